@@ -72,9 +72,26 @@ _SIGNATURES = {
     "hc_read_bwd": (_c_int, [_vp, _vp, _vp, _vp, _vp, _c_i64, _c_int, _c_int, _c_i64, _c_int, _vp]),
     "hc_mix_write_fwd": (_c_int, [_vp] * 6 + [_c_i64, _c_int, _c_int, _c_i64, _c_int, _vp]),
     "hc_mix_write_bwd": (_c_int, [_vp] * 11 + [_c_i64, _c_int, _c_int, _c_i64, _c_int, _vp]),
+    "hc_norm_scratch_words": (_c_i64, [_c_i64, _c_int, _c_int, _c_i64, _c_int]),
+    "hc_read_norm_fwd": (_c_int, [_vp] * 6 + [_c_i64, _c_int, _c_int, _c_i64, _c_int, ctypes.c_float, _c_int, _vp]),
+    "hc_read_norm_bwd": (_c_int, [_vp] * 10 + [_c_i64, _c_i64, _c_int, _c_int, _c_i64, _c_int, _c_int, _vp]),
+    "hc_mix_write_norm_fwd": (
+        _c_int,
+        [_vp] * 11 + [_c_i64, _c_int, _c_int, _c_i64, _c_int, _c_int, ctypes.c_float, ctypes.c_double, _vp, _c_i64,
+                      _c_i64, _c_int, _vp],
+    ),
+    "hc_mix_write_norm_bwd": (
+        _c_int,
+        [_vp] * 21 + [_c_i64, _c_i64, _c_int, _c_int, _c_i64, _c_int, _c_int, ctypes.c_double, _vp, _c_i64, _c_i64,
+                      _c_int, _vp],
+    ),
+    "hc_dropout": (_c_int, [_vp, _vp, _c_i64, ctypes.c_double, _vp, _c_i64, _c_i64, _c_int, _vp]),
+    "hc_gated_ffn_fwd": (_c_int, [_vp] * 9 + [_c_i64] * 5 + [_c_int, _c_int, _vp]),
+    "hc_gated_ffn_bwd": (_c_int, [_vp] * 15 + [_c_i64] * 5 + [_c_int, _c_int, _vp]),
+    "hc_gated_ffn_scratch_bytes": (_c_i64, [_c_int] + [_c_i64] * 4 + [_c_int]),
 }
 
-EXPECTED_ABI_VERSION = 7
+EXPECTED_ABI_VERSION = 8
 
 _lib: Optional[ctypes.CDLL] = None
 _load_error: Optional[str] = None

@@ -1,0 +1,111 @@
+// block.cuh — what the kernels of a layer's block share: arguments of the
+// norm kernels (hc_read_norm, hc_mix_write_norm), the dropout bits, and the
+// per-dtype launchers that block_capi.cu dispatches to.
+#pragma once
+
+#include "common.cuh"
+
+namespace hc {
+
+constexpr int kBlockMaxN = 8;  // streams
+constexpr int kBlockMaxM = 4;  // backbone blocks
+
+// ------------------------------------------------------------ dropout bits
+// Philox 4x32-10 (J. K. Salmon, M. A. Moraes, R. O. Dror, D. E. Shaw,
+// "Parallel random numbers: as easy as 1, 2, 3", SC 2011): ten rounds on a
+// 128-bit counter with a 64-bit key that grows by two Weyl constants. The
+// counter is (element / 4, offset), the key the seed, and element i takes word
+// i % 4, so the bits depend on nothing but the element's place: the forward,
+// the backward and every split of the work over threads draw the same ones.
+struct DropArgs {
+  const int64_t* state;  // device (seed, offset), or nullptr for the two below
+  uint64_t seed, offset;
+  uint64_t threshold;  // floor(p 2^32): an element is kept when its word is at least this
+  float scale;         // 1 / (1 - p); 0 at p = 1
+  int on;              // p > 0
+};
+
+struct DropKey {
+  uint32_t k0, k1, o0, o1;
+};
+
+__device__ __forceinline__ DropKey drop_key(const DropArgs& a) {
+  uint64_t seed = a.seed, offset = a.offset;
+  if (a.state) {
+    seed = static_cast<uint64_t>(a.state[0]);
+    offset = static_cast<uint64_t>(a.state[1]);
+  }
+  return DropKey{static_cast<uint32_t>(seed), static_cast<uint32_t>(seed >> 32), static_cast<uint32_t>(offset),
+                 static_cast<uint32_t>(offset >> 32)};
+}
+
+__device__ __forceinline__ uint4 philox4(const DropKey& key, uint64_t block) {
+  uint32_t c0 = static_cast<uint32_t>(block), c1 = static_cast<uint32_t>(block >> 32), c2 = key.o0, c3 = key.o1;
+  uint32_t k0 = key.k0, k1 = key.k1;
+#pragma unroll
+  for (int r = 0; r < 10; ++r) {
+    const uint64_t p0 = static_cast<uint64_t>(0xD2511F53u) * c0, p1 = static_cast<uint64_t>(0xCD9E8D57u) * c2;
+    c0 = static_cast<uint32_t>(p1 >> 32) ^ c1 ^ k0;
+    c1 = static_cast<uint32_t>(p1);
+    c2 = static_cast<uint32_t>(p0 >> 32) ^ c3 ^ k1;
+    c3 = static_cast<uint32_t>(p0);
+    k0 += 0x9E3779B9u;
+    k1 += 0xBB67AE85u;
+  }
+  return make_uint4(c0, c1, c2, c3);
+}
+
+// The word of one element.
+__device__ __forceinline__ uint32_t philox_word(const DropKey& key, uint64_t i) {
+  const uint4 w = philox4(key, i >> 2);
+  const uint32_t r = static_cast<uint32_t>(i) & 3u;
+  return r == 0 ? w.x : r == 1 ? w.y : r == 2 ? w.z : w.w;
+}
+
+// A dropped value is 0 whatever it was (an infinity or a NaN too), so it is
+// selected, not multiplied.
+__device__ __forceinline__ float drop_value(const DropArgs& a, uint32_t word, float v) {
+  return static_cast<uint64_t>(word) >= a.threshold ? v * a.scale : 0.f;
+}
+
+// ------------------------------------------------------------ norm kernels
+struct NormArgs {
+  const void* x;     // [T, n, D]
+  const void* g;     // upstream gradient: [T, m, D] (read), [T, n, D] (mix-write)
+  const void* f;     // [T, m, D] (mix-write)
+  const void* gate;  // [T, m, D] or nullptr
+  const float* R;    // [T, m, n] (read)
+  const float* H;    // [T, n, n] (mix-write)
+  const float* W;    // [T, n, m] (mix-write)
+  const float* v;    // [T, n] or nullptr
+  const float *weight, *bias, *scale;  // [m D] or nullptr
+  void* out;                           // y (read) or x' (mix-write)
+  float* stats;                        // [T, 2]: mean, 1 / root
+  void *grad_x, *grad_f, *grad_gate;
+  float *grad_R, *grad_H, *grad_W, *grad_v;
+  float* partial;  // [grid][2][m D]: the CTAs' sums over their tokens, or nullptr
+  int64_t T, D;
+  int n, m, norm, gate_act;
+  float eps;
+  DropArgs drop;
+};
+
+// Which kernels a call takes, and over how many CTAs.
+struct NormGeometry {
+  int grid;   // CTAs; also the rows of `partial`
+  int warps;  // warps of one token's group (the 8-column kernels); 0 = element by element
+};
+
+#define HC_BLOCK_DECL(SFX)                                                                            \
+  int norm_launch_##SFX(bool write, bool bwd, const NormGeometry& g, const NormArgs& a, cudaStream_t s); \
+  int dropout_launch_##SFX(const void* x, void* y, int64_t N, const DropArgs& d, cudaStream_t s);
+HC_BLOCK_DECL(f32)
+HC_BLOCK_DECL(f16)
+HC_BLOCK_DECL(bf16)
+#undef HC_BLOCK_DECL
+
+// grad_weight, grad_bias and grad_scale from the CTAs' sums (block_capi.cu).
+int norm_param_grads(const float* partial, int rows, int64_t E, const float* weight, const float* bias,
+                     const float* scale, float* grad_weight, float* grad_bias, float* grad_scale, cudaStream_t s);
+
+}  // namespace hc

@@ -1,0 +1,231 @@
+// block_capi.cu — C entry points of the norm kernels around a layer's block
+// and of dropout (see hcops.h). Host-side checks come first; then the kernels
+// of the stream dtype, and for the [m D] parameters' gradients one more launch
+// that adds the CTAs' sums.
+#include <math.h>
+
+#include "block.cuh"
+
+namespace hc {
+namespace {
+
+constexpr int64_t kMaxD = int64_t(1) << 24;
+constexpr int64_t kMaxTokens = (int64_t(1) << 31) - 1;
+
+int check_shape(int64_t T, int n, int m, int64_t D, int sdt) {
+  if (T < 0 || T > kMaxTokens || D < 0 || D > kMaxD) return HC_ERR_BAD_SIZE;
+  if (n < 1 || n > kBlockMaxN || m < 1 || m > kBlockMaxM) return HC_ERR_UNSUPPORTED_N;
+  if (dtype_size(sdt) == 0) return HC_ERR_DTYPE;
+  return HC_OK;
+}
+
+bool f32_ok(std::initializer_list<const float*> ps) {
+  for (const float* p : ps)
+    if (!aligned4(p)) return false;
+  return true;
+}
+
+// Dropout's arguments; false when p is not in [0, 1].
+bool drop_args(DropArgs& d, double p, const int64_t* state, int64_t seed, int64_t offset) {
+  if (!(p >= 0.0 && p <= 1.0)) return false;
+  d.state = state;
+  d.seed = static_cast<uint64_t>(seed);
+  d.offset = static_cast<uint64_t>(offset);
+  d.threshold = static_cast<uint64_t>(floor(p * 4294967296.0));
+  d.scale = p < 1.0 ? static_cast<float>(1.0 / (1.0 - p)) : 0.f;
+  d.on = p > 0.0;
+  return true;
+}
+
+NormGeometry geometry(int64_t T) {
+  NormGeometry g{};
+  const int64_t cap = 4 * static_cast<int64_t>(sm_count());
+  g.grid = static_cast<int>(T < cap ? T : cap);
+  return g;
+}
+
+int launch(int sdt, bool write, bool bwd, const NormGeometry& g, const NormArgs& a, cudaStream_t s) {
+  switch (sdt) {
+    case HC_DTYPE_F32: return norm_launch_f32(write, bwd, g, a, s);
+    case HC_DTYPE_F16: return norm_launch_f16(write, bwd, g, a, s);
+    case HC_DTYPE_BF16: return norm_launch_bf16(write, bwd, g, a, s);
+  }
+  return HC_ERR_DTYPE;
+}
+
+// ------------------------------------------------ the [E] parameters' grads
+// A = sum over rows of partial[.][0][c], B of partial[.][1][c]: a CTA takes 32
+// columns, its 8 warps every 8th row, and the warps' sums are added in order, so
+// the result does not depend on timing.
+constexpr int kParamWarps = 8;
+
+__global__ void __launch_bounds__(32 * kParamWarps)
+    norm_param_grads_kernel(const float* partial, int rows, int64_t E, const float* weight, const float* bias,
+                            const float* scale, float* gw, float* gb, float* gs) {
+  __shared__ float sA[kParamWarps][32], sB[kParamWarps][32];
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+  const int64_t c = static_cast<int64_t>(blockIdx.x) * 32 + lane;
+  float A = 0.f, B = 0.f;
+  if (c < E)
+    for (int r = w; r < rows; r += kParamWarps) {
+      A += partial[static_cast<int64_t>(r) * 2 * E + c];
+      B += partial[static_cast<int64_t>(r) * 2 * E + E + c];
+    }
+  sA[w][lane] = A;
+  sB[w][lane] = B;
+  __syncthreads();
+  if (w != 0 || c >= E) return;
+  for (int i = 1; i < kParamWarps; ++i) {
+    A += sA[i][lane];
+    B += sB[i][lane];
+  }
+  const float sc = scale ? scale[c] : 1.f;
+  if (gw) gw[c] = sc * A;
+  if (gb) gb[c] = sc * B;
+  if (gs) gs[c] = (weight ? weight[c] : 1.f) * A + (bias ? bias[c] : 0.f) * B;
+}
+
+}  // namespace
+
+int norm_param_grads(const float* partial, int rows, int64_t E, const float* weight, const float* bias,
+                     const float* scale, float* grad_weight, float* grad_bias, float* grad_scale, cudaStream_t s) {
+  norm_param_grads_kernel<<<static_cast<unsigned>((E + 31) / 32), 32 * kParamWarps, 0, s>>>(
+      partial, rows, E, weight, bias, scale, grad_weight, grad_bias, grad_scale);
+  return launch_status();
+}
+
+}  // namespace hc
+
+using namespace hc;
+
+extern "C" int64_t hc_norm_scratch_words(int64_t T, int n, int m, int64_t D, int stream_dtype) {
+  if (check_shape(T, n, m, D, stream_dtype) || T == 0 || D == 0) return 0;
+  return static_cast<int64_t>(geometry(T).grid) * 2 * m * D;
+}
+
+extern "C" int hc_read_norm_fwd(const float* R, const void* x, const float* weight, const float* bias, void* y,
+                                float* stats, int64_t T, int n, int m, int64_t D, int norm, float eps,
+                                int stream_dtype, void* stream) {
+  HC_ENTRY("hc_read_norm_fwd");
+  if (int rc = check_shape(T, n, m, D, stream_dtype)) return rc;
+  if (norm != HC_NORM_RMS && norm != HC_NORM_LAYER) return HC_ERR_BAD_SIZE;
+  if (!(eps >= 0.f)) return HC_ERR_BAD_SIZE;
+  if (T == 0 || D == 0) return HC_OK;
+  if (!R || !x || !y) return HC_ERR_NULL_POINTER;
+  if (!f32_ok({R, weight, bias, stats})) return HC_ERR_ALIGNMENT;
+  NormArgs a{};
+  a.R = R; a.x = x; a.weight = weight; a.bias = bias; a.out = y; a.stats = stats;
+  a.T = T; a.D = D; a.n = n; a.m = m; a.norm = norm; a.eps = eps;
+  return launch(stream_dtype, false, false, geometry(T), a, static_cast<cudaStream_t>(stream));
+}
+
+extern "C" int hc_read_norm_bwd(const void* g, const float* R, const void* x, const float* weight, const float* stats,
+                                void* grad_x, float* grad_R, float* grad_weight, float* grad_bias, float* scratch,
+                                int64_t scratch_words, int64_t T, int n, int m, int64_t D, int norm,
+                                int stream_dtype, void* stream) {
+  HC_ENTRY("hc_read_norm_bwd");
+  if (int rc = check_shape(T, n, m, D, stream_dtype)) return rc;
+  if (norm != HC_NORM_RMS && norm != HC_NORM_LAYER) return HC_ERR_BAD_SIZE;
+  const cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const int64_t E = m * D;
+  if (T == 0 || D == 0) {  // sums over nothing
+    if (!f32_ok({grad_R, grad_weight, grad_bias})) return HC_ERR_ALIGNMENT;
+    if (grad_R && T > 0 && cudaMemsetAsync(grad_R, 0, sizeof(float) * T * m * n, s) != cudaSuccess) return HC_ERR_LAUNCH;
+    for (float* p : {grad_weight, grad_bias})
+      if (p && E > 0 && cudaMemsetAsync(p, 0, sizeof(float) * E, s) != cudaSuccess) return HC_ERR_LAUNCH;
+    return HC_OK;
+  }
+  if (!g || !R || !x || !stats) return HC_ERR_NULL_POINTER;
+  if (!f32_ok({R, weight, stats, grad_R, grad_weight, grad_bias, scratch})) return HC_ERR_ALIGNMENT;
+  const bool params = grad_weight || grad_bias;
+  if (params && (!scratch || scratch_words < hc_norm_scratch_words(T, n, m, D, stream_dtype))) return HC_ERR_SCRATCH;
+  NormArgs a{};
+  a.g = g; a.R = R; a.x = x; a.weight = weight; a.stats = const_cast<float*>(stats);
+  a.grad_x = grad_x; a.grad_R = grad_R; a.partial = params ? scratch : nullptr;
+  a.T = T; a.D = D; a.n = n; a.m = m; a.norm = norm;
+  const NormGeometry geo = geometry(T);
+  if (int rc = launch(stream_dtype, false, true, geo, a, s)) return rc;
+  return params ? norm_param_grads(scratch, geo.grid, E, weight, nullptr, nullptr, grad_weight, grad_bias, nullptr, s)
+                : HC_OK;
+}
+
+namespace {
+int check_write(int norm, int gate_act, double p) {
+  if (norm != HC_NORM_NONE && norm != HC_NORM_RMS && norm != HC_NORM_LAYER) return HC_ERR_BAD_SIZE;
+  if (gate_act != HC_ACT_LINEAR && gate_act != HC_ACT_SIGMOID) return HC_ERR_BAD_SIZE;
+  return p >= 0.0 && p <= 1.0 ? HC_OK : HC_ERR_BAD_SIZE;
+}
+}  // namespace
+
+extern "C" int hc_mix_write_norm_fwd(const float* H, const void* x, const float* W, const void* f, const float* v,
+                                     const float* weight, const float* bias, const void* gate, const float* scale,
+                                     void* out, float* stats, int64_t T, int n, int m, int64_t D, int norm,
+                                     int gate_act, float eps, double p, const int64_t* state, int64_t seed,
+                                     int64_t offset, int stream_dtype, void* stream) {
+  HC_ENTRY("hc_mix_write_norm_fwd");
+  if (int rc = check_shape(T, n, m, D, stream_dtype)) return rc;
+  if (int rc = check_write(norm, gate_act, p)) return rc;
+  if (!(eps >= 0.f)) return HC_ERR_BAD_SIZE;
+  if (T == 0 || D == 0) return HC_OK;
+  if (!H || !x || !W || !f || !out) return HC_ERR_NULL_POINTER;
+  if (!f32_ok({H, W, v, weight, bias, scale, stats})) return HC_ERR_ALIGNMENT;
+  NormArgs a{};
+  a.H = H; a.x = x; a.W = W; a.f = f; a.v = v; a.weight = weight; a.bias = bias; a.gate = gate; a.scale = scale;
+  a.out = out; a.stats = stats; a.T = T; a.D = D; a.n = n; a.m = m; a.norm = norm; a.gate_act = gate_act; a.eps = eps;
+  drop_args(a.drop, p, state, seed, offset);
+  return launch(stream_dtype, true, false, geometry(T), a, static_cast<cudaStream_t>(stream));
+}
+
+extern "C" int hc_mix_write_norm_bwd(const void* g, const float* H, const void* x, const float* W, const void* f,
+                                     const float* v, const float* weight, const float* bias, const void* gate,
+                                     const float* scale, const float* stats, void* grad_x, void* grad_f,
+                                     void* grad_gate, float* grad_H, float* grad_W, float* grad_v, float* grad_weight,
+                                     float* grad_bias, float* grad_scale, float* scratch, int64_t scratch_words,
+                                     int64_t T, int n, int m, int64_t D, int norm, int gate_act, double p,
+                                     const int64_t* state, int64_t seed, int64_t offset, int stream_dtype,
+                                     void* stream) {
+  HC_ENTRY("hc_mix_write_norm_bwd");
+  if (int rc = check_shape(T, n, m, D, stream_dtype)) return rc;
+  if (int rc = check_write(norm, gate_act, p)) return rc;
+  const cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const int64_t E = m * D;
+  if (!f32_ok({H, W, v, weight, bias, scale, stats, grad_H, grad_W, grad_v, grad_weight, grad_bias, grad_scale, scratch}))
+    return HC_ERR_ALIGNMENT;
+  if (T == 0 || D == 0) {  // sums over nothing
+    const struct { float* p; int64_t words; } zero[] = {{grad_H, T * n * n}, {grad_W, T * n * m}, {grad_v, T * n},
+                                                        {grad_weight, E}, {grad_bias, E}, {grad_scale, E}};
+    for (const auto& z : zero)
+      if (z.p && z.words > 0 && cudaMemsetAsync(z.p, 0, sizeof(float) * z.words, s) != cudaSuccess) return HC_ERR_LAUNCH;
+    return HC_OK;
+  }
+  if (!g || !H || !x || !W || !f || (norm != HC_NORM_NONE && !stats)) return HC_ERR_NULL_POINTER;
+  const bool params = grad_weight || grad_bias || grad_scale;
+  if (params && (!scratch || scratch_words < hc_norm_scratch_words(T, n, m, D, stream_dtype))) return HC_ERR_SCRATCH;
+  NormArgs a{};
+  a.g = g; a.H = H; a.x = x; a.W = W; a.f = f; a.v = v; a.weight = weight; a.bias = bias; a.gate = gate;
+  a.scale = scale; a.stats = const_cast<float*>(stats); a.grad_x = grad_x; a.grad_f = grad_f;
+  a.grad_gate = gate ? grad_gate : nullptr; a.grad_H = grad_H; a.grad_W = grad_W; a.grad_v = v ? grad_v : nullptr;
+  a.partial = params ? scratch : nullptr;
+  a.T = T; a.D = D; a.n = n; a.m = m; a.norm = norm; a.gate_act = gate_act;
+  drop_args(a.drop, p, state, seed, offset);
+  const NormGeometry geo = geometry(T);
+  if (int rc = launch(stream_dtype, true, true, geo, a, s)) return rc;
+  return params ? norm_param_grads(scratch, geo.grid, E, weight, bias, scale, grad_weight, grad_bias, grad_scale, s)
+                : HC_OK;
+}
+
+extern "C" int hc_dropout(const void* x, void* y, int64_t N, double p, const int64_t* state, int64_t seed,
+                          int64_t offset, int stream_dtype, void* stream) {
+  HC_ENTRY("hc_dropout");
+  if (N < 0 || dtype_size(stream_dtype) == 0) return N < 0 ? HC_ERR_BAD_SIZE : HC_ERR_DTYPE;
+  DropArgs d{};
+  if (!drop_args(d, p, state, seed, offset)) return HC_ERR_BAD_SIZE;
+  if (N == 0) return HC_OK;
+  if (!x || !y) return HC_ERR_NULL_POINTER;
+  const cudaStream_t s = static_cast<cudaStream_t>(stream);
+  switch (stream_dtype) {
+    case HC_DTYPE_F32: return dropout_launch_f32(x, y, N, d, s);
+    case HC_DTYPE_F16: return dropout_launch_f16(x, y, N, d, s);
+    default: return dropout_launch_bf16(x, y, N, d, s);
+  }
+}

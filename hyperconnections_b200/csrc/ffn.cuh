@@ -1,0 +1,54 @@
+// ffn.cuh — the gated feed-forward's products, described once for every
+// kernel that computes them (ffn_capi.cu makes the descriptions).
+//
+//   forward   [a b] = x [w_gate; w_up]^T  -> h = act(a) * b      (kGlu)
+//             y     = h w_down^T                                 (kStore)
+//   backward  dh    = g w_down            -> da, db              (kGluBwd)
+//             dx    = da w_gate + db w_up                        (kStore, two terms)
+//             dw_gate = da^T x, dw_up = db^T x, dw_down = g^T h  (kStore)
+#pragma once
+
+#include "common.cuh"
+
+namespace hc {
+
+enum FfnEpilogue { kStore, kGlu, kGluBwd };
+
+// A matrix [rows, K] read as p[row * row_stride + k * k_stride]; one of the two
+// strides is 1.
+struct FfnOperand {
+  const void* p;
+  int64_t row_stride, k_stride;
+  int64_t rows;  // rows that exist: the others count as 0
+};
+
+struct FfnProduct {
+  int epilogue;
+  int terms;            // 1, or 2 products summed into one result
+  FfnOperand A[2];      // by term
+  FfnOperand B[2];      // by term; kGlu: w_gate and w_up of its one term
+  int64_t M, N, K;      // result [M, N], summed over K (for each term)
+  void* out;            // kStore: the result; kGlu: h; kGluBwd: da
+  void* out2;           // kGluBwd: db
+  void *pre_gate, *pre_up;  // kGlu: written (nullable); kGluBwd: read
+  int64_t ldo;          // row stride of the above
+  int act;
+};
+
+// act(a) and its derivative.
+__device__ __forceinline__ void ffn_act(int act, float a, float& val, float& der) {
+  if (act == HC_ACT_SILU) {
+    const float s = 1.f / (1.f + expf(-a));
+    val = a * s;
+    der = s + val * (1.f - s);
+  } else {  // 0.5 a (1 + tanh(c (a + 0.044715 a^3))), c = sqrt(2 / pi)
+    const float c = 0.7978845608028654f, a2 = a * a;
+    const float t = tanhf(c * a * (1.f + 0.044715f * a2));
+    val = 0.5f * a * (1.f + t);
+    der = 0.5f * (1.f + t) + 0.5f * a * (1.f - t * t) * c * (1.f + 3.f * 0.044715f * a2);
+  }
+}
+
+int ffn_simt_launch(const FfnProduct& p, int dtype, cudaStream_t s);
+
+}  // namespace hc

@@ -346,6 +346,128 @@ int hc_mix_write_bwd(const void* g, const float* H, const void* x,
                      float* grad_v, int64_t T, int n, int m, int64_t D,
                      int stream_dtype, void* stream);
 
+/* ===========================================================================
+ * The block between the read and the write: its norms, its gate, residual
+ * scale and dropout, and a gated feed-forward. E = m D is the block's width.
+ * Parameters (norm weight and bias, residual scale) are float32 [E]. No
+ * reference counterpart: the reference's layers leave all of this to the
+ * module they wrap.
+ * ======================================================================== */
+
+/* ---- norm kinds ----------------------------------------------------------- */
+#define HC_NORM_NONE   0  /* hc_mix_write_norm only: f is used as it is        */
+#define HC_NORM_RMS    1  /* u (mean(u^2) + eps)^-1/2                           */
+#define HC_NORM_LAYER  2  /* (u - mean u) (var u + eps)^-1/2                    */
+
+/* ---- activations ---------------------------------------------------------- */
+#define HC_ACT_LINEAR     0
+#define HC_ACT_SIGMOID    1  /* of a gate                                       */
+#define HC_ACT_SILU       2  /* of a gated feed-forward                         */
+#define HC_ACT_GELU_TANH  3  /* of a gated feed-forward                         */
+
+/* Dropout bits. Element i of a tensor (its row-major index) is kept when word
+ * i % 4 of Philox 4x32-10 (Salmon, Moraes, Dror and Shaw, SC 2011) with
+ * counter (i / 4, offset) and key seed is at least floor(p 2^32); what is kept
+ * is multiplied with 1 / (1 - p), what is not becomes 0 whatever it was.
+ * `state`, when not NULL, is a DEVICE pointer to two int64 (seed, offset)
+ * that replace the arguments `seed` and `offset` and are read when the kernel
+ * runs, so that a replayed graph can draw new bits. 0 <= p <= 1. */
+
+/* float32 words of scratch that the backward of hc_read_norm or
+ * hc_mix_write_norm needs for the gradients of its [E] parameters. Returns 0
+ * in error cases. Depends on the current device's SM count. */
+int64_t hc_norm_scratch_words(int64_t T, int n, int m, int64_t D, int stream_dtype);
+
+/* u[t,k,:] = sum_j R[t,k,j] x[t,j,:];  y[t] = weight * norm(u[t]) + bias over
+ * the E values of a token. R [T,m,n], x [T,n,D] -> y [T,m,D]; weight, bias
+ * [E] or NULL; norm HC_NORM_RMS or HC_NORM_LAYER, eps >= 0. stats [T,2]
+ * float32 (mean, 1 / root) for the backward, or NULL. u is never stored. */
+int hc_read_norm_fwd(const float* R, const void* x, const float* weight,
+                     const float* bias, void* y, float* stats, int64_t T,
+                     int n, int m, int64_t D, int norm, float eps,
+                     int stream_dtype, void* stream);
+
+/* Given g = dL/dy [T,m,D]: grad_x [T,n,D], grad_R [T,m,n] float32,
+ * grad_weight and grad_bias [E] float32, each nullable (u comes again from x
+ * and R). scratch is needed for grad_weight / grad_bias only. */
+int hc_read_norm_bwd(const void* g, const float* R, const void* x,
+                     const float* weight, const float* stats, void* grad_x,
+                     float* grad_R, float* grad_weight, float* grad_bias,
+                     float* scratch, int64_t scratch_words, int64_t T, int n,
+                     int m, int64_t D, int norm, int stream_dtype,
+                     void* stream);
+
+/* z[t]   = dropout(scale * act(gate[t]) * (weight * norm(f[t]) + bias))
+ * out[t,i,:] = sum_j H_ij x_j [+ (v_i - (H v)_i) (v^T x)] + sum_k W_ik z_k
+ * H [T,n,n], W [T,n,m], v [T,n] or NULL, f and gate [T,m,D] (gate or NULL),
+ * weight, bias, scale [E] or NULL; norm any HC_NORM_*, gate_act
+ * HC_ACT_LINEAR or HC_ACT_SIGMOID. z's elements are numbered over [T,m,D] for
+ * the dropout; p == 0 draws nothing. stats [T,2] as above (unused with
+ * HC_NORM_NONE). z is never stored. */
+int hc_mix_write_norm_fwd(const float* H, const void* x, const float* W,
+                          const void* f, const float* v, const float* weight,
+                          const float* bias, const void* gate,
+                          const float* scale, void* out, float* stats,
+                          int64_t T, int n, int m, int64_t D, int norm,
+                          int gate_act, float eps, double p,
+                          const int64_t* state, int64_t seed, int64_t offset,
+                          int stream_dtype, void* stream);
+
+/* Given g = dL/dout [T,n,D]: grad_x, grad_f, grad_gate (stream dtype),
+ * grad_H, grad_W, grad_v (float32, per token), grad_weight, grad_bias,
+ * grad_scale [E] float32, each nullable. The dropout bits are drawn again.
+ * scratch is needed for the [E] gradients only. */
+int hc_mix_write_norm_bwd(const void* g, const float* H, const void* x,
+                          const float* W, const void* f, const float* v,
+                          const float* weight, const float* bias,
+                          const void* gate, const float* scale,
+                          const float* stats, void* grad_x, void* grad_f,
+                          void* grad_gate, float* grad_H, float* grad_W,
+                          float* grad_v, float* grad_weight, float* grad_bias,
+                          float* grad_scale, float* scratch,
+                          int64_t scratch_words, int64_t T, int n, int m,
+                          int64_t D, int norm, int gate_act, double p,
+                          const int64_t* state, int64_t seed, int64_t offset,
+                          int stream_dtype, void* stream);
+
+/* y[i] = dropout(x[i]) for N elements (see "Dropout bits"); the backward is
+ * the same call on the upstream gradient. y may be x. */
+int hc_dropout(const void* x, void* y, int64_t N, double p,
+               const int64_t* state, int64_t seed, int64_t offset,
+               int stream_dtype, void* stream);
+
+/* Gated feed-forward: a = x w_gate^T, b = x w_up^T, h = act(a) * b (one
+ * kernel), y = h w_down^T. x [T,D], w_gate and w_up [F,D], w_down [O,F],
+ * y [T,O]; every tensor has `dtype`, products are summed in float32, and h (and
+ * a, b for the backward) are rounded once to dtype. act HC_ACT_SILU or
+ * HC_ACT_GELU_TANH. h, pre_gate (a) and pre_up (b) are [T,Fp] with
+ * Fp = F rounded up to a multiple of 8 (their last columns are written 0);
+ * pre_gate and pre_up NULL when no backward follows. scratch:
+ * hc_gated_ffn_scratch_bytes(0, ...) bytes, 256-byte aligned. */
+int hc_gated_ffn_fwd(const void* x, const void* w_gate, const void* w_up,
+                     const void* w_down, void* y, void* h, void* pre_gate,
+                     void* pre_up, void* scratch, int64_t scratch_bytes,
+                     int64_t T, int64_t D, int64_t F, int64_t O, int act,
+                     int dtype, void* stream);
+
+/* Given g = dL/dy [T,O]: grad_x [T,D], grad_w_gate and grad_w_up [F,D],
+ * grad_w_down [O,F], each nullable, from the forward's h, pre_gate and
+ * pre_up. d_gate and d_up: workspaces [T,Fp] (the gradients of a and b; not
+ * needed when grad_w_down alone is wanted). scratch:
+ * hc_gated_ffn_scratch_bytes(1, ...) bytes, 256-byte aligned. */
+int hc_gated_ffn_bwd(const void* g, const void* x, const void* w_gate,
+                     const void* w_up, const void* w_down, const void* h,
+                     const void* pre_gate, const void* pre_up, void* d_gate,
+                     void* d_up, void* grad_x, void* grad_w_gate,
+                     void* grad_w_up, void* grad_w_down, void* scratch,
+                     int64_t scratch_bytes, int64_t T, int64_t D, int64_t F,
+                     int64_t O, int act, int dtype, void* stream);
+
+/* Bytes of scratch of the two calls above (0 when none is needed, -1 for
+ * arguments they refuse). Depends on the current device's SM count. */
+int64_t hc_gated_ffn_scratch_bytes(int backward, int64_t T, int64_t D,
+                                   int64_t F, int64_t O, int dtype);
+
 #ifdef __cplusplus
 }
 #endif
