@@ -250,6 +250,8 @@ inline int dtype_size(int dt) {
 // Bounded waits of the expm kernels that gave up (expm.cu); summed into
 // hc_wait_timeouts() with those of the ring kernels.
 unsigned int expm_take_timeouts(bool reset);
+// The same of the feed-forward's tensor-core products (ffn_tc.cu).
+unsigned int ffn_take_timeouts(bool reset);
 
 // ------------------------------------------------------ bounded-wait status
 // Every spin-wait in the kernels polls at most a fixed number of times. A wait

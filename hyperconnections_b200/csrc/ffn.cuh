@@ -30,7 +30,7 @@ struct FfnProduct {
   int64_t M, N, K;      // result [M, N], summed over K (for each term)
   void* out;            // kStore: the result; kGlu: h; kGluBwd: da
   void* out2;           // kGluBwd: db
-  void *pre_gate, *pre_up;  // kGlu: written (nullable); kGluBwd: read
+  void *slope_gate, *slope_up;  // act'(a) b and act(a); kGlu: written (nullable); kGluBwd: read
   int64_t ldo;          // row stride of the above
   int act;
 };
@@ -49,6 +49,12 @@ __device__ __forceinline__ void ffn_act(int act, float a, float& val, float& der
   }
 }
 
-int ffn_simt_launch(const FfnProduct& p, int dtype, cudaStream_t s);
+// float32 (ffn_simt.cu).
+int ffn_simt_launch(const FfnProduct& p, cudaStream_t s);
 
+// bf16 and fp16 (ffn_tc.cu): operands 16-byte aligned with strides of whole 16
+// bytes. `parts`: splits * M * N floats where ffn_tc_splits says more than one
+// (kStore only), else nullptr.
+int ffn_tc_splits(int64_t M, int64_t N, int64_t K, int terms);
+int ffn_tc_launch(const FfnProduct& p, int dtype, float* parts, cudaStream_t s);
 }  // namespace hc

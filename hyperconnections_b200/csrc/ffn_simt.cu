@@ -1,7 +1,6 @@
-// ffn_simt.cu — the gated feed-forward's products on the FMA units: any type,
-// size, order and alignment. float32 products run here (the tensor cores have
-// no float32 inputs), 64 x 64 tiles of the result by 256 threads, 4 x 4 a
-// thread.
+// ffn_simt.cu — the gated feed-forward's float32 products on the FMA units (the
+// tensor cores have no float32 inputs): any size and order, 64 x 64 tiles of
+// the result by 256 threads, 4 x 4 a thread.
 #include "ffn.cuh"
 
 namespace hc {
@@ -86,16 +85,14 @@ __global__ void __launch_bounds__(kThreads) ffn_simt_kernel(FfnProduct p) {
         float val, der;
         ffn_act(p.act, a, val, der);
         static_cast<T*>(p.out)[at] = Elem<T>::from_f(val * b);
-        if (p.pre_gate) {
-          static_cast<T*>(p.pre_gate)[at] = Elem<T>::from_f(a);
-          static_cast<T*>(p.pre_up)[at] = Elem<T>::from_f(b);
+        if (p.slope_gate) {
+          static_cast<T*>(p.slope_gate)[at] = Elem<T>::from_f(der * b);
+          static_cast<T*>(p.slope_up)[at] = Elem<T>::from_f(val);
         }
       } else {
-        const float dh = acc[0][i][j], b = Elem<T>::to_f(static_cast<const T*>(p.pre_up)[at]);
-        float val, der;
-        ffn_act(p.act, Elem<T>::to_f(static_cast<const T*>(p.pre_gate)[at]), val, der);
-        static_cast<T*>(p.out)[at] = Elem<T>::from_f(dh * b * der);
-        static_cast<T*>(p.out2)[at] = Elem<T>::from_f(dh * val);
+        const float dh = acc[0][i][j];
+        static_cast<T*>(p.out)[at] = Elem<T>::from_f(dh * Elem<T>::to_f(static_cast<const T*>(p.slope_gate)[at]));
+        static_cast<T*>(p.out2)[at] = Elem<T>::from_f(dh * Elem<T>::to_f(static_cast<const T*>(p.slope_up)[at]));
       }
     }
 }
@@ -112,13 +109,6 @@ template <typename T> int launch(const FfnProduct& p, cudaStream_t s) {
 
 }  // namespace
 
-int ffn_simt_launch(const FfnProduct& p, int dtype, cudaStream_t s) {
-  switch (dtype) {
-    case HC_DTYPE_F32: return launch<float>(p, s);
-    case HC_DTYPE_F16: return launch<__half>(p, s);
-    case HC_DTYPE_BF16: return launch<__nv_bfloat16>(p, s);
-  }
-  return HC_ERR_DTYPE;
-}
+int ffn_simt_launch(const FfnProduct& p, cudaStream_t s) { return launch<float>(p, s); }
 
 }  // namespace hc

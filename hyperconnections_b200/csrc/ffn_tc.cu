@@ -1,0 +1,622 @@
+// ffn_tc.cu — the gated feed-forward's products on the 5th-generation tensor
+// cores, bf16 and fp16.
+//
+// A pair of CTAs (a cluster of two, on two SMs) owns a 256 x 256 tile of a
+// result: tcgen05.mma with cta_group::2, each CTA holding 128 rows of A, 128
+// rows of B and its 128 x 256 half of the float32 accumulator in tensor
+// memory. Against a CTA of its own with a 128 x 256 tile this halves the bytes
+// of B that an SM fetches: 32 KB for every 512 cycles of the tensor cores.
+// Clusters are persistent and walk the tiles; per CTA
+//
+//   warp 0      fetches: one lane issues the TMA copies of the CTA's halves of
+//               A and B into a ring of 6 stages of 32 KB (64 deep); both CTAs'
+//               copies are counted on the leader's barrier
+//   warp 1      multiplies (in the leader CTA): one lane issues the four
+//               16-deep steps of a stage for both CTAs
+//   warp 2      owns the tensor memory
+//   warps 4-11  finish: two groups of four warps read the accumulator out of
+//               tensor memory, half of the columns each, and write the result
+//               while the next tile is multiplied into the other half of
+//               tensor memory (2 x 256 of its 512 columns)
+//
+// An operand is read as it lies: summed along its unit stride ("K-major", x
+// and the weights of the forward) or across it ("MN-major", the weights of dx
+// and both operands of the weights' gradients); both come as boxes of 128-byte
+// lines with the 128-byte swizzle, and the matrix descriptor says which of the
+// two they are. For h, the CTAs of a pair fetch different weights: the leader
+// w_gate's 128 rows, its peer w_up's, so a accumulates in columns 0-127, b in
+// columns 128-255 of the same rows, and a thread that finishes a row holds
+// both.
+//
+// Products with few tiles and a long sum (the weights' gradients of a narrow
+// model, a few tokens) split the sum over several clusters, which write
+// float32 parts that one more kernel adds in order.
+//
+// Every wait is bounded (poll limit of status.cu): a warp that gives up
+// reports it, tells both CTAs to stop, and the pair leaves together after its
+// copies in flight have landed.
+#include "ffn.cuh"
+#include "mix_warp.cuh"
+
+namespace hc {
+namespace {
+
+__device__ unsigned int g_ffn_wait_timeouts;
+
+constexpr int kRows = 128;         // rows of A, and of B, that one CTA holds
+constexpr int kTileM = 2 * kRows;  // a pair's tile
+constexpr int kTileN = 2 * kRows;
+constexpr int kDepth = 64;         // elements of the sum in a stage: 128 bytes
+constexpr int kStages = 6;
+constexpr int kOperandBytes = kRows * kDepth * 2;
+constexpr int kStageBytes = 2 * kOperandBytes;
+constexpr int kThreads = 384;
+constexpr int kFinishWarp = 4;  // the first of the eight finishing warps
+constexpr int kSmemBytes = kStages * kStageBytes + 1024;
+constexpr int kGroupM = 8;  // tiles of A that neighbouring clusters share B with
+
+struct alignas(64) TcMaps {
+  CUtensorMap a[2], b[2];
+};
+
+struct TcArgs {
+  int64_t M, N, ldo;
+  void *out, *out2;
+  void *slope_gate, *slope_up;  // kGlu: written (nullable); kGluBwd: read
+  float* parts;                 // float32 parts [splits][M][N], or nullptr
+  int tiles_m, tiles_n, splits;
+  int blocks_term, blocks;  // 64-deep blocks of one term, and of all
+  int a_mn, b_mn;           // operands whose unit stride is their rows
+  int act, vec;             // vec: bytes that the result's rows are aligned to (32, 16, or 2)
+  uint32_t wait_limit;
+  unsigned int* status;
+};
+
+struct Shared {
+  uint64_t full[kStages], empty[kStages];
+  uint64_t acc_full[2], acc_empty[2], drain;
+  uint32_t tmem;
+  volatile int stop;
+};
+
+// ------------------------------------------------------------------- PTX
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// The address of a shared variable of CTA `rank` of the cluster.
+__device__ __forceinline__ uint32_t cluster_addr(const void* p, uint32_t rank) {
+  uint32_t r;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(smem_u32(p)), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ void arrive_cluster(uint32_t addr) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(addr) : "memory");
+}
+// A box of a matrix into this CTA, counted on a barrier of the pair.
+__device__ __forceinline__ void fetch_box(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], "
+      "[%4];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(bar)
+      : "memory");
+}
+__device__ __forceinline__ void mma_pair(uint32_t acc, uint64_t a, uint64_t b, uint32_t idesc, uint32_t add) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(acc),
+      "l"(a), "l"(b), "r"(idesc), "r"(add)
+      : "memory");
+}
+// The barrier at this offset in both CTAs is arrived at when the products issued so far are done.
+__device__ __forceinline__ void commit_pair(uint64_t* bar) {
+  asm volatile(
+      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
+          smem_u32(bar)),
+      "h"(static_cast<uint16_t>(3))
+      : "memory");
+}
+__device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+
+// 16 consecutive columns of this thread's accumulator row.
+__device__ __forceinline__ void acc_load16(uint32_t addr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(addr));
+}
+__device__ __forceinline__ void acc_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+
+// Shared-memory matrix descriptor with the 128-byte swizzle. K-major: groups of
+// 8 rows are 1024 bytes apart. MN-major: groups of 8 steps of the sum are 1024
+// bytes apart, and the next 64 rows begin a whole box (64 lines) on.
+__device__ __forceinline__ uint64_t matrix_desc(uint32_t addr, bool mn) {
+  const uint64_t lead = mn ? (kDepth * 128) >> 4 : 1, step = 1024 >> 4;
+  return static_cast<uint64_t>((addr & 0x3ffff) >> 4) | (lead << 16) | (step << 32) | (1ull << 46) | (2ull << 61);
+}
+
+// Bounded wait that also ends when the pair has been told to stop.
+__device__ __forceinline__ bool pair_wait(Shared& sh, uint64_t* bar, uint32_t parity, uint32_t limit) {
+  for (uint32_t i = 0; i < limit; ++i) {
+    if (mbar_try_wait(bar, parity)) return true;
+    if (sh.stop) return false;
+  }
+  return false;
+}
+
+__device__ __forceinline__ void tell_stop(Shared& sh, const TcArgs& a) {
+  if (!sh.stop) report_timeout(&g_ffn_wait_timeouts, a.status);
+  for (uint32_t r = 0; r < 2; ++r)
+    asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(cluster_addr(const_cast<int*>(&sh.stop), r)), "r"(1)
+                 : "memory");
+}
+
+// ------------------------------------------------------------------ tiles
+struct Item {
+  int m, n;          // tile
+  int split, k0, k1; // blocks of the sum
+};
+// Item i of the walk: kGroupM tiles of A for each tile of B, so that the
+// clusters at work share rows of both through L2.
+__device__ __forceinline__ Item item_at(const TcArgs& a, int i) {
+  const int tiles = a.tiles_m * a.tiles_n;
+  Item it;
+  it.split = i / tiles;
+  int t = i - it.split * tiles;
+  const int per_group = kGroupM * a.tiles_n;
+  const int g = t / per_group;
+  t -= g * per_group;
+  const int rows = min(kGroupM, a.tiles_m - g * kGroupM);
+  it.n = t / rows;
+  it.m = g * kGroupM + (t - it.n * rows);
+  it.k0 = static_cast<int>(static_cast<int64_t>(a.blocks) * it.split / a.splits);
+  it.k1 = static_cast<int>(static_cast<int64_t>(a.blocks) * (it.split + 1) / a.splits);
+  return it;
+}
+
+// ------------------------------------------------------------------ stores
+template <typename T> __device__ __forceinline__ uint32_t pack2(float a, float b);
+template <> __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float a, float b) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+template <> __device__ __forceinline__ uint32_t pack2<__half>(float a, float b) {
+  const __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ void st_v8(void* p, const uint32_t* w) {
+  asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]),
+               "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
+               : "memory");
+}
+// 16 values of one row from column n on; columns past N are not written.
+template <typename T>
+__device__ __forceinline__ void store16(T* row, int64_t n, int64_t N, int vec, const float (&v)[16]) {
+  uint32_t w[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) w[i] = pack2<T>(v[2 * i], v[2 * i + 1]);
+  if (vec == 32 && n + 16 <= N) {
+    st_v8(row + n, w);
+  } else if (vec >= 16) {
+    if (n + 8 <= N) st_v4(row + n, make_uint4(w[0], w[1], w[2], w[3]));
+    if (n + 16 <= N) st_v4(row + n + 8, make_uint4(w[4], w[5], w[6], w[7]));
+    // rows are whole multiples of 8 elements here, so nothing is left over
+  } else {
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+      if (n + i < N) row[n + i] = Elem<T>::from_f(v[i]);
+  }
+}
+template <typename T>
+__device__ __forceinline__ void load16(const T* row, int64_t n, int64_t N, float (&v)[16]) {
+  // the slopes' rows are multiples of 8 elements, 16-byte aligned
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    float t[8] = {};
+    if (n + 8 * h + 8 <= N) unpack<T>(ld_nc_v4(row + n + 8 * h), t);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[8 * h + i] = t[i];
+  }
+}
+
+// act(a) and act'(a) with the fast exponential: its error, a few 2^-22
+// relative, is far below the half step 2^-9 / 2^-12 of the types they go to.
+__device__ __forceinline__ void fast_act(int act, float a, float& val, float& der) {
+  if (act == HC_ACT_SILU) {
+    const float s = __fdividef(1.f, 1.f + __expf(-a));
+    val = a * s;
+    der = fmaf(val, 1.f - s, s);
+  } else {
+    const float c = 0.7978845608028654f, a2 = a * a;
+    const float t = 1.f - __fdividef(2.f, 1.f + __expf(2.f * c * a * fmaf(0.044715f, a2, 1.f)));
+    val = 0.5f * a * (1.f + t);
+    der = fmaf(0.5f * a * (1.f - t * t), c * fmaf(3.f * 0.044715f, a2, 1.f), 0.5f * (1.f + t));
+  }
+}
+
+template <typename T, int EPI>
+__device__ __forceinline__ void finish(const TcArgs& a, const Item& it, uint32_t acc, int rank, int quad, int half) {
+  const int lane = threadIdx.x & 31;
+  const int64_t row = static_cast<int64_t>(it.m) * kTileM + rank * kRows + 32 * quad + lane;
+  const bool live = row < a.M;
+  const uint32_t lanes = acc + (static_cast<uint32_t>(32 * quad) << 16);
+  if constexpr (EPI == kGlu) {
+    const int64_t n0 = static_cast<int64_t>(it.n) * kRows + half * 64;
+    T* h = static_cast<T*>(a.out) + row * a.ldo;
+    T* sg = a.slope_gate ? static_cast<T*>(a.slope_gate) + row * a.ldo : nullptr;
+    T* su = a.slope_up ? static_cast<T*>(a.slope_up) + row * a.ldo : nullptr;
+#pragma unroll 1
+    for (int c = 0; c < 64; c += 16) {
+      uint32_t ra[16], rb[16];
+      acc_load16(lanes + half * 64 + c, ra);
+      acc_load16(lanes + kRows + half * 64 + c, rb);
+      acc_wait();
+      if (live && n0 + c < a.N) {
+        float vh[16], vg[16], vu[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          float der;
+          const float b = __uint_as_float(rb[i]);
+          fast_act(a.act, __uint_as_float(ra[i]), vu[i], der);
+          vh[i] = vu[i] * b;
+          vg[i] = der * b;
+        }
+        store16<T>(h, n0 + c, a.N, a.vec, vh);
+        if (sg) {
+          store16<T>(sg, n0 + c, a.N, a.vec, vg);
+          store16<T>(su, n0 + c, a.N, a.vec, vu);
+        }
+      }
+      __syncwarp();  // the next load is the whole warp's
+    }
+  } else {
+    const int64_t n0 = static_cast<int64_t>(it.n) * kTileN + half * 128;
+#pragma unroll 1
+    for (int c = 0; c < 128; c += 16) {
+      uint32_t r[16];
+      acc_load16(lanes + half * 128 + c, r);
+      acc_wait();
+      if (live && n0 + c < a.N) {
+        float v[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
+        if constexpr (EPI == kGluBwd) {
+          float g[16], u[16];
+          load16<T>(static_cast<const T*>(a.slope_gate) + row * a.ldo, n0 + c, a.N, g);
+          load16<T>(static_cast<const T*>(a.slope_up) + row * a.ldo, n0 + c, a.N, u);
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            g[i] *= v[i];
+            u[i] *= v[i];
+          }
+          store16<T>(static_cast<T*>(a.out) + row * a.ldo, n0 + c, a.N, a.vec, g);
+          store16<T>(static_cast<T*>(a.out2) + row * a.ldo, n0 + c, a.N, a.vec, u);
+        } else if (a.parts) {
+          float* p = a.parts + (static_cast<int64_t>(it.split) * a.M + row) * a.N + n0 + c;
+          if ((a.N & 7) == 0) {
+            if (n0 + c + 8 <= a.N) st_v8(p, r);
+            if (n0 + c + 16 <= a.N) st_v8(p + 8, r + 8);
+          } else {
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+              if (n0 + c + i < a.N) p[i] = v[i];
+          }
+        } else {
+          store16<T>(static_cast<T*>(a.out) + row * a.ldo, n0 + c, a.N, a.vec, v);
+        }
+      }
+      __syncwarp();
+    }
+  }
+}
+
+template <typename T, int EPI>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
+    ffn_tc_kernel(const __grid_constant__ TcMaps maps, const __grid_constant__ TcArgs a) {
+  extern __shared__ uint8_t raw[];
+  __shared__ Shared sh;
+  const uint32_t ring = (smem_u32(raw) + 1023) & ~1023u;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = cluster_rank();
+  const int items = a.tiles_m * a.tiles_n * a.splits;
+  const int first = blockIdx.x >> 1, step = gridDim.x >> 1;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kStages; ++s) {
+      mbar_init(&sh.full[s], 1);
+      mbar_init(&sh.empty[s], 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(&sh.acc_full[b], 1);
+      mbar_init(&sh.acc_empty[b], 16);  // the eight finishing warps of both CTAs
+    }
+    mbar_init(&sh.drain, 1);
+    sh.stop = 0;
+    fence_mbar_init();
+  }
+  if (warp == 2) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&sh.tmem))
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    tc_fence_before();
+  }
+  __syncthreads();
+  cluster_sync();
+  tc_fence_after();
+  const uint32_t tmem = sh.tmem;
+
+  if (warp == 0) {
+    if (lane == 0) {
+      int s = 0;
+      uint32_t ph = 0;
+      bool ok = true;
+      for (int i = first; i < items && ok; i += step) {
+        const Item it = item_at(a, i);
+        const int row_a = it.m * kTileM + static_cast<int>(rank) * kRows;
+        const int row_b = EPI == kGlu ? it.n * kRows : it.n * kTileN + static_cast<int>(rank) * kRows;
+        for (int kb = it.k0; kb < it.k1; ++kb) {
+          if (!pair_wait(sh, &sh.empty[s], ph ^ 1, a.wait_limit)) {
+            ok = false;
+            break;
+          }
+          const int term = kb >= a.blocks_term ? 1 : 0;
+          const int k = (kb - term * a.blocks_term) * kDepth;
+          const CUtensorMap* ma = &maps.a[term];
+          const CUtensorMap* mb = &maps.b[EPI == kGlu ? rank : term];
+          const uint32_t bar = cluster_addr(&sh.full[s], 0);
+          const uint32_t da = ring + s * kStageBytes, db = da + kOperandBytes;
+          if (rank == 0) mbar_expect_tx(&sh.full[s], 2 * kStageBytes);
+          if (a.a_mn) {
+            fetch_box(da, ma, row_a, k, bar);
+            fetch_box(da + kOperandBytes / 2, ma, row_a + 64, k, bar);
+          } else {
+            fetch_box(da, ma, k, row_a, bar);
+          }
+          if (a.b_mn) {
+            fetch_box(db, mb, row_b, k, bar);
+            fetch_box(db + kOperandBytes / 2, mb, row_b + 64, k, bar);
+          } else {
+            fetch_box(db, mb, k, row_b, bar);
+          }
+          if (++s == kStages) {
+            s = 0;
+            ph ^= 1;
+          }
+        }
+      }
+      // every stage's last release has arrived before the CTA leaves
+      for (int j = 0; j < kStages && ok; ++j) {
+        ok = pair_wait(sh, &sh.empty[s], ph ^ 1, a.wait_limit);
+        if (++s == kStages) {
+          s = 0;
+          ph ^= 1;
+        }
+      }
+      if (!ok) tell_stop(sh, a);
+    }
+  } else if (warp == 1) {
+    if (rank == 0 && lane == 0) {
+      // float32 sums of bf16 (format 1) or fp16 (0) operands, 256 x 256
+      constexpr uint32_t fmt = sizeof(T) == 2 && std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
+      const uint32_t idesc = (1u << 4) | (fmt << 7) | (fmt << 10) | (static_cast<uint32_t>(a.a_mn) << 15) |
+                             (static_cast<uint32_t>(a.b_mn) << 16) | ((kTileN >> 3) << 17) | ((kTileM >> 4) << 24);
+      const uint64_t step_a = (a.a_mn ? 16 * 128 : 32) >> 4, step_b = (a.b_mn ? 16 * 128 : 32) >> 4;
+      int s = 0, buf = 0;
+      uint32_t ph = 0, acc_ph = 0;
+      bool ok = true;
+      for (int i = first; i < items && ok; i += step) {
+        const Item it = item_at(a, i);
+        if (!pair_wait(sh, &sh.acc_empty[buf], acc_ph ^ 1, a.wait_limit)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        for (int kb = it.k0; kb < it.k1; ++kb) {
+          if (!pair_wait(sh, &sh.full[s], ph, a.wait_limit)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          uint64_t da = matrix_desc(ring + s * kStageBytes, a.a_mn);
+          uint64_t db = matrix_desc(ring + s * kStageBytes + kOperandBytes, a.b_mn);
+#pragma unroll
+          for (int k = 0; k < kDepth / 16; ++k) {
+            mma_pair(tmem + buf * kTileN, da, db, idesc, kb > it.k0 || k > 0);
+            da += step_a;
+            db += step_b;
+          }
+          commit_pair(&sh.empty[s]);
+          if (++s == kStages) {
+            s = 0;
+            ph ^= 1;
+          }
+        }
+        if (!ok) break;
+        commit_pair(&sh.acc_full[buf]);
+        buf ^= 1;
+        if (buf == 0) acc_ph ^= 1;
+      }
+      if (!ok) {  // stop, and let the products in flight end before the tensor memory goes
+        tell_stop(sh, a);
+        commit_pair(&sh.drain);
+        for (uint32_t i = 0; i < kWaitPolls && !mbar_try_wait(&sh.drain, 0); ++i) {
+        }
+      }
+    }
+  } else if (warp >= kFinishWarp) {
+    const int quad = warp & 3, half = (warp - kFinishWarp) >> 2;
+    int buf = 0;
+    uint32_t acc_ph = 0;
+    for (int i = first; i < items; i += step) {
+      const Item it = item_at(a, i);
+      const bool ok = pair_wait(sh, &sh.acc_full[buf], acc_ph, a.wait_limit);
+      if (!__all_sync(kFull, ok)) {
+        if (lane == 0) tell_stop(sh, a);
+        break;
+      }
+      tc_fence_after();
+      finish<T, EPI>(a, it, tmem + buf * kTileN, static_cast<int>(rank), quad, half);
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) arrive_cluster(cluster_addr(&sh.acc_empty[buf], 0));
+      buf ^= 1;
+      if (buf == 0) acc_ph ^= 1;
+    }
+  }
+  __syncwarp();
+  __syncthreads();
+  if (sh.stop && threadIdx.x == 0)  // copies in flight may be counted on the other CTA's barrier: give them 4 ms
+    for (int i = 0; i < 4096; ++i) __nanosleep(1000);
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync();
+  tc_fence_after();
+  if (warp == 2)
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+  __syncthreads();
+  cluster_sync();
+}
+
+// ----------------------------------------------------- parts of a split sum
+template <typename T>
+__global__ void __launch_bounds__(256) ffn_add_parts(const float* parts, T* out, int64_t count, int splits) {
+  for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < count;
+       i += static_cast<int64_t>(gridDim.x) * 256) {
+    float s = 0.f;
+    for (int p = 0; p < splits; ++p) s += parts[p * count + i];
+    out[i] = Elem<T>::from_f(s);
+  }
+}
+
+// ------------------------------------------------------------------- host
+int pairs_resident() {
+  static int cached[64] = {0};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return sm_count() / 2;
+  if (cached[dev] > 0) return cached[dev];
+  int n = 0;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(2 * (sm_count() / 2));
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = kSmemBytes;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = 2;
+  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  auto* k = ffn_tc_kernel<__nv_bfloat16, kStore>;
+  if (cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes) != cudaSuccess ||
+      cudaOccupancyMaxActiveClusters(&n, k, &cfg) != cudaSuccess || n <= 0) {
+    cudaGetLastError();
+    n = sm_count() / 2;
+  }
+  cached[dev] = n;
+  return n;
+}
+
+int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+// The matrix of an operand as a tensor map: 128-byte lines along its unit stride.
+bool encode_operand(CUtensorMap* map, const FfnOperand& o, int64_t K) {
+  const auto encode = tensor_map_encoder();
+  if (!encode) return false;
+  const bool mn = o.k_stride != 1;
+  const int64_t inner = mn ? o.rows : K, outer = mn ? K : o.rows, ld = mn ? o.k_stride : o.row_stride;
+  const cuuint64_t dims[2] = {static_cast<cuuint64_t>(inner), static_cast<cuuint64_t>(outer)};
+  const cuuint64_t strides[1] = {static_cast<cuuint64_t>(ld) * 2};
+  const cuuint32_t box[2] = {64, static_cast<cuuint32_t>(mn ? kDepth : kRows)};
+  const cuuint32_t ones[2] = {1, 1};
+  return encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT16, 2, const_cast<void*>(o.p), dims, strides, box, ones,
+                CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+using Kernel = void (*)(TcMaps, TcArgs);
+template <typename T> Kernel kernel_of(int epi) {
+  return epi == kStore ? ffn_tc_kernel<T, kStore> : epi == kGlu ? ffn_tc_kernel<T, kGlu> : ffn_tc_kernel<T, kGluBwd>;
+}
+
+}  // namespace
+
+// Clusters that share the sum of one tile: as many as there are for every
+// tile, each with at least 4 blocks (256 deep) of its own.
+int ffn_tc_splits(int64_t M, int64_t N, int64_t K, int terms) {
+  const int64_t tiles = ceil_div(M, kTileM) * ceil_div(N, kTileN), blocks = ceil_div(K, kDepth) * terms;
+  const int64_t by_pairs = pairs_resident() / tiles, by_depth = blocks / 4;
+  const int64_t s = by_pairs < by_depth ? by_pairs : by_depth;
+  return static_cast<int>(s < 1 ? 1 : s > 32 ? 32 : s);
+}
+
+int ffn_tc_launch(const FfnProduct& p, int dtype, float* parts, cudaStream_t s) {
+  const bool bf = dtype == HC_DTYPE_BF16;
+  const Kernel kernel = bf ? kernel_of<__nv_bfloat16>(p.epilogue) : kernel_of<__half>(p.epilogue);
+  // A call of the runtime before the first one of the driver's encoder: on a
+  // thread that has made none (autograd's), the encoder finds no context.
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes) != cudaSuccess) {
+    cudaGetLastError();
+    return HC_ERR_LAUNCH;
+  }
+  TcMaps maps{};
+  TcArgs a{};
+  const int nb = p.epilogue == kGlu ? 2 : p.terms;
+  for (int t = 0; t < 2; ++t)
+    if (!encode_operand(&maps.a[t], p.A[t < p.terms ? t : 0], p.K) ||
+        !encode_operand(&maps.b[t], p.B[t < nb ? t : 0], p.K))
+      return HC_ERR_LAUNCH;
+  a.M = p.M; a.N = p.N; a.ldo = p.ldo;
+  a.out = p.out; a.out2 = p.out2; a.slope_gate = p.slope_gate; a.slope_up = p.slope_up;
+  a.tiles_m = static_cast<int>(ceil_div(p.M, kTileM));
+  a.tiles_n = static_cast<int>(ceil_div(p.N, p.epilogue == kGlu ? kRows : kTileN));
+  a.splits = p.epilogue == kStore ? ffn_tc_splits(p.M, p.N, p.K, p.terms) : 1;
+  a.parts = a.splits > 1 ? parts : nullptr;
+  if (a.splits > 1 && !parts) return HC_ERR_SCRATCH;
+  a.blocks_term = static_cast<int>(ceil_div(p.K, kDepth));
+  a.blocks = a.blocks_term * p.terms;
+  a.a_mn = p.A[0].k_stride != 1;
+  a.b_mn = p.B[0].k_stride != 1;
+  a.act = p.act;
+  const uintptr_t base = reinterpret_cast<uintptr_t>(p.out) | reinterpret_cast<uintptr_t>(p.out2) |
+                         reinterpret_cast<uintptr_t>(p.epilogue == kGlu ? p.slope_gate : nullptr) |
+                         reinterpret_cast<uintptr_t>(p.epilogue == kGlu ? p.slope_up : nullptr) |
+                         static_cast<uintptr_t>(2 * p.ldo);
+  a.vec = base % 32 == 0 ? 32 : base % 16 == 0 ? 16 : 2;
+  a.wait_limit = wait_poll_limit();
+  a.status = timeout_word(s);
+  const int64_t items = static_cast<int64_t>(a.tiles_m) * a.tiles_n * a.splits;
+  if (items > (int64_t(1) << 30)) return HC_ERR_BAD_SIZE;
+  const int pairs = static_cast<int>(items < pairs_resident() ? items : pairs_resident());
+  kernel<<<2 * pairs, kThreads, kSmemBytes, s>>>(maps, a);
+  if (int rc = launch_status()) return rc;
+  if (a.splits == 1) return HC_OK;
+  const int64_t count = p.M * p.N;
+  const int64_t want = ceil_div(count, 256), most = 8 * sm_count();
+  const int grid = static_cast<int>(want < most ? want : most);
+  if (bf)
+    ffn_add_parts<<<grid, 256, 0, s>>>(parts, static_cast<__nv_bfloat16*>(p.out), count, a.splits);
+  else
+    ffn_add_parts<<<grid, 256, 0, s>>>(parts, static_cast<__half*>(p.out), count, a.splits);
+  return launch_status();
+}
+
+unsigned int ffn_take_timeouts(bool reset) {
+  unsigned int v = 0;
+  if (cudaMemcpyFromSymbol(&v, g_ffn_wait_timeouts, sizeof(v)) != cudaSuccess) {
+    cudaGetLastError();
+    return 0;
+  }
+  if (reset && v != 0) {
+    const unsigned int z = 0;
+    cudaMemcpyToSymbol(g_ffn_wait_timeouts, &z, sizeof(z));
+  }
+  return v;
+}
+
+}  // namespace hc

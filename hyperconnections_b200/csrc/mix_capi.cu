@@ -230,7 +230,7 @@ extern "C" int hc_wait_timeouts(unsigned int* count, int reset) {
   *count = mix_warp_take_timeouts_f32(r) + mix_warp_take_timeouts_f16(r) + mix_warp_take_timeouts_bf16(r) +
            rw_fwd_take_timeouts_f32(r) + rw_fwd_take_timeouts_f16(r) + rw_fwd_take_timeouts_bf16(r) +
            rw_bwd_take_timeouts_f32(r) + rw_bwd_take_timeouts_f16(r) + rw_bwd_take_timeouts_bf16(r) +
-           expm_take_timeouts(r);
+           expm_take_timeouts(r) + ffn_take_timeouts(r);
   if (r) clear_timeout_word();
   return HC_OK;
 }

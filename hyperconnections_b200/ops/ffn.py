@@ -6,14 +6,14 @@
 x [*, D], w_gate and w_up [F, D], w_down [O, F] (the layouts of
 ``nn.Linear.weight``) -> y [*, O]; activation "silu" or "gelu_tanh" (the
 tanh form of GELU). Both projections, the activation and the product are one
-kernel, which writes h = act(a) * b and, when a backward follows, a and b; the
-backward applies the activation's derivative where it makes dh = g w_down, and
-sums dx = da w_gate + db w_up in one product.
+kernel, which writes h = act(a) * b and, when a backward follows, what dh is
+multiplied with there: act'(a) b and act(a). The backward does that where it
+makes dh = g w_down, and sums dx = da w_gate + db w_up in one product.
 
 Weights are cast to x's dtype (float32, float16 or bfloat16; under autocast
 all four tensors to the autocast dtype, as ``F.linear`` does). Products are
-summed in float32; h, a, b and their gradients are rounded to that dtype, since
-they are the operands of the products that follow.
+summed in float32; h, the two slopes and the gradients da and db are rounded
+once to that dtype (h, da and db are operands of the products that follow).
 """
 
 from __future__ import annotations
@@ -33,41 +33,47 @@ def _scratch(backward: int, T, D, F, O, code, device):
     return (torch.empty(size, dtype=torch.uint8, device=device) if size > 0 else None), max(size, 0)
 
 
+def _dense(t):
+    """t itself, or a copy where it is strided or starts off a 16-byte boundary (the tensor copies need one)."""
+    t = t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
 def _forward(x, w_gate, w_up, w_down, act, keep):
     D, (O, F) = x.shape[-1], w_down.shape
     lead = x.shape[:-1]
     T = math.prod(lead)
-    dense = [t.contiguous() for t in (x, w_gate, w_up, w_down)]
+    dense = [_dense(t) for t in (x, w_gate, w_up, w_down)]
     x_c = dense[0]
     dev, dt, code = x.device, x.dtype, _lib.dtype_code(x.dtype)
     Fp = (F + 7) // 8 * 8
     y = torch.empty(*lead, O, dtype=dt, device=dev)
     h = torch.empty(T, Fp, dtype=dt, device=dev)
-    pre = [torch.empty(T, Fp, dtype=dt, device=dev) if keep else None for _ in range(2)]
+    slopes = [torch.empty(T, Fp, dtype=dt, device=dev) if keep else None for _ in range(2)]
     with _lib.on_device(x_c):
         scratch, size = _scratch(0, T, D, F, O, code, dev)
         rc = _lib.lib().hc_gated_ffn_fwd(*[t.data_ptr() for t in dense], y.data_ptr(), h.data_ptr(),
-                                         *[_lib.ptr(t) for t in pre], _lib.ptr(scratch), size, T, D, F, O, act, code,
+                                         *[_lib.ptr(t) for t in slopes], _lib.ptr(scratch), size, T, D, F, O, act, code,
                                          _lib.stream_of(x_c))
     _lib.check(rc, "hc_gated_ffn_fwd")
-    return y, dense, h, pre
+    return y, dense, h, slopes
 
 
 class _GatedFfnFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w_gate, w_up, w_down, act):
-        y, dense, h, pre = _forward(x, w_gate, w_up, w_down, act, True)
-        ctx.save_for_backward(*dense, h, *pre)
+        y, dense, h, slopes = _forward(x, w_gate, w_up, w_down, act, True)
+        ctx.save_for_backward(*dense, h, *slopes)
         ctx.act = act
         return y
 
     @staticmethod
     @once_differentiable
     def backward(ctx, g):
-        x, w_gate, w_up, w_down, h, pre_gate, pre_up = ctx.saved_tensors
+        x, w_gate, w_up, w_down, h, slope_gate, slope_up = ctx.saved_tensors
         (O, F), D, T = w_down.shape, x.shape[-1], h.shape[0]
         code = _lib.dtype_code(x.dtype)
-        g_c = g.to(x.dtype).contiguous()
+        g_c = _dense(g.to(x.dtype))
         grads = [torch.empty_like(t) if need else None
                  for t, need in zip((x, w_gate, w_up, w_down), ctx.needs_input_grad)]
         inner = any(t is not None for t in grads[:3])
@@ -75,7 +81,7 @@ class _GatedFfnFn(torch.autograd.Function):
         with _lib.on_device(x):
             scratch, size = _scratch(1, T, D, F, O, code, x.device)
             rc = _lib.lib().hc_gated_ffn_bwd(
-                *[t.data_ptr() for t in (g_c, x, w_gate, w_up, w_down, h, pre_gate, pre_up)],
+                *[t.data_ptr() for t in (g_c, x, w_gate, w_up, w_down, h, slope_gate, slope_up)],
                 *[_lib.ptr(t) for t in (*d_pre, *grads, scratch)], size, T, D, F, O, ctx.act, code, _lib.stream_of(x))
         _lib.check(rc, "hc_gated_ffn_bwd")
         return (*grads, None)

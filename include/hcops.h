@@ -438,26 +438,28 @@ int hc_dropout(const void* x, void* y, int64_t N, double p,
 
 /* Gated feed-forward: a = x w_gate^T, b = x w_up^T, h = act(a) * b (one
  * kernel), y = h w_down^T. x [T,D], w_gate and w_up [F,D], w_down [O,F],
- * y [T,O]; every tensor has `dtype`, products are summed in float32, and h (and
- * a, b for the backward) are rounded once to dtype. act HC_ACT_SILU or
- * HC_ACT_GELU_TANH. h, pre_gate (a) and pre_up (b) are [T,Fp] with
- * Fp = F rounded up to a multiple of 8 (their last columns are written 0);
- * pre_gate and pre_up NULL when no backward follows. scratch:
+ * y [T,O]; every tensor has `dtype`, products are summed in float32. act
+ * HC_ACT_SILU or HC_ACT_GELU_TANH. For the backward the forward keeps not a
+ * and b but what dh is multiplied with: slope_gate = act'(a) b, slope_up =
+ * act(a), computed in float32 and rounded once, like h. These three are
+ * [T,Fp] with Fp = F rounded up to a multiple of 8 (their last columns are
+ * written 0); the slopes are NULL when no backward follows. Half-precision
+ * tensors start on 16-byte boundaries. scratch:
  * hc_gated_ffn_scratch_bytes(0, ...) bytes, 256-byte aligned. */
 int hc_gated_ffn_fwd(const void* x, const void* w_gate, const void* w_up,
-                     const void* w_down, void* y, void* h, void* pre_gate,
-                     void* pre_up, void* scratch, int64_t scratch_bytes,
+                     const void* w_down, void* y, void* h, void* slope_gate,
+                     void* slope_up, void* scratch, int64_t scratch_bytes,
                      int64_t T, int64_t D, int64_t F, int64_t O, int act,
                      int dtype, void* stream);
 
 /* Given g = dL/dy [T,O]: grad_x [T,D], grad_w_gate and grad_w_up [F,D],
- * grad_w_down [O,F], each nullable, from the forward's h, pre_gate and
- * pre_up. d_gate and d_up: workspaces [T,Fp] (the gradients of a and b; not
+ * grad_w_down [O,F], each nullable, from the forward's h and
+ * slopes. d_gate and d_up: workspaces [T,Fp] (the gradients of a and b; not
  * needed when grad_w_down alone is wanted). scratch:
  * hc_gated_ffn_scratch_bytes(1, ...) bytes, 256-byte aligned. */
 int hc_gated_ffn_bwd(const void* g, const void* x, const void* w_gate,
                      const void* w_up, const void* w_down, const void* h,
-                     const void* pre_gate, const void* pre_up, void* d_gate,
+                     const void* slope_gate, const void* slope_up, void* d_gate,
                      void* d_up, void* grad_x, void* grad_w_gate,
                      void* grad_w_up, void* grad_w_down, void* scratch,
                      int64_t scratch_bytes, int64_t T, int64_t D, int64_t F,
