@@ -83,7 +83,7 @@ struct NormArgs {
   float* stats;                        // [T, 2]: mean, 1 / root
   void *grad_x, *grad_f, *grad_gate;
   float *grad_R, *grad_H, *grad_W, *grad_v;
-  float* partial;  // [grid][2][m D]: the CTAs' sums over their tokens, or nullptr
+  float* partial;  // [rows][2][m D]: the groups' sums over their tokens, or nullptr
   int64_t T, D;
   int n, m, norm, gate_act;
   float eps;
@@ -92,12 +92,15 @@ struct NormArgs {
 
 // Which kernels a call takes, and over how many CTAs.
 struct NormGeometry {
-  int grid;   // CTAs; also the rows of `partial`
   int warps;  // warps of one token's group (the 8-column kernels); 0 = element by element
+  int grid;   // CTAs
+  int rows;   // rows of `partial` that are written
 };
 
-#define HC_BLOCK_DECL(SFX)                                                                            \
-  int norm_launch_##SFX(bool write, bool bwd, const NormGeometry& g, const NormArgs& a, cudaStream_t s); \
+// Launchers of one stream dtype; the 8-column ones set grid and rows.
+#define HC_BLOCK_DECL(SFX)                                                                     \
+  int read_norm_launch_##SFX(bool bwd, NormGeometry& g, const NormArgs& a, cudaStream_t s);     \
+  int write_norm_launch_##SFX(bool bwd, NormGeometry& g, const NormArgs& a, cudaStream_t s);    \
   int dropout_launch_##SFX(const void* x, void* y, int64_t N, const DropArgs& d, cudaStream_t s);
 HC_BLOCK_DECL(f32)
 HC_BLOCK_DECL(f16)

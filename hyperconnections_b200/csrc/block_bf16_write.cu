@@ -1,0 +1,10 @@
+// bf16 streams: the post-norm + mix-write kernels.
+#include "block_norm.cuh"
+
+namespace hc {
+
+int write_norm_launch_bf16(bool bwd, NormGeometry& g, const NormArgs& a, cudaStream_t s) {
+  return norm_launch<__nv_bfloat16, true>(bwd, g, a, s);
+}
+
+}  // namespace hc

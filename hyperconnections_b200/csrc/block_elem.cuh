@@ -382,7 +382,9 @@ __global__ void __launch_bounds__(kElemThreads) write_norm_bwd_elem(NormArgs a) 
 }
 
 template <typename T>
-int norm_launch_elem(bool write, bool bwd, const NormGeometry& geo, const NormArgs& a, cudaStream_t s) {
+int norm_launch_elem(bool write, bool bwd, NormGeometry& geo, const NormArgs& a, cudaStream_t s) {
+  const int64_t most = 4 * static_cast<int64_t>(sm_count());
+  geo.grid = geo.rows = static_cast<int>(a.T < most ? a.T : most);
   if (write)
     (bwd ? write_norm_bwd_elem<T> : write_norm_fwd_elem<T>)<<<geo.grid, kElemThreads, 0, s>>>(a);
   else
