@@ -127,9 +127,12 @@ torch::Tensor matrix_exp(const torch::Tensor& A) { return MatrixExp::apply(A); }
 
 }  // namespace
 
+void bind_block_ops(pybind11::module_& m);  // torch_block.cpp
+
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
-  m.doc() = "autograd Functions of the batched matrix exponentials over libhcops.so";
+  m.doc() = "autograd Functions of the batched matrix exponentials and of the operators around a block over libhcops.so";
   m.def("expm_t18", &expm_t18, "T18 matrix exponential (global or per-matrix scaling), differentiable");
   m.def("matrix_exp", &matrix_exp, "Pade [7/7] matrix exponential, differentiable");
+  bind_block_ops(m);
   m.def("abi_version", &hc_abi_version, "ABI version of the linked libhcops.so");
 }

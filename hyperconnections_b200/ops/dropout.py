@@ -18,7 +18,6 @@ step also moves that tensor on.
 from __future__ import annotations
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from .. import _lib
 
@@ -40,45 +39,16 @@ def drop_state(name: str, seed, offset, x: torch.Tensor):
 
 def drop_words(seed: int, offset: int):
     """Both modulo 2^64, as the signed words of the C call."""
-    return tuple((int(k) + (1 << 63)) % (1 << 64) - (1 << 63) for k in (seed, offset))
-
-
-def _run(x_c, p, state, words):
-    y = torch.empty_like(x_c)
-    with _lib.on_device(x_c):
-        rc = _lib.lib().hc_dropout(x_c.data_ptr(), y.data_ptr(), x_c.numel(), p, _lib.ptr(state), *words,
-                                   _lib.dtype_code(x_c.dtype), _lib.stream_of(x_c))
-    _lib.check(rc, "hc_dropout")
-    return y
-
-
-class _DropoutFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, state, p, words):
-        ctx.save_for_backward(state)
-        ctx.p, ctx.words, ctx.dtype = p, words, x.dtype
-        return _run(x.contiguous(), p, state, words)
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, g):
-        (state,) = ctx.saved_tensors
-        return _run(g.to(ctx.dtype).contiguous(), ctx.p, state, ctx.words), None, None, None
+    return tuple((k + (1 << 63)) % (1 << 64) - (1 << 63) for k in (seed, offset))
 
 
 def hc_dropout(x: torch.Tensor, p: float, seed, offset: int = 0) -> torch.Tensor:
     """x with each element kept (times 1 / (1 - p)) or zeroed (see module doc)."""
-    if not _lib.available():
-        raise RuntimeError("hc_dropout requires the hyperconnections_b200 CUDA kernels (libhcops.so)")
     if not x.is_cuda or (torch.is_tensor(seed) and not seed.is_cuda):
         raise RuntimeError("hc_dropout requires CUDA tensors")
-    p = float(p)
-    if not 0.0 <= p <= 1.0:
-        raise ValueError(f"p must lie in [0, 1], got {p}")
-    _lib.dtype_code(x.dtype)
     state, seed, offset = drop_state("hc_dropout", seed, offset, x)
-    words = drop_words(seed, offset)
-    if torch.is_grad_enabled() and x.requires_grad:
-        # the caller may move its seed on before the backward draws the bits again
-        return _DropoutFn.apply(x, None if state is None else state.clone(), p, words)
-    return _run(x.contiguous(), p, state, words)
+    out = _lib.torch_ext().dropout(x, state, p, *drop_words(seed, offset))
+    if out is None:
+        _lib.dtype_code(x.dtype)
+        raise ValueError(f"p must lie in [0, 1], got {p}")
+    return out
