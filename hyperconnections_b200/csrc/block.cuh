@@ -23,6 +23,7 @@ struct DropArgs {
   uint64_t threshold;  // floor(p 2^32): an element is kept when its word is at least this
   float scale;         // 1 / (1 - p); 0 at p = 1
   int on;              // p > 0
+  uint32_t bar, kept;  // min(threshold, 2^32 - 1), and the mask of a word that reaches it (0 at p = 1)
 };
 
 struct DropKey {
@@ -92,9 +93,10 @@ struct NormArgs {
 
 // Which kernels a call takes, and over how many CTAs.
 struct NormGeometry {
-  int warps;  // warps of one token's group (the 8-column kernels); 0 = element by element
-  int grid;   // CTAs
-  int rows;   // rows of `partial` that are written
+  int warps;   // warps of one token's group (the 8-column kernels); 0 = element by element
+  int chunks;  // 8-column chunks a thread owns (forward)
+  int grid;    // CTAs
+  int rows;    // rows of `partial` that are written
 };
 
 // Launchers of one stream dtype; the 8-column ones set grid and rows.

@@ -34,6 +34,9 @@ bool drop_args(DropArgs& d, double p, const int64_t* state, int64_t seed, int64_
   d.threshold = static_cast<uint64_t>(floor(p * 4294967296.0));
   d.scale = p < 1.0 ? static_cast<float>(1.0 / (1.0 - p)) : 0.f;
   d.on = p > 0.0;
+  // the same test on 32 bits: at p = 1 no bar keeps every word out, so what is kept is masked instead
+  d.bar = d.threshold > 0xffffffffu ? 0xffffffffu : static_cast<uint32_t>(d.threshold);
+  d.kept = d.threshold > 0xffffffffu ? 0u : 0xffffffffu;
   return true;
 }
 
@@ -41,13 +44,11 @@ bool drop_args(DropArgs& d, double p, const int64_t* state, int64_t seed, int64_
 // CTA, with every stream and parameter on a 16-byte boundary; the others go
 // element by element. (16,384 tokens of n = 4, D = 768, bf16, forward and
 // backward: NN against 3,222 us for the mix-write, MM against 668 us for the read.)
-NormGeometry geometry(bool bwd, int n, int64_t D, int esize, std::initializer_list<const void*> ps) {
-  NormGeometry g{};
-  const int64_t warps = (D + 32 * kColumns - 1) / (32 * kColumns);
-  bool fits = D % kColumns == 0 && 32 * warps <= norm_max_threads(bwd, n <= 1 ? 1 : n <= 2 ? 2 : n <= 4 ? 4 : 8, esize);
-  for (const void* p : ps) fits = fits && aligned16(p);
-  g.warps = fits ? static_cast<int>(warps) : 0;
-  return g;
+NormGeometry geometry(bool write, bool bwd, int n, int m, int64_t D, int esize,
+                      std::initializer_list<const void*> ps) {
+  for (const void* p : ps)
+    if (!aligned16(p)) return NormGeometry{};
+  return norm_geometry(write, bwd, n, m, D, esize);
 }
 
 int launch(int sdt, bool write, bool bwd, NormGeometry& g, const NormArgs& a, cudaStream_t s) {
@@ -126,7 +127,8 @@ extern "C" int hc_read_norm_fwd(const float* R, const void* x, const float* weig
   NormArgs a{};
   a.R = R; a.x = x; a.weight = weight; a.bias = bias; a.out = y; a.stats = stats;
   a.T = T; a.D = D; a.n = n; a.m = m; a.norm = norm; a.eps = eps;
-  NormGeometry geo = geometry(false, n, D, dtype_size(stream_dtype), {x, y, weight, bias});
+  NormGeometry geo = geometry(false, false, n, m, D, dtype_size(stream_dtype),
+                              {x, y, weight, bias, stats});
   return launch(stream_dtype, false, false, geo, a, static_cast<cudaStream_t>(stream));
 }
 
@@ -154,7 +156,8 @@ extern "C" int hc_read_norm_bwd(const void* g, const float* R, const void* x, co
   a.g = g; a.R = R; a.x = x; a.weight = weight; a.stats = const_cast<float*>(stats);
   a.grad_x = grad_x; a.grad_R = grad_R; a.partial = params ? scratch : nullptr;
   a.T = T; a.D = D; a.n = n; a.m = m; a.norm = norm;
-  NormGeometry geo = geometry(true, n, D, dtype_size(stream_dtype), {g, x, grad_x, weight});
+  NormGeometry geo = geometry(false, true, n, m, D, dtype_size(stream_dtype),
+                              {g, x, grad_x, weight, scratch});
   if (int rc = launch(stream_dtype, false, true, geo, a, s)) return rc;
   return params ? norm_param_grads(scratch, geo.rows, E, weight, nullptr, nullptr, grad_weight, grad_bias, nullptr, s)
                 : HC_OK;
@@ -184,8 +187,8 @@ extern "C" int hc_mix_write_norm_fwd(const float* H, const void* x, const float*
   a.H = H; a.x = x; a.W = W; a.f = f; a.v = v; a.weight = weight; a.bias = bias; a.gate = gate; a.scale = scale;
   a.out = out; a.stats = stats; a.T = T; a.D = D; a.n = n; a.m = m; a.norm = norm; a.gate_act = gate_act; a.eps = eps;
   drop_args(a.drop, p, state, seed, offset);
-  NormGeometry geo =
-      geometry(false, n, D, dtype_size(stream_dtype), {x, f, gate, out, weight, bias, scale});
+  NormGeometry geo = geometry(true, false, n, m, D, dtype_size(stream_dtype),
+                              {x, f, gate, out, weight, bias, scale, stats});
   return launch(stream_dtype, true, false, geo, a, static_cast<cudaStream_t>(stream));
 }
 
@@ -221,8 +224,8 @@ extern "C" int hc_mix_write_norm_bwd(const void* g, const float* H, const void* 
   a.partial = params ? scratch : nullptr;
   a.T = T; a.D = D; a.n = n; a.m = m; a.norm = norm; a.gate_act = gate_act;
   drop_args(a.drop, p, state, seed, offset);
-  NormGeometry geo = geometry(true, n, D, dtype_size(stream_dtype),
-                              {g, x, f, gate, grad_x, grad_f, grad_gate, weight, bias, scale});
+  NormGeometry geo = geometry(true, true, n, m, D, dtype_size(stream_dtype),
+                              {g, x, f, gate, grad_x, grad_f, grad_gate, weight, bias, scale, scratch});
   if (int rc = launch(stream_dtype, true, true, geo, a, s)) return rc;
   return params ? norm_param_grads(scratch, geo.rows, E, weight, bias, scale, grad_weight, grad_bias, grad_scale, s)
                 : HC_OK;

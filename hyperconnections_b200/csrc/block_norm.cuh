@@ -1,25 +1,38 @@
 // block_norm.cuh — the norm kernels for rows of whole 8-column chunks (D a
-// multiple of 8, 16-byte aligned streams).
+// multiple of 8, streams and parameters on 16-byte boundaries).
 //
 // A token belongs to a group of W = ceil(D / 256) warps: a CTA for W > 1, one
-// of a CTA's four warps for W = 1. A thread owns eight columns of every row, so
-// that a token is read once, kept in registers (16-bit rows stay packed) over
-// the norm's sums, and written once. The groups walk the tokens grid-strided;
-// several CTAs an SM keep enough loads in flight.
+// of a CTA's four warps for W = 1. A thread owns eight columns of every row,
+// reads them once and writes its outputs once. The groups walk the tokens
+// grid-strided.
 //
-// Sums over a token: a warp folds its values by halving exchanges (every
-// exchange sends half of the live values, so k values cost about k + 5 - log k
-// shuffles), writes them to shared memory, and after the group's barrier every
-// thread adds the W warps' in order. The backward has two rounds: the norm's
-// two sums, which the gradients wait for, and the token's small matrices (R, or
-// H and W), which nothing waits for: those are added one token later, behind
-// the next token's barrier, so a token costs one barrier. Shared memory is
-// double-buffered by token for that.
-//
+// What bounds these kernels is HBM, as long as enough loads are in flight and
+// the instructions keep up; both shaped the layout:
+//   * a thread copies its own 16 bytes of every row of the next token to shared
+//     memory (cp.async) while it works on this one. It reads nothing that
+//     another thread copied, so the rows need no barrier, and they cost no
+//     registers while they travel;
+//   * the token's small matrices (R, or H, W and v) and its norm's statistics
+//     are copied one token earlier still, so that the barrier between them and
+//     their use is one that the group passes anyway;
+//   * arithmetic is on pairs of float32 (fma.rn.f32x2); the small matrices'
+//     entries lie in shared memory twice, as the pairs that it multiplies with;
+//   * kernels exist for 1, 2, 4, 8 streams and 1, 2, 4 blocks. Rows and entries
+//     past n and m are zeros in shared memory, never fetched and never stored,
+//     so that no product asks for n or m;
+//   * a warp folds k sums by halving exchanges (every exchange sends half of
+//     the live values: about k + 5 - log k shuffles), writes them to shared
+//     memory, and behind the group's barrier every thread adds the W warps' in
+//     order. The backward's sums come in two rounds, the norm's two, which the
+//     gradients wait for, and the token's small matrices', which nothing waits
+//     for: those are added behind the next token's barrier. A token costs one
+//     barrier.
 // The [m D] parameters' gradients are sums over tokens: a thread keeps its
 // columns' sums in registers over all of its group's tokens and writes them
 // once; block_capi.cu adds the groups' sums in order.
 #pragma once
+
+#include <type_traits>
 
 #include "block_elem.cuh"
 
@@ -27,40 +40,110 @@ namespace hc {
 
 constexpr int kColumns = 8;      // a thread's columns
 constexpr int kSmallGroups = 4;  // groups of a CTA when a group is one warp
+constexpr int kSmallSlots = 8;   // tokens whose small matrices are held (5 are live; a power of two)
+constexpr int kNormSmemMax = 210 * 1024;  // of the 227 KB a CTA can have; up to 10 KB are static
 
-// Threads of a CTA at most, which bounds the registers of one: the backward of
-// 8 streams holds 16 rows, the float32 kernels twice the words a row.
-constexpr int norm_max_threads(bool bwd, int N, int esize) {
-  return N == 8 ? (bwd || esize == 4 ? 256 : 512) : (bwd && N == 4 && esize == 4) ? 256 : 512;
+// Threads of a CTA at most, which bounds the registers of one.
+constexpr int norm_bwd_threads(int N, int M, int esize) { return M >= 2 || N == 8 || (N == 4 && esize == 4) ? 256 : 512; }
+// Chunks a thread may own in the forward (a token's rows then need fewer warps,
+// down to one without barriers): as many as keep a block's rows in registers.
+constexpr int norm_fwd_chunks(int N, int M, int esize) { return M == 1 && N <= 4 && esize == 2 ? 3 : 1; }
+constexpr int norm_fwd_threads(int N, int M, int CH, int esize) { return CH > 1 || (N == 8 && M > 1) ? 384 : 512; }
+
+// ------------------------------------------------------- pairs of float32
+using f2 = unsigned long long;
+__device__ __forceinline__ f2 pair(float a, float b) {
+  f2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ f2 both(float a) { return pair(a, a); }
+__device__ __forceinline__ void split(f2 v, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+__device__ __forceinline__ float fold2(f2 v) {
+  float a, b;
+  split(v, a, b);
+  return a + b;
+}
+__device__ __forceinline__ f2 fma2(f2 a, f2 b, f2 c) {
+  f2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ f2 mul2(f2 a, f2 b) {
+  f2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ f2 add2(f2 a, f2 b) {
+  f2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
 }
 
-template <typename T> struct Raw8 {
-  static constexpr int Q = sizeof(T) / 2;  // 16-byte words
-  uint4 q[Q];
-  __device__ __forceinline__ void load(const T* p, bool ok) {
+struct V8 {  // eight columns
+  f2 v[4];
+  __device__ __forceinline__ void fill(float a) {
 #pragma unroll
-    for (int i = 0; i < Q; ++i) q[i] = ok ? ld_nc_v4(p + i * (16 / sizeof(T))) : make_uint4(0u, 0u, 0u, 0u);
-  }
-  __device__ __forceinline__ void get(float (&f)[8]) const {
-#pragma unroll
-    for (int i = 0; i < Q; ++i) unpack<T>(q[i], f + i * (16 / sizeof(T)));
+    for (int i = 0; i < 4; ++i) v[i] = both(a);
   }
 };
-template <typename T> __device__ __forceinline__ void put8(T* p, const float (&f)[8]) {
+__device__ __forceinline__ float dot(const V8& a, const V8& b) {
+  f2 s = mul2(a.v[0], b.v[0]);
 #pragma unroll
-  for (int i = 0; i < Raw8<T>::Q; ++i) st_v4(p + i * (16 / sizeof(T)), pack<T>(f + i * (16 / sizeof(T))));
+  for (int i = 1; i < 4; ++i) s = fma2(a.v[i], b.v[i], s);
+  return fold2(s);
 }
-// Eight values of a 16-byte aligned float32 parameter, or `none`.
-__device__ __forceinline__ void param8(const float* p, int64_t c, bool ok, float none, float (&f)[8]) {
-  float4 q[2] = {make_float4(none, none, none, none), make_float4(none, none, none, none)};
-  if (p && ok) {
-    q[0] = __ldg(reinterpret_cast<const float4*>(p + c));
-    q[1] = __ldg(reinterpret_cast<const float4*>(p + c) + 1);
-  }
-  f[0] = q[0].x; f[1] = q[0].y; f[2] = q[0].z; f[3] = q[0].w;
-  f[4] = q[1].x; f[5] = q[1].y; f[6] = q[1].z; f[7] = q[1].w;
+__device__ __forceinline__ void axpy(f2 aa, const V8& x, V8& y) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) y.v[i] = fma2(aa, x.v[i], y.v[i]);
 }
 
+template <typename T> constexpr int kWords = sizeof(T) / 2;  // 16-byte words of eight columns
+
+template <typename T> __device__ __forceinline__ V8 expand(const uint4 (&q)[kWords<T>]) {
+  float f[8];
+#pragma unroll
+  for (int i = 0; i < kWords<T>; ++i) unpack<T>(q[i], f + i * (16 / sizeof(T)));
+  V8 r;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) r.v[i] = pair(f[2 * i], f[2 * i + 1]);
+  return r;
+}
+template <typename T> __device__ __forceinline__ void put8(T* p, const V8& r) {
+  float f[8];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) split(r.v[i], f[2 * i], f[2 * i + 1]);
+#pragma unroll
+  for (int i = 0; i < kWords<T>; ++i) st_v4(p + i * (16 / sizeof(T)), pack<T>(f + i * (16 / sizeof(T))));
+}
+// Eight values of a float32 parameter, or `none`.
+__device__ __forceinline__ V8 param8(const float* p, int64_t c, bool ok, float none) {
+  V8 r;
+  r.fill(none);
+  if (p && ok) {
+    const float4 a = __ldg(reinterpret_cast<const float4*>(p + c)), b = __ldg(reinterpret_cast<const float4*>(p + c) + 1);
+    r.v[0] = pair(a.x, a.y);
+    r.v[1] = pair(a.z, a.w);
+    r.v[2] = pair(b.x, b.y);
+    r.v[3] = pair(b.z, b.w);
+  }
+  return r;
+}
+
+// ------------------------------------------------------------- async copies
+__device__ __forceinline__ uint32_t shared_addr(const void* p) {
+  return static_cast<uint32_t>(__cvta_generic_to_shared(p));
+}
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void copy4(uint32_t dst, const void* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int K> __device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(K) : "memory"); }
+
+// ------------------------------------------------------------------- sums
 constexpr int log2_of(int k) { return k <= 1 ? 0 : 1 + log2_of(k / 2); }
 
 // Warp-wide sums of K values (a power of two up to 32): lane l ends with the
@@ -82,7 +165,7 @@ template <int K> __device__ __forceinline__ void fold_to(float* v, int lane, flo
   if ((lane & ((1 << shift) - 1)) == 0) dst[lane >> shift] = v[0];
 }
 
-// Where a thread stands: group, warp and thread in it, and its columns.
+// Where a thread stands: its group, its warp in it, its columns.
 struct Place {
   int W, group, warp, lane, tid;
   int64_t d0;
@@ -113,18 +196,31 @@ struct Place {
   __device__ __forceinline__ int slot0() const { return W == 1 ? group : 0; }
 };
 
-// Mean and 1 / root of the group's values u[0..K) of each live thread; `red` is
-// one buffer, a float4 a warp. The variance of a LayerNorm is merged from
-// (count, mean, sum of squared deviations) triples pair by pair, which loses
-// nothing where the mean is large against the deviations.
-template <int K, int MAXW>
-__device__ __forceinline__ void group_stats(const Place& p, const float* u, int per_thread, int norm, float eps,
-                                            float total, float4 (&red)[MAXW], float& mean, float& rstd) {
+// Chunks of eight columns that a thread owns, 32 W apart.
+__device__ __forceinline__ int owned_chunks(const Place& p, int64_t D) {
+  const int total = static_cast<int>(D / kColumns), per = 32 * p.W;
+  return p.tid < total ? (total - p.tid + per - 1) / per : 0;
+}
+
+// Mean and 1 / root of the group's values: u[c][k] of each chunk c that the
+// thread owns (`chunks` of them) and each block k < m; what does not exist
+// holds 0. `red` is one buffer, a float4 a warp; one barrier where W > 1. The
+// variance of a LayerNorm is merged from (count, mean, sum of squared
+// deviations) triples pair by pair, which loses nothing where the mean is large
+// against the deviations.
+template <int CH, int M, int MAXW>
+__device__ __forceinline__ void group_stats(const Place& p, const V8 (&u)[CH][M], int chunks, int m, int norm, float eps,
+                                            float inv, float4 (&red)[MAXW], float& mean, float& rstd) {
   mean = 0.f;
   if (norm == HC_NORM_RMS) {
-    float s = 0.f;
+    f2 s2 = both(0.f);
 #pragma unroll
-    for (int i = 0; i < K; ++i) s = fmaf(u[i], u[i], s);  // columns and blocks that do not exist hold 0
+    for (int c = 0; c < CH; ++c)
+#pragma unroll
+      for (int k = 0; k < M; ++k)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s2 = fma2(u[c][k].v[i], u[c][k].v[i], s2);
+    float s = fold2(s2);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(kFull, s, o);
     if (p.W > 1) {
@@ -133,22 +229,40 @@ __device__ __forceinline__ void group_stats(const Place& p, const float* u, int 
       s = 0.f;
       for (int w = 0; w < p.W; ++w) s += red[w].x;
     }
-    rstd = 1.f / sqrtf(s / total + eps);
+    rstd = rsqrtf(fmaf(s, inv, eps));
     return;
   }
-  float c = p.live ? static_cast<float>(per_thread) : 0.f, mu = 0.f, m2 = 0.f;
-  if (p.live) {
+  float c = static_cast<float>(8 * m * chunks), mu = 0.f, m2 = 0.f;
+  if (chunks > 0) {
+    f2 s2 = both(0.f);
 #pragma unroll
-    for (int i = 0; i < K; ++i) mu += u[i];
-    mu /= c;
+    for (int j = 0; j < CH; ++j)
 #pragma unroll
-    for (int i = 0; i < K; ++i)
-      if (i < per_thread) m2 = fmaf(u[i] - mu, u[i] - mu, m2);
+      for (int k = 0; k < M; ++k)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s2 = add2(u[j][k].v[i], s2);
+    mu = fold2(s2) / c;
+    const f2 less = both(-mu);
+    f2 q2 = both(0.f);
+#pragma unroll
+    for (int j = 0; j < CH; ++j) {
+      if (j >= chunks) break;
+#pragma unroll
+      for (int k = 0; k < M; ++k) {
+        if (k >= m) break;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const f2 d = add2(u[j][k].v[i], less);
+          q2 = fma2(d, d, q2);
+        }
+      }
+    }
+    m2 = fold2(q2);
   }
   auto merge = [&](float c2, float mu2, float m22) {
     const float n = c + c2;
     if (n > 0.f) {
-      const float d = mu2 - mu, share = c2 / n;
+      const float d = mu2 - mu, share = __fdividef(c2, n);
       mu = fmaf(d, share, mu);
       m2 += m22 + d * d * c * share;
       c = n;
@@ -177,552 +291,919 @@ __device__ __forceinline__ void group_stats(const Place& p, const float* u, int 
     }
   }
   mean = mu;
-  rstd = 1.f / sqrtf(m2 / total + eps);
+  rstd = rsqrtf(fmaf(m2, inv, eps));
 }
 
-// u[k] = sum_j R[k][j] x[j] of this thread's columns.
-template <typename T, int N, int M>
-__device__ __forceinline__ void read_rows(const float* R, const Raw8<T> (&x)[N], int n, int m, float (&u)[M][8]) {
+// ------------------------------------------------------ the token's rows
+// A thread's words of ROWS rows of its CH chunks, at [chunk][row][word][thread].
+// A row's threads lie side by side (a warp's copies to scattered words took a
+// quarter more time), and a row ends with 16 bytes of padding, so that the
+// same thread's words of eight rows lie in different banks (warp_gram).
+template <typename T, int ROWS, int CH> struct Rows {
+  uint8_t* mem;
+  int base, pitch;
+  __device__ __forceinline__ Rows(uint8_t* smem) : mem(smem), base(threadIdx.x * 16), pitch(blockDim.x * 16 + 16) {
+    for (int i = 0; i < CH * ROWS * kWords<T>; ++i) *reinterpret_cast<uint4*>(mem + base + i * pitch) = make_uint4(0u, 0u, 0u, 0u);
+  }
+  __device__ __forceinline__ int at(int c, int row) const { return base + (c * ROWS + row) * kWords<T> * pitch; }
+  __device__ __forceinline__ int bytes() const { return CH * ROWS * kWords<T> * pitch; }
+  __device__ __forceinline__ void fetch(int c, int row, const T* src) const {
+    const uint32_t dst = shared_addr(mem) + at(c, row);
 #pragma unroll
-  for (int k = 0; k < M; ++k)
+    for (int i = 0; i < kWords<T>; ++i) copy16(dst + i * pitch, src + i * (16 / sizeof(T)));
+  }
+  __device__ __forceinline__ V8 get(int c, int row) const {
+    uint4 q[kWords<T>];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) u[k][e] = 0.f;
-#pragma unroll
-  for (int j = 0; j < N; ++j) {
-    if (j >= n) break;
-    float xv[8];
-    x[j].get(xv);
-#pragma unroll
-    for (int k = 0; k < M; ++k) {
-      if (k >= m) break;
-      const float r = __ldg(R + k * n + j);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) u[k][e] = fmaf(r, xv[e], u[k][e]);
-    }
+    for (int i = 0; i < kWords<T>; ++i) q[i] = *reinterpret_cast<const uint4*>(mem + at(c, row) + i * pitch);
+    return expand<T>(q);
+  }
+};
+__device__ __forceinline__ float one(f2 v) {
+  float a, b;
+  split(v, a, b);
+  return a;
+}
+
+// The loop over a group's tokens. all(t) issues the copies of a token's rows,
+// small(t, slot) those of its small matrices. work(t, next, slot, parity) does
+// token t, whose rows have arrived and whose small matrices have since the
+// barrier before; it passes the group's barrier exactly once, and where
+// next < T asks for that token's rows, each as soon as it has read this
+// token's.
+template <typename All, typename Small, typename Start, typename Work>
+__device__ __forceinline__ void walk_tokens(const Place& p, int64_t T, All all, Small small, Start start, Work work) {
+  const int64_t t0 = p.first(), step = p.stride();
+  if (t0 >= T) return;
+  p.sync();  // the zeros of the rows and of the small matrices
+  small(t0, 0);
+  copy_commit();
+  all(t0);
+  if (t0 + step < T) small(t0 + step, 1);
+  copy_commit();
+  copy_wait<1>();
+  p.sync();
+  start(0);
+  int i = 0;
+  for (int64_t t = t0; t < T; t += step, ++i) {
+    if (t + 2 * step < T) small(t + 2 * step, (i + 2) & (kSmallSlots - 1));
+    copy_commit();
+    copy_wait<1>();
+    work(t, t + step, i & (kSmallSlots - 1), i & 1);
+    copy_commit();
   }
 }
+
+// A group's small entries of a token, dealt to its threads once: R rounds of
+// 32 W entries, each from src + t stride to entry dst of a slot.
+template <int R> struct SmallCopies {
+  const float* src[R];
+  int stride[R], dst[R];
+  template <typename Decode> __device__ __forceinline__ SmallCopies(const Place& p, int total, Decode decode) {
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      const int id = p.tid + r * 32 * p.W;
+      src[r] = nullptr;
+      stride[r] = 0;
+      dst[r] = -1;
+      if (id < total) decode(id, src[r], stride[r], dst[r]);
+    }
+  }
+  __device__ __forceinline__ void fetch(f2* slot, int64_t t) const {
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+      if (dst[r] >= 0) {
+        const float* s = src[r] + t * stride[r];
+        const uint32_t d = shared_addr(slot + dst[r]);
+        copy4(d, s);
+        copy4(d + 4, s);
+      }
+  }
+};
+
+// Where the sums of a token's small gradients go, dealt to threads likewise;
+// nullptr where nobody wants one.
+template <int R> struct SmallGrads {
+  float* out[R];
+  int stride[R];
+  template <typename Decode> __device__ __forceinline__ SmallGrads(const Place& p, int total, Decode decode) {
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      const int id = p.tid + r * 32 * p.W;
+      out[r] = nullptr;
+      stride[r] = 0;
+      if (id < total) decode(id, out[r], stride[r]);
+    }
+  }
+  // The W warps' sums of entry id, which lie `per` floats apart.
+  template <typename Sums> __device__ __forceinline__ void store(const Place& p, int64_t t, Sums sums) const {
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+      if (out[r]) {
+        const int id = p.tid + r * 32 * p.W;
+        float s = 0.f;
+        for (int q = 0; q < p.W; ++q) s += sums(q, id);
+        out[r][t * stride[r]] = s;
+      }
+  }
+};
 
 // The groups' sums of the [m D] parameters' gradients; with several groups a
 // CTA each adds its own row.
-template <int M>
-__device__ __forceinline__ void store_param_sums(const NormArgs& a, const Place& p, const float (&A)[M][8],
-                                                 const float (&B)[M][8]) {
-  if (!a.partial || !p.live) return;
+template <int CH, int M>
+__device__ __forceinline__ void store_param_sums(const NormArgs& a, const Place& p, int chunks, const V8 (&A)[CH][M],
+                                                 const V8 (&B)[CH][M]) {
+  if (!a.partial) return;
   const int64_t E = a.D * a.m;
   const int64_t row = p.W == 1 ? static_cast<int64_t>(blockIdx.x) * kSmallGroups + p.group : blockIdx.x;
-  float* dst = a.partial + row * 2 * E;
+  float* dst = a.partial + row * 2 * E + p.d0;
 #pragma unroll
-  for (int k = 0; k < M; ++k) {
-    if (k >= a.m) break;
-    const int64_t c = k * a.D + p.d0;
+  for (int c = 0; c < CH; ++c) {
+    if (c >= chunks) break;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      dst[c + e] = A[k][e];
-      dst[E + c + e] = B[k][e];
+    for (int k = 0; k < M; ++k) {
+      if (k >= a.m) break;
+      put8<float>(dst + k * a.D + c * 256 * p.W, A[c][k]);
+      put8<float>(dst + E + k * a.D + c * 256 * p.W, B[c][k]);
     }
   }
+}
+
+// The group's small matrices, all slots, to zero.
+template <int K> __device__ __forceinline__ void clear_small(const Place& p, f2 (&s)[kSmallSlots][K]) {
+  for (int i = p.tid; i < kSmallSlots * K; i += 32 * p.W) (&s[0][0])[i] = 0ull;
+}
+
+// A group's part of dynamic shared memory, behind the rows.
+template <int N, int M> struct ReadMemory {
+  static constexpr int kEntries = N * M + 2;
+  alignas(16) f2 R[kSmallSlots][kEntries];  // R [N][M], and for the backward mean and 1 / root
+};
+template <typename Memory>
+__device__ __forceinline__ Memory& group_memory(uint8_t* dyn, const Place& p, int row_bytes) {
+  return reinterpret_cast<Memory*>(dyn + row_bytes)[p.group];
 }
 
 // ------------------------------------------------------------------- read
-template <typename T, int N, int M>
-__global__ void __launch_bounds__(norm_max_threads(false, N, sizeof(T)))
+template <typename T, int N, int M, int CH>
+__global__ void __launch_bounds__(norm_fwd_threads(N, M, CH, sizeof(T)))
     read_norm_fwd_kernel(const __grid_constant__ NormArgs a, int warps) {
-  constexpr int MAXW = norm_max_threads(false, N, sizeof(T)) / 32;
+  constexpr int MAXW = norm_fwd_threads(N, M, CH, sizeof(T)) / 32;
+  extern __shared__ __align__(16) uint8_t dyn[];
   __shared__ float4 red[2][MAXW];
   const Place p(warps, a.D);
-  const int n = a.n, m = a.m;
+  const int n = a.n, m = a.m, chunks = owned_chunks(p, a.D), step = 256 * p.W;
   const int64_t D = a.D, E = D * m;
-  int buf = 0;
-  for (int64_t t = p.first(); t < a.T; t += p.stride(), buf ^= 1) {
-    const T* x = static_cast<const T*>(a.x) + t * n * D + p.d0;
-    Raw8<T> xr[N];
+  const float inv = 1.f / static_cast<float>(E);
+  const Rows<T, N, CH> rows(dyn);
+  auto& sR = group_memory<ReadMemory<N, M>>(dyn, p, rows.bytes()).R;
+  clear_small(p, sR);
+  const SmallCopies<(N * M + 31) / 32> copies(p, n * m, [&](int id, const float*& src, int& stride, int& dst) {
+    src = a.R + id;
+    stride = n * m;
+    dst = id % n * M + id / n;
+  });
+  auto fetch = [&](int64_t t, int c) {
+    if (c >= chunks) return;
+    const T* x = static_cast<const T*>(a.x) + t * n * D + p.d0 + c * step;
 #pragma unroll
-    for (int j = 0; j < N; ++j) xr[j].load(x + j * D, p.live && j < n);
-    float u[M][8];
-    read_rows<T, N, M>(a.R + t * m * n, xr, n, m, u);
-    float mean, rstd;
-    group_stats<8 * M>(p, &u[0][0], 8 * m, a.norm, a.eps, static_cast<float>(E), red[buf], mean, rstd);
-    if (a.stats && p.tid == 0) {
-      a.stats[2 * t] = mean;
-      a.stats[2 * t + 1] = rstd;
-    }
-    if (p.live) {
-      T* y = static_cast<T*>(a.out) + t * E + p.d0;
+    for (int j = 0; j < N; ++j)
+      if (j < n) rows.fetch(c, j, x + j * D);
+  };
+  walk_tokens(
+      p, a.T,
+      [&](int64_t t) {
 #pragma unroll
-      for (int k = 0; k < M; ++k) {
-        if (k >= m) break;
-        float w[8], b[8];
-        param8(a.weight, k * D + p.d0, true, 1.f, w);
-        param8(a.bias, k * D + p.d0, true, 0.f, b);
+        for (int c = 0; c < CH; ++c) fetch(t, c);
+      },
+      [&](int64_t t, int slot) { copies.fetch(sR[slot], t); }, [](int) {},
+      [&](int64_t t, int64_t next, int slot, int parity) {
+        const f2* R = sR[slot];
+        V8 u[CH][M];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) u[k][e] = fmaf((u[k][e] - mean) * rstd, w[e], b[e]);
-        put8<T>(y + k * D, u[k]);
-      }
-    }
-    __syncwarp();
-  }
+        for (int c = 0; c < CH; ++c) {
+#pragma unroll
+          for (int k = 0; k < M; ++k) u[c][k].fill(0.f);
+#pragma unroll
+          for (int j = 0; j < N; ++j) {
+            const V8 x = rows.get(c, j);
+#pragma unroll
+            for (int k = 0; k < M; ++k) axpy(R[j * M + k], x, u[c][k]);
+          }
+          if (next < a.T) fetch(next, c);
+        }
+        float mean, rstd;
+        group_stats<CH, M, MAXW>(p, u, chunks, m, a.norm, a.eps, inv, red[parity], mean, rstd);
+        if (a.stats && p.tid == 0) *reinterpret_cast<float2*>(a.stats + 2 * t) = make_float2(mean, rstd);
+        T* y = static_cast<T*>(a.out) + t * E + p.d0;
+        const f2 less = both(-mean), r2 = both(rstd);
+#pragma unroll
+        for (int c = 0; c < CH; ++c) {
+          if (c >= chunks) break;
+#pragma unroll
+          for (int k = 0; k < M; ++k) {
+            if (k >= m) break;
+            const int64_t col = k * D + c * step;
+            const V8 w = param8(a.weight, col + p.d0, true, 1.f), b = param8(a.bias, col + p.d0, true, 0.f);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) u[c][k].v[i] = fma2(mul2(add2(u[c][k].v[i], less), r2), w.v[i], b.v[i]);
+            put8<T>(y + col, u[c][k]);
+          }
+        }
+        __syncwarp();
+      });
 }
 
-template <typename T, int N, int M>
-__global__ void __launch_bounds__(norm_max_threads(true, N, sizeof(T)))
+template <typename T, int N, int M, int CH>
+__global__ void __launch_bounds__(norm_bwd_threads(N, M, sizeof(T)))
     read_norm_bwd_kernel(const __grid_constant__ NormArgs a, int warps) {
-  constexpr int MAXW = norm_max_threads(true, N, sizeof(T)) / 32, G = N * M;
+  static_assert(CH == 1, "the backward's threads own one chunk");
+  constexpr int MAXW = norm_bwd_threads(N, M, sizeof(T)) / 32, G = N * M;
+  extern __shared__ __align__(16) uint8_t dyn[];
   __shared__ float red[2][MAXW][2], gram[2][MAXW][G];
   const Place p(warps, a.D);
   const int n = a.n, m = a.m;
   const int64_t D = a.D, E = D * m;
-  float A[M][8] = {}, B[M][8] = {};
-  int buf = 0;
-  int64_t last = -1;
-  // grad_R of token t, whose warps' sums lie in buffer b
-  auto flush = [&](int64_t t, int b) {
-    if (!a.grad_R || t < 0) return;
-    for (int i = p.tid; i < G; i += 32 * p.W) {
-      const int k = i / N, j = i % N;
-      if (k >= m || j >= n) continue;
-      float s = 0.f;
-      for (int w = 0; w < p.W; ++w) s += gram[b][p.slot0() + w][i];
-      a.grad_R[t * m * n + k * n + j] = s;
-    }
-  };
-  for (int64_t t = p.first(); t < a.T; t += p.stride(), buf ^= 1) {
-    const T* x = static_cast<const T*>(a.x) + t * n * D + p.d0;
-    const T* g = static_cast<const T*>(a.g) + t * E + p.d0;
-    const float* R = a.R + t * m * n;
-    Raw8<T> xr[N], gr[M];
+  const float inv = 1.f / static_cast<float>(E);
+  const Rows<T, N + M, 1> rows(dyn);
+  auto& sR = group_memory<ReadMemory<N, M>>(dyn, p, rows.bytes()).R;
+  clear_small(p, sR);
+  const SmallCopies<(G + 33) / 32> copies(p, n * m + 2, [&](int id, const float*& src, int& stride, int& dst) {
+    const bool st = id >= n * m;
+    src = st ? a.stats + (id - n * m) : a.R + id;
+    stride = st ? 2 : n * m;
+    dst = st ? G + id - n * m : id % n * M + id / n;
+  });
+  const SmallGrads<(G + 31) / 32> grads(p, G, [&](int id, float*& out, int& stride) {  // [stream][block]
+    const int j = id / M, k = id % M;
+    if (a.grad_R && j < n && k < m) out = a.grad_R + k * n + j;
+    stride = n * m;
+  });
+  V8 A[1][M], B[1][M];
 #pragma unroll
-    for (int k = 0; k < M; ++k) gr[k].load(g + k * D, p.live && k < m);
-#pragma unroll
-    for (int j = 0; j < N; ++j) xr[j].load(x + j * D, p.live && j < n);
-    const float mean = __ldg(a.stats + 2 * t), rstd = __ldg(a.stats + 2 * t + 1);
-    float u[M][8];
-    read_rows<T, N, M>(R, xr, n, m, u);
-    float s[2] = {0.f, 0.f};
-#pragma unroll
-    for (int k = 0; k < M; ++k) {
-      if (k >= m) break;
-      float w[8], gv[8];
-      gr[k].get(gv);
-      param8(a.weight, k * D + p.d0, p.live, 1.f, w);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        u[k][e] = (u[k][e] - mean) * rstd;  // xhat
-        const float q = gv[e] * w[e];
-        s[0] = fmaf(q, u[k][e], s[0]);
-        s[1] += q;
-        A[k][e] = fmaf(gv[e], u[k][e], A[k][e]);
-        B[k][e] += gv[e];
-      }
-    }
-    if (!p.live) s[0] = s[1] = 0.f;
-    fold_to<2>(s, p.lane, red[buf][p.slot()]);
-    p.sync();
-    flush(last, buf ^ 1);
-    float c1 = 0.f, c2 = 0.f;
-    for (int w = 0; w < p.W; ++w) {
-      c1 += red[buf][p.slot0() + w][0];
-      c2 += red[buf][p.slot0() + w][1];
-    }
-    c1 /= static_cast<float>(E);
-    c2 = a.norm == HC_NORM_LAYER ? c2 / static_cast<float>(E) : 0.f;
-#pragma unroll
-    for (int k = 0; k < M; ++k) {
-      if (k >= m) {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) u[k][e] = 0.f;
-        continue;
-      }
-      float w[8], gv[8];
-      gr[k].get(gv);
-      param8(a.weight, k * D + p.d0, p.live, 1.f, w);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) u[k][e] = p.live ? rstd * (gv[e] * w[e] - c2 - u[k][e] * c1) : 0.f;  // du
-    }
-    if (a.grad_x && p.live) {
-      T* gx = static_cast<T*>(a.grad_x) + t * n * D + p.d0;
-#pragma unroll
-      for (int j = 0; j < N; ++j) {
-        if (j >= n) break;
-        float r[8] = {};
-#pragma unroll
-        for (int k = 0; k < M; ++k) {
-          if (k >= m) break;
-          const float rk = __ldg(R + k * n + j);
-#pragma unroll
-          for (int e = 0; e < 8; ++e) r[e] = fmaf(rk, u[k][e], r[e]);
-        }
-        put8<T>(gx + j * D, r);
-      }
-    }
-    if (a.grad_R) {
-      float acc[G];
-#pragma unroll
-      for (int j = 0; j < N; ++j) {
-        float xv[8];
-        xr[j].get(xv);
-#pragma unroll
-        for (int k = 0; k < M; ++k) {
-          float r = 0.f;
-#pragma unroll
-          for (int e = 0; e < 8; ++e) r = fmaf(u[k][e], xv[e], r);
-          acc[k * N + j] = r;
-        }
-      }
-      fold_to<G>(acc, p.lane, gram[buf][p.slot()]);
-    }
-    last = t;
+  for (int k = 0; k < M; ++k) {
+    A[0][k].fill(0.f);
+    B[0][k].fill(0.f);
   }
+  int64_t last = -1;
+  int last_parity = 0;
+  // grad_R of the last token, whose warps' sums lie in the other buffer
+  auto flush = [&] {
+    if (last >= 0) grads.store(p, last, [&](int q, int id) { return gram[last_parity][p.slot0() + q][id]; });
+  };
+  auto fetch_x = [&](int64_t t) {
+    if (!p.live) return;
+    const T* x = static_cast<const T*>(a.x) + t * n * D + p.d0;
+#pragma unroll
+    for (int j = 0; j < N; ++j)
+      if (j < n) rows.fetch(0, j, x + j * D);
+  };
+  auto fetch_g = [&](int64_t t) {
+    if (!p.live) return;
+    const T* g = static_cast<const T*>(a.g) + t * E + p.d0;
+#pragma unroll
+    for (int k = 0; k < M; ++k)
+      if (k < m) rows.fetch(0, N + k, g + k * D);
+  };
+  walk_tokens(
+      p, a.T,
+      [&](int64_t t) {
+        fetch_x(t);
+        fetch_g(t);
+      },
+      [&](int64_t t, int slot) { copies.fetch(sR[slot], t); }, [](int) {},
+      [&](int64_t t, int64_t next, int slot, int parity) {
+        const f2* R = sR[slot];
+        const f2 less = both(-one(R[G])), r2 = R[G + 1];
+        f2 s1 = both(0.f), s2 = both(0.f);
+        V8 u[M], q[M];
+#pragma unroll
+        for (int k = 0; k < M; ++k) u[k].fill(0.f);
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+          const V8 x = rows.get(0, j);
+#pragma unroll
+          for (int k = 0; k < M; ++k) axpy(R[j * M + k], x, u[k]);
+        }
+#pragma unroll
+        for (int k = 0; k < M; ++k) {
+          const V8 g = rows.get(0, N + k);
+          const V8 w = param8(a.weight, k * D + p.d0, p.live && k < m, 1.f);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            u[k].v[i] = mul2(add2(u[k].v[i], less), r2);  // xhat
+            q[k].v[i] = mul2(g.v[i], w.v[i]);
+            s1 = fma2(q[k].v[i], u[k].v[i], s1);
+            s2 = add2(q[k].v[i], s2);
+            A[0][k].v[i] = fma2(g.v[i], u[k].v[i], A[0][k].v[i]);
+            B[0][k].v[i] = add2(g.v[i], B[0][k].v[i]);
+          }
+        }
+        if (next < a.T) fetch_g(next);
+        float s[2] = {fold2(s1), fold2(s2)};  // g is 0 where there are no columns
+        fold_to<2>(s, p.lane, red[parity][p.slot()]);
+        p.sync();
+        flush();
+        float c1 = 0.f, c2 = 0.f;
+        for (int i = 0; i < p.W; ++i) {
+          c1 += red[parity][p.slot0() + i][0];
+          c2 += red[parity][p.slot0() + i][1];
+        }
+        const f2 k1 = both(-c1 * inv), k2 = both(a.norm == HC_NORM_LAYER ? -c2 * inv : 0.f);
+#pragma unroll
+        for (int k = 0; k < M; ++k)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) u[k].v[i] = mul2(r2, fma2(u[k].v[i], k1, add2(q[k].v[i], k2)));  // du
+        float acc[G];
+        T* gx = static_cast<T*>(a.grad_x) + t * n * D + p.d0;
+        const bool store = a.grad_x && p.live;
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+          V8 r;
+          r.fill(0.f);
+#pragma unroll
+          for (int k = 0; k < M; ++k) axpy(R[j * M + k], u[k], r);
+          if (store && j < n) put8<T>(gx + j * D, r);
+          const V8 x = rows.get(0, j);  // 0 where there are no columns
+#pragma unroll
+          for (int k = 0; k < M; ++k) acc[j * M + k] = dot(u[k], x);
+        }
+        if (next < a.T) fetch_x(next);
+        fold_to<G>(acc, p.lane, gram[parity][p.slot()]);
+        last = t;
+        last_parity = parity;
+      });
   p.sync();
-  flush(last, buf ^ 1);
-  store_param_sums<M>(a, p, A, B);
+  flush();
+  store_param_sums<1, M>(a, p, p.live ? 1 : 0, A, B);
 }
 
 // -------------------------------------------------------------- mix-write
-// Keep factors (0 or 1 / (1 - p)) of this thread's eight columns of block k.
-__device__ __forceinline__ void keep8(const DropArgs& d, const DropKey& key, uint64_t element, float (&f)[8]) {
+// All ones where one of eight columns is kept, the first a multiple of 8.
+__device__ __forceinline__ void keep8(const DropArgs& d, const DropKey& key, uint64_t element, uint32_t (&mask)[8]) {
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
     const uint4 w = philox4(key, (element >> 2) + h);
-    f[4 * h] = w.x >= d.threshold ? d.scale : 0.f;
-    f[4 * h + 1] = w.y >= d.threshold ? d.scale : 0.f;
-    f[4 * h + 2] = w.z >= d.threshold ? d.scale : 0.f;
-    f[4 * h + 3] = w.w >= d.threshold ? d.scale : 0.f;
+    mask[4 * h] = w.x >= d.bar ? d.kept : 0u;
+    mask[4 * h + 1] = w.y >= d.bar ? d.kept : 0u;
+    mask[4 * h + 2] = w.z >= d.bar ? d.kept : 0u;
+    mask[4 * h + 3] = w.w >= d.bar ? d.kept : 0u;
+  }
+}
+// v / (1 - p) where kept, else 0 whatever v is.
+__device__ __forceinline__ void keep_mul(V8& v, float scale, const uint32_t (&mask)[8]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    float x, y;
+    split(mul2(v.v[i], both(scale)), x, y);
+    v.v[i] = pair(__uint_as_float(__float_as_uint(x) & mask[2 * i]), __uint_as_float(__float_as_uint(y) & mask[2 * i + 1]));
+  }
+}
+// act(a) of a gate, and act'(a).
+__device__ __forceinline__ void gate8(int act, const V8& a, V8& val, V8& der) {
+  if (act == HC_ACT_SIGMOID) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      float x, y;
+      split(a.v[i], x, y);
+      x = __fdividef(1.f, 1.f + __expf(-x));
+      y = __fdividef(1.f, 1.f + __expf(-y));
+      val.v[i] = pair(x, y);
+      der.v[i] = fma2(val.v[i], pair(-x, -y), val.v[i]);  // s - s^2
+    }
+  } else {
+    val = a;
+    der.fill(1.f);
   }
 }
 
-// H + (v - H v) v^T of token t into shared memory, by the group's first threads.
-template <int N>
-__device__ __forceinline__ void stage_mix(const NormArgs& a, const Place& p, int64_t t, float (&sH)[N * N]) {
-  const int n = a.n;
-  for (int i = p.tid; i < n * n; i += 32 * p.W)
-    sH[(i / n) * N + i % n] = mix_entry(a.H + t * n * n, a.v ? a.v + t * n : nullptr, n, i / n, i % n);
+// A token's small matrices in shared memory: H [column][row] (TRANSPOSED) or
+// [row][column], W [N][M], v, then mean and 1 / root.
+template <int N, int M, bool TRANSPOSED> struct Small {
+  static constexpr int kW = N * N, kV = kW + N * M, kStats = kV + N, kEntries = (kStats + 3) / 2 * 2;
+  static constexpr int kRounds = (kStats + 2 + 31) / 32;
+  __device__ static __forceinline__ int h(int r, int c) { return TRANSPOSED ? c * N + r : r * N + c; }
+  __device__ static __forceinline__ SmallCopies<kRounds> copies(const NormArgs& a, const Place& p, bool stats) {
+    const int n = a.n, m = a.m, w0 = n * n, v0 = w0 + n * m, s0 = a.v ? v0 + n : v0;
+    return SmallCopies<kRounds>(p, stats ? s0 + 2 : s0, [&](int id, const float*& src, int& stride, int& dst) {
+      if (id < w0) {
+        src = a.H + id;
+        stride = w0;
+        dst = h(id / n, id % n);
+      } else if (id < v0) {
+        src = a.W + (id - w0);
+        stride = n * m;
+        dst = kW + (id - w0) / m * M + (id - w0) % m;
+      } else if (id < s0) {
+        src = a.v + (id - v0);
+        stride = n;
+        dst = kV + id - v0;
+      } else {
+        src = a.stats + (id - s0);
+        stride = 2;
+        dst = kStats + id - s0;
+      }
+    });
+  }
+  // H + (v - H v) v^T, by the group's first threads.
+  __device__ static __forceinline__ void project(const Place& p, const f2* s, f2* dst) {
+    for (int i = p.tid; i < N * N; i += 32 * p.W) {
+      const int r = i / N, c = i % N;
+      float q = one(s[kV + r]);
+      for (int k = 0; k < N; ++k) q -= one(s[h(r, k)]) * one(s[kV + k]);
+      dst[h(r, c)] = both(one(s[h(r, c)]) + q * one(s[kV + c]));
+    }
+  }
+  // grad_H and grad_v of the token from G = dL/d(H + (v - H v) v^T), [row][column].
+  __device__ static __forceinline__ void grads(const NormArgs& a, const Place& p, const f2* s, const float* G, int64_t t) {
+    const int n = a.n;
+    for (int i = p.tid; i < N * N; i += 32 * p.W) {
+      const int r = i / N, c = i % N;
+      if (r >= n || c >= n || !a.grad_H) continue;
+      float dq = 0.f;
+      for (int j = 0; j < n; ++j) dq += G[r * N + j] * one(s[kV + j]);
+      a.grad_H[t * n * n + r * n + c] = G[i] - dq * one(s[kV + c]);
+    }
+    if (a.grad_v && p.tid < n) {
+      const int c = p.tid;
+      float g = 0.f;
+      for (int r = 0; r < n; ++r) {
+        float q = one(s[kV + r]), dq = 0.f;
+        for (int j = 0; j < n; ++j) {
+          q -= one(s[h(r, j)]) * one(s[kV + j]);
+          dq += G[r * N + j] * one(s[kV + j]);
+        }
+        g += q * G[r * N + c] + (r == c ? dq : 0.f) - one(s[h(r, c)]) * dq;
+      }
+      a.grad_v[t * n + c] = g;
+    }
+  }
+};
+
+template <int N, int M> struct WriteMemory {
+  alignas(16) f2 small[kSmallSlots][Small<N, M, true>::kEntries];
+  f2 mixed[2][N * N];  // H + (v - H v) v^T of this token and the next
+  float G[N * N];
+};
+
+// g x^T of a warp's 256 columns by mma.m16n8k16 (products of 16-bit values are
+// exact in float32): a lane's 16 bytes of a row are a row of an 8 x 8 tile, so
+// that the tiles g and x of two lanes' columns are one ldmatrix, and the sums
+// over the lanes come out of the products instead of exchanges. Rows past N
+// repeat the others and are not stored; dst is [column][row].
+template <typename T, int N, typename R>
+__device__ __forceinline__ void warp_gram(const R& rows, float (&c)[4]) {
+  const int lane = threadIdx.x & 31;
+  // matrices 0, 1: rows g of an even and an odd lane's columns; 2, 3: rows x
+  const uint32_t addr = shared_addr(rows.mem) + rows.at(0, 0) - lane * 16 + ((lane >> 3) & 1) * 16 +
+                        static_cast<uint32_t>(((lane >> 4) * N + (lane & 7) % N) * rows.pitch);
+#pragma unroll
+  for (int l = 0; l < 32; l += 2) {
+    uint32_t g0, g1, x0, x1;
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(g0), "=r"(g1), "=r"(x0), "=r"(x1)
+                 : "r"(addr + l * 16)
+                 : "memory");
+    if constexpr (std::is_same<T, __nv_bfloat16>::value)
+      asm volatile(
+          "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+          : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+          : "r"(g0), "r"(0), "r"(g1), "r"(0), "r"(x0), "r"(x1));
+    else
+      asm volatile(
+          "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+          : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+          : "r"(g0), "r"(0), "r"(g1), "r"(0), "r"(x0), "r"(x1));
+  }
+}
+template <int N> __device__ __forceinline__ void store_gram(const float (&c)[4], int lane, float* dst) {
+  const int r = lane >> 2, col = (lane & 3) * 2;  // c[0], c[1]: row r, columns col and col + 1
+  if (r < N) {
+    if (col < N) dst[col * N + r] = c[0];
+    if (col + 1 < N) dst[(col + 1) * N + r] = c[1];
+  }
 }
 
-template <typename T, int N, int M>
-__global__ void __launch_bounds__(norm_max_threads(false, N, sizeof(T)))
+// scale * weight and scale * bias of eight columns from c on.
+__device__ __forceinline__ void scaled_params(const NormArgs& a, int64_t c, bool ok, V8& ws, V8& bs) {
+  const V8 sc = param8(a.scale, c, ok, 1.f);
+  ws = param8(a.weight, c, ok, 1.f);
+  bs = param8(a.bias, c, ok, 0.f);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    ws.v[i] = mul2(ws.v[i], sc.v[i]);
+    bs.v[i] = mul2(bs.v[i], sc.v[i]);
+  }
+}
+
+template <typename T, int N, int M, int CH>
+__global__ void __launch_bounds__(norm_fwd_threads(N, M, CH, sizeof(T)))
     write_norm_fwd_kernel(const __grid_constant__ NormArgs a, int warps) {
-  constexpr int MAXW = norm_max_threads(false, N, sizeof(T)) / 32;
+  constexpr int MAXW = norm_fwd_threads(N, M, CH, sizeof(T)) / 32;
+  using S = Small<N, M, false>;
+  extern __shared__ __align__(16) uint8_t dyn[];
   __shared__ float4 red[2][MAXW];
-  __shared__ float sH[2][kSmallGroups][N * N];
   const Place p(warps, a.D);
-  const int n = a.n, m = a.m;
+  const int n = a.n, m = a.m, chunks = owned_chunks(p, a.D), step = 256 * p.W;
   const int64_t D = a.D, E = D * m;
+  const float inv = 1.f / static_cast<float>(E);
   const DropKey key = a.drop.on ? drop_key(a.drop) : DropKey{};
-  int buf = 0;
-  for (int64_t t = p.first(); t < a.T; t += p.stride(), buf ^= 1) {
-    const T* x = static_cast<const T*>(a.x) + t * n * D + p.d0;
-    const T* f = static_cast<const T*>(a.f) + t * E + p.d0;
-    const T* gate = a.gate ? static_cast<const T*>(a.gate) + t * E + p.d0 : nullptr;
-    Raw8<T> fr[M], xr[N], ar[M];
-#pragma unroll
-    for (int k = 0; k < M; ++k) fr[k].load(f + k * D, p.live && k < m);
-#pragma unroll
-    for (int k = 0; k < M; ++k) ar[k].load(gate + k * D, gate && p.live && k < m);
-#pragma unroll
-    for (int j = 0; j < N; ++j) xr[j].load(x + j * D, p.live && j < n);
-    stage_mix<N>(a, p, t, sH[buf][p.group]);
-    float z[M][8];
-#pragma unroll
-    for (int k = 0; k < M; ++k) fr[k].get(z[k]);
-    float mean = 0.f, rstd = 1.f;
-    if (a.norm != HC_NORM_NONE) {
-      group_stats<8 * M>(p, &z[0][0], 8 * m, a.norm, a.eps, static_cast<float>(E), red[buf], mean, rstd);
-      if (a.stats && p.tid == 0) {
-        a.stats[2 * t] = mean;
-        a.stats[2 * t + 1] = rstd;
-      }
-    }
-    if (a.norm == HC_NORM_NONE || p.W == 1) p.sync();  // sH; with a norm over several warps its barrier did it
-#pragma unroll
-    for (int k = 0; k < M; ++k) {
-      if (k >= m || !p.live) {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) z[k][e] = 0.f;
-        continue;
-      }
-      const int64_t c = k * D + p.d0;
-      float w[8], b[8];
-      param8(a.weight, c, true, 1.f, w);
-      param8(a.bias, c, true, 0.f, b);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) z[k][e] = fmaf((z[k][e] - mean) * rstd, w[e], b[e]);
-      if (gate) {
-        ar[k].get(w);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) z[k][e] *= gate_value(a.gate_act, w[e]);
-      }
-      if (a.scale) {
-        param8(a.scale, c, true, 1.f, w);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) z[k][e] *= w[e];
-      }
-      if (a.drop.on) {
-        keep8(a.drop, key, static_cast<uint64_t>(t * E + c), w);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) z[k][e] = w[e] != 0.f ? z[k][e] * w[e] : 0.f;
-      }
-    }
-    if (p.live) {
-      float xv[N][8];
-#pragma unroll
-      for (int j = 0; j < N; ++j) xr[j].get(xv[j]);
-      T* out = static_cast<T*>(a.out) + t * n * D + p.d0;
-      const float* W = a.W + t * n * m;
-#pragma unroll
-      for (int i = 0; i < N; ++i) {
-        if (i >= n) break;
-        float r[8] = {};
-#pragma unroll
-        for (int j = 0; j < N; ++j) {
-          if (j >= n) break;
-          const float h = sH[buf][p.group][i * N + j];
-#pragma unroll
-          for (int e = 0; e < 8; ++e) r[e] = fmaf(h, xv[j][e], r[e]);
-        }
-#pragma unroll
-        for (int k = 0; k < M; ++k) {
-          if (k >= m) break;
-          const float w = __ldg(W + i * m + k);
-#pragma unroll
-          for (int e = 0; e < 8; ++e) r[e] = fmaf(w, z[k][e], r[e]);
-        }
-        put8<T>(out + i * D, r);
-      }
-    }
-    __syncwarp();
-  }
-}
-
-template <typename T, int N, int M>
-__global__ void __launch_bounds__(norm_max_threads(true, N, sizeof(T)))
-    write_norm_bwd_kernel(const __grid_constant__ NormArgs a, int warps) {
-  constexpr int MAXW = norm_max_threads(true, N, sizeof(T)) / 32;
-  constexpr int GB = N * N < 32 ? N * N : 32, G = N * N + N * M;  // H's sums by batches of GB, then W's
-  __shared__ float red[2][MAXW][2], gram[2][MAXW][G], sH[2][kSmallGroups][N * N], sG[kSmallGroups][N * N];
-  const Place p(warps, a.D);
-  const int n = a.n, m = a.m;
-  const int64_t D = a.D, E = D * m;
-  const DropKey key = a.drop.on ? drop_key(a.drop) : DropKey{};
-  float A[M][8] = {}, B[M][8] = {};
-  int buf = 0;
-  int64_t last = -1;
-  // grad_H, grad_v and grad_W of token t, whose warps' sums lie in buffer b
-  auto flush = [&](int64_t t, int b) {
-    if (t < 0) return;
-    for (int i = p.tid; i < G; i += 32 * p.W) {
-      float s = 0.f;
-      for (int w = 0; w < p.W; ++w) s += gram[b][p.slot0() + w][i];
-      if (i < N * N) {
-        const int r = i / N, c = i % N;
-        if (r >= n || c >= n) continue;
-        if (a.v)
-          sG[p.group][r * n + c] = s;
-        else if (a.grad_H)
-          a.grad_H[t * n * n + r * n + c] = s;
-      } else if (a.grad_W) {
-        const int r = (i - N * N) / M, k = (i - N * N) % M;
-        if (r < n && k < m) a.grad_W[(t * n + r) * m + k] = s;
-      }
-    }
-    if (a.v) {
-      p.sync();
-      for (int i = p.tid; i < n * n; i += 32 * p.W)
-        mix_grads(sG[p.group], a.H + t * n * n, a.v + t * n, n, i, a.grad_H ? a.grad_H + t * n * n : nullptr,
-                  a.grad_v ? a.grad_v + t * n : nullptr);
-    }
-  };
-  for (int64_t t = p.first(); t < a.T; t += p.stride(), buf ^= 1) {
-    const T* x = static_cast<const T*>(a.x) + t * n * D + p.d0;
-    const T* g = static_cast<const T*>(a.g) + t * n * D + p.d0;
-    const T* f = static_cast<const T*>(a.f) + t * E + p.d0;
-    const T* gate = a.gate ? static_cast<const T*>(a.gate) + t * E + p.d0 : nullptr;
-    const float* W = a.W + t * n * m;
-    Raw8<T> gr[N], xr[N], fr[M], ar[M];
-#pragma unroll
-    for (int j = 0; j < N; ++j) gr[j].load(g + j * D, p.live && j < n);
-#pragma unroll
-    for (int k = 0; k < M; ++k) fr[k].load(f + k * D, p.live && k < m);
-#pragma unroll
-    for (int k = 0; k < M; ++k) ar[k].load(gate + k * D, gate && p.live && k < m);
-#pragma unroll
-    for (int j = 0; j < N; ++j) xr[j].load(x + j * D, p.live && j < n);
-    const float mean = a.norm == HC_NORM_NONE ? 0.f : __ldg(a.stats + 2 * t);
-    const float rstd = a.norm == HC_NORM_NONE ? 1.f : __ldg(a.stats + 2 * t + 1);
-    stage_mix<N>(a, p, t, sH[buf][p.group]);
-    // pg[k] = dz behind dropout, times act(gate); z; the gradients of gate
-    float pg[M][8], z[M][8];
-    float s[2] = {0.f, 0.f};
+  const Rows<T, N + 2 * M, CH> rows(dyn);  // x, f, gate
+  auto& memory = group_memory<WriteMemory<N, M>>(dyn, p, rows.bytes());
+  auto& small = memory.small;
+  auto& mixed = memory.mixed;
+  clear_small(p, small);
+  const auto copies = S::copies(a, p, false);
+  auto fetch_f = [&](int64_t t, int c) {
+    if (c >= chunks) return;
+    const T* f = static_cast<const T*>(a.f) + t * E + p.d0 + c * step;
 #pragma unroll
     for (int k = 0; k < M; ++k)
+      if (k < m) rows.fetch(c, N + k, f + k * D);
+  };
+  auto fetch_rest = [&](int64_t t, int c) {  // gate and x
+    if (c >= chunks) return;
+    const T* x = static_cast<const T*>(a.x) + t * n * D + p.d0 + c * step;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) pg[k][e] = z[k][e] = 0.f;
+    for (int k = 0; k < M; ++k)
+      if (a.gate && k < m) rows.fetch(c, N + M + k, static_cast<const T*>(a.gate) + t * E + p.d0 + c * step + k * D);
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      if (i >= n) break;
-      float gv[8];
-      gr[i].get(gv);
+    for (int j = 0; j < N; ++j)
+      if (j < n) rows.fetch(c, j, x + j * D);
+  };
+  walk_tokens(
+      p, a.T,
+      [&](int64_t t) {
 #pragma unroll
-      for (int k = 0; k < M; ++k) {
-        if (k >= m) break;
-        const float w = __ldg(W + i * m + k);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) pg[k][e] = fmaf(w, gv[e], pg[k][e]);
-      }
-    }
-#pragma unroll
-    for (int k = 0; k < M; ++k) {
-      if (k >= m || !p.live) continue;
-      const int64_t c = k * D + p.d0;
-      float fac[8], xh[8], w[8], b[8], sc[8];
-#pragma unroll
-      for (int e = 0; e < 8; ++e) fac[e] = 1.f;
-      if (a.drop.on) {
-        keep8(a.drop, key, static_cast<uint64_t>(t * E + c), fac);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) pg[k][e] = fac[e] != 0.f ? pg[k][e] * fac[e] : 0.f;
-      }
-      fr[k].get(xh);
-      param8(a.weight, c, true, 1.f, w);
-      param8(a.bias, c, true, 0.f, b);
-      param8(a.scale, c, true, 1.f, sc);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        xh[e] = (xh[e] - mean) * rstd;
-        b[e] = fmaf(xh[e], w[e], b[e]);  // weight xhat + bias
-      }
-      if (gate) {
-        float ga[8], gd[8];
-        ar[k].get(ga);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const float v = gate_value(a.gate_act, ga[e]);
-          gd[e] = pg[k][e] * sc[e] * b[e] * (a.gate_act == HC_ACT_SIGMOID ? v * (1.f - v) : 1.f);
-          pg[k][e] *= v;
-          b[e] *= v;
+        for (int c = 0; c < CH; ++c) {
+          fetch_f(t, c);
+          fetch_rest(t, c);
         }
-        if (a.grad_gate) put8<T>(static_cast<T*>(a.grad_gate) + t * E + c, gd);
-      }
+      },
+      [&](int64_t t, int slot) { copies.fetch(small[slot], t); },
+      [&](int slot) {
+        if (a.v) S::project(p, small[slot], mixed[0]);
+      },
+      [&](int64_t t, int64_t next, int slot, int parity) {
+        V8 z[CH][M];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        z[k][e] = fac[e] != 0.f ? sc[e] * b[e] * fac[e] : 0.f;
-        A[k][e] = fmaf(pg[k][e], xh[e], A[k][e]);
-        B[k][e] += pg[k][e];
-        pg[k][e] *= sc[e] * w[e];  // q
-        s[0] = fmaf(pg[k][e], xh[e], s[0]);
-        s[1] += pg[k][e];
-      }
-    }
-    fold_to<2>(s, p.lane, red[buf][p.slot()]);
-    p.sync();
-    flush(last, buf ^ 1);
-    if (a.grad_f && p.live) {
-      float c1 = 0.f, c2 = 0.f;
-      for (int w = 0; w < p.W; ++w) {
-        c1 += red[buf][p.slot0() + w][0];
-        c2 += red[buf][p.slot0() + w][1];
-      }
-      c1 /= static_cast<float>(E);
-      c2 = a.norm == HC_NORM_LAYER ? c2 / static_cast<float>(E) : 0.f;
+        for (int c = 0; c < CH; ++c) {
 #pragma unroll
-      for (int k = 0; k < M; ++k) {
-        if (k >= m) break;
-        if (a.norm != HC_NORM_NONE) {  // without a norm f's value plays no part, be it a NaN
-          float xh[8];
-          fr[k].get(xh);
-#pragma unroll
-          for (int e = 0; e < 8; ++e) pg[k][e] = rstd * (pg[k][e] - c2 - (xh[e] - mean) * rstd * c1);
+          for (int k = 0; k < M; ++k) z[c][k] = rows.get(c, N + k);
+          if (next < a.T) fetch_f(next, c);
         }
-        put8<T>(static_cast<T*>(a.grad_f) + t * E + k * D + p.d0, pg[k]);
-      }
-    }
-    // grad_x = Heff^T g; g x^T, g z^T
-    float xv[N][8], gx[N][8] = {}, acc[GB], accW[N * M];
-#pragma unroll
-    for (int j = 0; j < N; ++j) xr[j].get(xv[j]);
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      float gv[8];
-      gr[i].get(gv);
-#pragma unroll
-      for (int j = 0; j < N; ++j) {
-        float r = 0.f;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) r = fmaf(gv[e], xv[j][e], r);
-        acc[(i * N + j) % GB] = r;
-        if (i < n && j < n) {
-          const float h = sH[buf][p.group][i * N + j];
-#pragma unroll
-          for (int e = 0; e < 8; ++e) gx[j][e] = fmaf(h, gv[e], gx[j][e]);
+        float mean = 0.f, rstd = 1.f;
+        if (a.norm != HC_NORM_NONE) {
+          group_stats<CH, M, MAXW>(p, z, chunks, m, a.norm, a.eps, inv, red[parity], mean, rstd);
+          if (a.stats && p.tid == 0) *reinterpret_cast<float2*>(a.stats + 2 * t) = make_float2(mean, rstd);
+        } else {
+          p.sync();
         }
+        const f2* s = small[slot];
+        if (a.v) S::project(p, small[(slot + 1) & (kSmallSlots - 1)], mixed[parity ^ 1]);
+        const f2* H = a.v ? mixed[parity] : s;
+        const f2 less = both(-mean), r2 = both(rstd);
+#pragma unroll
+        for (int c = 0; c < CH; ++c) {
+#pragma unroll
+          for (int k = 0; k < M; ++k) {
+            if (M > 1 && k >= m) {  // a block that does not exist
+              z[c][k].fill(0.f);
+              continue;
+            }
+            const int64_t col = k * D + p.d0 + c * step;
+            V8 ws, bs;
+            scaled_params(a, col, c < chunks, ws, bs);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) z[c][k].v[i] = fma2(mul2(add2(z[c][k].v[i], less), r2), ws.v[i], bs.v[i]);
+            if (a.gate) {
+              V8 val, der;
+              gate8(a.gate_act, rows.get(c, N + M + k), val, der);
+#pragma unroll
+              for (int i = 0; i < 4; ++i) z[c][k].v[i] = mul2(z[c][k].v[i], val.v[i]);
+            }
+            if (a.drop.on) {
+              uint32_t keep[8];
+              keep8(a.drop, key, static_cast<uint64_t>(t * E + col), keep);
+              keep_mul(z[c][k], a.drop.scale, keep);
+            }
+          }
+          V8 x[N];
+#pragma unroll
+          for (int j = 0; j < N; ++j) x[j] = rows.get(c, j);
+          if (next < a.T) fetch_rest(next, c);
+          T* out = static_cast<T*>(a.out) + t * n * D + p.d0 + c * step;
+#pragma unroll
+          for (int i = 0; i < N; ++i) {
+            V8 r;
+            r.fill(0.f);
+#pragma unroll
+            for (int j = 0; j < N; ++j) axpy(H[i * N + j], x[j], r);
+#pragma unroll
+            for (int k = 0; k < M; ++k) axpy(s[S::kW + i * M + k], z[c][k], r);
+            if (c < chunks && i < n) put8<T>(out + i * D, r);
+          }
+        }
+        __syncwarp();
+      });
+}
+
+template <typename T, int N, int M, int CH>
+__global__ void __launch_bounds__(norm_bwd_threads(N, M, sizeof(T)))
+    write_norm_bwd_kernel(const __grid_constant__ NormArgs a, int warps) {
+  static_assert(CH == 1, "the backward's threads own one chunk");
+  constexpr int MAXW = norm_bwd_threads(N, M, sizeof(T)) / 32;
+  constexpr int GB = N * N < 32 ? N * N : 32, G = N * N + N * M;  // H's sums [column][row] by batches of GB, then W's
+  using S = Small<N, M, true>;
+  extern __shared__ __align__(16) uint8_t dyn[];
+  __shared__ float red[2][MAXW][2], gram[2][MAXW][G];
+  const Place p(warps, a.D);
+  const int n = a.n, m = a.m;
+  const int64_t D = a.D, E = D * m;
+  const float inv = 1.f / static_cast<float>(E);
+  const DropKey key = a.drop.on ? drop_key(a.drop) : DropKey{};
+  const Rows<T, 2 * N + 2 * M, 1> rows(dyn);  // g, x, f, gate
+  auto& memory = group_memory<WriteMemory<N, M>>(dyn, p, rows.bytes());
+  auto& small = memory.small;
+  auto& mixed = memory.mixed;
+  clear_small(p, small);
+  const auto copies = S::copies(a, p, a.norm != HC_NORM_NONE);
+  const SmallGrads<(G + 31) / 32> grads(p, G, [&](int id, float*& out, int& stride) {
+    if (id < N * N) {
+      const int c = id / N, r = id % N;
+      if (a.grad_H && r < n && c < n) out = a.grad_H + r * n + c;
+      stride = n * n;
+      if (a.v) {  // first to the projection's gradients
+        out = memory.G + r * N + c;
+        stride = 0;
       }
-#pragma unroll
-      for (int k = 0; k < M; ++k) {
-        float r = 0.f;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) r = fmaf(gv[e], z[k][e], r);
-        accW[i * M + k] = r;
-      }
-      if ((i + 1) * N % GB == 0) fold_to<GB>(acc, p.lane, &gram[buf][p.slot()][(i + 1) * N - GB]);
+    } else {
+      const int r = (id - N * N) / M, k = (id - N * N) % M;
+      if (a.grad_W && r < n && k < m) out = a.grad_W + r * m + k;
+      stride = n * m;
     }
-    fold_to<N * M>(accW, p.lane, &gram[buf][p.slot()][N * N]);
-    if (a.grad_x && p.live) {
-      T* dst = static_cast<T*>(a.grad_x) + t * n * D + p.d0;
+  });
+  V8 A[1][M], B[1][M];
 #pragma unroll
-      for (int j = 0; j < N; ++j)
-        if (j < n) put8<T>(dst + j * D, gx[j]);
-    }
-    last = t;
+  for (int k = 0; k < M; ++k) {
+    A[0][k].fill(0.f);
+    B[0][k].fill(0.f);
   }
+  int64_t last = -1;
+  int last_parity = 0, last_slot = 0;
+  // grad_H, grad_v and grad_W of the last token, whose warps' sums lie in the other buffer
+  auto flush = [&] {
+    if (last < 0) return;
+    grads.store(p, last, [&](int q, int id) { return gram[last_parity][p.slot0() + q][id]; });
+    if (a.v) {
+      p.sync();
+      S::grads(a, p, small[last_slot], memory.G, last);
+    }
+  };
+  auto fetch_outer = [&](int64_t t) {  // g, x and gate
+    if (!p.live) return;
+    const int64_t xo = t * n * D + p.d0;
+    const T *g = static_cast<const T*>(a.g) + xo, *x = static_cast<const T*>(a.x) + xo;
+#pragma unroll
+    for (int j = 0; j < N; ++j)
+      if (j < n) rows.fetch(0, j, g + j * D);
+#pragma unroll
+    for (int k = 0; k < M; ++k)
+      if (a.gate && k < m) rows.fetch(0, 2 * N + M + k, static_cast<const T*>(a.gate) + t * E + p.d0 + k * D);
+#pragma unroll
+    for (int j = 0; j < N; ++j)
+      if (j < n) rows.fetch(0, N + j, x + j * D);
+  };
+  auto fetch_f = [&](int64_t t) {
+    if (!p.live) return;
+    const T* f = static_cast<const T*>(a.f) + t * E + p.d0;
+#pragma unroll
+    for (int k = 0; k < M; ++k)
+      if (k < m) rows.fetch(0, 2 * N + k, f + k * D);
+  };
+  walk_tokens(
+      p, a.T,
+      [&](int64_t t) {
+        fetch_outer(t);
+        fetch_f(t);
+      },
+      [&](int64_t t, int slot) { copies.fetch(small[slot], t); },
+      [&](int slot) {
+        if (a.v) {
+          S::project(p, small[slot], mixed[0]);
+          p.sync();
+        }
+      },
+      [&](int64_t t, int64_t next, int slot, int parity) {
+        const f2* s = small[slot];
+        const f2* H = a.v ? mixed[parity] : s;
+        const f2 less = a.norm == HC_NORM_NONE ? both(0.f) : both(-one(s[S::kStats]));
+        const f2 r2 = a.norm == HC_NORM_NONE ? both(1.f) : s[S::kStats + 1];
+        __syncwarp();  // the other lanes' copies have arrived
+        // dz, from W^T g
+        V8 q[M];
+        {
+          V8 g[N];
+#pragma unroll
+          for (int k = 0; k < M; ++k) q[k].fill(0.f);
+#pragma unroll
+          for (int i = 0; i < N; ++i) {
+            g[i] = rows.get(0, i);
+#pragma unroll
+            for (int k = 0; k < M; ++k) axpy(s[S::kW + i * M + k], g[i], q[k]);
+          }
+          // a column of the mix at a time: grad_x_j = sum_i Heff_ij g_i, and for float32 streams g x_j
+          T* gx = static_cast<T*>(a.grad_x) + t * n * D + p.d0;
+          const bool store = a.grad_x && p.live;
+          float acc[GB];
+#pragma unroll
+          for (int j = 0; j < N; ++j) {
+            V8 r;
+            r.fill(0.f);
+#pragma unroll
+            for (int i = 0; i < N; ++i) axpy(H[j * N + i], g[i], r);
+            if (store && j < n) put8<T>(gx + j * D, r);
+            if constexpr (sizeof(T) == 4) {
+              const V8 x = rows.get(0, N + j);
+#pragma unroll
+              for (int i = 0; i < N; ++i) acc[(j * N + i) % GB] = dot(g[i], x);
+              if ((j + 1) * N % GB == 0) fold_to<GB>(acc, p.lane, &gram[parity][p.slot()][(j + 1) * N - GB]);
+            }
+          }
+        }
+        if constexpr (sizeof(T) == 2) {
+          float gsum[4] = {0.f, 0.f, 0.f, 0.f};
+          warp_gram<T, N>(rows, gsum);
+          store_gram<N>(gsum, p.lane, gram[parity][p.slot()]);
+        }
+        // dropout's and the gate's backward; z
+        f2 s1 = both(0.f), s2 = both(0.f);
+        V8 z[M];
+#pragma unroll
+        for (int k = 0; k < M; ++k) {
+          if (M > 1 && k >= m) {
+            z[k].fill(0.f);
+            continue;
+          }
+          const int64_t col = k * D + p.d0;
+          uint32_t keep[8];
+          if (a.drop.on) {
+            keep8(a.drop, key, static_cast<uint64_t>(t * E + col), keep);
+            keep_mul(q[k], a.drop.scale, keep);
+          }
+          V8 ws, bs, xh = rows.get(0, 2 * N + k);
+          scaled_params(a, col, p.live, ws, bs);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            xh.v[i] = mul2(add2(xh.v[i], less), r2);
+            z[k].v[i] = fma2(xh.v[i], ws.v[i], bs.v[i]);  // scale (weight xhat + bias)
+          }
+          if (a.gate) {
+            V8 val, der;
+            gate8(a.gate_act, rows.get(0, 2 * N + M + k), val, der);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              der.v[i] = mul2(der.v[i], mul2(q[k].v[i], z[k].v[i]));
+              q[k].v[i] = mul2(q[k].v[i], val.v[i]);
+              z[k].v[i] = mul2(z[k].v[i], val.v[i]);
+            }
+            if (a.grad_gate && p.live) put8<T>(static_cast<T*>(a.grad_gate) + t * E + col, der);
+          }
+          if (a.drop.on) keep_mul(z[k], a.drop.scale, keep);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            A[0][k].v[i] = fma2(q[k].v[i], xh.v[i], A[0][k].v[i]);
+            B[0][k].v[i] = add2(q[k].v[i], B[0][k].v[i]);
+            q[k].v[i] = mul2(q[k].v[i], ws.v[i]);
+            s1 = fma2(q[k].v[i], xh.v[i], s1);
+            s2 = add2(q[k].v[i], s2);
+          }
+        }
+        float sums[2] = {fold2(s1), fold2(s2)};  // g is 0 where there are no columns
+        fold_to<2>(sums, p.lane, red[parity][p.slot()]);
+        float accW[N * M];
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+          const V8 g = rows.get(0, i);  // again: held over the block's part above it costs the registers of two warps in five
+#pragma unroll
+          for (int k = 0; k < M; ++k) accW[i * M + k] = dot(g, z[k]);
+        }
+        fold_to<N * M>(accW, p.lane, &gram[parity][p.slot()][N * N]);
+        __syncwarp();  // warp_gram's reads are done before the next token's copies overwrite the rows
+        if (next < a.T) fetch_outer(next);
+        p.sync();
+        flush();
+        if (a.v) {  // the next token's mix, which its work begins with
+          S::project(p, small[(slot + 1) & (kSmallSlots - 1)], mixed[parity ^ 1]);
+          p.sync();
+        }
+        float c1 = 0.f, c2 = 0.f;
+        for (int i = 0; i < p.W; ++i) {
+          c1 += red[parity][p.slot0() + i][0];
+          c2 += red[parity][p.slot0() + i][1];
+        }
+        const f2 k1 = both(-c1 * inv), k2 = both(a.norm == HC_NORM_LAYER ? -c2 * inv : 0.f);
+        if (a.grad_f && p.live) {
+#pragma unroll
+          for (int k = 0; k < M; ++k) {
+            if (k >= m) break;
+            if (a.norm != HC_NORM_NONE) {  // without a norm f's value plays no part, be it a NaN
+              const V8 f = rows.get(0, 2 * N + k);
+#pragma unroll
+              for (int i = 0; i < 4; ++i)
+                q[k].v[i] = mul2(r2, fma2(mul2(add2(f.v[i], less), r2), k1, add2(q[k].v[i], k2)));
+            }
+            put8<T>(static_cast<T*>(a.grad_f) + t * E + k * D + p.d0, q[k]);
+          }
+        }
+        if (next < a.T) fetch_f(next);
+        last = t;
+        last_parity = parity;
+        last_slot = slot;
+      });
   p.sync();
-  flush(last, buf ^ 1);
-  store_param_sums<M>(a, p, A, B);
+  flush();
+  store_param_sums<1, M>(a, p, p.live ? 1 : 0, A, B);
 }
 
 // ------------------------------------------------------------------- host
 using NormKernel = void (*)(NormArgs, int);
 
-template <typename T, bool WRITE, int N, int M> NormKernel norm_kernel(bool bwd) {
-  if constexpr (WRITE)
-    return bwd ? write_norm_bwd_kernel<T, N, M> : write_norm_fwd_kernel<T, N, M>;
-  else
-    return bwd ? read_norm_bwd_kernel<T, N, M> : read_norm_fwd_kernel<T, N, M>;
-}
+inline int padded_streams(int n) { return n <= 1 ? 1 : n <= 2 ? 2 : n <= 4 ? 4 : 8; }
+inline int padded_blocks(int m) { return m <= 1 ? 1 : m <= 2 ? 2 : 4; }
 
-// The kernel for n streams and m blocks: the next larger of 1, 2, 4, 8 and of
-// 1, 2, 4 (rows past n and m are neither read nor written); nullptr for more
-// blocks than streams, which the element kernels take.
-template <typename T, bool WRITE> NormKernel norm_kernel_for(bool bwd, int n, int m) {
-  if (n == 1) return m == 1 ? norm_kernel<T, WRITE, 1, 1>(bwd) : nullptr;
-  if (n == 2) return m == 1 ? norm_kernel<T, WRITE, 2, 1>(bwd) : m == 2 ? norm_kernel<T, WRITE, 2, 2>(bwd) : nullptr;
-  if (n <= 4)
-    return m == 1   ? norm_kernel<T, WRITE, 4, 1>(bwd)
-           : m == 2 ? norm_kernel<T, WRITE, 4, 2>(bwd)
-                    : norm_kernel<T, WRITE, 4, 4>(bwd);
-  return m == 1   ? norm_kernel<T, WRITE, 8, 1>(bwd)
-         : m == 2 ? norm_kernel<T, WRITE, 8, 2>(bwd)
-                  : norm_kernel<T, WRITE, 8, 4>(bwd);
+// Shared memory of a CTA: its threads' rows and its groups' small matrices.
+inline int64_t norm_smem_bytes(bool write, bool bwd, int N, int M, int chunks, int threads, int groups, int esize) {
+  const int rows = write ? (bwd ? 2 * N : N) + 2 * M : N + (bwd ? M : 0);
+  const int64_t entries = write ? (N * N + N * M + N + 3) / 2 * 2 : N * M + 2;
+  const int64_t group = (entries * 8 * kSmallSlots + (write ? N * N * 20 : 0) + 15) / 16 * 16;
+  return static_cast<int64_t>(rows * esize / 2) * chunks * (16 * threads + 16) + groups * group;
 }
+static_assert(sizeof(ReadMemory<8, 4>) == (34 * 8 * kSmallSlots + 15) / 16 * 16);
+static_assert(sizeof(WriteMemory<8, 4>) == (106 * 8 * kSmallSlots + 64 * 20 + 15) / 16 * 16);
+static_assert(sizeof(WriteMemory<1, 1>) == (6 * 8 * kSmallSlots + 20 + 15) / 16 * 16);
 
-// CTAs that fit on the device at once.
-inline int norm_resident(NormKernel k, int threads) {
-  int per_sm = 0;
-  if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, k, threads, 0) != cudaSuccess || per_sm < 1) {
-    cudaGetLastError();
-    per_sm = 1;
+// The kernel for n streams, m blocks and ch chunks a thread: the next larger of
+// 1, 2, 4, 8 and of 1, 2, 4 (rows past n and m are neither read nor written).
+template <typename T, bool WRITE, bool BWD, int N, int M, int CH> NormKernel norm_kernel_of() {
+  if constexpr (WRITE && BWD) return write_norm_bwd_kernel<T, N, M, CH>;
+  if constexpr (WRITE && !BWD) return write_norm_fwd_kernel<T, N, M, CH>;
+  if constexpr (!WRITE && BWD) return read_norm_bwd_kernel<T, N, M, CH>;
+  if constexpr (!WRITE && !BWD) return read_norm_fwd_kernel<T, N, M, CH>;
+}
+template <typename T, bool WRITE, int N, int M> NormKernel norm_kernel_for(bool bwd, int ch) {
+  if (bwd) return norm_kernel_of<T, WRITE, true, N, M, 1>();
+  if constexpr (norm_fwd_chunks(N, M, sizeof(T)) >= 3) {
+    if (ch == 3) return norm_kernel_of<T, WRITE, false, N, M, 3>();
+    if (ch == 2) return norm_kernel_of<T, WRITE, false, N, M, 2>();
   }
-  return per_sm * sm_count();
+  return norm_kernel_of<T, WRITE, false, N, M, 1>();
+}
+template <typename T, bool WRITE> NormKernel norm_kernel(bool bwd, int n, int m, int ch) {
+#define HC_NM(N, M) norm_kernel_for<T, WRITE, N, M>(bwd, ch)
+  if (n == 1) return HC_NM(1, 1);
+  if (n == 2) return m == 1 ? HC_NM(2, 1) : HC_NM(2, 2);
+  if (n <= 4) return m == 1 ? HC_NM(4, 1) : m == 2 ? HC_NM(4, 2) : HC_NM(4, 4);
+  return m == 1 ? HC_NM(8, 1) : m == 2 ? HC_NM(8, 2) : HC_NM(8, 4);
+#undef HC_NM
+}
+
+// Warps of a token's group, and for the forward the chunks a thread owns; 0
+// warps where the 8-column kernels do not take the shape (rows that are not
+// whole chunks or do not fit a CTA, more blocks than streams).
+inline NormGeometry norm_geometry(bool write, bool bwd, int n, int m, int64_t D, int esize) {
+  NormGeometry g{};
+  const int N = padded_streams(n), M = padded_blocks(m);
+  if (D % kColumns != 0 || M > N) return g;
+  const int64_t lines = (D + 32 * kColumns - 1) / (32 * kColumns);  // warps with a chunk a thread
+  const int most = bwd ? 1 : norm_fwd_chunks(N, M, esize);
+  g.chunks = static_cast<int>(lines < most ? lines : most);
+  const int64_t warps = (lines + g.chunks - 1) / g.chunks;
+  const int groups = warps == 1 ? kSmallGroups : 1;
+  if (32 * warps * groups > (bwd ? norm_bwd_threads(N, M, esize) : norm_fwd_threads(N, M, g.chunks, esize)) ||
+      norm_smem_bytes(write, bwd, N, M, g.chunks, static_cast<int>(32 * warps * groups), groups, esize) > kNormSmemMax)
+    return g;
+  g.warps = static_cast<int>(warps);
+  return g;
 }
 
 template <typename T, bool WRITE>
 int norm_launch(bool bwd, NormGeometry& geo, const NormArgs& a, cudaStream_t s) {
-  const NormKernel k = geo.warps > 0 ? norm_kernel_for<T, WRITE>(bwd, a.n, a.m) : nullptr;
-  if (!k) return norm_launch_elem<T>(WRITE, bwd, geo, a, s);
+  if (geo.warps == 0) return norm_launch_elem<T>(WRITE, bwd, geo, a, s);
   const int groups = geo.warps == 1 ? kSmallGroups : 1, threads = 32 * geo.warps * groups;
-  const int64_t want = (a.T + groups - 1) / groups;
-  const int most = norm_resident(k, threads);
+  const NormKernel k = norm_kernel<T, WRITE>(bwd, a.n, a.m, geo.chunks);
+  const int smem = static_cast<int>(norm_smem_bytes(WRITE, bwd, padded_streams(a.n), padded_blocks(a.m), geo.chunks,
+                                                    threads, groups, sizeof(T)));
+  int per_sm = 0;
+  if (cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, kNormSmemMax) != cudaSuccess ||
+      cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, k, threads, smem) != cudaSuccess || per_sm < 1) {
+    cudaGetLastError();
+    return HC_ERR_LAUNCH;
+  }
+  const int64_t want = (a.T + groups - 1) / groups, most = static_cast<int64_t>(per_sm) * sm_count();
   geo.grid = static_cast<int>(want < most ? want : most);
   geo.rows = geo.grid * groups;
-  k<<<geo.grid, threads, 0, s>>>(a, geo.warps);
+  k<<<geo.grid, threads, smem, s>>>(a, geo.warps);
   return launch_status();
 }
 
