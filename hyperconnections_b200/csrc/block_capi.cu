@@ -61,30 +61,50 @@ int launch(int sdt, bool write, bool bwd, NormGeometry& g, const NormArgs& a, cu
 }
 
 // ------------------------------------------------ the [E] parameters' grads
-// A = sum over rows of partial[.][0][c], B of partial[.][1][c]: a CTA takes 32
-// columns, its 32 warps every 32nd row, and the warps' sums are added in order,
-// so the result does not depend on timing.
-constexpr int kParamWarps = 32;
+// A = sum over rows of partial[.][0][c], B of partial[.][1][c]: a CTA takes 8
+// columns (so that narrow blocks fill the device too) and 128 rows at a time,
+// eight loads of each in flight; the lanes' and warps' sums are added in a
+// fixed order, so the result does not depend on timing.
+constexpr int kParamCols = 8, kParamThreads = 1024, kParamLines = kParamThreads / kParamCols;
 
-__global__ void __launch_bounds__(32 * kParamWarps)
+__global__ void __launch_bounds__(kParamThreads)
     norm_param_grads_kernel(const float* partial, int rows, int64_t E, const float* weight, const float* bias,
                             const float* scale, float* gw, float* gb, float* gs) {
-  __shared__ float sA[kParamWarps][32], sB[kParamWarps][32];
-  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
-  const int64_t c = static_cast<int64_t>(blockIdx.x) * 32 + lane;
+  __shared__ float sA[kParamThreads / 32][kParamCols], sB[kParamThreads / 32][kParamCols];
+  const int col = threadIdx.x % kParamCols, line = threadIdx.x / kParamCols;
+  const int64_t c = static_cast<int64_t>(blockIdx.x) * kParamCols + col;
   float A = 0.f, B = 0.f;
-  if (c < E)
-    for (int r = w; r < rows; r += kParamWarps) {
-      A += partial[static_cast<int64_t>(r) * 2 * E + c];
-      B += partial[static_cast<int64_t>(r) * 2 * E + E + c];
+  constexpr int kBatch = 8;
+  for (int r0 = line; r0 < rows; r0 += kBatch * kParamLines) {
+    float a[kBatch], b[kBatch];
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) {
+      const int r = r0 + i * kParamLines;
+      const bool ok = c < E && r < rows;
+      a[i] = ok ? __ldg(partial + static_cast<int64_t>(r) * 2 * E + c) : 0.f;
+      b[i] = ok ? __ldg(partial + static_cast<int64_t>(r) * 2 * E + E + c) : 0.f;
     }
-  sA[w][lane] = A;
-  sB[w][lane] = B;
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) {
+      A += a[i];
+      B += b[i];
+    }
+  }
+#pragma unroll
+  for (int o = 16; o >= kParamCols; o >>= 1) {
+    A += __shfl_xor_sync(kFull, A, o);
+    B += __shfl_xor_sync(kFull, B, o);
+  }
+  if ((threadIdx.x & 31) < kParamCols) {
+    sA[threadIdx.x >> 5][col] = A;
+    sB[threadIdx.x >> 5][col] = B;
+  }
   __syncthreads();
-  if (w != 0 || c >= E) return;
-  for (int i = 1; i < kParamWarps; ++i) {
-    A += sA[i][lane];
-    B += sB[i][lane];
+  if (threadIdx.x >= kParamCols || c >= E) return;
+  A = B = 0.f;
+  for (int i = 0; i < kParamThreads / 32; ++i) {
+    A += sA[i][col];
+    B += sB[i][col];
   }
   const float sc = scale ? scale[c] : 1.f;
   if (gw) gw[c] = sc * A;
@@ -96,7 +116,7 @@ __global__ void __launch_bounds__(32 * kParamWarps)
 
 int norm_param_grads(const float* partial, int rows, int64_t E, const float* weight, const float* bias,
                      const float* scale, float* grad_weight, float* grad_bias, float* grad_scale, cudaStream_t s) {
-  norm_param_grads_kernel<<<static_cast<unsigned>((E + 31) / 32), 32 * kParamWarps, 0, s>>>(
+  norm_param_grads_kernel<<<static_cast<unsigned>((E + kParamCols - 1) / kParamCols), kParamThreads, 0, s>>>(
       partial, rows, E, weight, bias, scale, grad_weight, grad_bias, grad_scale);
   return launch_status();
 }

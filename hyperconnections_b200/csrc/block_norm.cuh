@@ -44,11 +44,11 @@ constexpr int kSmallSlots = 8;   // tokens whose small matrices are held (5 are 
 constexpr int kNormSmemMax = 210 * 1024;  // of the 227 KB a CTA can have; up to 10 KB are static
 
 // Threads of a CTA at most, which bounds the registers of one.
-constexpr int norm_bwd_threads(int N, int M, int esize) { return M >= 2 || N == 8 || (N == 4 && esize == 4) ? 256 : 512; }
+constexpr int norm_bwd_threads(int N, int M, int esize) { return M >= 4 || (N == 8 && esize == 4) ? 256 : M == 2 || N == 8 ? 384 : 512; }
 // Chunks a thread may own in the forward (a token's rows then need fewer warps,
 // down to one without barriers): as many as keep a block's rows in registers.
-constexpr int norm_fwd_chunks(int N, int M, int esize) { return M == 1 && N <= 4 && esize == 2 ? 3 : 1; }
-constexpr int norm_fwd_threads(int N, int M, int CH, int esize) { return CH > 1 || (N == 8 && M > 1) ? 384 : 512; }
+constexpr int norm_fwd_chunks(bool write, int N, int M, int esize) { return 1; }
+constexpr int norm_fwd_threads(int N, int M, int CH, int esize) { return M >= 4 || CH > 1 ? 384 : 640; }
 
 // ------------------------------------------------------- pairs of float32
 using f2 = unsigned long long;
@@ -80,6 +80,18 @@ __device__ __forceinline__ f2 add2(f2 a, f2 b) {
   return r;
 }
 
+// K pairs of a row of a small matrix, loaded where they are used: kept for both
+// halves of the columns, a mix of 8 streams alone would fill the registers.
+template <int K> __device__ __forceinline__ void pairs(const f2* p, f2 (&v)[K]) {
+  const uint32_t at = static_cast<uint32_t>(__cvta_generic_to_shared(p));
+  if constexpr (K == 1) {
+    asm volatile("ld.shared.b64 %0, [%1];" : "=l"(v[0]) : "r"(at));
+  } else {
+#pragma unroll
+    for (int i = 0; i < K; i += 2) asm volatile("ld.shared.v2.b64 {%0, %1}, [%2];" : "=l"(v[i]), "=l"(v[i + 1]) : "r"(at + 8 * i));
+  }
+}
+
 struct V8 {  // eight columns
   f2 v[4];
   __device__ __forceinline__ void fill(float a) {
@@ -99,6 +111,28 @@ __device__ __forceinline__ void axpy(f2 aa, const V8& x, V8& y) {
 }
 
 template <typename T> constexpr int kWords = sizeof(T) / 2;  // 16-byte words of eight columns
+
+// Four of the eight columns: the products with all rows at once are done by
+// halves where N rows of eight would not leave registers for more warps.
+struct V4 {
+  f2 v[2];
+};
+__device__ __forceinline__ void axpy(f2 aa, const V4& x, V4& y) {
+  y.v[0] = fma2(aa, x.v[0], y.v[0]);
+  y.v[1] = fma2(aa, x.v[1], y.v[1]);
+}
+template <typename T> __device__ __forceinline__ void put4(T* p, const V4& r) {
+  float f[4];
+  split(r.v[0], f[0], f[1]);
+  split(r.v[1], f[2], f[3]);
+  if constexpr (sizeof(T) == 4) {
+    st_v4(p, pack<float>(f));
+  } else {
+    const float g[8] = {f[0], f[1], f[2], f[3], 0.f, 0.f, 0.f, 0.f};
+    const uint4 q = pack<T>(g);
+    asm volatile("st.global.v2.u32 [%0], {%1, %2};" ::"l"(p), "r"(q.x), "r"(q.y) : "memory");
+  }
+}
 
 template <typename T> __device__ __forceinline__ V8 expand(const uint4 (&q)[kWords<T>]) {
   float f[8];
@@ -295,27 +329,50 @@ __device__ __forceinline__ void group_stats(const Place& p, const V8 (&u)[CH][M]
 }
 
 // ------------------------------------------------------ the token's rows
-// A thread's words of ROWS rows of its CH chunks, at [chunk][row][word][thread].
-// A row's threads lie side by side (a warp's copies to scattered words took a
-// quarter more time), and a row ends with 16 bytes of padding, so that the
-// same thread's words of eight rows lie in different banks (warp_gram).
+// A thread's words of ROWS rows of its CH chunks, at
+// [warp][chunk][row][word][lane]. A row's lanes lie side by side (a warp's
+// copies to scattered words took a quarter more time), and a row ends with 16
+// bytes of padding, so that the same lane's words of eight rows lie in
+// different banks (warp_gram). All of a thread's addresses are one register and
+// a constant.
+constexpr int kRowPitch = 32 * 16 + 16;
 template <typename T, int ROWS, int CH> struct Rows {
   uint8_t* mem;
-  int base, pitch;
-  __device__ __forceinline__ Rows(uint8_t* smem) : mem(smem), base(threadIdx.x * 16), pitch(blockDim.x * 16 + 16) {
-    for (int i = 0; i < CH * ROWS * kWords<T>; ++i) *reinterpret_cast<uint4*>(mem + base + i * pitch) = make_uint4(0u, 0u, 0u, 0u);
+  int base;
+  __device__ __forceinline__ Rows(uint8_t* smem)
+      : mem(smem), base((threadIdx.x >> 5) * (CH * ROWS * kWords<T> * kRowPitch) + (threadIdx.x & 31) * 16) {
+    for (int i = 0; i < CH * ROWS * kWords<T>; ++i)
+      *reinterpret_cast<uint4*>(mem + base + i * kRowPitch) = make_uint4(0u, 0u, 0u, 0u);
   }
-  __device__ __forceinline__ int at(int c, int row) const { return base + (c * ROWS + row) * kWords<T> * pitch; }
-  __device__ __forceinline__ int bytes() const { return CH * ROWS * kWords<T> * pitch; }
+  __device__ __forceinline__ int at(int c, int row) const { return base + (c * ROWS + row) * kWords<T> * kRowPitch; }
+  __device__ __forceinline__ int bytes() const { return (blockDim.x >> 5) * (CH * ROWS * kWords<T> * kRowPitch); }
   __device__ __forceinline__ void fetch(int c, int row, const T* src) const {
     const uint32_t dst = shared_addr(mem) + at(c, row);
 #pragma unroll
-    for (int i = 0; i < kWords<T>; ++i) copy16(dst + i * pitch, src + i * (16 / sizeof(T)));
+    for (int i = 0; i < kWords<T>; ++i) copy16(dst + i * kRowPitch, src + i * (16 / sizeof(T)));
+  }
+  // Rows row .. row + K - 1 of a chunk, of which the first `count` exist, D elements apart.
+  template <int K> __device__ __forceinline__ void fetch_rows(int c, int row, const T* src, int count, int64_t D) const {
+#pragma unroll
+    for (int j = 0; j < K; ++j) {
+      if (j < count) fetch(c, row + j, src);
+      src += D;
+    }
+  }
+  __device__ __forceinline__ V4 half(int c, int row, int h) const {  // columns 4 h .. 4 h + 3
+    float f[8];
+    if constexpr (kWords<T> == 2) {
+      unpack<T>(*reinterpret_cast<const uint4*>(mem + at(c, row) + h * kRowPitch), f);
+    } else {
+      const uint2 q = *reinterpret_cast<const uint2*>(mem + at(c, row) + h * 8);
+      unpack<T>(make_uint4(q.x, q.y, 0u, 0u), f);
+    }
+    return V4{{pair(f[0], f[1]), pair(f[2], f[3])}};
   }
   __device__ __forceinline__ V8 get(int c, int row) const {
     uint4 q[kWords<T>];
 #pragma unroll
-    for (int i = 0; i < kWords<T>; ++i) q[i] = *reinterpret_cast<const uint4*>(mem + at(c, row) + i * pitch);
+    for (int i = 0; i < kWords<T>; ++i) q[i] = *reinterpret_cast<const uint4*>(mem + at(c, row) + i * kRowPitch);
     return expand<T>(q);
   }
 };
@@ -466,9 +523,7 @@ __global__ void __launch_bounds__(norm_fwd_threads(N, M, CH, sizeof(T)))
   auto fetch = [&](int64_t t, int c) {
     if (c >= chunks) return;
     const T* x = static_cast<const T*>(a.x) + t * n * D + p.d0 + c * step;
-#pragma unroll
-    for (int j = 0; j < N; ++j)
-      if (j < n) rows.fetch(c, j, x + j * D);
+    rows.template fetch_rows<N>(c, 0, x, n, D);
   };
   walk_tokens(
       p, a.T,
@@ -554,16 +609,12 @@ __global__ void __launch_bounds__(norm_bwd_threads(N, M, sizeof(T)))
   auto fetch_x = [&](int64_t t) {
     if (!p.live) return;
     const T* x = static_cast<const T*>(a.x) + t * n * D + p.d0;
-#pragma unroll
-    for (int j = 0; j < N; ++j)
-      if (j < n) rows.fetch(0, j, x + j * D);
+    rows.template fetch_rows<N>(0, 0, x, n, D);
   };
   auto fetch_g = [&](int64_t t) {
     if (!p.live) return;
     const T* g = static_cast<const T*>(a.g) + t * E + p.d0;
-#pragma unroll
-    for (int k = 0; k < M; ++k)
-      if (k < m) rows.fetch(0, N + k, g + k * D);
+    rows.template fetch_rows<M>(0, N, g, m, D);
   };
   walk_tokens(
       p, a.T,
@@ -623,7 +674,8 @@ __global__ void __launch_bounds__(norm_bwd_threads(N, M, sizeof(T)))
           r.fill(0.f);
 #pragma unroll
           for (int k = 0; k < M; ++k) axpy(R[j * M + k], u[k], r);
-          if (store && j < n) put8<T>(gx + j * D, r);
+          if (store && j < n) put8<T>(gx, r);
+          gx += D;
           const V8 x = rows.get(0, j);  // 0 where there are no columns
 #pragma unroll
           for (int k = 0; k < M; ++k) acc[j * M + k] = dot(u[k], x);
@@ -742,7 +794,7 @@ template <int N, int M, bool TRANSPOSED> struct Small {
 
 template <int N, int M> struct WriteMemory {
   alignas(16) f2 small[kSmallSlots][Small<N, M, true>::kEntries];
-  f2 mixed[2][N * N];  // H + (v - H v) v^T of this token and the next
+  alignas(16) f2 mixed[2][N * N];  // H + (v - H v) v^T of this token and the next
   float G[N * N];
 };
 
@@ -756,7 +808,7 @@ __device__ __forceinline__ void warp_gram(const R& rows, float (&c)[4]) {
   const int lane = threadIdx.x & 31;
   // matrices 0, 1: rows g of an even and an odd lane's columns; 2, 3: rows x
   const uint32_t addr = shared_addr(rows.mem) + rows.at(0, 0) - lane * 16 + ((lane >> 3) & 1) * 16 +
-                        static_cast<uint32_t>(((lane >> 4) * N + (lane & 7) % N) * rows.pitch);
+                        static_cast<uint32_t>(((lane >> 4) * N + (lane & 7) % N) * kRowPitch);
 #pragma unroll
   for (int l = 0; l < 32; l += 2) {
     uint32_t g0, g1, x0, x1;
@@ -817,19 +869,13 @@ __global__ void __launch_bounds__(norm_fwd_threads(N, M, CH, sizeof(T)))
   auto fetch_f = [&](int64_t t, int c) {
     if (c >= chunks) return;
     const T* f = static_cast<const T*>(a.f) + t * E + p.d0 + c * step;
-#pragma unroll
-    for (int k = 0; k < M; ++k)
-      if (k < m) rows.fetch(c, N + k, f + k * D);
+    rows.template fetch_rows<M>(c, N, f, m, D);
   };
   auto fetch_rest = [&](int64_t t, int c) {  // gate and x
     if (c >= chunks) return;
     const T* x = static_cast<const T*>(a.x) + t * n * D + p.d0 + c * step;
-#pragma unroll
-    for (int k = 0; k < M; ++k)
-      if (a.gate && k < m) rows.fetch(c, N + M + k, static_cast<const T*>(a.gate) + t * E + p.d0 + c * step + k * D);
-#pragma unroll
-    for (int j = 0; j < N; ++j)
-      if (j < n) rows.fetch(c, j, x + j * D);
+    if (a.gate) rows.template fetch_rows<M>(c, N + M, static_cast<const T*>(a.gate) + t * E + p.d0 + c * step, m, D);
+    rows.template fetch_rows<N>(c, 0, x, n, D);
   };
   walk_tokens(
       p, a.T,
@@ -888,21 +934,33 @@ __global__ void __launch_bounds__(norm_fwd_threads(N, M, CH, sizeof(T)))
               keep_mul(z[c][k], a.drop.scale, keep);
             }
           }
-          V8 x[N];
-#pragma unroll
-          for (int j = 0; j < N; ++j) x[j] = rows.get(c, j);
-          if (next < a.T) fetch_rest(next, c);
           T* out = static_cast<T*>(a.out) + t * n * D + p.d0 + c * step;
+#pragma unroll 1  // one half's registers at a time
+          for (int h = 0; h < 2; ++h) {
+            V4 x[N], zh[M];
 #pragma unroll
-          for (int i = 0; i < N; ++i) {
-            V8 r;
-            r.fill(0.f);
+            for (int k = 0; k < M; ++k) {
+              zh[k].v[0] = h ? z[c][k].v[2] : z[c][k].v[0];
+              zh[k].v[1] = h ? z[c][k].v[3] : z[c][k].v[1];
+            }
 #pragma unroll
-            for (int j = 0; j < N; ++j) axpy(H[i * N + j], x[j], r);
+            for (int j = 0; j < N; ++j) x[j] = rows.half(c, j, h);
+            T* dst = out + 4 * h;
 #pragma unroll
-            for (int k = 0; k < M; ++k) axpy(s[S::kW + i * M + k], z[c][k], r);
-            if (c < chunks && i < n) put8<T>(out + i * D, r);
+            for (int i = 0; i < N; ++i) {
+              V4 r{{both(0.f), both(0.f)}};
+              f2 hi[N], wi[M];
+              pairs<N>(H + i * N, hi);
+              pairs<M>(s + S::kW + i * M, wi);
+#pragma unroll
+              for (int j = 0; j < N; ++j) axpy(hi[j], x[j], r);
+#pragma unroll
+              for (int k = 0; k < M; ++k) axpy(wi[k], zh[k], r);
+              if (c < chunks && i < n) put4<T>(dst, r);
+              dst += D;
+            }
           }
+          if (next < a.T) fetch_rest(next, c);
         }
         __syncwarp();
       });
@@ -964,22 +1022,14 @@ __global__ void __launch_bounds__(norm_bwd_threads(N, M, sizeof(T)))
     if (!p.live) return;
     const int64_t xo = t * n * D + p.d0;
     const T *g = static_cast<const T*>(a.g) + xo, *x = static_cast<const T*>(a.x) + xo;
-#pragma unroll
-    for (int j = 0; j < N; ++j)
-      if (j < n) rows.fetch(0, j, g + j * D);
-#pragma unroll
-    for (int k = 0; k < M; ++k)
-      if (a.gate && k < m) rows.fetch(0, 2 * N + M + k, static_cast<const T*>(a.gate) + t * E + p.d0 + k * D);
-#pragma unroll
-    for (int j = 0; j < N; ++j)
-      if (j < n) rows.fetch(0, N + j, x + j * D);
+    rows.template fetch_rows<N>(0, 0, g, n, D);
+    if (a.gate) rows.template fetch_rows<M>(0, 2 * N + M, static_cast<const T*>(a.gate) + t * E + p.d0, m, D);
+    rows.template fetch_rows<N>(0, N, x, n, D);
   };
   auto fetch_f = [&](int64_t t) {
     if (!p.live) return;
     const T* f = static_cast<const T*>(a.f) + t * E + p.d0;
-#pragma unroll
-    for (int k = 0; k < M; ++k)
-      if (k < m) rows.fetch(0, 2 * N + k, f + k * D);
+    rows.template fetch_rows<M>(0, 2 * N, f, m, D);
   };
   walk_tokens(
       p, a.T,
@@ -1000,35 +1050,50 @@ __global__ void __launch_bounds__(norm_bwd_threads(N, M, sizeof(T)))
         const f2 less = a.norm == HC_NORM_NONE ? both(0.f) : both(-one(s[S::kStats]));
         const f2 r2 = a.norm == HC_NORM_NONE ? both(1.f) : s[S::kStats + 1];
         __syncwarp();  // the other lanes' copies have arrived
-        // dz, from W^T g
+        // dz, from W^T g; a column of the mix at a time, grad_x_j = sum_i Heff_ij g_i
         V8 q[M];
-        {
-          V8 g[N];
+        T* gx = static_cast<T*>(a.grad_x) + t * n * D + p.d0;
+        const bool store = a.grad_x && p.live;
+#pragma unroll 1  // one half's registers at a time
+        for (int h = 0; h < 2; ++h) {
+          V4 g[N], d[M];
 #pragma unroll
-          for (int k = 0; k < M; ++k) q[k].fill(0.f);
+          for (int k = 0; k < M; ++k) d[k].v[0] = d[k].v[1] = both(0.f);
 #pragma unroll
           for (int i = 0; i < N; ++i) {
-            g[i] = rows.get(0, i);
+            g[i] = rows.half(0, i, h);
+            f2 wi[M];
+            pairs<M>(s + S::kW + i * M, wi);
 #pragma unroll
-            for (int k = 0; k < M; ++k) axpy(s[S::kW + i * M + k], g[i], q[k]);
+            for (int k = 0; k < M; ++k) axpy(wi[k], g[i], d[k]);
           }
-          // a column of the mix at a time: grad_x_j = sum_i Heff_ij g_i, and for float32 streams g x_j
-          T* gx = static_cast<T*>(a.grad_x) + t * n * D + p.d0;
-          const bool store = a.grad_x && p.live;
+#pragma unroll
+          for (int k = 0; k < M; ++k) {
+            q[k].v[0] = h ? q[k].v[0] : d[k].v[0];
+            q[k].v[1] = h ? q[k].v[1] : d[k].v[1];
+            q[k].v[2] = d[k].v[0];  // the second half stays
+            q[k].v[3] = d[k].v[1];
+          }
+          T* dst = gx + 4 * h;
+#pragma unroll
+          for (int j = 0; j < N; ++j) {
+            V4 r{{both(0.f), both(0.f)}};
+            f2 hj[N];
+            pairs<N>(H + j * N, hj);
+#pragma unroll
+            for (int i = 0; i < N; ++i) axpy(hj[i], g[i], r);
+            if (store && j < n) put4<T>(dst, r);
+            dst += D;
+          }
+        }
+        if constexpr (sizeof(T) == 4) {  // g x^T of float32 streams
           float acc[GB];
 #pragma unroll
           for (int j = 0; j < N; ++j) {
-            V8 r;
-            r.fill(0.f);
+            const V8 x = rows.get(0, N + j);
 #pragma unroll
-            for (int i = 0; i < N; ++i) axpy(H[j * N + i], g[i], r);
-            if (store && j < n) put8<T>(gx + j * D, r);
-            if constexpr (sizeof(T) == 4) {
-              const V8 x = rows.get(0, N + j);
-#pragma unroll
-              for (int i = 0; i < N; ++i) acc[(j * N + i) % GB] = dot(g[i], x);
-              if ((j + 1) * N % GB == 0) fold_to<GB>(acc, p.lane, &gram[parity][p.slot()][(j + 1) * N - GB]);
-            }
+            for (int i = 0; i < N; ++i) acc[(j * N + i) % GB] = dot(rows.get(0, i), x);
+            if ((j + 1) * N % GB == 0) fold_to<GB>(acc, p.lane, &gram[parity][p.slot()][(j + 1) * N - GB]);
           }
         }
         if constexpr (sizeof(T) == 2) {
@@ -1137,7 +1202,7 @@ inline int64_t norm_smem_bytes(bool write, bool bwd, int N, int M, int chunks, i
   const int rows = write ? (bwd ? 2 * N : N) + 2 * M : N + (bwd ? M : 0);
   const int64_t entries = write ? (N * N + N * M + N + 3) / 2 * 2 : N * M + 2;
   const int64_t group = (entries * 8 * kSmallSlots + (write ? N * N * 20 : 0) + 15) / 16 * 16;
-  return static_cast<int64_t>(rows * esize / 2) * chunks * (16 * threads + 16) + groups * group;
+  return static_cast<int64_t>(rows * esize / 2) * chunks * kRowPitch * (threads / 32) + groups * group;
 }
 static_assert(sizeof(ReadMemory<8, 4>) == (34 * 8 * kSmallSlots + 15) / 16 * 16);
 static_assert(sizeof(WriteMemory<8, 4>) == (106 * 8 * kSmallSlots + 64 * 20 + 15) / 16 * 16);
@@ -1153,7 +1218,7 @@ template <typename T, bool WRITE, bool BWD, int N, int M, int CH> NormKernel nor
 }
 template <typename T, bool WRITE, int N, int M> NormKernel norm_kernel_for(bool bwd, int ch) {
   if (bwd) return norm_kernel_of<T, WRITE, true, N, M, 1>();
-  if constexpr (norm_fwd_chunks(N, M, sizeof(T)) >= 3) {
+  if constexpr (norm_fwd_chunks(WRITE, N, M, sizeof(T)) >= 3) {
     if (ch == 3) return norm_kernel_of<T, WRITE, false, N, M, 3>();
     if (ch == 2) return norm_kernel_of<T, WRITE, false, N, M, 2>();
   }
@@ -1176,7 +1241,7 @@ inline NormGeometry norm_geometry(bool write, bool bwd, int n, int m, int64_t D,
   const int N = padded_streams(n), M = padded_blocks(m);
   if (D % kColumns != 0 || M > N) return g;
   const int64_t lines = (D + 32 * kColumns - 1) / (32 * kColumns);  // warps with a chunk a thread
-  const int most = bwd ? 1 : norm_fwd_chunks(N, M, esize);
+  const int most = bwd ? 1 : norm_fwd_chunks(write, N, M, esize);
   g.chunks = static_cast<int>(lines < most ? lines : most);
   const int64_t warps = (lines + g.chunks - 1) / g.chunks;
   const int groups = warps == 1 ? kSmallGroups : 1;
