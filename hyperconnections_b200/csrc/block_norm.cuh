@@ -47,8 +47,8 @@ constexpr int kNormSmemMax = 210 * 1024;  // of the 227 KB a CTA can have; up to
 constexpr int norm_bwd_threads(int N, int M, int esize) { return M >= 4 || (N == 8 && esize == 4) ? 256 : M == 2 || N == 8 ? 384 : 512; }
 // Chunks a thread may own in the forward (a token's rows then need fewer warps,
 // down to one without barriers): as many as keep a block's rows in registers.
-constexpr int norm_fwd_chunks(bool write, int N, int M, int esize) { return 1; }
-constexpr int norm_fwd_threads(int N, int M, int CH, int esize) { return M >= 4 || CH > 1 ? 384 : 640; }
+constexpr int norm_fwd_chunks(bool write, int N, int M, int esize) { return M == 1 && N <= 4 && esize == 2 ? 3 : 1; }
+constexpr int norm_fwd_threads(int N, int M, int CH, int esize) { return M >= 4 ? 384 : CH > 1 ? 512 : 640; }
 
 // ------------------------------------------------------- pairs of float32
 using f2 = unsigned long long;

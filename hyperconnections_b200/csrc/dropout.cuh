@@ -1,4 +1,9 @@
 // dropout.cuh — y = x / (1 - p) where the element's Philox word says so, else 0.
+//
+// Bound by HBM as long as the generator keeps up: a block of four words is ten
+// rounds of two 32 x 32 -> 64 bit products and two three-input xors (the round
+// keys, the same for all, stay in registers), about 80 instructions for the
+// eight elements that a thread moves at a time.
 #pragma once
 
 #include "block.cuh"
@@ -7,27 +12,55 @@ namespace hc {
 
 constexpr int kDropThreads = 256;
 
-// One Philox block serves four consecutive elements, so a thread takes four.
-template <typename T>
-__global__ void __launch_bounds__(kDropThreads) dropout_elem(const T* x, T* y, int64_t N, DropArgs d) {
+// Groups of eight elements: two generator blocks, one or two 16-byte words.
+// VECTOR: x and y on 16-byte boundaries. The last N % 8 elements go to the
+// thread behind the last whole group.
+template <typename T, bool VECTOR>
+__global__ void __launch_bounds__(kDropThreads) dropout_kernel(const T* x, T* y, int64_t N, const __grid_constant__ DropArgs d) {
+  constexpr int Q = sizeof(T) / 2;
   const DropKey key = drop_key(d);
-  const int64_t stride = static_cast<int64_t>(gridDim.x) * kDropThreads;
-  for (int64_t b = static_cast<int64_t>(blockIdx.x) * kDropThreads + threadIdx.x; 4 * b < N; b += stride) {
-    const uint4 w = philox4(key, static_cast<uint64_t>(b));
-    const uint32_t word[4] = {w.x, w.y, w.z, w.w};
+  const int64_t stride = static_cast<int64_t>(gridDim.x) * kDropThreads, groups = N / 8;
+  for (int64_t b = static_cast<int64_t>(blockIdx.x) * kDropThreads + threadIdx.x; 8 * b < N; b += stride) {
+    float f[8];
+    const bool whole = b < groups;
+    if (VECTOR && whole) {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const int64_t i = 4 * b + e;
-      if (i < N) y[i] = Elem<T>::from_f(drop_value(d, word[e], Elem<T>::to_f(x[i])));
+      for (int i = 0; i < Q; ++i) unpack<T>(ld_nc_v4(x + 8 * b + i * (16 / sizeof(T))), f + i * (16 / sizeof(T)));
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) f[e] = 8 * b + e < N ? Elem<T>::to_f(x[8 * b + e]) : 0.f;
+    }
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const uint4 w = philox4(key, static_cast<uint64_t>(2 * b + h));
+      const uint32_t word[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const uint32_t mask = word[e] >= d.bar ? d.kept : 0u;  // a dropped value is 0 whatever it was
+        f[4 * h + e] = __uint_as_float(__float_as_uint(f[4 * h + e] * d.scale) & mask);
+      }
+    }
+    if (VECTOR && whole) {
+#pragma unroll
+      for (int i = 0; i < Q; ++i) st_v4(y + 8 * b + i * (16 / sizeof(T)), pack<T>(f + i * (16 / sizeof(T))));
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (8 * b + e < N) y[8 * b + e] = Elem<T>::from_f(f[e]);
     }
   }
 }
 
 template <typename T>
 int dropout_launch(const void* x, void* y, int64_t N, const DropArgs& d, cudaStream_t s) {
-  const int64_t want = ((N + 3) / 4 + kDropThreads - 1) / kDropThreads;
-  const int grid = static_cast<int>(want < 8 * sm_count() ? want : 8 * sm_count());
-  dropout_elem<T><<<grid, kDropThreads, 0, s>>>(static_cast<const T*>(x), static_cast<T*>(y), N, d);
+  const int64_t want = ((N + 7) / 8 + kDropThreads - 1) / kDropThreads, most = 8 * static_cast<int64_t>(sm_count());
+  const int grid = static_cast<int>(want < most ? want : most);
+  // x may be y, which the non-coherent loads of the vector kernel allow: a
+  // thread reads its own elements before it writes them
+  if (aligned16(x) && aligned16(y))
+    dropout_kernel<T, true><<<grid, kDropThreads, 0, s>>>(static_cast<const T*>(x), static_cast<T*>(y), N, d);
+  else
+    dropout_kernel<T, false><<<grid, kDropThreads, 0, s>>>(static_cast<const T*>(x), static_cast<T*>(y), N, d);
   return launch_status();
 }
 
