@@ -20,10 +20,9 @@ constexpr int kBlockMaxM = 4;  // backbone blocks
 struct DropArgs {
   const int64_t* state;  // device (seed, offset), or nullptr for the two below
   uint64_t seed, offset;
-  uint64_t threshold;  // floor(p 2^32): an element is kept when its word is at least this
+  uint32_t below;      // floor(p 2^32) - 1: an element is kept when its word is above
   float scale;         // 1 / (1 - p); 0 at p = 1
-  int on;              // p > 0
-  uint32_t bar, kept;  // min(threshold, 2^32 - 1), and the mask of a word that reaches it (0 at p = 1)
+  int on;              // floor(p 2^32) > 0; else nothing is dropped
 };
 
 struct DropKey {
@@ -40,20 +39,32 @@ __device__ __forceinline__ DropKey drop_key(const DropArgs& a) {
                  static_cast<uint32_t>(offset >> 32)};
 }
 
-__device__ __forceinline__ uint4 philox4(const DropKey& key, uint64_t block) {
-  uint32_t c0 = static_cast<uint32_t>(block), c1 = static_cast<uint32_t>(block >> 32), c2 = key.o0, c3 = key.o1;
-  uint32_t k0 = key.k0, k1 = key.k1;
+// The ten round keys. A kernel that draws many blocks makes them once.
+struct RoundKeys {
+  uint32_t a[10], b[10];
+  __device__ __forceinline__ explicit RoundKeys(const DropKey& k) {
+#pragma unroll
+    for (int r = 0; r < 10; ++r) {
+      a[r] = k.k0 + r * 0x9E3779B9u;
+      b[r] = k.k1 + r * 0xBB67AE85u;
+    }
+  }
+};
+
+__device__ __forceinline__ uint4 philox4(const RoundKeys& k, uint32_t o0, uint32_t o1, uint64_t block) {
+  uint32_t c0 = static_cast<uint32_t>(block), c1 = static_cast<uint32_t>(block >> 32), c2 = o0, c3 = o1;
 #pragma unroll
   for (int r = 0; r < 10; ++r) {
     const uint64_t p0 = static_cast<uint64_t>(0xD2511F53u) * c0, p1 = static_cast<uint64_t>(0xCD9E8D57u) * c2;
-    c0 = static_cast<uint32_t>(p1 >> 32) ^ c1 ^ k0;
+    c0 = static_cast<uint32_t>(p1 >> 32) ^ c1 ^ k.a[r];
     c1 = static_cast<uint32_t>(p1);
-    c2 = static_cast<uint32_t>(p0 >> 32) ^ c3 ^ k1;
+    c2 = static_cast<uint32_t>(p0 >> 32) ^ c3 ^ k.b[r];
     c3 = static_cast<uint32_t>(p0);
-    k0 += 0x9E3779B9u;
-    k1 += 0xBB67AE85u;
   }
   return make_uint4(c0, c1, c2, c3);
+}
+__device__ __forceinline__ uint4 philox4(const DropKey& key, uint64_t block) {
+  return philox4(RoundKeys(key), key.o0, key.o1, block);
 }
 
 // The word of one element.
@@ -66,7 +77,7 @@ __device__ __forceinline__ uint32_t philox_word(const DropKey& key, uint64_t i) 
 // A dropped value is 0 whatever it was (an infinity or a NaN too), so it is
 // selected, not multiplied.
 __device__ __forceinline__ float drop_value(const DropArgs& a, uint32_t word, float v) {
-  return static_cast<uint64_t>(word) >= a.threshold ? v * a.scale : 0.f;
+  return word > a.below ? v * a.scale : 0.f;
 }
 
 // ------------------------------------------------------------ norm kernels

@@ -31,12 +31,10 @@ bool drop_args(DropArgs& d, double p, const int64_t* state, int64_t seed, int64_
   d.state = state;
   d.seed = static_cast<uint64_t>(seed);
   d.offset = static_cast<uint64_t>(offset);
-  d.threshold = static_cast<uint64_t>(floor(p * 4294967296.0));
+  const uint64_t threshold = static_cast<uint64_t>(floor(p * 4294967296.0));
+  d.on = threshold > 0;  // of p < 2^-32 nothing is left
+  d.below = static_cast<uint32_t>(threshold - (threshold > 0));
   d.scale = p < 1.0 ? static_cast<float>(1.0 / (1.0 - p)) : 0.f;
-  d.on = p > 0.0;
-  // the same test on 32 bits: at p = 1 no bar keeps every word out, so what is kept is masked instead
-  d.bar = d.threshold > 0xffffffffu ? 0xffffffffu : static_cast<uint32_t>(d.threshold);
-  d.kept = d.threshold > 0xffffffffu ? 0u : 0xffffffffu;
   return true;
 }
 
@@ -260,6 +258,13 @@ extern "C" int hc_dropout(const void* x, void* y, int64_t N, double p, const int
   if (N == 0) return HC_OK;
   if (!x || !y) return HC_ERR_NULL_POINTER;
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (!d.on) {  // every element is kept, times 1
+    if (x == y) return HC_OK;
+    return cudaMemcpyAsync(y, x, static_cast<size_t>(N) * dtype_size(stream_dtype), cudaMemcpyDeviceToDevice, s) ==
+                   cudaSuccess
+               ? HC_OK
+               : HC_ERR_LAUNCH;
+  }
   switch (stream_dtype) {
     case HC_DTYPE_F32: return dropout_launch_f32(x, y, N, d, s);
     case HC_DTYPE_F16: return dropout_launch_f16(x, y, N, d, s);

@@ -281,7 +281,7 @@ __global__ void __launch_bounds__(kElemThreads) write_norm_bwd_elem(NormArgs a) 
       factor = 1.f;
       if (a.drop.on) {
         const uint32_t w = philox_word(key, static_cast<uint64_t>(t * E + k * D + d));
-        factor = static_cast<uint64_t>(w) >= a.drop.threshold ? a.drop.scale : 0.f;
+        factor = w > a.drop.below ? a.drop.scale : 0.f;
         return factor != 0.f ? s * factor : 0.f;
       }
       return s;

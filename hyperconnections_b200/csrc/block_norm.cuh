@@ -696,10 +696,10 @@ __device__ __forceinline__ void keep8(const DropArgs& d, const DropKey& key, uin
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
     const uint4 w = philox4(key, (element >> 2) + h);
-    mask[4 * h] = w.x >= d.bar ? d.kept : 0u;
-    mask[4 * h + 1] = w.y >= d.bar ? d.kept : 0u;
-    mask[4 * h + 2] = w.z >= d.bar ? d.kept : 0u;
-    mask[4 * h + 3] = w.w >= d.bar ? d.kept : 0u;
+    mask[4 * h] = w.x > d.below ? 0xffffffffu : 0u;
+    mask[4 * h + 1] = w.y > d.below ? 0xffffffffu : 0u;
+    mask[4 * h + 2] = w.z > d.below ? 0xffffffffu : 0u;
+    mask[4 * h + 3] = w.w > d.below ? 0xffffffffu : 0u;
   }
 }
 // v / (1 - p) where kept, else 0 whatever v is.

@@ -19,6 +19,9 @@ template <typename T, bool VECTOR>
 __global__ void __launch_bounds__(kDropThreads) dropout_kernel(const T* x, T* y, int64_t N, const __grid_constant__ DropArgs d) {
   constexpr int Q = sizeof(T) / 2;
   const DropKey key = drop_key(d);
+  RoundKeys rk(key);
+#pragma unroll
+  for (int r = 0; r < 10; ++r) asm volatile("" : "+r"(rk.a[r]), "+r"(rk.b[r]));  // made once, not in every round again
   const int64_t stride = static_cast<int64_t>(gridDim.x) * kDropThreads, groups = N / 8;
   for (int64_t b = static_cast<int64_t>(blockIdx.x) * kDropThreads + threadIdx.x; 8 * b < N; b += stride) {
     float f[8];
@@ -32,12 +35,11 @@ __global__ void __launch_bounds__(kDropThreads) dropout_kernel(const T* x, T* y,
     }
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const uint4 w = philox4(key, static_cast<uint64_t>(2 * b + h));
+      const uint4 w = philox4(rk, key.o0, key.o1, static_cast<uint64_t>(2 * b + h));
       const uint32_t word[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const uint32_t mask = word[e] >= d.bar ? d.kept : 0u;  // a dropped value is 0 whatever it was
-        f[4 * h + e] = __uint_as_float(__float_as_uint(f[4 * h + e] * d.scale) & mask);
+        f[4 * h + e] = drop_value(d, word[e], f[4 * h + e]);
       }
     }
     if (VECTOR && whole) {
@@ -53,7 +55,7 @@ __global__ void __launch_bounds__(kDropThreads) dropout_kernel(const T* x, T* y,
 
 template <typename T>
 int dropout_launch(const void* x, void* y, int64_t N, const DropArgs& d, cudaStream_t s) {
-  const int64_t want = ((N + 7) / 8 + kDropThreads - 1) / kDropThreads, most = 8 * static_cast<int64_t>(sm_count());
+  const int64_t want = ((N + 7) / 8 + kDropThreads - 1) / kDropThreads, most = 24 * static_cast<int64_t>(sm_count());
   const int grid = static_cast<int>(want < most ? want : most);
   // x may be y, which the non-coherent loads of the vector kernel allow: a
   // thread reads its own elements before it writes them
