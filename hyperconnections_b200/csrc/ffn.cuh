@@ -57,4 +57,10 @@ int ffn_simt_launch(const FfnProduct& p, cudaStream_t s);
 // (kStore only), else nullptr.
 int ffn_tc_splits(int64_t M, int64_t N, int64_t K, int terms);
 int ffn_tc_launch(const FfnProduct& p, int dtype, float* parts, cudaStream_t s);
+
+// bf16 and fp16, the forward's products for at most kFewTokens rows of A
+// (ffn_few.cu): operands aligned as above.
+constexpr int64_t kFewTokens = 32;
+int ffn_few_launch(const FfnProduct& p, int dtype, cudaStream_t s);
+
 }  // namespace hc

@@ -67,6 +67,10 @@ int fit(Matrix& out, Scratch& scratch, const void* p, int64_t rows, int64_t cols
   return launch_status();
 }
 
+// A few tokens: the weights bound the forward, and ffn_few.cu streams them. (D =
+// 2048, F = 8192, bf16, 8 tokens: XX us against 44.8 on the tensor-core tiles.)
+bool few(int64_t T, int dtype) { return half(dtype) && T <= kFewTokens; }
+
 int64_t parts_bytes(int64_t M, int64_t N, int64_t K, int terms, int dtype) {
   const int splits = half(dtype) ? ffn_tc_splits(M, N, K, terms) : 1;
   return splits > 1 ? splits * M * N * 4 : 0;
@@ -74,7 +78,7 @@ int64_t parts_bytes(int64_t M, int64_t N, int64_t K, int terms, int dtype) {
 
 // The sums of products one after the other share the largest one's parts.
 int64_t most_parts(int backward, int64_t T, int64_t D, int64_t F, int64_t O, int dtype) {
-  if (!backward) return parts_bytes(T, O, F, 1, dtype);
+  if (!backward) return few(T, dtype) ? 0 : parts_bytes(T, O, F, 1, dtype);
   int64_t m = parts_bytes(T, D, F, 2, dtype);
   for (const int64_t b : {parts_bytes(F, D, T, 1, dtype), parts_bytes(O, F, T, 1, dtype)})
     if (b > m) m = b;
@@ -147,8 +151,13 @@ extern "C" int hc_gated_ffn_fwd(const void* x, const void* w_gate, const void* w
   p.B[1] = {mu.p, mu.ld, 1, F};
   p.M = T; p.N = Fp; p.K = D;
   p.out = h; p.slope_gate = slope_gate; p.slope_up = slope_up; p.ldo = Fp; p.act = act;
+  const FfnProduct down = store(T, O, F, {h, Fp, 1, T}, {md.p, md.ld, 1, O}, y);
+  if (few(T, dtype)) {
+    if (int rc = ffn_few_launch(p, dtype, s)) return rc;
+    return ffn_few_launch(down, dtype, s);
+  }
   if (int rc = run(p, dtype, nullptr, s)) return rc;
-  return run(store(T, O, F, {h, Fp, 1, T}, {md.p, md.ld, 1, O}, y), dtype, space.take(0), s);
+  return run(down, dtype, space.take(0), s);
 }
 
 extern "C" int hc_gated_ffn_bwd(const void* g, const void* x, const void* w_gate, const void* w_up, const void* w_down,
