@@ -49,8 +49,12 @@ __device__ __forceinline__ void ffn_act(int act, float a, float& val, float& der
   }
 }
 
-// float32 (ffn_simt.cu).
-int ffn_simt_launch(const FfnProduct& p, cudaStream_t s);
+// out[i] = the sum of `splits` float32 parts, count apart, in order (ffn_tc.cu).
+int ffn_add_parts(const float* parts, void* out, int64_t count, int splits, int dtype, cudaStream_t s);
+
+// float32 (ffn_simt.cu); parts as below.
+int ffn_simt_splits(int64_t M, int64_t N, int64_t K, int terms);
+int ffn_simt_launch(const FfnProduct& p, float* parts, cudaStream_t s);
 
 // bf16 and fp16 (ffn_tc.cu): operands 16-byte aligned with strides of whole 16
 // bytes. `parts`: splits * M * N floats where ffn_tc_splits says more than one

@@ -72,7 +72,7 @@ int fit(Matrix& out, Scratch& scratch, const void* p, int64_t rows, int64_t cols
 bool few(int64_t T, int dtype) { return half(dtype) && T <= kFewTokens; }
 
 int64_t parts_bytes(int64_t M, int64_t N, int64_t K, int terms, int dtype) {
-  const int splits = half(dtype) ? ffn_tc_splits(M, N, K, terms) : 1;
+  const int splits = half(dtype) ? ffn_tc_splits(M, N, K, terms) : ffn_simt_splits(M, N, K, terms);
   return splits > 1 ? splits * M * N * 4 : 0;
 }
 
@@ -86,7 +86,8 @@ int64_t most_parts(int backward, int64_t T, int64_t D, int64_t F, int64_t O, int
 }
 
 int run(const FfnProduct& p, int dtype, void* parts, cudaStream_t s) {
-  return half(dtype) ? ffn_tc_launch(p, dtype, static_cast<float*>(parts), s) : ffn_simt_launch(p, s);
+  float* f = static_cast<float*>(parts);
+  return half(dtype) ? ffn_tc_launch(p, dtype, f, s) : ffn_simt_launch(p, f, s);
 }
 
 FfnProduct store(int64_t M, int64_t N, int64_t K, FfnOperand A, FfnOperand B, void* out) {

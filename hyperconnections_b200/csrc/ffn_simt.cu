@@ -1,85 +1,127 @@
 // ffn_simt.cu — the gated feed-forward's float32 products on the FMA units (the
-// tensor cores have no float32 inputs): any size and order, 64 x 64 tiles of
-// the result by 256 threads, 4 x 4 a thread.
+// tensor cores have no float32 inputs): any size and order.
+//
+// 256 threads make a TM x TN tile of the result, TM / 16 x TN / 16 values a
+// thread, over stages of 16 steps of the sum in two shared-memory buffers. A
+// thread's loads are a pointer and constant steps from it. With 8 x 8 values a
+// thread the FMA units bound the kernel (64 FMAs on four 16-byte shared loads);
+// smaller products take 64 x 64 tiles, and where even those are few they split
+// their sum over CTAs, whose parts one more kernel adds in order: a lone CTA on
+// an SM waits for its loads at every stage.
 #include "ffn.cuh"
 
 namespace hc {
 namespace {
 
-constexpr int kTile = 64, kDepth = 16, kThreads = 256, kPitch = kTile + 4;
+constexpr int kDepth = 16, kThreads = 256;
 
-// The tile [64 rows][16 k] of an operand into shared memory as [k][row],
-// neighbouring threads along the operand's unit stride.
-template <typename T>
-__device__ __forceinline__ void load_tile(const FfnOperand& o, int64_t row0, int64_t k0, int64_t K, float (&r)[4]) {
-  const T* p = static_cast<const T*>(o.p);
+// ROWS rows of an operand, 16 steps at a time, neighbouring threads along its
+// unit stride. Rows and steps past the operand's end count as 0.
+template <typename T, int ROWS> struct Loader {
+  static constexpr int kLoads = ROWS * kDepth / kThreads;
+  const T* p;
+  int64_t step, advance;  // from one of a thread's loads to the next; from stage to stage
+  uint32_t rows;          // bit i: the row of load i exists
+  int k, k_step;          // of load 0, and from load to load
+  int at, at_step;        // place in the [step][row] buffer
+  __device__ __forceinline__ Loader(const FfnOperand& o, int64_t row0, int64_t k0, int pitch) {
+    const bool along = o.k_stride == 1;  // else along the rows
+    const int row = along ? threadIdx.x / kDepth : threadIdx.x % ROWS;
+    const int row_step = along ? kThreads / kDepth : 0;
+    k = along ? threadIdx.x % kDepth : threadIdx.x / ROWS;
+    k_step = along ? 0 : kThreads / ROWS;
+    p = static_cast<const T*>(o.p) + (row0 + row) * o.row_stride + (k0 + k) * o.k_stride;
+    step = row_step * o.row_stride + k_step * o.k_stride;
+    advance = kDepth * o.k_stride;
+    at = k * pitch + row;
+    at_step = k_step * pitch + row_step;
+    rows = 0;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int e = threadIdx.x + i * kThreads;
-    const int64_t row = row0 + (o.k_stride == 1 ? e / kDepth : e % kTile);
-    const int64_t k = k0 + (o.k_stride == 1 ? e % kDepth : e / kTile);
-    r[i] = row < o.rows && k < K ? Elem<T>::to_f(p[row * o.row_stride + k * o.k_stride]) : 0.f;
+    for (int i = 0; i < kLoads; ++i) rows |= (row0 + row + i * row_step < o.rows ? 1u : 0u) << i;
   }
-}
-__device__ __forceinline__ void put_tile(const FfnOperand& o, const float (&r)[4], float (*s)[kPitch]) {
+  __device__ __forceinline__ void load(int64_t left, float (&r)[kLoads]) {  // `left` steps of the sum from this stage on
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int e = threadIdx.x + i * kThreads;
-    if (o.k_stride == 1)
-      s[e % kDepth][e / kDepth] = r[i];
-    else
-      s[e / kTile][e % kTile] = r[i];
+    for (int i = 0; i < kLoads; ++i)
+      r[i] = (rows >> i & 1u) && k + i * k_step < left ? Elem<T>::to_f(__ldg(p + i * step)) : 0.f;
+    p += advance;
   }
-}
+  __device__ __forceinline__ void put(const float (&r)[kLoads], float* buffer) const {
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) buffer[at + i * at_step] = r[i];
+  }
+};
 
-template <typename T, int EPI>
-__global__ void __launch_bounds__(kThreads) ffn_simt_kernel(FfnProduct p) {
-  constexpr int NB = EPI == kGlu ? 2 : 1;
-  __shared__ float sA[kDepth][kPitch], sB[NB][kDepth][kPitch];
+template <typename T, int EPI, int TM, int TN>
+__global__ void __launch_bounds__(kThreads) ffn_simt_kernel(const __grid_constant__ FfnProduct p, float* parts, int splits) {
+  constexpr int NB = EPI == kGlu ? 2 : 1, VM = TM / 16, VN = TN / 16, PM = TM + 4, PN = TN + 4;
+  __shared__ __align__(16) float sA[2][kDepth * PM], sB[2][NB][kDepth * PN];
   const int tx = threadIdx.x % 16, ty = threadIdx.x / 16;
-  const int64_t m0 = static_cast<int64_t>(blockIdx.y) * kTile, n0 = static_cast<int64_t>(blockIdx.x) * kTile;
-  float acc[NB][4][4] = {};
+  const int64_t m0 = static_cast<int64_t>(blockIdx.y) * TM, n0 = static_cast<int64_t>(blockIdx.x) * TN;
+  float acc[NB][VM][VN] = {};
+  // this CTA's stages of all terms' sums
+  const int64_t per_term = (p.K + kDepth - 1) / kDepth, stages = per_term * p.terms;
+  const int64_t s0 = stages * blockIdx.z / splits, s1 = stages * (blockIdx.z + 1) / splits;
   for (int term = 0; term < p.terms; ++term) {
-    float ra[4], rb[NB][4];
-    load_tile<T>(p.A[term], m0, 0, p.K, ra);
-#pragma unroll
-    for (int b = 0; b < NB; ++b) load_tile<T>(p.B[term + b], n0, 0, p.K, rb[b]);
-    for (int64_t k0 = 0; k0 < p.K; k0 += kDepth) {
-      put_tile(p.A[term], ra, sA);
-#pragma unroll
-      for (int b = 0; b < NB; ++b) put_tile(p.B[term + b], rb[b], sB[b]);
-      __syncthreads();
-      if (k0 + kDepth < p.K) {  // the next tile travels while this one is used
-        load_tile<T>(p.A[term], m0, k0 + kDepth, p.K, ra);
-#pragma unroll
-        for (int b = 0; b < NB; ++b) load_tile<T>(p.B[term + b], n0, k0 + kDepth, p.K, rb[b]);
-      }
+    const int64_t first = s0 > term * per_term ? s0 - term * per_term : 0;
+    const int64_t last = s1 - term * per_term < per_term ? s1 - term * per_term : per_term;
+    if (first >= last) continue;
+    Loader<T, TM> la(p.A[term], m0, first * kDepth, PM);
+    Loader<T, TN> lb(p.B[term], n0, first * kDepth, PN), lb2(p.B[NB == 2 ? 1 : term], n0, first * kDepth, PN);
+    float ra[la.kLoads], rb[NB][Loader<T, TN>::kLoads];
+    auto load = [&](int64_t st) {
+      la.load(p.K - st * kDepth, ra);
+      lb.load(p.K - st * kDepth, rb[0]);
+      if constexpr (NB == 2) lb2.load(p.K - st * kDepth, rb[NB - 1]);
+    };
+    auto put = [&](int buf) {
+      la.put(ra, sA[buf]);
+      lb.put(rb[0], sB[buf][0]);
+      if constexpr (NB == 2) lb2.put(rb[NB - 1], sB[buf][NB - 1]);
+    };
+    load(first);
+    put(0);
+    __syncthreads();
+    int buf = 0;
+    for (int64_t st = first; st < last; ++st, buf ^= 1) {
+      if (st + 1 < last) load(st + 1);  // the next stage travels while this one is used
 #pragma unroll
       for (int k = 0; k < kDepth; ++k) {
-        const float4 av = *reinterpret_cast<const float4*>(&sA[k][4 * ty]);
-        const float a[4] = {av.x, av.y, av.z, av.w};
+        float a[VM];
+#pragma unroll
+        for (int h = 0; h < VM; h += 4) {  // rows 4 ty + 64 (h / 4) + 0 .. 3
+          const float4 v = *reinterpret_cast<const float4*>(&sA[buf][k * PM + 16 * h + 4 * ty]);
+          a[h] = v.x; a[h + 1] = v.y; a[h + 2] = v.z; a[h + 3] = v.w;
+        }
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
-          const float4 bv = *reinterpret_cast<const float4*>(&sB[b][k][4 * tx]);
-          const float w[4] = {bv.x, bv.y, bv.z, bv.w};
+          float w[VN];
 #pragma unroll
-          for (int i = 0; i < 4; ++i)
+          for (int h = 0; h < VN; h += 4) {
+            const float4 v = *reinterpret_cast<const float4*>(&sB[buf][b][k * PN + 16 * h + 4 * tx]);
+            w[h] = v.x; w[h + 1] = v.y; w[h + 2] = v.z; w[h + 3] = v.w;
+          }
 #pragma unroll
-            for (int j = 0; j < 4; ++j) acc[b][i][j] = fmaf(a[i], w[j], acc[b][i][j]);
+          for (int i = 0; i < VM; ++i)
+#pragma unroll
+            for (int j = 0; j < VN; ++j) acc[b][i][j] = fmaf(a[i], w[j], acc[b][i][j]);
         }
       }
+      if (st + 1 < last) put(buf ^ 1);
       __syncthreads();
     }
   }
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
+  for (int i = 0; i < VM; ++i)
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int64_t m = m0 + 4 * ty + i, n = n0 + 4 * tx + j;
+    for (int j = 0; j < VN; ++j) {
+      const int64_t m = m0 + 4 * ty + 64 * (i / 4) + i % 4, n = n0 + 4 * tx + 64 * (j / 4) + j % 4;
       if (m >= p.M || n >= p.N) continue;
       const int64_t at = m * p.ldo + n;
       if constexpr (EPI == kStore) {
-        static_cast<T*>(p.out)[at] = Elem<T>::from_f(acc[0][i][j]);
+        if (parts)
+          parts[(blockIdx.z * p.M + m) * p.N + n] = acc[0][i][j];
+        else
+          static_cast<T*>(p.out)[at] = Elem<T>::from_f(acc[0][i][j]);
       } else if constexpr (EPI == kGlu) {
         const float a = acc[0][i][j], b = acc[NB - 1][i][j];
         float val, der;
@@ -97,18 +139,44 @@ __global__ void __launch_bounds__(kThreads) ffn_simt_kernel(FfnProduct p) {
     }
 }
 
-template <typename T> int launch(const FfnProduct& p, cudaStream_t s) {
-  const dim3 grid(static_cast<unsigned>((p.N + kTile - 1) / kTile), static_cast<unsigned>((p.M + kTile - 1) / kTile));
-  switch (p.epilogue) {
-    case kStore: ffn_simt_kernel<T, kStore><<<grid, kThreads, 0, s>>>(p); break;
-    case kGlu: ffn_simt_kernel<T, kGlu><<<grid, kThreads, 0, s>>>(p); break;
-    default: ffn_simt_kernel<T, kGluBwd><<<grid, kThreads, 0, s>>>(p); break;
-  }
-  return launch_status();
-}
-
 }  // namespace
 
-int ffn_simt_launch(const FfnProduct& p, cudaStream_t s) { return launch<float>(p, s); }
+namespace {
+int64_t tiles(int64_t M, int64_t N, int tm, int tn) { return (M + tm - 1) / tm * ((N + tn - 1) / tn); }
+
+// 128 x 128 tiles (128 x 64 of two weights) where they give every SM one.
+bool wide(int64_t M, int64_t N, bool glu) { return tiles(M, N, 128, glu ? 64 : 128) >= sm_count(); }
+
+template <int EPI> int launch(const FfnProduct& p, float* parts, int splits, cudaStream_t s) {
+  constexpr int kWideN = EPI == kGlu ? 64 : 128;
+  const bool w = wide(p.M, p.N, EPI == kGlu);
+  const int tm = w ? 128 : 64, tn = w ? kWideN : 64;
+  const dim3 grid(static_cast<unsigned>((p.N + tn - 1) / tn), static_cast<unsigned>((p.M + tm - 1) / tm), splits);
+  if (w)
+    ffn_simt_kernel<float, EPI, 128, kWideN><<<grid, kThreads, 0, s>>>(p, parts, splits);
+  else
+    ffn_simt_kernel<float, EPI, 64, 64><<<grid, kThreads, 0, s>>>(p, parts, splits);
+  return launch_status();
+}
+}  // namespace
+
+// CTAs that share the sum of one 64 x 64 tile: until there are four an SM, each
+// with at least 8 stages (128 steps) of its own. (517 x 333 x 887, forward and
+// backward: XX us against 354 without.)
+int ffn_simt_splits(int64_t M, int64_t N, int64_t K, int terms) {
+  if (wide(M, N, false)) return 1;
+  const int64_t by_sms = 4 * sm_count() / tiles(M, N, 64, 64), by_depth = (K + kDepth - 1) / kDepth * terms / 8;
+  const int64_t s = by_sms < by_depth ? by_sms : by_depth;
+  return static_cast<int>(s < 1 ? 1 : s > 32 ? 32 : s);
+}
+
+int ffn_simt_launch(const FfnProduct& p, float* parts, cudaStream_t s) {
+  if (p.epilogue == kGlu) return launch<kGlu>(p, nullptr, 1, s);
+  if (p.epilogue == kGluBwd) return launch<kGluBwd>(p, nullptr, 1, s);
+  const int splits = ffn_simt_splits(p.M, p.N, p.K, p.terms);
+  if (splits > 1 && !parts) return HC_ERR_SCRATCH;
+  if (int rc = launch<kStore>(p, splits > 1 ? parts : nullptr, splits, s)) return rc;
+  return splits > 1 ? ffn_add_parts(parts, p.out, p.M * p.N, splits, HC_DTYPE_F32, s) : HC_OK;
+}
 
 }  // namespace hc

@@ -486,7 +486,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 
 // ----------------------------------------------------- parts of a split sum
 template <typename T>
-__global__ void __launch_bounds__(256) ffn_add_parts(const float* parts, T* out, int64_t count, int splits) {
+__global__ void __launch_bounds__(256) add_parts_kernel(const float* parts, T* out, int64_t count, int splits) {
   for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < count;
        i += static_cast<int64_t>(gridDim.x) * 256) {
     float s = 0.f;
@@ -595,14 +595,17 @@ int ffn_tc_launch(const FfnProduct& p, int dtype, float* parts, cudaStream_t s) 
   const int pairs = static_cast<int>(items < pairs_resident() ? items : pairs_resident());
   kernel<<<2 * pairs, kThreads, kSmemBytes, s>>>(maps, a);
   if (int rc = launch_status()) return rc;
-  if (a.splits == 1) return HC_OK;
-  const int64_t count = p.M * p.N;
-  const int64_t want = ceil_div(count, 256), most = 8 * sm_count();
+  return a.splits > 1 ? ffn_add_parts(parts, p.out, p.M * p.N, a.splits, dtype, s) : HC_OK;
+}
+
+int ffn_add_parts(const float* parts, void* out, int64_t count, int splits, int dtype, cudaStream_t s) {
+  const int64_t want = ceil_div(count, 256), most = 8 * static_cast<int64_t>(sm_count());
   const int grid = static_cast<int>(want < most ? want : most);
-  if (bf)
-    ffn_add_parts<<<grid, 256, 0, s>>>(parts, static_cast<__nv_bfloat16*>(p.out), count, a.splits);
-  else
-    ffn_add_parts<<<grid, 256, 0, s>>>(parts, static_cast<__half*>(p.out), count, a.splits);
+  switch (dtype) {
+    case HC_DTYPE_F32: add_parts_kernel<<<grid, 256, 0, s>>>(parts, static_cast<float*>(out), count, splits); break;
+    case HC_DTYPE_F16: add_parts_kernel<<<grid, 256, 0, s>>>(parts, static_cast<__half*>(out), count, splits); break;
+    default: add_parts_kernel<<<grid, 256, 0, s>>>(parts, static_cast<__nv_bfloat16*>(out), count, splits); break;
+  }
   return launch_status();
 }
 
