@@ -57,10 +57,14 @@ int ffn_simt_splits(int64_t M, int64_t N, int64_t K, int terms);
 int ffn_simt_launch(const FfnProduct& p, float* parts, cudaStream_t s);
 
 // bf16 and fp16 (ffn_tc.cu): operands 16-byte aligned with strides of whole 16
-// bytes. `parts`: splits * M * N floats where ffn_tc_splits says more than one
-// (kStore only), else nullptr.
-int ffn_tc_splits(int64_t M, int64_t N, int64_t K, int terms);
-int ffn_tc_launch(const FfnProduct& p, int dtype, float* parts, cudaStream_t s);
+// bytes. Up to kFfnMaxJobs products in one launch, which then share K, one term,
+// the order of their operands and the epilogue kStore. `parts`: the sum of
+// splits * M * N floats where ffn_tc_splits of all their tiles says more than
+// one (kStore only), else nullptr.
+constexpr int kFfnMaxJobs = 3;
+int64_t ffn_tc_tiles(int64_t M, int64_t N);
+int ffn_tc_splits(int64_t tiles, int64_t K, int terms);
+int ffn_tc_launch(const FfnProduct* p, int jobs, int dtype, float* parts, cudaStream_t s);
 
 // bf16 and fp16, the forward's products for at most kFewTokens rows of A
 // (ffn_few.cu): operands aligned as above.

@@ -71,24 +71,43 @@ int fit(Matrix& out, Scratch& scratch, const void* p, int64_t rows, int64_t cols
 // 2048, F = 8192, bf16, 8 tokens: XX us against 44.8 on the tensor-core tiles.)
 bool few(int64_t T, int dtype) { return half(dtype) && T <= kFewTokens; }
 
-int64_t parts_bytes(int64_t M, int64_t N, int64_t K, int terms, int dtype) {
-  const int splits = half(dtype) ? ffn_tc_splits(M, N, K, terms) : ffn_simt_splits(M, N, K, terms);
-  return splits > 1 ? splits * M * N * 4 : 0;
+// Float32 parts of products [M, N] summed over K, in one launch on the tensor
+// cores and one after the other on the FMA units (which then share them).
+struct Size {
+  int64_t M, N;
+};
+int64_t parts_bytes(std::initializer_list<Size> results, int64_t K, int terms, int dtype) {
+  int64_t tiles = 0, count = 0, most = 0;
+  for (const Size& r : results) {
+    tiles += ffn_tc_tiles(r.M, r.N);
+    count += r.M * r.N;
+    const int64_t splits = ffn_simt_splits(r.M, r.N, K, terms);
+    if (splits > 1 && splits * r.M * r.N * 4 > most) most = splits * r.M * r.N * 4;
+  }
+  if (!half(dtype)) return most;
+  const int64_t splits = ffn_tc_splits(tiles, K, terms);
+  return splits > 1 ? splits * count * 4 : 0;
 }
 
-// The sums of products one after the other share the largest one's parts.
+// The largest of what a call's launches need, whichever gradients it wants.
 int64_t most_parts(int backward, int64_t T, int64_t D, int64_t F, int64_t O, int dtype) {
-  if (!backward) return few(T, dtype) ? 0 : parts_bytes(T, O, F, 1, dtype);
-  int64_t m = parts_bytes(T, D, F, 2, dtype);
-  for (const int64_t b : {parts_bytes(F, D, T, 1, dtype), parts_bytes(O, F, T, 1, dtype)})
-    if (b > m) m = b;
-  return m;
+  if (!backward) return few(T, dtype) ? 0 : parts_bytes({{T, O}}, F, 1, dtype);
+  int64_t most = parts_bytes({{T, D}}, F, 2, dtype);
+  const Size g{F, D}, d{O, F};  // w_gate's or w_up's, w_down's
+  for (const int64_t b : {parts_bytes({g}, T, 1, dtype), parts_bytes({g, g}, T, 1, dtype), parts_bytes({d}, T, 1, dtype),
+                          parts_bytes({g, d}, T, 1, dtype), parts_bytes({g, g, d}, T, 1, dtype)})
+    if (b > most) most = b;
+  return most;
 }
 
-int run(const FfnProduct& p, int dtype, void* parts, cudaStream_t s) {
+int run(const FfnProduct* p, int jobs, int dtype, void* parts, cudaStream_t s) {
   float* f = static_cast<float*>(parts);
-  return half(dtype) ? ffn_tc_launch(p, dtype, f, s) : ffn_simt_launch(p, f, s);
+  if (half(dtype)) return ffn_tc_launch(p, jobs, dtype, f, s);
+  for (int j = 0; j < jobs; ++j)
+    if (int rc = ffn_simt_launch(p[j], f, s)) return rc;
+  return HC_OK;
 }
+int run(const FfnProduct& p, int dtype, void* parts, cudaStream_t s) { return run(&p, 1, dtype, parts, s); }
 
 FfnProduct store(int64_t M, int64_t N, int64_t K, FfnOperand A, FfnOperand B, void* out) {
   FfnProduct p{};
@@ -213,11 +232,10 @@ extern "C" int hc_gated_ffn_bwd(const void* g, const void* x, const void* w_gate
     p.B[1] = {wu.p, 1, wu.ld, D};
     if (int rc = run(p, dtype, parts, s)) return rc;
   }
-  if (grad_w_gate)
-    if (int rc = run(store(F, D, T, {d_gate, 1, Fp, F}, {mx.p, 1, mx.ld, D}, grad_w_gate), dtype, parts, s)) return rc;
-  if (grad_w_up)
-    if (int rc = run(store(F, D, T, {d_up, 1, Fp, F}, {mx.p, 1, mx.ld, D}, grad_w_up), dtype, parts, s)) return rc;
-  if (grad_w_down)
-    if (int rc = run(store(O, F, T, {mg.p, 1, mg.ld, O}, {h, 1, Fp, F}, grad_w_down), dtype, parts, s)) return rc;
-  return HC_OK;
+  FfnProduct weights[kFfnMaxJobs];  // the weights' gradients, all sums over the tokens
+  int jobs = 0;
+  if (grad_w_gate) weights[jobs++] = store(F, D, T, {d_gate, 1, Fp, F}, {mx.p, 1, mx.ld, D}, grad_w_gate);
+  if (grad_w_up) weights[jobs++] = store(F, D, T, {d_up, 1, Fp, F}, {mx.p, 1, mx.ld, D}, grad_w_up);
+  if (grad_w_down) weights[jobs++] = store(O, F, T, {mg.p, 1, mg.ld, O}, {h, 1, Fp, F}, grad_w_down);
+  return jobs ? run(weights, jobs, dtype, parts, s) : HC_OK;
 }

@@ -1,40 +1,41 @@
 // ffn_simt.cu — the gated feed-forward's float32 products on the FMA units (the
 // tensor cores have no float32 inputs): any size and order.
 //
-// 256 threads make a TM x TN tile of the result, TM / 16 x TN / 16 values a
-// thread, over stages of 16 steps of the sum in two shared-memory buffers. A
-// thread's loads are a pointer and constant steps from it. With 8 x 8 values a
-// thread the FMA units bound the kernel (64 FMAs on four 16-byte shared loads);
-// smaller products take 64 x 64 tiles, and where even those are few they split
-// their sum over CTAs, whose parts one more kernel adds in order: a lone CTA on
-// an SM waits for its loads at every stage.
+// 256 threads make a 64 x 64 tile of the result, 4 x 4 values a thread, over
+// stages of 16 steps of the sum in two shared-memory buffers; a thread's loads
+// are a pointer and constant steps from it. Three or four CTAs an SM hide each
+// other's waits (0.75 instructions a cycle; 128 x 128 tiles of 8 x 8 values, one
+// or two CTAs an SM, ran at 0.58 and took 12-18% more time at 4096 x 1024 x
+// 2048, and pairs of float32 in one instruction changed nothing). Products with
+// few tiles split their sum over CTAs, whose parts one more kernel adds in
+// order.
 #include "ffn.cuh"
 
 namespace hc {
 namespace {
 
-constexpr int kDepth = 16, kThreads = 256;
+constexpr int kTile = 64, kDepth = 16, kThreads = 256, kPitch = kTile + 4;
 
-// ROWS rows of an operand, 16 steps at a time, neighbouring threads along its
+// kTile rows of an operand, 16 steps at a time, neighbouring threads along its
 // unit stride. Rows and steps past the operand's end count as 0.
-template <typename T, int ROWS> struct Loader {
-  static constexpr int kLoads = ROWS * kDepth / kThreads;
+template <typename T> struct Loader {
+  static constexpr int kLoads = kTile * kDepth / kThreads;
   const T* p;
   int64_t step, advance;  // from one of a thread's loads to the next; from stage to stage
   uint32_t rows;          // bit i: the row of load i exists
   int k, k_step;          // of load 0, and from load to load
   int at, at_step;        // place in the [step][row] buffer
-  __device__ __forceinline__ Loader(const FfnOperand& o, int64_t row0, int64_t k0, int pitch) {
+  __device__ __forceinline__ Loader(const FfnOperand& o, int64_t row0, int64_t k0) {
     const bool along = o.k_stride == 1;  // else along the rows
-    const int row = along ? threadIdx.x / kDepth : threadIdx.x % ROWS;
+    const int row = along ? threadIdx.x / kDepth : threadIdx.x % kTile;
     const int row_step = along ? kThreads / kDepth : 0;
-    k = along ? threadIdx.x % kDepth : threadIdx.x / ROWS;
-    k_step = along ? 0 : kThreads / ROWS;
+    k = along ? threadIdx.x % kDepth : threadIdx.x / kTile;
+    k_step = along ? 0 : kThreads / kTile;
     p = static_cast<const T*>(o.p) + (row0 + row) * o.row_stride + (k0 + k) * o.k_stride;
     step = row_step * o.row_stride + k_step * o.k_stride;
     advance = kDepth * o.k_stride;
-    at = k * pitch + row;
-    at_step = k_step * pitch + row_step;
+    at = k * kPitch + row;
+    at_step = k_step * kPitch + row_step;
     rows = 0;
 #pragma unroll
     for (int i = 0; i < kLoads; ++i) rows |= (row0 + row + i * row_step < o.rows ? 1u : 0u) << i;
@@ -51,13 +52,13 @@ template <typename T, int ROWS> struct Loader {
   }
 };
 
-template <typename T, int EPI, int TM, int TN>
+template <typename T, int EPI>
 __global__ void __launch_bounds__(kThreads) ffn_simt_kernel(const __grid_constant__ FfnProduct p, float* parts, int splits) {
-  constexpr int NB = EPI == kGlu ? 2 : 1, VM = TM / 16, VN = TN / 16, PM = TM + 4, PN = TN + 4;
-  __shared__ __align__(16) float sA[2][kDepth * PM], sB[2][NB][kDepth * PN];
+  constexpr int NB = EPI == kGlu ? 2 : 1, V = kTile / 16;
+  __shared__ __align__(16) float sA[2][kDepth * kPitch], sB[2][NB][kDepth * kPitch];
   const int tx = threadIdx.x % 16, ty = threadIdx.x / 16;
-  const int64_t m0 = static_cast<int64_t>(blockIdx.y) * TM, n0 = static_cast<int64_t>(blockIdx.x) * TN;
-  float acc[NB][VM][VN] = {};
+  const int64_t m0 = static_cast<int64_t>(blockIdx.y) * kTile, n0 = static_cast<int64_t>(blockIdx.x) * kTile;
+  float acc[NB][V][V] = {};
   // this CTA's stages of all terms' sums
   const int64_t per_term = (p.K + kDepth - 1) / kDepth, stages = per_term * p.terms;
   const int64_t s0 = stages * blockIdx.z / splits, s1 = stages * (blockIdx.z + 1) / splits;
@@ -65,9 +66,9 @@ __global__ void __launch_bounds__(kThreads) ffn_simt_kernel(const __grid_constan
     const int64_t first = s0 > term * per_term ? s0 - term * per_term : 0;
     const int64_t last = s1 - term * per_term < per_term ? s1 - term * per_term : per_term;
     if (first >= last) continue;
-    Loader<T, TM> la(p.A[term], m0, first * kDepth, PM);
-    Loader<T, TN> lb(p.B[term], n0, first * kDepth, PN), lb2(p.B[NB == 2 ? 1 : term], n0, first * kDepth, PN);
-    float ra[la.kLoads], rb[NB][Loader<T, TN>::kLoads];
+    Loader<T> la(p.A[term], m0, first * kDepth);
+    Loader<T> lb(p.B[term], n0, first * kDepth), lb2(p.B[NB == 2 ? 1 : term], n0, first * kDepth);
+    float ra[Loader<T>::kLoads], rb[NB][Loader<T>::kLoads];
     auto load = [&](int64_t st) {
       la.load(p.K - st * kDepth, ra);
       lb.load(p.K - st * kDepth, rb[0]);
@@ -86,24 +87,16 @@ __global__ void __launch_bounds__(kThreads) ffn_simt_kernel(const __grid_constan
       if (st + 1 < last) load(st + 1);  // the next stage travels while this one is used
 #pragma unroll
       for (int k = 0; k < kDepth; ++k) {
-        float a[VM];
-#pragma unroll
-        for (int h = 0; h < VM; h += 4) {  // rows 4 ty + 64 (h / 4) + 0 .. 3
-          const float4 v = *reinterpret_cast<const float4*>(&sA[buf][k * PM + 16 * h + 4 * ty]);
-          a[h] = v.x; a[h + 1] = v.y; a[h + 2] = v.z; a[h + 3] = v.w;
-        }
+        const float4 av = *reinterpret_cast<const float4*>(&sA[buf][k * kPitch + V * ty]);
+        const float a[V] = {av.x, av.y, av.z, av.w};
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
-          float w[VN];
+          const float4 bv = *reinterpret_cast<const float4*>(&sB[buf][b][k * kPitch + V * tx]);
+          const float w[V] = {bv.x, bv.y, bv.z, bv.w};
 #pragma unroll
-          for (int h = 0; h < VN; h += 4) {
-            const float4 v = *reinterpret_cast<const float4*>(&sB[buf][b][k * PN + 16 * h + 4 * tx]);
-            w[h] = v.x; w[h + 1] = v.y; w[h + 2] = v.z; w[h + 3] = v.w;
-          }
+          for (int i = 0; i < V; ++i)
 #pragma unroll
-          for (int i = 0; i < VM; ++i)
-#pragma unroll
-            for (int j = 0; j < VN; ++j) acc[b][i][j] = fmaf(a[i], w[j], acc[b][i][j]);
+            for (int j = 0; j < V; ++j) acc[b][i][j] = fmaf(a[i], w[j], acc[b][i][j]);
         }
       }
       if (st + 1 < last) put(buf ^ 1);
@@ -111,10 +104,10 @@ __global__ void __launch_bounds__(kThreads) ffn_simt_kernel(const __grid_constan
     }
   }
 #pragma unroll
-  for (int i = 0; i < VM; ++i)
+  for (int i = 0; i < V; ++i)
 #pragma unroll
-    for (int j = 0; j < VN; ++j) {
-      const int64_t m = m0 + 4 * ty + 64 * (i / 4) + i % 4, n = n0 + 4 * tx + 64 * (j / 4) + j % 4;
+    for (int j = 0; j < V; ++j) {
+      const int64_t m = m0 + V * ty + i, n = n0 + V * tx + j;
       if (m >= p.M || n >= p.N) continue;
       const int64_t at = m * p.ldo + n;
       if constexpr (EPI == kStore) {
@@ -142,30 +135,19 @@ __global__ void __launch_bounds__(kThreads) ffn_simt_kernel(const __grid_constan
 }  // namespace
 
 namespace {
-int64_t tiles(int64_t M, int64_t N, int tm, int tn) { return (M + tm - 1) / tm * ((N + tn - 1) / tn); }
-
-// 128 x 128 tiles (128 x 64 of two weights) where they give every SM one.
-bool wide(int64_t M, int64_t N, bool glu) { return tiles(M, N, 128, glu ? 64 : 128) >= sm_count(); }
-
 template <int EPI> int launch(const FfnProduct& p, float* parts, int splits, cudaStream_t s) {
-  constexpr int kWideN = EPI == kGlu ? 64 : 128;
-  const bool w = wide(p.M, p.N, EPI == kGlu);
-  const int tm = w ? 128 : 64, tn = w ? kWideN : 64;
-  const dim3 grid(static_cast<unsigned>((p.N + tn - 1) / tn), static_cast<unsigned>((p.M + tm - 1) / tm), splits);
-  if (w)
-    ffn_simt_kernel<float, EPI, 128, kWideN><<<grid, kThreads, 0, s>>>(p, parts, splits);
-  else
-    ffn_simt_kernel<float, EPI, 64, 64><<<grid, kThreads, 0, s>>>(p, parts, splits);
+  const dim3 grid(static_cast<unsigned>((p.N + kTile - 1) / kTile), static_cast<unsigned>((p.M + kTile - 1) / kTile), splits);
+  ffn_simt_kernel<float, EPI><<<grid, kThreads, 0, s>>>(p, parts, splits);
   return launch_status();
 }
 }  // namespace
 
-// CTAs that share the sum of one 64 x 64 tile: until there are four an SM, each
-// with at least 8 stages (128 steps) of its own. (517 x 333 x 887, forward and
-// backward: XX us against 354 without.)
+// CTAs that share the sum of one tile: until there are four an SM, each with at
+// least 8 stages (128 steps) of its own. (517 x 333 x 887, forward and
+// backward: 210 us against 354 without.)
 int ffn_simt_splits(int64_t M, int64_t N, int64_t K, int terms) {
-  if (wide(M, N, false)) return 1;
-  const int64_t by_sms = 4 * sm_count() / tiles(M, N, 64, 64), by_depth = (K + kDepth - 1) / kDepth * terms / 8;
+  const int64_t tiles = ((M + kTile - 1) / kTile) * ((N + kTile - 1) / kTile);
+  const int64_t by_sms = 4 * sm_count() / tiles, by_depth = (K + kDepth - 1) / kDepth * terms / 8;
   const int64_t s = by_sms < by_depth ? by_sms : by_depth;
   return static_cast<int>(s < 1 ? 1 : s > 32 ? 32 : s);
 }

@@ -55,19 +55,29 @@ constexpr int kFinishWarp = 4;  // the first of the eight finishing warps
 constexpr int kSmemBytes = kStages * kStageBytes + 1024;
 constexpr int kGroupM = 8;  // tiles of A that neighbouring clusters share B with
 
+// Operands by term of a sum of two products, or by job of a launch of several.
 struct alignas(64) TcMaps {
-  CUtensorMap a[2], b[2];
+  CUtensorMap a[kFfnMaxJobs], b[kFfnMaxJobs];
+};
+
+// One result. A launch of several shares the depth of the sum and the operands'
+// order.
+struct TcJob {
+  int64_t M, N, ldo;
+  void* out;
+  float* parts;  // float32 parts [splits][M][N], or nullptr
+  int tiles_m, tiles_n;
+  int vec;  // bytes that the result's rows are aligned to (32, 16, or 2)
 };
 
 struct TcArgs {
-  int64_t M, N, ldo;
-  void *out, *out2;
+  TcJob job[kFfnMaxJobs];
+  void* out2;
   void *slope_gate, *slope_up;  // kGlu: written (nullable); kGluBwd: read
-  float* parts;                 // float32 parts [splits][M][N], or nullptr
-  int tiles_m, tiles_n, splits;
+  int jobs, tiles, splits;  // tiles of all jobs
   int blocks_term, blocks;  // 64-deep blocks of one term, and of all
   int a_mn, b_mn;           // operands whose unit stride is their rows
-  int act, vec;             // vec: bytes that the result's rows are aligned to (32, 16, or 2)
+  int act;
   uint32_t wait_limit;
   unsigned int* status;
 };
@@ -132,7 +142,14 @@ __device__ __forceinline__ void acc_load16(uint32_t addr, uint32_t (&r)[16]) {
         "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
       : "r"(addr));
 }
-__device__ __forceinline__ void acc_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+// Until the loads issued so far are done; r is theirs, so that no use of it moves up.
+__device__ __forceinline__ void acc_wait(uint32_t (&r)[16]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                 "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
+               :
+               : "memory");
+}
 
 // Shared-memory matrix descriptor with the 128-byte swizzle. K-major: groups of
 // 8 rows are 1024 bytes apart. MN-major: groups of 8 steps of the sum are 1024
@@ -160,20 +177,30 @@ __device__ __forceinline__ void tell_stop(Shared& sh, const TcArgs& a) {
 
 // ------------------------------------------------------------------ tiles
 struct Item {
-  int m, n;          // tile
-  int split, k0, k1; // blocks of the sum
+  int job, m, n;       // result, and tile of it
+  int split, k0, k1;   // blocks of the sum
 };
-// Item i of the walk: kGroupM tiles of A for each tile of B, so that the
-// clusters at work share rows of both through L2.
+// Item i of the walk: the splits one after the other, in each the jobs, in each
+// kGroupM tiles of A for each tile of B, so that the clusters at work share
+// rows of both through L2.
 __device__ __forceinline__ Item item_at(const TcArgs& a, int i) {
-  const int tiles = a.tiles_m * a.tiles_n;
   Item it;
-  it.split = i / tiles;
-  int t = i - it.split * tiles;
-  const int per_group = kGroupM * a.tiles_n;
+  it.split = i / a.tiles;
+  int t = i - it.split * a.tiles;
+  it.job = 0;
+#pragma unroll
+  for (int j = 0; j + 1 < kFfnMaxJobs; ++j) {
+    const int n = a.job[j].tiles_m * a.job[j].tiles_n;
+    if (it.job == j && j + 1 < a.jobs && t >= n) {
+      t -= n;
+      it.job = j + 1;
+    }
+  }
+  const int tiles_m = a.job[it.job].tiles_m, tiles_n = a.job[it.job].tiles_n;
+  const int per_group = kGroupM * tiles_n;
   const int g = t / per_group;
   t -= g * per_group;
-  const int rows = min(kGroupM, a.tiles_m - g * kGroupM);
+  const int rows = min(kGroupM, tiles_m - g * kGroupM);
   it.n = t / rows;
   it.m = g * kGroupM + (t - it.n * rows);
   it.k0 = static_cast<int>(static_cast<int64_t>(a.blocks) * it.split / a.splits);
@@ -214,16 +241,39 @@ __device__ __forceinline__ void store16(T* row, int64_t n, int64_t N, int vec, c
       if (n + i < N) row[n + i] = Elem<T>::from_f(v[i]);
   }
 }
-template <typename T>
-__device__ __forceinline__ void load16(const T* row, int64_t n, int64_t N, float (&v)[16]) {
-  // the slopes' rows are multiples of 8 elements, 16-byte aligned
+// 16 values of a slope's row from column n on, as they lie (zeros past N; rows
+// are multiples of 8 elements on 16-byte boundaries).
+struct Raw16 {
+  uint32_t w[8];
+};
+template <typename T> __device__ __forceinline__ Raw16 load16(const T* row, int64_t n, int64_t N, int vec, bool live) {
+  Raw16 r;
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    float t[8] = {};
-    if (n + 8 * h + 8 <= N) unpack<T>(ld_nc_v4(row + n + 8 * h), t);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[8 * h + i] = t[i];
+  for (int i = 0; i < 8; ++i) r.w[i] = 0u;
+  if (!live) return r;
+  if (vec == 32 && n + 16 <= N) {
+    asm volatile("ld.global.nc.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                 : "=r"(r.w[0]), "=r"(r.w[1]), "=r"(r.w[2]), "=r"(r.w[3]), "=r"(r.w[4]), "=r"(r.w[5]), "=r"(r.w[6]),
+                   "=r"(r.w[7])
+                 : "l"(row + n));
+    return r;
   }
+#pragma unroll
+  for (int h = 0; h < 2; ++h)
+    if (n + 8 * h + 8 <= N) {
+      const uint4 q = ld_nc_v4(row + n + 8 * h);
+      r.w[4 * h] = q.x; r.w[4 * h + 1] = q.y; r.w[4 * h + 2] = q.z; r.w[4 * h + 3] = q.w;
+    }
+  return r;
+}
+template <typename T> __device__ __forceinline__ void values(const Raw16& r, float (&v)[16]) {
+  float t[8];
+  unpack<T>(make_uint4(r.w[0], r.w[1], r.w[2], r.w[3]), t);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] = t[i];
+  unpack<T>(make_uint4(r.w[4], r.w[5], r.w[6], r.w[7]), t);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[8 + i] = t[i];
 }
 
 // act(a) and act'(a) with the fast exponential: its error, a few 2^-22
@@ -241,81 +291,95 @@ __device__ __forceinline__ void fast_act(int act, float a, float& val, float& de
   }
 }
 
-template <typename T, int EPI>
-__device__ __forceinline__ void finish(const TcArgs& a, const Item& it, uint32_t acc, int rank, int quad, int half) {
-  const int lane = threadIdx.x & 31;
-  const int64_t row = static_cast<int64_t>(it.m) * kTileM + rank * kRows + 32 * quad + lane;
-  const bool live = row < a.M;
-  const uint32_t lanes = acc + (static_cast<uint32_t>(32 * quad) << 16);
-  if constexpr (EPI == kGlu) {
-    const int64_t n0 = static_cast<int64_t>(it.n) * kRows + half * 64;
-    T* h = static_cast<T*>(a.out) + row * a.ldo;
-    T* sg = a.slope_gate ? static_cast<T*>(a.slope_gate) + row * a.ldo : nullptr;
-    T* su = a.slope_up ? static_cast<T*>(a.slope_up) + row * a.ldo : nullptr;
-#pragma unroll 1
-    for (int c = 0; c < 64; c += 16) {
-      uint32_t ra[16], rb[16];
-      acc_load16(lanes + half * 64 + c, ra);
-      acc_load16(lanes + kRows + half * 64 + c, rb);
-      acc_wait();
-      if (live && n0 + c < a.N) {
-        float vh[16], vg[16], vu[16];
+// A finishing warp's part of a tile: 32 rows, half of the columns, 16 at a time.
+// The next columns' accumulators (and slopes) are on their way while these are
+// worked on. begin() asks for the first slopes before the accumulator is done.
+template <typename T, int EPI> struct Finish {
+  static constexpr int kColumns = EPI == kGlu ? 64 : 128, kSteps = kColumns / 16;
+  const TcArgs& a;
+  const TcJob& job;
+  int64_t row, n0;
+  bool live;
+  int split;
+  Raw16 g[2], u[2];
+
+  __device__ __forceinline__ Finish(const TcArgs& args, const Item& it, int rank, int quad, int half)
+      : a(args), job(args.job[it.job]), split(it.split) {
+    row = static_cast<int64_t>(it.m) * kTileM + rank * kRows + 32 * quad + (threadIdx.x & 31);
+    n0 = static_cast<int64_t>(it.n) * (EPI == kGlu ? kRows : kTileN) + half * kColumns;
+    live = row < job.M;
+  }
+  __device__ __forceinline__ void ask(int step) {
+    if constexpr (EPI == kGluBwd) {
+      const int64_t n = n0 + 16 * step;
+      g[step & 1] = load16<T>(static_cast<const T*>(a.slope_gate) + row * job.ldo, n, job.N, job.vec, live);
+      u[step & 1] = load16<T>(static_cast<const T*>(a.slope_up) + row * job.ldo, n, job.N, job.vec, live);
+    }
+  }
+  __device__ __forceinline__ void begin() { ask(0); }
+  // acc: this warp's lanes of the tile's accumulator, at its half of the columns
+  __device__ __forceinline__ void run(uint32_t acc) {
+    uint32_t r[2][16], q[2][16];
+    acc_load16(acc, r[0]);
+    if constexpr (EPI == kGlu) acc_load16(acc + kRows, q[0]);
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          float der;
-          const float b = __uint_as_float(rb[i]);
-          fast_act(a.act, __uint_as_float(ra[i]), vu[i], der);
-          vh[i] = vu[i] * b;
-          vg[i] = der * b;
-        }
-        store16<T>(h, n0 + c, a.N, a.vec, vh);
-        if (sg) {
-          store16<T>(sg, n0 + c, a.N, a.vec, vg);
-          store16<T>(su, n0 + c, a.N, a.vec, vu);
+    for (int st = 0; st < kSteps; ++st) {
+      const int64_t n = n0 + 16 * st;
+      acc_wait(r[st & 1]);
+      if constexpr (EPI == kGlu) acc_wait(q[st & 1]);
+      if (st + 1 < kSteps) {
+        acc_load16(acc + 16 * (st + 1), r[(st + 1) & 1]);
+        if constexpr (EPI == kGlu) acc_load16(acc + kRows + 16 * (st + 1), q[(st + 1) & 1]);
+        ask(st + 1);
+      }
+      float v[16];
+#pragma unroll
+      for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[st & 1][i]);
+      if (live && n < job.N) {
+        if constexpr (EPI == kGlu) {
+          float h[16], sg[16];
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            float der;
+            const float b = __uint_as_float(q[st & 1][i]);
+            fast_act(a.act, v[i], v[i], der);
+            h[i] = v[i] * b;
+            sg[i] = der * b;
+          }
+          store16<T>(static_cast<T*>(job.out) + row * job.ldo, n, job.N, job.vec, h);
+          if (a.slope_gate) {
+            store16<T>(static_cast<T*>(a.slope_gate) + row * job.ldo, n, job.N, job.vec, sg);
+            store16<T>(static_cast<T*>(a.slope_up) + row * job.ldo, n, job.N, job.vec, v);
+          }
+        } else if constexpr (EPI == kGluBwd) {
+          float x[16], y[16];
+          values<T>(g[st & 1], x);
+          values<T>(u[st & 1], y);
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            x[i] *= v[i];
+            y[i] *= v[i];
+          }
+          store16<T>(static_cast<T*>(job.out) + row * job.ldo, n, job.N, job.vec, x);
+          store16<T>(static_cast<T*>(a.out2) + row * job.ldo, n, job.N, job.vec, y);
+        } else if (job.parts) {
+          float* p = job.parts + (static_cast<int64_t>(split) * job.M + row) * job.N + n;
+          if ((job.N & 7) == 0) {
+            if (n + 8 <= job.N) st_v8(p, r[st & 1]);
+            if (n + 16 <= job.N) st_v8(p + 8, r[st & 1] + 8);
+          } else {
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+              if (n + i < job.N) p[i] = v[i];
+          }
+        } else {
+          store16<T>(static_cast<T*>(job.out) + row * job.ldo, n, job.N, job.vec, v);
         }
       }
       __syncwarp();  // the next load is the whole warp's
     }
-  } else {
-    const int64_t n0 = static_cast<int64_t>(it.n) * kTileN + half * 128;
-#pragma unroll 1
-    for (int c = 0; c < 128; c += 16) {
-      uint32_t r[16];
-      acc_load16(lanes + half * 128 + c, r);
-      acc_wait();
-      if (live && n0 + c < a.N) {
-        float v[16];
-#pragma unroll
-        for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
-        if constexpr (EPI == kGluBwd) {
-          float g[16], u[16];
-          load16<T>(static_cast<const T*>(a.slope_gate) + row * a.ldo, n0 + c, a.N, g);
-          load16<T>(static_cast<const T*>(a.slope_up) + row * a.ldo, n0 + c, a.N, u);
-#pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            g[i] *= v[i];
-            u[i] *= v[i];
-          }
-          store16<T>(static_cast<T*>(a.out) + row * a.ldo, n0 + c, a.N, a.vec, g);
-          store16<T>(static_cast<T*>(a.out2) + row * a.ldo, n0 + c, a.N, a.vec, u);
-        } else if (a.parts) {
-          float* p = a.parts + (static_cast<int64_t>(it.split) * a.M + row) * a.N + n0 + c;
-          if ((a.N & 7) == 0) {
-            if (n0 + c + 8 <= a.N) st_v8(p, r);
-            if (n0 + c + 16 <= a.N) st_v8(p + 8, r + 8);
-          } else {
-#pragma unroll
-            for (int i = 0; i < 16; ++i)
-              if (n0 + c + i < a.N) p[i] = v[i];
-          }
-        } else {
-          store16<T>(static_cast<T*>(a.out) + row * a.ldo, n0 + c, a.N, a.vec, v);
-        }
-      }
-      __syncwarp();
-    }
   }
-}
+};
 
 template <typename T, int EPI>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
@@ -325,7 +389,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   const uint32_t ring = (smem_u32(raw) + 1023) & ~1023u;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = cluster_rank();
-  const int items = a.tiles_m * a.tiles_n * a.splits;
+  const int items = a.tiles * a.splits;
   const int first = blockIdx.x >> 1, step = gridDim.x >> 1;
 
   if (threadIdx.x == 0) {
@@ -368,8 +432,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           }
           const int term = kb >= a.blocks_term ? 1 : 0;
           const int k = (kb - term * a.blocks_term) * kDepth;
-          const CUtensorMap* ma = &maps.a[term];
-          const CUtensorMap* mb = &maps.b[EPI == kGlu ? rank : term];
+          const CUtensorMap* ma = &maps.a[it.job + term];
+          const CUtensorMap* mb = &maps.b[EPI == kGlu ? static_cast<int>(rank) : it.job + term];
           const uint32_t bar = cluster_addr(&sh.full[s], 0);
           const uint32_t da = ring + s * kStageBytes, db = da + kOperandBytes;
           if (rank == 0) mbar_expect_tx(&sh.full[s], 2 * kStageBytes);
@@ -455,14 +519,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     int buf = 0;
     uint32_t acc_ph = 0;
     for (int i = first; i < items; i += step) {
-      const Item it = item_at(a, i);
+      Finish<T, EPI> tile(a, item_at(a, i), static_cast<int>(rank), quad, half);
+      tile.begin();
       const bool ok = pair_wait(sh, &sh.acc_full[buf], acc_ph, a.wait_limit);
       if (!__all_sync(kFull, ok)) {
         if (lane == 0) tell_stop(sh, a);
         break;
       }
       tc_fence_after();
-      finish<T, EPI>(a, it, tmem + buf * kTileN, static_cast<int>(rank), quad, half);
+      tile.run(tmem + buf * kTileN + (static_cast<uint32_t>(32 * quad) << 16) + half * tile.kColumns);
       tc_fence_before();
       __syncwarp();
       if (lane == 0) arrive_cluster(cluster_addr(&sh.acc_empty[buf], 0));
@@ -548,14 +613,16 @@ template <typename T> Kernel kernel_of(int epi) {
 
 // Clusters that share the sum of one tile: as many as there are for every
 // tile, each with at least 4 blocks (256 deep) of its own.
-int ffn_tc_splits(int64_t M, int64_t N, int64_t K, int terms) {
-  const int64_t tiles = ceil_div(M, kTileM) * ceil_div(N, kTileN), blocks = ceil_div(K, kDepth) * terms;
+int ffn_tc_splits(int64_t tiles, int64_t K, int terms) {
+  const int64_t blocks = ceil_div(K, kDepth) * terms;
   const int64_t by_pairs = pairs_resident() / tiles, by_depth = blocks / 4;
   const int64_t s = by_pairs < by_depth ? by_pairs : by_depth;
   return static_cast<int>(s < 1 ? 1 : s > 32 ? 32 : s);
 }
+int64_t ffn_tc_tiles(int64_t M, int64_t N) { return ceil_div(M, kTileM) * ceil_div(N, kTileN); }
 
-int ffn_tc_launch(const FfnProduct& p, int dtype, float* parts, cudaStream_t s) {
+int ffn_tc_launch(const FfnProduct* ps, int jobs, int dtype, float* parts, cudaStream_t s) {
+  const FfnProduct& p = ps[0];
   const bool bf = dtype == HC_DTYPE_BF16;
   const Kernel kernel = bf ? kernel_of<__nv_bfloat16>(p.epilogue) : kernel_of<__half>(p.epilogue);
   // A call of the runtime before the first one of the driver's encoder: on a
@@ -566,36 +633,48 @@ int ffn_tc_launch(const FfnProduct& p, int dtype, float* parts, cudaStream_t s) 
   }
   TcMaps maps{};
   TcArgs a{};
-  const int nb = p.epilogue == kGlu ? 2 : p.terms;
-  for (int t = 0; t < 2; ++t)
-    if (!encode_operand(&maps.a[t], p.A[t < p.terms ? t : 0], p.K) ||
-        !encode_operand(&maps.b[t], p.B[t < nb ? t : 0], p.K))
-      return HC_ERR_LAUNCH;
-  a.M = p.M; a.N = p.N; a.ldo = p.ldo;
-  a.out = p.out; a.out2 = p.out2; a.slope_gate = p.slope_gate; a.slope_up = p.slope_up;
-  a.tiles_m = static_cast<int>(ceil_div(p.M, kTileM));
-  a.tiles_n = static_cast<int>(ceil_div(p.N, p.epilogue == kGlu ? kRows : kTileN));
-  a.splits = p.epilogue == kStore ? ffn_tc_splits(p.M, p.N, p.K, p.terms) : 1;
-  a.parts = a.splits > 1 ? parts : nullptr;
-  if (a.splits > 1 && !parts) return HC_ERR_SCRATCH;
+  a.jobs = jobs;
+  for (int j = 0; j < jobs; ++j) {
+    const int nb = ps[j].epilogue == kGlu ? 2 : ps[j].terms;
+    for (int t = 0; t < ps[j].terms; ++t)
+      if (!encode_operand(&maps.a[j + t], ps[j].A[t], p.K)) return HC_ERR_LAUNCH;
+    for (int t = 0; t < nb; ++t)
+      if (!encode_operand(&maps.b[j + t], ps[j].B[t], p.K)) return HC_ERR_LAUNCH;
+    TcJob& job = a.job[j];
+    job.M = ps[j].M; job.N = ps[j].N; job.ldo = ps[j].ldo; job.out = ps[j].out;
+    job.tiles_m = static_cast<int>(ceil_div(job.M, kTileM));
+    job.tiles_n = static_cast<int>(ceil_div(job.N, p.epilogue == kGlu ? kRows : kTileN));
+    const uintptr_t base = reinterpret_cast<uintptr_t>(job.out) | reinterpret_cast<uintptr_t>(ps[j].out2) |
+                           reinterpret_cast<uintptr_t>(ps[j].slope_gate) | reinterpret_cast<uintptr_t>(ps[j].slope_up) |
+                           static_cast<uintptr_t>(2 * job.ldo);
+    job.vec = base % 32 == 0 ? 32 : base % 16 == 0 ? 16 : 2;
+    if (static_cast<int64_t>(job.tiles_m) * job.tiles_n > (int64_t(1) << 24)) return HC_ERR_BAD_SIZE;
+    a.tiles += job.tiles_m * job.tiles_n;
+  }
+  a.out2 = p.out2; a.slope_gate = p.slope_gate; a.slope_up = p.slope_up;
+  a.splits = p.epilogue == kStore ? ffn_tc_splits(a.tiles, p.K, p.terms) : 1;
+  if (a.splits > 1) {
+    if (!parts) return HC_ERR_SCRATCH;
+    float* at = parts;
+    for (int j = 0; j < jobs; ++j) {
+      a.job[j].parts = at;
+      at += a.splits * ps[j].M * ps[j].N;
+    }
+  }
   a.blocks_term = static_cast<int>(ceil_div(p.K, kDepth));
   a.blocks = a.blocks_term * p.terms;
   a.a_mn = p.A[0].k_stride != 1;
   a.b_mn = p.B[0].k_stride != 1;
   a.act = p.act;
-  const uintptr_t base = reinterpret_cast<uintptr_t>(p.out) | reinterpret_cast<uintptr_t>(p.out2) |
-                         reinterpret_cast<uintptr_t>(p.epilogue == kGlu ? p.slope_gate : nullptr) |
-                         reinterpret_cast<uintptr_t>(p.epilogue == kGlu ? p.slope_up : nullptr) |
-                         static_cast<uintptr_t>(2 * p.ldo);
-  a.vec = base % 32 == 0 ? 32 : base % 16 == 0 ? 16 : 2;
   a.wait_limit = wait_poll_limit();
   a.status = timeout_word(s);
-  const int64_t items = static_cast<int64_t>(a.tiles_m) * a.tiles_n * a.splits;
-  if (items > (int64_t(1) << 30)) return HC_ERR_BAD_SIZE;
-  const int pairs = static_cast<int>(items < pairs_resident() ? items : pairs_resident());
+  const int items = a.tiles * a.splits, pairs = items < pairs_resident() ? items : pairs_resident();
   kernel<<<2 * pairs, kThreads, kSmemBytes, s>>>(maps, a);
   if (int rc = launch_status()) return rc;
-  return a.splits > 1 ? ffn_add_parts(parts, p.out, p.M * p.N, a.splits, dtype, s) : HC_OK;
+  if (a.splits > 1)
+    for (int j = 0; j < jobs; ++j)
+      if (int rc = ffn_add_parts(a.job[j].parts, ps[j].out, ps[j].M * ps[j].N, a.splits, dtype, s)) return rc;
+  return HC_OK;
 }
 
 int ffn_add_parts(const float* parts, void* out, int64_t count, int splits, int dtype, cudaStream_t s) {
