@@ -42,7 +42,7 @@ __device__ __forceinline__ void ffn_act(int act, float a, float& val, float& der
     val = a * s;
     der = s + val * (1.f - s);
   } else {  // 0.5 a (1 + tanh(c (a + 0.044715 a^3))), c = sqrt(2 / pi)
-    const float c = 0.7978845608028654f, a2 = a * a;
+    const float c = 0.7978845608028654f, a2 = fminf(a * a, 1e4f);  // past |a| = 10 the tanh is 1: a^2 need not grow
     const float t = tanhf(c * a * (1.f + 0.044715f * a2));
     val = 0.5f * a * (1.f + t);
     der = 0.5f * (1.f + t) + 0.5f * a * (1.f - t * t) * c * (1.f + 3.f * 0.044715f * a2);

@@ -14,9 +14,9 @@
 //   warp 1      multiplies (in the leader CTA): one lane issues the four
 //               16-deep steps of a stage for both CTAs
 //   warp 2      owns the tensor memory
-//   warps 4-11  finish: two groups of four warps read the accumulator out of
-//               tensor memory, half of the columns each, and write the result
-//               while the next tile is multiplied into the other half of
+//   warps 4-19  finish: four groups of four warps read the accumulator out of
+//               tensor memory, a quarter of the columns each, and write the
+//               result while the next tile is multiplied into the other half of
 //               tensor memory (2 x 256 of its 512 columns)
 //
 // An operand is read as it lies: summed along its unit stride ("K-major", x
@@ -50,8 +50,9 @@ constexpr int kDepth = 64;         // elements of the sum in a stage: 128 bytes
 constexpr int kStages = 6;
 constexpr int kOperandBytes = kRows * kDepth * 2;
 constexpr int kStageBytes = 2 * kOperandBytes;
-constexpr int kThreads = 384;
-constexpr int kFinishWarp = 4;  // the first of the eight finishing warps
+constexpr int kFinishWarp = 4;    // the first of the finishing warps
+constexpr int kFinishWarps = 16;  // four a scheduler: with two, the activation's chains left it idle two cycles in three
+constexpr int kThreads = 32 * (kFinishWarp + kFinishWarps);
 constexpr int kSmemBytes = kStages * kStageBytes + 1024;
 constexpr int kGroupM = 8;  // tiles of A that neighbouring clusters share B with
 
@@ -223,12 +224,9 @@ __device__ __forceinline__ void st_v8(void* p, const uint32_t* w) {
                "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
                : "memory");
 }
-// 16 values of one row from column n on; columns past N are not written.
+// 16 values of one row from column n on, in pairs; columns past N are not written.
 template <typename T>
-__device__ __forceinline__ void store16(T* row, int64_t n, int64_t N, int vec, const float (&v)[16]) {
-  uint32_t w[8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) w[i] = pack2<T>(v[2 * i], v[2 * i + 1]);
+__device__ __forceinline__ void store16(T* row, int64_t n, int64_t N, int vec, const uint32_t (&w)[8]) {
   if (vec == 32 && n + 16 <= N) {
     st_v8(row + n, w);
   } else if (vec >= 16) {
@@ -238,7 +236,7 @@ __device__ __forceinline__ void store16(T* row, int64_t n, int64_t N, int vec, c
   } else {
 #pragma unroll
     for (int i = 0; i < 16; ++i)
-      if (n + i < N) row[n + i] = Elem<T>::from_f(v[i]);
+      if (n + i < N) reinterpret_cast<uint16_t*>(row)[n + i] = static_cast<uint16_t>(w[i / 2] >> (16 * (i % 2)));
   }
 }
 // 16 values of a slope's row from column n on, as they lie (zeros past N; rows
@@ -276,26 +274,40 @@ template <typename T> __device__ __forceinline__ void values(const Raw16& r, flo
   for (int i = 0; i < 8; ++i) v[8 + i] = t[i];
 }
 
-// act(a) and act'(a) with the fast exponential: its error, a few 2^-22
-// relative, is far below the half step 2^-9 / 2^-12 of the types they go to.
+__device__ __forceinline__ float exp2_fast(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+__device__ __forceinline__ float inverse_fast(float x) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+// act(a) and act'(a) with the approximate exponential and inverse: their
+// errors, a few 2^-22 relative, are far below the half steps 2^-8 and 2^-11 of
+// the types they go to.
 __device__ __forceinline__ void fast_act(int act, float a, float& val, float& der) {
+  constexpr float kLog2e = 1.4426950408889634f;
   if (act == HC_ACT_SILU) {
-    const float s = __fdividef(1.f, 1.f + __expf(-a));
+    const float s = inverse_fast(1.f + exp2_fast(-kLog2e * a));
     val = a * s;
     der = fmaf(val, 1.f - s, s);
-  } else {
-    const float c = 0.7978845608028654f, a2 = a * a;
-    const float t = 1.f - __fdividef(2.f, 1.f + __expf(2.f * c * a * fmaf(0.044715f, a2, 1.f)));
-    val = 0.5f * a * (1.f + t);
-    der = fmaf(0.5f * a * (1.f - t * t), c * fmaf(3.f * 0.044715f, a2, 1.f), 0.5f * (1.f + t));
+  } else {  // tanh(u) = 1 - 2 / (1 + e^2u); past |a| = 10 it is 1, and a^2 need not grow
+    constexpr float c = 0.7978845608028654f;
+    const float a2 = fminf(a * a, 1e4f), half = 0.5f * a;
+    const float i = inverse_fast(1.f + exp2_fast((2.f * c * kLog2e) * a * fmaf(0.044715f, a2, 1.f)));
+    const float t = fmaf(-2.f, i, 1.f);
+    val = fmaf(half, t, half);
+    der = fmaf(half * fmaf(-t, t, 1.f), fmaf(3.f * 0.044715f * c, a2, c), fmaf(0.5f, t, 0.5f));
   }
 }
 
-// A finishing warp's part of a tile: 32 rows, half of the columns, 16 at a time.
-// The next columns' accumulators (and slopes) are on their way while these are
-// worked on. begin() asks for the first slopes before the accumulator is done.
+// A finishing warp's part of a tile: 32 rows, a quarter of the columns, 16 at a
+// time. begin() asks for the first slopes before the accumulator is done, each
+// step for the next one's.
 template <typename T, int EPI> struct Finish {
-  static constexpr int kColumns = EPI == kGlu ? 64 : 128, kSteps = kColumns / 16;
+  static constexpr int kColumns = (EPI == kGlu ? kRows : kTileN) / (kFinishWarps / 4), kSteps = kColumns / 16;
   const TcArgs& a;
   const TcJob& job;
   int64_t row, n0;
@@ -303,10 +315,10 @@ template <typename T, int EPI> struct Finish {
   int split;
   Raw16 g[2], u[2];
 
-  __device__ __forceinline__ Finish(const TcArgs& args, const Item& it, int rank, int quad, int half)
+  __device__ __forceinline__ Finish(const TcArgs& args, const Item& it, int rank, int quad, int part)
       : a(args), job(args.job[it.job]), split(it.split) {
     row = static_cast<int64_t>(it.m) * kTileM + rank * kRows + 32 * quad + (threadIdx.x & 31);
-    n0 = static_cast<int64_t>(it.n) * (EPI == kGlu ? kRows : kTileN) + half * kColumns;
+    n0 = static_cast<int64_t>(it.n) * (EPI == kGlu ? kRows : kTileN) + part * kColumns;
     live = row < job.M;
   }
   __device__ __forceinline__ void ask(int step) {
@@ -317,63 +329,65 @@ template <typename T, int EPI> struct Finish {
     }
   }
   __device__ __forceinline__ void begin() { ask(0); }
-  // acc: this warp's lanes of the tile's accumulator, at its half of the columns
+  // acc: this warp's lanes of the tile's accumulator, at its quarter of the columns
   __device__ __forceinline__ void run(uint32_t acc) {
-    uint32_t r[2][16], q[2][16];
-    acc_load16(acc, r[0]);
-    if constexpr (EPI == kGlu) acc_load16(acc + kRows, q[0]);
 #pragma unroll
     for (int st = 0; st < kSteps; ++st) {
       const int64_t n = n0 + 16 * st;
-      acc_wait(r[st & 1]);
-      if constexpr (EPI == kGlu) acc_wait(q[st & 1]);
-      if (st + 1 < kSteps) {
-        acc_load16(acc + 16 * (st + 1), r[(st + 1) & 1]);
-        if constexpr (EPI == kGlu) acc_load16(acc + kRows + 16 * (st + 1), q[(st + 1) & 1]);
-        ask(st + 1);
-      }
-      float v[16];
-#pragma unroll
-      for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[st & 1][i]);
+      uint32_t r[16], q[16];
+      acc_load16(acc + 16 * st, r);
+      if constexpr (EPI == kGlu) acc_load16(acc + kRows + 16 * st, q);
+      if (st + 1 < kSteps) ask(st + 1);
+      acc_wait(r);
+      if constexpr (EPI == kGlu) acc_wait(q);
       if (live && n < job.N) {
         if constexpr (EPI == kGlu) {
-          float h[16], sg[16];
+          uint32_t h[8], sg[8], su[8];
 #pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            float der;
-            const float b = __uint_as_float(q[st & 1][i]);
-            fast_act(a.act, v[i], v[i], der);
-            h[i] = v[i] * b;
-            sg[i] = der * b;
+          for (int i = 0; i < 8; ++i) {
+            float v[2], d[2], b[2];
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              b[e] = __uint_as_float(q[2 * i + e]);
+              fast_act(a.act, __uint_as_float(r[2 * i + e]), v[e], d[e]);
+            }
+            h[i] = pack2<T>(v[0] * b[0], v[1] * b[1]);
+            sg[i] = pack2<T>(d[0] * b[0], d[1] * b[1]);
+            su[i] = pack2<T>(v[0], v[1]);
           }
           store16<T>(static_cast<T*>(job.out) + row * job.ldo, n, job.N, job.vec, h);
           if (a.slope_gate) {
             store16<T>(static_cast<T*>(a.slope_gate) + row * job.ldo, n, job.N, job.vec, sg);
-            store16<T>(static_cast<T*>(a.slope_up) + row * job.ldo, n, job.N, job.vec, v);
+            store16<T>(static_cast<T*>(a.slope_up) + row * job.ldo, n, job.N, job.vec, su);
           }
         } else if constexpr (EPI == kGluBwd) {
-          float x[16], y[16];
+          uint32_t w[8];
+          float x[16];
           values<T>(g[st & 1], x);
-          values<T>(u[st & 1], y);
 #pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            x[i] *= v[i];
-            y[i] *= v[i];
-          }
-          store16<T>(static_cast<T*>(job.out) + row * job.ldo, n, job.N, job.vec, x);
-          store16<T>(static_cast<T*>(a.out2) + row * job.ldo, n, job.N, job.vec, y);
+          for (int i = 0; i < 8; ++i)
+            w[i] = pack2<T>(x[2 * i] * __uint_as_float(r[2 * i]), x[2 * i + 1] * __uint_as_float(r[2 * i + 1]));
+          store16<T>(static_cast<T*>(job.out) + row * job.ldo, n, job.N, job.vec, w);
+          values<T>(u[st & 1], x);
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            w[i] = pack2<T>(x[2 * i] * __uint_as_float(r[2 * i]), x[2 * i + 1] * __uint_as_float(r[2 * i + 1]));
+          store16<T>(static_cast<T*>(a.out2) + row * job.ldo, n, job.N, job.vec, w);
         } else if (job.parts) {
           float* p = job.parts + (static_cast<int64_t>(split) * job.M + row) * job.N + n;
           if ((job.N & 7) == 0) {
-            if (n + 8 <= job.N) st_v8(p, r[st & 1]);
-            if (n + 16 <= job.N) st_v8(p + 8, r[st & 1] + 8);
+            if (n + 8 <= job.N) st_v8(p, r);
+            if (n + 16 <= job.N) st_v8(p + 8, r + 8);
           } else {
 #pragma unroll
             for (int i = 0; i < 16; ++i)
-              if (n + i < job.N) p[i] = v[i];
+              if (n + i < job.N) p[i] = __uint_as_float(r[i]);
           }
         } else {
-          store16<T>(static_cast<T*>(job.out) + row * job.ldo, n, job.N, job.vec, v);
+          uint32_t w[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) w[i] = pack2<T>(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1]));
+          store16<T>(static_cast<T*>(job.out) + row * job.ldo, n, job.N, job.vec, w);
         }
       }
       __syncwarp();  // the next load is the whole warp's
@@ -399,7 +413,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(&sh.acc_full[b], 1);
-      mbar_init(&sh.acc_empty[b], 16);  // the eight finishing warps of both CTAs
+      mbar_init(&sh.acc_empty[b], 2 * kFinishWarps);  // of both CTAs
     }
     mbar_init(&sh.drain, 1);
     sh.stop = 0;
@@ -515,11 +529,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       }
     }
   } else if (warp >= kFinishWarp) {
-    const int quad = warp & 3, half = (warp - kFinishWarp) >> 2;
+    const int quad = warp & 3, part = (warp - kFinishWarp) >> 2;
     int buf = 0;
     uint32_t acc_ph = 0;
     for (int i = first; i < items; i += step) {
-      Finish<T, EPI> tile(a, item_at(a, i), static_cast<int>(rank), quad, half);
+      Finish<T, EPI> tile(a, item_at(a, i), static_cast<int>(rank), quad, part);
       tile.begin();
       const bool ok = pair_wait(sh, &sh.acc_full[buf], acc_ph, a.wait_limit);
       if (!__all_sync(kFull, ok)) {
@@ -527,7 +541,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         break;
       }
       tc_fence_after();
-      tile.run(tmem + buf * kTileN + (static_cast<uint32_t>(32 * quad) << 16) + half * tile.kColumns);
+      tile.run(tmem + buf * kTileN + (static_cast<uint32_t>(32 * quad) << 16) + part * tile.kColumns);
       tc_fence_before();
       __syncwarp();
       if (lane == 0) arrive_cluster(cluster_addr(&sh.acc_empty[buf], 0));
