@@ -801,6 +801,7 @@ def run_b200(args):
         import e2e_models as em
 
         for spec in (em.VIT, em.LM):
+            spec = em.gated(spec) if args.gated_models else spec
             models[spec.name] = time_model(spec, device, world, rank, steps=max(3, min(args.steps, 5)),
                                            warmup=3)
 
@@ -1205,6 +1206,8 @@ def main():
     ap.add_argument("--impl", choices=["b200", "reference"], default="b200")
     ap.add_argument("--no-cpu-baseline", action="store_true", help="skip the CPU baseline leg")
     ap.add_argument("--no-models", action="store_true", help="skip the end-to-end ViT / LM training legs")
+    ap.add_argument("--gated-models", action="store_true",
+                    help="time the ViT / LM legs with gated blocks (e2e_models.gated) instead")
     ap.add_argument("--fused-only", action="store_true",
                     help="time the headline fused step alone and print a short line (profiling, comparisons)")
     ap.add_argument("--n", type=int, default=N_STREAMS, help="with --fused-only: streams (16,384 tokens)")

@@ -20,19 +20,28 @@ is split evenly over the ranks (strong scaling), the model is wrapped in
 DistributedDataParallel (NCCL gradient all-reduce in buckets overlapped with
 the backward), and a rank's share is processed in micro-batches with
 gradient accumulation (all but the last under ``no_sync``).
+
+``gated(spec)`` is the same workload with gated blocks: the MLP is a gated
+feed-forward of the same hidden width (``ops.gated_ffn``, SiLU), each block's
+norm and a post-norm, a residual scale a channel and dropout are the
+hyper-connection layer's own (``BlockOptions``: ``ops.hc_read_norm`` and
+``ops.hc_mix_write_norm``), and the embedding is dropped out
+(``ops.hc_dropout``).
 """
 
 from __future__ import annotations
 
 import math
 import time
-from dataclasses import dataclass
+from dataclasses import dataclass, replace
 
 import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
+from hyperconnections_b200.block import BlockOptions
 from hyperconnections_b200.cghc import ContinuousGenHyperConnections
+from hyperconnections_b200.ops import gated_ffn, hc_dropout
 
 N_STREAMS = 4
 
@@ -49,16 +58,31 @@ class Spec:
     classes: int = 10       # vit
     vocab: int = 32000      # lm
     patch: int = 4          # vit
+    block: BlockOptions | None = None  # what the layers do around their blocks (None: LayerNorm in the block)
+    gated: bool = False                # gated feed-forward instead of the MLP
+    dropout: float = 0.0               # of the embedding
 
 
 VIT = Spec("vit", dim=384, depth=6, heads=6, global_batch=512, seq=64, micro_batch=512)
 LM = Spec("lm", dim=2048, depth=12, heads=16, global_batch=64, seq=2048, micro_batch=8)
 
+GATED = BlockOptions(pre_norm="rms", post_norm="rms", residual_scale=0.1, dropout=0.1)
+
+
+def gated(spec: Spec) -> Spec:
+    """The workload with gated blocks (see module doc)."""
+    return replace(spec, block=GATED, gated=True, dropout=GATED.dropout)
+
+
+def own_norm(dim: int, block: BlockOptions | None) -> nn.Module:
+    """A block's norm, unless its layer reads through one."""
+    return nn.Identity() if block is not None and block.pre_norm else nn.LayerNorm(dim)
+
 
 class Attention(nn.Module):
-    def __init__(self, dim: int, heads: int, causal: bool):
+    def __init__(self, dim: int, heads: int, causal: bool, block: BlockOptions | None = None):
         super().__init__()
-        self.norm = nn.LayerNorm(dim)
+        self.norm = own_norm(dim, block)
         self.qkv = nn.Linear(dim, 3 * dim)
         self.out = nn.Linear(dim, dim)
         self.heads, self.causal = heads, causal
@@ -81,8 +105,36 @@ class MLP(nn.Module):
         return self.fc2(F.gelu(self.fc1(self.norm(x)), approximate="tanh"))
 
 
-def hc(dim: int, module: nn.Module) -> ContinuousGenHyperConnections:
-    return ContinuousGenHyperConnections(N_STREAMS, 1, N_STREAMS * dim, dim, module)
+class GatedMLP(nn.Module):
+    def __init__(self, dim: int, block: BlockOptions | None = None):
+        super().__init__()
+        self.norm = own_norm(dim, block)
+        self.w_gate, self.w_up = (nn.Linear(dim, 4 * dim, bias=False) for _ in range(2))
+        self.w_down = nn.Linear(4 * dim, dim, bias=False)
+
+    def forward(self, x):
+        return gated_ffn(self.norm(x), self.w_gate.weight, self.w_up.weight, self.w_down.weight)
+
+
+class EmbeddingDropout(nn.Module):
+    """hc_dropout whose seed and step live on the device."""
+
+    def __init__(self, p: float):
+        super().__init__()
+        self.p = p
+        self.register_buffer("state", torch.stack([torch.randint(1 << 62, ()), torch.zeros((), dtype=torch.int64)]),
+                             persistent=False)
+
+    def forward(self, h):
+        if not self.training:
+            return h
+        out = hc_dropout(h, self.p, self.state)
+        self.state[1].add_(1)
+        return out
+
+
+def hc(dim: int, module: nn.Module, block: BlockOptions | None = None) -> ContinuousGenHyperConnections:
+    return ContinuousGenHyperConnections(N_STREAMS, 1, N_STREAMS * dim, dim, module, block=block)
 
 
 class Backbone(nn.Module):
@@ -92,11 +144,15 @@ class Backbone(nn.Module):
         super().__init__()
         self.layers = nn.ModuleList()
         for _ in range(spec.depth):
-            self.layers.append(hc(spec.dim, Attention(spec.dim, spec.heads, causal)))
-            self.layers.append(hc(spec.dim, MLP(spec.dim)))
+            self.layers.append(hc(spec.dim, Attention(spec.dim, spec.heads, causal, spec.block), spec.block))
+            mlp = GatedMLP(spec.dim, spec.block) if spec.gated else MLP(spec.dim)
+            self.layers.append(hc(spec.dim, mlp, spec.block))
         self.norm = nn.LayerNorm(spec.dim)
+        self.drop = EmbeddingDropout(spec.dropout) if spec.dropout else None
 
     def forward(self, h):
+        if self.drop is not None:
+            h = self.drop(h)
         x = h.to(torch.bfloat16).repeat(1, 1, N_STREAMS)  # the embedding in every stream
         for layer in self.layers:
             x = layer(x)
@@ -249,7 +305,7 @@ def flops_per_token(spec: Spec) -> float:
     """Dense training FLOPs per token (6 per weight of the blocks and head,
     plus the attention score / value products), for context only."""
     D, L = spec.dim, spec.depth
-    block = 12 * D * D
+    block = (16 if spec.gated else 12) * D * D  # attention 4, MLP 8, gated feed-forward 12
     head = D * (spec.vocab if spec.name == "lm" else 0)
     attn = 2 * 2 * spec.seq * D * (0.5 if spec.name == "lm" else 1.0)
     return 6 * (L * block + head) + 3 * L * attn
@@ -258,7 +314,7 @@ def flops_per_token(spec: Spec) -> float:
 def describe(spec: Spec) -> dict:
     return {"model": spec.name, "dim": spec.dim, "depth": spec.depth, "heads": spec.heads,
             "global_batch": spec.global_batch, "seq_len": spec.seq, "hc_streams": N_STREAMS,
-            "tokens_per_step": spec.global_batch * spec.seq, "mlp": "4x", "dtype": "bf16 autocast, fp32 master weights",
+            "tokens_per_step": spec.global_batch * spec.seq, "mlp": "4x gated" if spec.gated else "4x", "dtype": "bf16 autocast, fp32 master weights",
             **({"vocab": spec.vocab} if spec.name == "lm" else {"patch": spec.patch, "classes": spec.classes,
                                                                "image": "32x32x3"})}
 

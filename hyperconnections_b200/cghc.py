@@ -36,7 +36,8 @@ import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
-from .ops import cghc_transition, hc_mix_write, hc_read
+from .block import BlockOptions, BlockParts, read_block, write_block
+from .ops import cghc_transition
 
 GeneratorType = Literal["conservative", "psd_diss", "diagonal_diss", "laplacian", "conservative_diag_diss",
                         "conservative_psd_diss", "conservative_laplacian"]
@@ -59,14 +60,16 @@ class ContinuousGenHyperConnections(nn.Module):
     Args are the reference's (cghc.py:15-40): n streams, m backbone blocks,
     input_dim = n / m * embed_dim, the wrapped module, the generator type,
     projection ("mean" / "v" / "none"), dt and its range, learn_dt, bias of
-    the read / write heads, elementwise_affine of the RMSNorm, vec_dt.
+    the read / write heads, elementwise_affine of the RMSNorm, vec_dt; and
+    ``block``, what the layer does around the module itself (``block.py``; None,
+    the default, is the reference's layer).
     """
 
     def __init__(self, n: int, m: int, input_dim: int, embed_dim: int, module: nn.Module, dt: float = 0.01,
                  generator_type: GeneratorType = "conservative_psd_diss",
                  projection: Literal["mean", "v", "none"] = "none", learn_dt: bool = False, dt_min: float = 0.001,
                  dt_max: float = 1.0, bias: bool = False, elementwise_affine: bool = False, use_triton: bool = True,
-                 vec_dt: bool = False):
+                 vec_dt: bool = False, block: BlockOptions | None = None):
         super().__init__()
         if embed_dim % m:
             raise ValueError(f"embed_dim ({embed_dim}) must be divisible by m ({m})")
@@ -116,6 +119,7 @@ class ContinuousGenHyperConnections(nn.Module):
             raise ValueError(f"unknown projection {projection!r}")
         self.norm = nn.RMSNorm(input_dim, elementwise_affine=elementwise_affine)
         self.module = module
+        self.block = None if block is None else BlockParts(block, embed_dim)
         self.init_weights()
 
     # ------------------------------------------------------------------ init
@@ -190,7 +194,7 @@ class ContinuousGenHyperConnections(nn.Module):
 
         read = torch.sigmoid(self.alpha_read_in * h["read"].view(T, n, m) + self.read_in).transpose(1, 2)
         write = 2.0 * torch.sigmoid(self.alpha_write_out * h["write"].view(T, n, m) + self.write_out)
-        u = hc_read(read, xs)
+        u = read_block(self.block, read, xs)
         f = self.module(u.reshape(*lead, self.embed_dim), **kwargs).reshape(T, m, blk)
 
         gt = self.generator_type
@@ -210,5 +214,5 @@ class ContinuousGenHyperConnections(nn.Module):
             v = F.normalize(h["v"], dim=-1)
         else:
             v = None
-        out = hc_mix_write(Phi, xs, write, f, v)
+        out = write_block(self.block, Phi, xs, write, f, v, u)
         return out.reshape(*lead, n * blk)

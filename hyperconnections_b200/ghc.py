@@ -27,15 +27,16 @@ import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
-from .ops import hc_mix_write, hc_read
+from .block import BlockOptions, BlockParts, read_block, write_block
 
 
 class GeneralizedHyperConnections(nn.Module):
     """Generalised hyper-connection layer (see module doc). Args are the
-    reference's (ghc.py:15-24)."""
+    reference's (ghc.py:15-24), and ``block``: what the layer does around the
+    module itself (``block.py``; None is the reference's layer)."""
 
     def __init__(self, n: int, m: int, input_dim: int, embed_dim: int, module: nn.Module, bias: bool = False,
-                 elementwise_affine: bool = False):
+                 elementwise_affine: bool = False, block: BlockOptions | None = None):
         super().__init__()
         if embed_dim % m:
             raise ValueError(f"embed_dim ({embed_dim}) must be divisible by m ({m})")
@@ -56,6 +57,7 @@ class GeneralizedHyperConnections(nn.Module):
         self.dynamic_scaling_weight_stream_mixing = nn.Linear(blk, n, bias=bias)
         self.norm = nn.RMSNorm(blk, elementwise_affine=elementwise_affine)
         self.module = module
+        self.block = None if block is None else BlockParts(block, embed_dim)
         self.init_weights()
 
     @torch.no_grad()
@@ -92,6 +94,6 @@ class GeneralizedHyperConnections(nn.Module):
         write = self.dynamic_scaling_write_out * torch.tanh(h_w) + self.write_out
         read = (self.dynamic_scaling_read_in * torch.tanh(h_r) + self.read_in).transpose(1, 2)
         mix = self.dynamic_scaling_stream_mixing * torch.tanh(h_s) + self.stream_mixing
-        u = hc_read(read, xs)
+        u = read_block(self.block, read, xs)
         f = self.module(u.reshape(*lead, self.embed_dim), **kwargs).reshape(T, m, blk)
-        return hc_mix_write(mix, xs, write, f).reshape(*lead, n * blk)
+        return write_block(self.block, mix, xs, write, f, None, u).reshape(*lead, n * blk)

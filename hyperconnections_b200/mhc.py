@@ -28,7 +28,8 @@ import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
-from .ops import hc_mix_write, hc_read, sinkhorn_knopp
+from .block import BlockOptions, BlockParts, read_block, write_block
+from .ops import sinkhorn_knopp
 
 
 class ManifoldHyperConnections(nn.Module):
@@ -36,7 +37,8 @@ class ManifoldHyperConnections(nn.Module):
     the reference's (mhc.py:22-33)."""
 
     def __init__(self, n: int, m: int, input_dim: int, embed_dim: int, module: nn.Module, bias: bool = False,
-                 elementwise_affine: bool = False, sinkhorn_iters: int = 20, sinkhorn_bias_init: float = 0.0):
+                 elementwise_affine: bool = False, sinkhorn_iters: int = 20, sinkhorn_bias_init: float = 0.0,
+                 block: BlockOptions | None = None):
         super().__init__()
         if embed_dim % m:
             raise ValueError(f"embed_dim ({embed_dim}) must be divisible by m ({m})")
@@ -56,6 +58,7 @@ class ManifoldHyperConnections(nn.Module):
         self.proj_stream_mixing = nn.Linear(input_dim, n * n, bias=bias)
         self.norm = nn.RMSNorm(input_dim, elementwise_affine=elementwise_affine)
         self.module = module
+        self.block = None if block is None else BlockParts(block, embed_dim)
         self.init_weights()
 
     @torch.no_grad()
@@ -90,6 +93,6 @@ class ManifoldHyperConnections(nn.Module):
         read = torch.sigmoid(self.alpha_read_in * h_r.view(T, n, m) + self.read_in).transpose(1, 2)
         write = 2.0 * torch.sigmoid(self.alpha_write_out * h_w.view(T, n, m) + self.write_out)
         mix = sinkhorn_knopp(self.alpha_stream_mixing * h_s.view(T, n, n) + self.stream_mixing, self.sinkhorn_iters)
-        u = hc_read(read, xs)
+        u = read_block(self.block, read, xs)
         f = self.module(u.reshape(*lead, self.embed_dim), **kwargs).reshape(T, m, blk)
-        return hc_mix_write(mix, xs, write, f).reshape(*lead, n * blk)
+        return write_block(self.block, mix, xs, write, f, None, u).reshape(*lead, n * blk)

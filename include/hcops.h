@@ -15,7 +15,8 @@
  *
  * Bounded waits. Kernels that wait on each other's work (the bulk-copy ring
  * of the stream-mixing kernels, the grid barrier of the cooperative expm
- * forward) poll a bounded number of times. A wait that gives up leaves that
+ * forward, the tensor-core pipeline of the gated feed-forward) poll a bounded
+ * number of times. A wait that gives up leaves that
  * launch's outputs incomplete; the kernel records it in one word of pinned,
  * device-mapped host memory, and from then on every entry point that launches
  * work returns HC_ERR_TIMEOUT without launching, until hc_wait_timeouts(..., 1)
