@@ -41,7 +41,7 @@ bool drop_args(DropArgs& d, double p, const int64_t* state, int64_t seed, int64_
 // The 8-column kernels take rows of whole 8-column chunks whose group fits a
 // CTA, with every stream and parameter on a 16-byte boundary; the others go
 // element by element. (16,384 tokens of n = 4, D = 768, bf16, forward and
-// backward: NN against 3,222 us for the mix-write, MM against 668 us for the read.)
+// backward: 180 us against 3,222 for the mix-write, 90 against 668 for the read.)
 NormGeometry geometry(bool write, bool bwd, int n, int m, int64_t D, int esize,
                       std::initializer_list<const void*> ps) {
   for (const void* p : ps)

@@ -9,15 +9,23 @@
 // Clusters are persistent and walk the tiles; per CTA
 //
 //   warp 0      fetches: one lane issues the TMA copies of the CTA's halves of
-//               A and B into a ring of 6 stages of 32 KB (64 deep); both CTAs'
+//               A and B into a ring of 5 stages of 32 KB (64 deep); both CTAs'
 //               copies are counted on the leader's barrier
 //   warp 1      multiplies (in the leader CTA): one lane issues the four
 //               16-deep steps of a stage for both CTAs
 //   warp 2      owns the tensor memory
+//   warp 3      (for da, db) fetches the tile's slopes, 32 columns at a time for
+//               each quarter, into the quarters' 16 KB slots
 //   warps 4-19  finish: four groups of four warps read the accumulator out of
 //               tensor memory, a quarter of the columns each, and write the
 //               result while the next tile is multiplied into the other half of
 //               tensor memory (2 x 256 of its 512 columns)
+//
+// Results leave through shared memory and TMA stores, and slopes come by TMA
+// loads: a warp holds a row a lane, so its own loads and stores would touch 32
+// lines each (da and db of 32,768 tokens, 384 x 1536, fp16: 134 us that way, 99
+// with the copies). A quarter's slopes come in two halves of 32 columns, so that
+// all four quarters fetch and finish at once.
 //
 // An operand is read as it lies: summed along its unit stride ("K-major", x
 // and the weights of the forward) or across it ("MN-major", the weights of dx
@@ -47,19 +55,25 @@ constexpr int kRows = 128;         // rows of A, and of B, that one CTA holds
 constexpr int kTileM = 2 * kRows;  // a pair's tile
 constexpr int kTileN = 2 * kRows;
 constexpr int kDepth = 64;         // elements of the sum in a stage: 128 bytes
-constexpr int kStages = 6;
+constexpr int kStages = 5;
 constexpr int kOperandBytes = kRows * kDepth * 2;
 constexpr int kStageBytes = 2 * kOperandBytes;
 constexpr int kFinishWarp = 4;    // the first of the finishing warps
 constexpr int kFinishWarps = 16;  // four a scheduler: with two, the activation's chains left it idle two cycles in three
 constexpr int kThreads = 32 * (kFinishWarp + kFinishWarps);
-constexpr int kSmemBytes = kStages * kStageBytes + 1024;
+constexpr int kSlotBytes = kOperandBytes;       // a quarter's: 32 columns of both slopes, and of da and db in their place
+constexpr int kWarpBytes = 4096;                // a finishing warp's results elsewhere: 32 rows of 128 bytes
+constexpr int kStagingBytes = 4 * kSlotBytes;   // the four slots, or the sixteen warps' results
+constexpr int kSmemBytes = kStages * kStageBytes + kStagingBytes + 1024;
 constexpr int kGroupM = 8;  // tiles of A that neighbouring clusters share B with
 
 // Operands by term of a sum of two products, or by job of a launch of several.
 struct alignas(64) TcMaps {
   CUtensorMap a[kFfnMaxJobs], b[kFfnMaxJobs];
+  CUtensorMap out[kFfnMaxJobs];  // kStore: by job; kGlu: h and the slopes; kGluBwd: da and db
+  CUtensorMap in[2];             // kGluBwd: the slopes
 };
+static_assert(kStagingBytes == kFinishWarps * kWarpBytes);
 
 // One result. A launch of several shares the depth of the sum and the operands'
 // order.
@@ -68,13 +82,12 @@ struct TcJob {
   void* out;
   float* parts;  // float32 parts [splits][M][N], or nullptr
   int tiles_m, tiles_n;
-  int vec;  // bytes that the result's rows are aligned to (32, 16, or 2)
+  int tma;  // the result's rows start on 16-byte boundaries: TMA stores
 };
 
 struct TcArgs {
   TcJob job[kFfnMaxJobs];
-  void* out2;
-  void *slope_gate, *slope_up;  // kGlu: written (nullable); kGluBwd: read
+  const void* slope_gate;  // kGlu: whether the slopes are written
   int jobs, tiles, splits;  // tiles of all jobs
   int blocks_term, blocks;  // 64-deep blocks of one term, and of all
   int a_mn, b_mn;           // operands whose unit stride is their rows
@@ -86,6 +99,7 @@ struct TcArgs {
 struct Shared {
   uint64_t full[kStages], empty[kStages];
   uint64_t acc_full[2], acc_empty[2], drain;
+  uint64_t part_full[4], part_done[4];  // a quarter's slopes have arrived, its results have left: twice a tile
   uint32_t tmem;
   volatile int stop;
 };
@@ -116,6 +130,38 @@ __device__ __forceinline__ void fetch_box(uint32_t dst, const CUtensorMap* map, 
       "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(bar)
       : "memory");
 }
+// A box into this CTA, counted on its own barrier.
+__device__ __forceinline__ void fetch_own(uint32_t dst, const CUtensorMap* map, int x, int y, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(smem_u32(bar))
+      : "memory");
+}
+__device__ __forceinline__ void store_box(const CUtensorMap* map, int x, int y, uint32_t src) {
+  asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%1, %2}], [%3];" ::"l"(
+                   reinterpret_cast<uint64_t>(map)),
+               "r"(x), "r"(y), "r"(src)
+               : "memory");
+}
+__device__ __forceinline__ void store_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
+// Until all but the last K groups of this thread's stores have read their source.
+template <int K> __device__ __forceinline__ void store_wait_read() {
+  asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(K) : "memory");
+}
+__device__ __forceinline__ void store_wait_all() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
+__device__ __forceinline__ void put16(uint32_t at, const uint32_t* w) {
+  asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(at), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
+}
+__device__ __forceinline__ uint4 get16(uint32_t at) {
+  uint4 q;
+  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(q.x), "=r"(q.y), "=r"(q.z), "=r"(q.w) : "r"(at));
+  return q;
+}
+// 16-byte word c of line r of a box as the TMA swizzles it: lines of 128 bytes
+// (8 words, the line's number modulo 8 mixed in) and of 64 bytes (4 words).
+__device__ __forceinline__ uint32_t word128(uint32_t base, int r, int c) { return base + r * 128 + ((c ^ (r & 7)) << 4); }
+__device__ __forceinline__ uint32_t word64(uint32_t base, int r, int c) { return base + r * 64 + ((c ^ ((r >> 1) & 3)) << 4); }
+
 __device__ __forceinline__ void mma_pair(uint32_t acc, uint64_t a, uint64_t b, uint32_t idesc, uint32_t add) {
   asm volatile(
       "{\n\t.reg .pred p;\n\t"
@@ -224,56 +270,6 @@ __device__ __forceinline__ void st_v8(void* p, const uint32_t* w) {
                "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
                : "memory");
 }
-// 16 values of one row from column n on, in pairs; columns past N are not written.
-template <typename T>
-__device__ __forceinline__ void store16(T* row, int64_t n, int64_t N, int vec, const uint32_t (&w)[8]) {
-  if (vec == 32 && n + 16 <= N) {
-    st_v8(row + n, w);
-  } else if (vec >= 16) {
-    if (n + 8 <= N) st_v4(row + n, make_uint4(w[0], w[1], w[2], w[3]));
-    if (n + 16 <= N) st_v4(row + n + 8, make_uint4(w[4], w[5], w[6], w[7]));
-    // rows are whole multiples of 8 elements here, so nothing is left over
-  } else {
-#pragma unroll
-    for (int i = 0; i < 16; ++i)
-      if (n + i < N) reinterpret_cast<uint16_t*>(row)[n + i] = static_cast<uint16_t>(w[i / 2] >> (16 * (i % 2)));
-  }
-}
-// 16 values of a slope's row from column n on, as they lie (zeros past N; rows
-// are multiples of 8 elements on 16-byte boundaries).
-struct Raw16 {
-  uint32_t w[8];
-};
-template <typename T> __device__ __forceinline__ Raw16 load16(const T* row, int64_t n, int64_t N, int vec, bool live) {
-  Raw16 r;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) r.w[i] = 0u;
-  if (!live) return r;
-  if (vec == 32 && n + 16 <= N) {
-    asm volatile("ld.global.nc.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
-                 : "=r"(r.w[0]), "=r"(r.w[1]), "=r"(r.w[2]), "=r"(r.w[3]), "=r"(r.w[4]), "=r"(r.w[5]), "=r"(r.w[6]),
-                   "=r"(r.w[7])
-                 : "l"(row + n));
-    return r;
-  }
-#pragma unroll
-  for (int h = 0; h < 2; ++h)
-    if (n + 8 * h + 8 <= N) {
-      const uint4 q = ld_nc_v4(row + n + 8 * h);
-      r.w[4 * h] = q.x; r.w[4 * h + 1] = q.y; r.w[4 * h + 2] = q.z; r.w[4 * h + 3] = q.w;
-    }
-  return r;
-}
-template <typename T> __device__ __forceinline__ void values(const Raw16& r, float (&v)[16]) {
-  float t[8];
-  unpack<T>(make_uint4(r.w[0], r.w[1], r.w[2], r.w[3]), t);
-#pragma unroll
-  for (int i = 0; i < 8; ++i) v[i] = t[i];
-  unpack<T>(make_uint4(r.w[4], r.w[5], r.w[6], r.w[7]), t);
-#pragma unroll
-  for (int i = 0; i < 8; ++i) v[8 + i] = t[i];
-}
-
 __device__ __forceinline__ float exp2_fast(float x) {
   float r;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
@@ -303,77 +299,38 @@ __device__ __forceinline__ void fast_act(int act, float a, float& val, float& de
   }
 }
 
-// A finishing warp's part of a tile: 32 rows, a quarter of the columns, 16 at a
-// time. begin() asks for the first slopes before the accumulator is done, each
-// step for the next one's.
-template <typename T, int EPI> struct Finish {
-  static constexpr int kColumns = (EPI == kGlu ? kRows : kTileN) / (kFinishWarps / 4), kSteps = kColumns / 16;
+// A finishing warp's part of a tile: 32 rows (one a lane), a quarter of the
+// columns. `acc` is the warp's lanes of the accumulator at its columns, `release`
+// gives the accumulator back once it has been read.
+template <typename T> struct Part {
   const TcArgs& a;
   const TcJob& job;
-  int64_t row, n0;
-  bool live;
-  int split;
-  Raw16 g[2], u[2];
+  const TcMaps& maps;
+  int lane, split, job_id;
+  int64_t row0, n0;
+  bool inside;  // any of it lies in the result
+  __device__ __forceinline__ Part(const TcArgs& args, const TcMaps& m, const Item& it, int rank, int quad, int part, int tile_n)
+      : a(args), job(args.job[it.job]), maps(m), lane(threadIdx.x & 31), split(it.split), job_id(it.job) {
+    row0 = static_cast<int64_t>(it.m) * kTileM + rank * kRows + 32 * quad;
+    n0 = static_cast<int64_t>(it.n) * tile_n + part * (tile_n / 4);
+    inside = row0 < job.M && n0 < job.N;
+  }
 
-  __device__ __forceinline__ Finish(const TcArgs& args, const Item& it, int rank, int quad, int part)
-      : a(args), job(args.job[it.job]), split(it.split) {
-    row = static_cast<int64_t>(it.m) * kTileM + rank * kRows + 32 * quad + (threadIdx.x & 31);
-    n0 = static_cast<int64_t>(it.n) * (EPI == kGlu ? kRows : kTileN) + part * kColumns;
-    live = row < job.M;
-  }
-  __device__ __forceinline__ void ask(int step) {
-    if constexpr (EPI == kGluBwd) {
-      const int64_t n = n0 + 16 * step;
-      g[step & 1] = load16<T>(static_cast<const T*>(a.slope_gate) + row * job.ldo, n, job.N, job.vec, live);
-      u[step & 1] = load16<T>(static_cast<const T*>(a.slope_up) + row * job.ldo, n, job.N, job.vec, live);
+  // 64 columns of the result, or of a part of its sum.
+  template <typename Release> __device__ __forceinline__ void store(uint32_t acc, uint32_t mine, Release release) {
+    if (job.tma && !job.parts) {
+      if (lane == 0) store_wait_read<0>();  // the last tile's results have left
+      __syncwarp();
     }
-  }
-  __device__ __forceinline__ void begin() { ask(0); }
-  // acc: this warp's lanes of the tile's accumulator, at its quarter of the columns
-  __device__ __forceinline__ void run(uint32_t acc) {
 #pragma unroll
-    for (int st = 0; st < kSteps; ++st) {
-      const int64_t n = n0 + 16 * st;
-      uint32_t r[16], q[16];
+    for (int st = 0; st < 4; ++st) {
+      uint32_t r[16];
       acc_load16(acc + 16 * st, r);
-      if constexpr (EPI == kGlu) acc_load16(acc + kRows + 16 * st, q);
-      if (st + 1 < kSteps) ask(st + 1);
       acc_wait(r);
-      if constexpr (EPI == kGlu) acc_wait(q);
-      if (live && n < job.N) {
-        if constexpr (EPI == kGlu) {
-          uint32_t h[8], sg[8], su[8];
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            float v[2], d[2], b[2];
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              b[e] = __uint_as_float(q[2 * i + e]);
-              fast_act(a.act, __uint_as_float(r[2 * i + e]), v[e], d[e]);
-            }
-            h[i] = pack2<T>(v[0] * b[0], v[1] * b[1]);
-            sg[i] = pack2<T>(d[0] * b[0], d[1] * b[1]);
-            su[i] = pack2<T>(v[0], v[1]);
-          }
-          store16<T>(static_cast<T*>(job.out) + row * job.ldo, n, job.N, job.vec, h);
-          if (a.slope_gate) {
-            store16<T>(static_cast<T*>(a.slope_gate) + row * job.ldo, n, job.N, job.vec, sg);
-            store16<T>(static_cast<T*>(a.slope_up) + row * job.ldo, n, job.N, job.vec, su);
-          }
-        } else if constexpr (EPI == kGluBwd) {
-          uint32_t w[8];
-          float x[16];
-          values<T>(g[st & 1], x);
-#pragma unroll
-          for (int i = 0; i < 8; ++i)
-            w[i] = pack2<T>(x[2 * i] * __uint_as_float(r[2 * i]), x[2 * i + 1] * __uint_as_float(r[2 * i + 1]));
-          store16<T>(static_cast<T*>(job.out) + row * job.ldo, n, job.N, job.vec, w);
-          values<T>(u[st & 1], x);
-#pragma unroll
-          for (int i = 0; i < 8; ++i)
-            w[i] = pack2<T>(x[2 * i] * __uint_as_float(r[2 * i]), x[2 * i + 1] * __uint_as_float(r[2 * i + 1]));
-          store16<T>(static_cast<T*>(a.out2) + row * job.ldo, n, job.N, job.vec, w);
-        } else if (job.parts) {
+      if (st == 3) release();
+      const int64_t row = row0 + lane, n = n0 + 16 * st;
+      if (job.parts) {
+        if (row < job.M && n < job.N) {
           float* p = job.parts + (static_cast<int64_t>(split) * job.M + row) * job.N + n;
           if ((job.N & 7) == 0) {
             if (n + 8 <= job.N) st_v8(p, r);
@@ -383,14 +340,123 @@ template <typename T, int EPI> struct Finish {
             for (int i = 0; i < 16; ++i)
               if (n + i < job.N) p[i] = __uint_as_float(r[i]);
           }
-        } else {
-          uint32_t w[8];
-#pragma unroll
-          for (int i = 0; i < 8; ++i) w[i] = pack2<T>(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1]));
-          store16<T>(static_cast<T*>(job.out) + row * job.ldo, n, job.N, job.vec, w);
         }
+      } else if (job.tma) {
+        uint32_t w[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) w[i] = pack2<T>(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1]));
+        put16(word128(mine, lane, 2 * st), w);
+        put16(word128(mine, lane, 2 * st + 1), w + 4);
+      } else if (row < job.M) {
+        T* p = static_cast<T*>(job.out) + row * job.ldo + n;
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          if (n + i < job.N) p[i] = Elem<T>::from_f(__uint_as_float(r[i]));
       }
       __syncwarp();  // the next load is the whole warp's
+    }
+    if (job.tma && !job.parts) {
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0 && inside) store_box(&maps.out[job_id], static_cast<int>(n0), static_cast<int>(row0), mine);
+      if (lane == 0) store_commit();
+    }
+  }
+
+  // 32 columns of h, act'(a) b and act(a); a at acc, b at acc + 128. Two of the
+  // three leave from the warp's two boxes, the third from the first's once it has.
+  template <typename Release> __device__ __forceinline__ void glu(uint32_t acc, uint32_t mine, Release release) {
+    const uint32_t box0 = mine, box1 = mine + kWarpBytes / 2;
+    const bool keep = a.slope_gate != nullptr;
+    if (lane == 0) store_wait_read<0>();
+    __syncwarp();
+    uint32_t su[16];
+#pragma unroll
+    for (int st = 0; st < 2; ++st) {
+      uint32_t r[16], q[16];
+      acc_load16(acc + 16 * st, r);
+      acc_load16(acc + kRows + 16 * st, q);
+      acc_wait(r);
+      acc_wait(q);
+      if (st == 1) release();
+      uint32_t h[8], sg[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        float v[2], d[2], b[2];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          b[e] = __uint_as_float(q[2 * i + e]);
+          fast_act(a.act, __uint_as_float(r[2 * i + e]), v[e], d[e]);
+        }
+        h[i] = pack2<T>(v[0] * b[0], v[1] * b[1]);
+        sg[i] = pack2<T>(d[0] * b[0], d[1] * b[1]);
+        su[8 * st + i] = pack2<T>(v[0], v[1]);
+      }
+      put16(word64(box0, lane, 2 * st), h);
+      put16(word64(box0, lane, 2 * st + 1), h + 4);
+      if (keep) {
+        put16(word64(box1, lane, 2 * st), sg);
+        put16(word64(box1, lane, 2 * st + 1), sg + 4);
+      }
+    }
+    const int x = static_cast<int>(n0), y = static_cast<int>(row0);
+    fence_proxy_async_smem();
+    __syncwarp();
+    if (lane == 0) {
+      if (inside) store_box(&maps.out[0], x, y, box0);
+      store_commit();
+      if (inside && keep) store_box(&maps.out[1], x, y, box1);
+      store_commit();
+      if (keep) store_wait_read<1>();
+    }
+    if (!keep) return;
+    __syncwarp();
+#pragma unroll
+    for (int c = 0; c < 4; ++c) put16(word64(box0, lane, c), su + 4 * c);
+    fence_proxy_async_smem();
+    __syncwarp();
+    if (lane == 0) {
+      if (inside) store_box(&maps.out[2], x, y, box0);
+      store_commit();
+    }
+  }
+
+  // 32 columns (the part's first or second) of da and db, from dh and the slopes in the warp's lines of a slot, where
+  // the results take their place.
+  __device__ __forceinline__ void glu_bwd(uint32_t acc, int half, uint32_t gate, uint32_t up) {
+#pragma unroll
+    for (int st = 0; st < 2; ++st) {
+      uint32_t r[16];
+      acc_load16(acc + 32 * half + 16 * st, r);
+      acc_wait(r);
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          const uint32_t at = word64(k ? up : gate, lane, 2 * st + c);
+          float x[8];
+          unpack<T>(get16(at), x);
+          uint32_t w[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            w[i] = pack2<T>(x[2 * i] * __uint_as_float(r[8 * c + 2 * i]), x[2 * i + 1] * __uint_as_float(r[8 * c + 2 * i + 1]));
+          put16(at, w);
+        }
+      }
+      __syncwarp();
+    }
+  }
+  __device__ __forceinline__ void glu_bwd_leave(int half, uint32_t gate, uint32_t up) {
+    fence_proxy_async_smem();
+    __syncwarp();
+    if (lane == 0) {
+      const int x = static_cast<int>(n0) + 32 * half, y = static_cast<int>(row0);
+      if (row0 < job.M && x < job.N) {
+        store_box(&maps.out[0], x, y, gate);
+        store_box(&maps.out[1], x, y, up);
+      }
+      store_commit();
+      store_wait_read<0>();  // before the slot is given back
     }
   }
 };
@@ -400,7 +466,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     ffn_tc_kernel(const __grid_constant__ TcMaps maps, const __grid_constant__ TcArgs a) {
   extern __shared__ uint8_t raw[];
   __shared__ Shared sh;
-  const uint32_t ring = (smem_u32(raw) + 1023) & ~1023u;
+  const uint32_t ring = (smem_u32(raw) + 1023) & ~1023u, staging = ring + kStages * kStageBytes;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = cluster_rank();
   const int items = a.tiles * a.splits;
@@ -414,6 +480,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     for (int b = 0; b < 2; ++b) {
       mbar_init(&sh.acc_full[b], 1);
       mbar_init(&sh.acc_empty[b], 2 * kFinishWarps);  // of both CTAs
+    }
+    for (int q = 0; q < 4; ++q) {
+      mbar_init(&sh.part_full[q], 1);
+      mbar_init(&sh.part_done[q], 4);  // the quarter's warps
     }
     mbar_init(&sh.drain, 1);
     sh.stop = 0;
@@ -528,26 +598,71 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         }
       }
     }
+  } else if (EPI == kGluBwd && warp == 3) {
+    if (lane == 0) {
+      bool ok = true;
+      for (int i = first; i < items && ok; i += step) {
+        const Item it = item_at(a, i);
+        const int row = it.m * kTileM + static_cast<int>(rank) * kRows;
+        for (int use = 0; use < 8; ++use) {  // the quarters' first halves, then their second ones
+          const int half = use >> 2, part = use & 3;
+          // the slot's use before this one has left: its parity is the other half's
+          if ((half || i != first) && !pair_wait(sh, &sh.part_done[part], half ^ 1, a.wait_limit)) {
+            ok = false;
+            break;
+          }
+          const uint32_t dst = staging + part * kSlotBytes;
+          const int n = it.n * kTileN + part * 64 + half * 32;
+          mbar_expect_tx(&sh.part_full[part], kSlotBytes);
+          fetch_own(dst, &maps.in[0], n, row, &sh.part_full[part]);
+          fetch_own(dst + kSlotBytes / 2, &maps.in[1], n, row, &sh.part_full[part]);
+        }
+      }
+      if (!ok) tell_stop(sh, a);
+    }
   } else if (warp >= kFinishWarp) {
     const int quad = warp & 3, part = (warp - kFinishWarp) >> 2;
+    constexpr int tile_n = EPI == kGlu ? kRows : kTileN;
     int buf = 0;
     uint32_t acc_ph = 0;
     for (int i = first; i < items; i += step) {
-      Finish<T, EPI> tile(a, item_at(a, i), static_cast<int>(rank), quad, part);
-      tile.begin();
-      const bool ok = pair_wait(sh, &sh.acc_full[buf], acc_ph, a.wait_limit);
+      Part<T> tile(a, maps, item_at(a, i), static_cast<int>(rank), quad, part, tile_n);
+      bool ok = pair_wait(sh, &sh.acc_full[buf], acc_ph, a.wait_limit);
       if (!__all_sync(kFull, ok)) {
         if (lane == 0) tell_stop(sh, a);
         break;
       }
       tc_fence_after();
-      tile.run(tmem + buf * kTileN + (static_cast<uint32_t>(32 * quad) << 16) + part * tile.kColumns);
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) arrive_cluster(cluster_addr(&sh.acc_empty[buf], 0));
+      const uint32_t acc = tmem + buf * kTileN + (static_cast<uint32_t>(32 * quad) << 16) + part * (tile_n / 4);
+      const auto release = [&] {
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) arrive_cluster(cluster_addr(&sh.acc_empty[buf], 0));
+      };
+      if constexpr (EPI == kGlu) {
+        tile.glu(acc, staging + (warp - kFinishWarp) * kWarpBytes, release);
+      } else if constexpr (EPI == kGluBwd) {
+        const uint32_t gate = staging + part * kSlotBytes + quad * 32 * 64, up = gate + kSlotBytes / 2;
+        for (int half = 0; half < 2; ++half) {
+          ok = pair_wait(sh, &sh.part_full[part], half, a.wait_limit);
+          if (!__all_sync(kFull, ok)) break;
+          tile.glu_bwd(acc, half, gate, up);
+          if (half) release();
+          tile.glu_bwd_leave(half, gate, up);
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&sh.part_done[part]);
+        }
+        if (!__all_sync(kFull, ok)) {
+          if (lane == 0) tell_stop(sh, a);
+          break;
+        }
+      } else {
+        tile.store(acc, staging + (warp - kFinishWarp) * kWarpBytes, release);
+      }
       buf ^= 1;
       if (buf == 0) acc_ph ^= 1;
     }
+    if (lane == 0) store_wait_all();
   }
   __syncwarp();
   __syncthreads();
@@ -618,6 +733,20 @@ bool encode_operand(CUtensorMap* map, const FfnOperand& o, int64_t K) {
                 CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+// Rows of a result or of the slopes in boxes of `cols` x `rows`, a box's line of
+// 64 or 128 bytes swizzled.
+bool encode_rows(CUtensorMap* map, void* p, int64_t M, int64_t N, int64_t ld, int cols, int rows) {
+  const auto encode = tensor_map_encoder();
+  if (!encode) return false;
+  const cuuint64_t dims[2] = {static_cast<cuuint64_t>(N), static_cast<cuuint64_t>(M)};
+  const cuuint64_t strides[1] = {static_cast<cuuint64_t>(ld) * 2};
+  const cuuint32_t box[2] = {static_cast<cuuint32_t>(cols), static_cast<cuuint32_t>(rows)};
+  const cuuint32_t ones[2] = {1, 1};
+  return encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT16, 2, p, dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                cols == 32 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 using Kernel = void (*)(TcMaps, TcArgs);
 template <typename T> Kernel kernel_of(int epi) {
   return epi == kStore ? ffn_tc_kernel<T, kStore> : epi == kGlu ? ffn_tc_kernel<T, kGlu> : ffn_tc_kernel<T, kGluBwd>;
@@ -658,14 +787,22 @@ int ffn_tc_launch(const FfnProduct* ps, int jobs, int dtype, float* parts, cudaS
     job.M = ps[j].M; job.N = ps[j].N; job.ldo = ps[j].ldo; job.out = ps[j].out;
     job.tiles_m = static_cast<int>(ceil_div(job.M, kTileM));
     job.tiles_n = static_cast<int>(ceil_div(job.N, p.epilogue == kGlu ? kRows : kTileN));
-    const uintptr_t base = reinterpret_cast<uintptr_t>(job.out) | reinterpret_cast<uintptr_t>(ps[j].out2) |
-                           reinterpret_cast<uintptr_t>(ps[j].slope_gate) | reinterpret_cast<uintptr_t>(ps[j].slope_up) |
-                           static_cast<uintptr_t>(2 * job.ldo);
-    job.vec = base % 32 == 0 ? 32 : base % 16 == 0 ? 16 : 2;
+    // the hidden tensors' rows always start on 16-byte boundaries
+    job.tma = job.ldo % 8 == 0;
+    if (job.tma) {
+      const FfnProduct& q = ps[j];
+      void* const outs[3] = {q.out, q.epilogue == kGlu ? q.slope_gate : q.out2, q.epilogue == kGlu ? q.slope_up : nullptr};
+      for (int k = 0; k < (q.epilogue == kStore ? 1 : 3); ++k)
+        if (outs[k] && !encode_rows(&maps.out[j + k], outs[k], job.M, job.N, job.ldo, q.epilogue == kStore ? 64 : 32, 32))
+          return HC_ERR_LAUNCH;
+    }
     if (static_cast<int64_t>(job.tiles_m) * job.tiles_n > (int64_t(1) << 24)) return HC_ERR_BAD_SIZE;
     a.tiles += job.tiles_m * job.tiles_n;
   }
-  a.out2 = p.out2; a.slope_gate = p.slope_gate; a.slope_up = p.slope_up;
+  if (p.epilogue == kGluBwd && (!encode_rows(&maps.in[0], p.slope_gate, p.M, p.N, p.ldo, 32, kRows) ||
+                                !encode_rows(&maps.in[1], p.slope_up, p.M, p.N, p.ldo, 32, kRows)))
+    return HC_ERR_LAUNCH;
+  a.slope_gate = p.slope_gate;
   a.splits = p.epilogue == kStore ? ffn_tc_splits(a.tiles, p.K, p.terms) : 1;
   if (a.splits > 1) {
     if (!parts) return HC_ERR_SCRATCH;

@@ -102,6 +102,8 @@ SHAPES = [
     (300, 384, 1536, 384, "bf16", "silu"),
     (1000, 192, 448, 320, "fp16", "silu"),
     (5000, 64, 72, 64, "bf16", "silu"),
+    (9000, 72, 1112, 64, "bf16", "silu"),  # several tiles a pair of CTAs in every product
+    (20000, 64, 264, 136, "fp16", "gelu_tanh"),
     (50, 333, 887, 101, "bf16", "silu"),
     (50, 333, 880, 104, "fp16", "silu"),
     (129, 63, 65, 67, "fp16", "gelu_tanh"),
