@@ -121,6 +121,8 @@ FfnProduct store(int64_t M, int64_t N, int64_t K, FfnOperand A, FfnOperand B, vo
   return p;
 }
 
+bool aligned256(const void* p) { return reinterpret_cast<uintptr_t>(p) % 256 == 0; }
+
 bool aligned_for(int dtype, std::initializer_list<const void*> ps) {
   for (const void* p : ps)
     if (half(dtype) ? !aligned16(p) : !aligned4(p)) return false;
@@ -155,6 +157,7 @@ extern "C" int hc_gated_ffn_fwd(const void* x, const void* w_gate, const void* w
   if (!aligned_for(dtype, {x, w_gate, w_up, w_down, y, h, slope_gate, slope_up})) return HC_ERR_ALIGNMENT;
   const int64_t need = hc_gated_ffn_scratch_bytes(0, T, D, F, O, dtype);
   if (need > 0 && (!scratch || scratch_bytes < need)) return HC_ERR_SCRATCH;
+  if (need > 0 && !aligned256(scratch)) return HC_ERR_ALIGNMENT;
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
   const int64_t Fp = padded(F);
   Scratch space{static_cast<uint8_t*>(scratch), 0};
@@ -204,6 +207,7 @@ extern "C" int hc_gated_ffn_bwd(const void* g, const void* x, const void* w_gate
     return HC_ERR_ALIGNMENT;
   const int64_t need = hc_gated_ffn_scratch_bytes(1, T, D, F, O, dtype);
   if (need > 0 && (!scratch || scratch_bytes < need)) return HC_ERR_SCRATCH;
+  if (need > 0 && !aligned256(scratch)) return HC_ERR_ALIGNMENT;
   const int64_t Fp = padded(F);
   Scratch space{static_cast<uint8_t*>(scratch), 0};
   Matrix mg, mx, wg, wu, wd;  // what is not needed is not copied

@@ -95,6 +95,7 @@ def test_gated_ffn():
 
     assert fwd(T=-1) == SIZE and fwd(D=0) == SIZE and fwd(act=1) == SIZE and fwd(act=4) == SIZE and fwd(dt=9) == DTYPE
     assert fwd([(0, None)]) == NULL and fwd([(5, None)]) == NULL and fwd([(6, None)]) == NULL and fwd(T=0) == OK
+    assert fwd([(4, P + 2)]) == ALIGN and fwd(D=63, scratch=P + 32) == ALIGN and fwd(D=63, scratch=None) == SCRATCH
 
     def bwd(ptrs=(), T=8, act=2, dt=2):
         a = [P] * 15
