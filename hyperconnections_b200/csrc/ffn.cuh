@@ -52,16 +52,19 @@ __device__ __forceinline__ void ffn_act(int act, float a, float& val, float& der
 // out[i] = the sum of `splits` float32 parts, count apart, in order (ffn_tc.cu).
 int ffn_add_parts(const float* parts, void* out, int64_t count, int splits, int dtype, cudaStream_t s);
 
-// float32 (ffn_simt.cu); parts as below.
-int ffn_simt_splits(int64_t M, int64_t N, int64_t K, int terms);
-int ffn_simt_launch(const FfnProduct& p, float* parts, cudaStream_t s);
+// Up to kFfnMaxJobs products in one launch, which then share K, one term, the
+// order of their operands and the epilogue kStore. `parts`: the sum of splits *
+// M * N floats where *_splits of all their tiles says more than one (kStore
+// only), else nullptr.
+constexpr int kFfnMaxJobs = 3;
+
+// float32 (ffn_simt.cu).
+int64_t ffn_simt_tiles(int64_t M, int64_t N);
+int ffn_simt_splits(int64_t tiles, int64_t K, int terms);
+int ffn_simt_launch(const FfnProduct* p, int jobs, float* parts, cudaStream_t s);
 
 // bf16 and fp16 (ffn_tc.cu): operands 16-byte aligned with strides of whole 16
-// bytes. Up to kFfnMaxJobs products in one launch, which then share K, one term,
-// the order of their operands and the epilogue kStore. `parts`: the sum of
-// splits * M * N floats where ffn_tc_splits of all their tiles says more than
-// one (kStore only), else nullptr.
-constexpr int kFfnMaxJobs = 3;
+// bytes.
 int64_t ffn_tc_tiles(int64_t M, int64_t N);
 int ffn_tc_splits(int64_t tiles, int64_t K, int terms);
 int ffn_tc_launch(const FfnProduct* p, int jobs, int dtype, float* parts, cudaStream_t s);

@@ -5,8 +5,8 @@
 namespace hc {
 namespace {
 
-// A CTA's 64 rows in grid.y (at most 65,535) bound the rows of every product.
-constexpr int64_t kMaxRows = int64_t(65535) * 64, kMaxWidth = int64_t(1) << 20;
+// Within these every product's tiles and coordinates are 32-bit numbers.
+constexpr int64_t kMaxRows = int64_t(1) << 22, kMaxWidth = int64_t(1) << 20;
 
 int check(int64_t T, int64_t D, int64_t F, int64_t O, int act, int dtype) {
   if (T < 0 || T > kMaxRows) return HC_ERR_BAD_SIZE;
@@ -71,21 +71,17 @@ int fit(Matrix& out, Scratch& scratch, const void* p, int64_t rows, int64_t cols
 // 2048, F = 8192, bf16, 8 tokens: 24.4 us against 44.8 on the tensor-core tiles.)
 bool few(int64_t T, int dtype) { return half(dtype) && T <= kFewTokens; }
 
-// Float32 parts of products [M, N] summed over K, in one launch on the tensor
-// cores and one after the other on the FMA units (which then share them).
+// Float32 parts of products [M, N] summed over K in one launch.
 struct Size {
   int64_t M, N;
 };
 int64_t parts_bytes(std::initializer_list<Size> results, int64_t K, int terms, int dtype) {
-  int64_t tiles = 0, count = 0, most = 0;
+  int64_t tiles = 0, count = 0;
   for (const Size& r : results) {
-    tiles += ffn_tc_tiles(r.M, r.N);
+    tiles += half(dtype) ? ffn_tc_tiles(r.M, r.N) : ffn_simt_tiles(r.M, r.N);
     count += r.M * r.N;
-    const int64_t splits = ffn_simt_splits(r.M, r.N, K, terms);
-    if (splits > 1 && splits * r.M * r.N * 4 > most) most = splits * r.M * r.N * 4;
   }
-  if (!half(dtype)) return most;
-  const int64_t splits = ffn_tc_splits(tiles, K, terms);
+  const int64_t splits = half(dtype) ? ffn_tc_splits(tiles, K, terms) : ffn_simt_splits(tiles, K, terms);
   return splits > 1 ? splits * count * 4 : 0;
 }
 
@@ -102,10 +98,7 @@ int64_t most_parts(int backward, int64_t T, int64_t D, int64_t F, int64_t O, int
 
 int run(const FfnProduct* p, int jobs, int dtype, void* parts, cudaStream_t s) {
   float* f = static_cast<float*>(parts);
-  if (half(dtype)) return ffn_tc_launch(p, jobs, dtype, f, s);
-  for (int j = 0; j < jobs; ++j)
-    if (int rc = ffn_simt_launch(p[j], f, s)) return rc;
-  return HC_OK;
+  return half(dtype) ? ffn_tc_launch(p, jobs, dtype, f, s) : ffn_simt_launch(p, jobs, f, s);
 }
 int run(const FfnProduct& p, int dtype, void* parts, cudaStream_t s) { return run(&p, 1, dtype, parts, s); }
 

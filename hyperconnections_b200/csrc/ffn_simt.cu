@@ -1,164 +1,289 @@
 // ffn_simt.cu — the gated feed-forward's float32 products on the FMA units (the
 // tensor cores have no float32 inputs): any size and order.
 //
-// 256 threads make a 64 x 64 tile of the result, 4 x 4 values a thread, over
-// stages of 16 steps of the sum in two shared-memory buffers; a thread's loads
-// are a pointer and constant steps from it. Three or four CTAs an SM hide each
-// other's waits (0.75 instructions a cycle; 128 x 128 tiles of 8 x 8 values, one
-// or two CTAs an SM, ran at 0.58 and took 12-18% more time at 4096 x 1024 x
-// 2048, and pairs of float32 in one instruction changed nothing). Products with
-// few tiles split their sum over CTAs, whose parts one more kernel adds in
+// 256 threads make a 64 x 64 tile of the result (for h: 64 x 32 of a and of b)
+// in four groups, each of which sums every fourth stage of 16 steps on its own
+// and over the whole tile; the groups' sums are added in their order at the end.
+// So a few hundred rows fill the device's schedulers, and a thread still makes 8
+// x 8 values: four 16-byte reads of shared memory for 64 FMAs, where 4 x 4
+// values take two for 16 and the reads bound the kernel. A warp's lanes are 4
+// rows x 8 columns of such blocks, whose reads of a step are 64 and 128
+// consecutive bytes. Stages arrive by 4-byte asynchronous copies, which take any
+// alignment, stride and order, two of the group's stages ahead. Products with
+// few tiles also split their sum over CTAs, whose parts one more kernel adds in
 // order.
 #include "ffn.cuh"
+#include "mix_warp.cuh"  // smem_u32
 
 namespace hc {
 namespace {
 
-constexpr int kTile = 64, kDepth = 16, kThreads = 256, kPitch = kTile + 4;
+constexpr int kTile = 64, kDepth = 16, kPitch = kTile + 4, kStages = 3;
+constexpr int kGroup = 64, kGroups = 4, kThreads = kGroup * kGroups;
+constexpr int kStageFloats = 2 * kDepth * kPitch, kGroupFloats = kStages * kStageFloats;
+constexpr int kSmemBytes = kGroups * kGroupFloats * 4;
+static_assert(kGroupFloats >= kTile * kTile);  // a group's sums take its stages' place
 
-// kTile rows of an operand, 16 steps at a time, neighbouring threads along its
-// unit stride. Rows and steps past the operand's end count as 0.
-template <typename T> struct Loader {
-  static constexpr int kLoads = kTile * kDepth / kThreads;
-  const T* p;
-  int64_t step, advance;  // from one of a thread's loads to the next; from stage to stage
+__device__ __forceinline__ void copy4(uint32_t dst, const float* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
+}
+// 4 bytes, or zeros with nothing read.
+__device__ __forceinline__ void copy4_or_zero(uint32_t dst, const float* src, bool there) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(there ? 4 : 0) : "memory");
+}
+
+// ROWS rows of an operand, 16 steps at a time by the 64 threads of a group,
+// neighbouring threads along its unit stride (ALONG: the sum's), into a
+// [step][row] buffer. Rows and steps past the operand's end count as 0.
+template <int ROWS, bool ALONG> struct Loader {
+  static constexpr int kLoads = ROWS * kDepth / kGroup;
+  static constexpr int kRowStep = ALONG ? kGroup / kDepth : 0, kStep = ALONG ? 0 : kGroup / ROWS;  // from load to load
+  const float* p;
+  int64_t step, advance;  // from one of a thread's loads to the next; from the group's stage to its next
   uint32_t rows;          // bit i: the row of load i exists
-  int k, k_step;          // of load 0, and from load to load
-  int at, at_step;        // place in the [step][row] buffer
-  __device__ __forceinline__ Loader(const FfnOperand& o, int64_t row0, int64_t k0) {
-    const bool along = o.k_stride == 1;  // else along the rows
-    const int row = along ? threadIdx.x / kDepth : threadIdx.x % kTile;
-    const int row_step = along ? kThreads / kDepth : 0;
-    k = along ? threadIdx.x % kDepth : threadIdx.x / kTile;
-    k_step = along ? 0 : kThreads / kTile;
-    p = static_cast<const T*>(o.p) + (row0 + row) * o.row_stride + (k0 + k) * o.k_stride;
-    step = row_step * o.row_stride + k_step * o.k_stride;
-    advance = kDepth * o.k_stride;
-    at = k * kPitch + row;
-    at_step = k_step * kPitch + row_step;
+  __device__ __forceinline__ static int row(int tid) { return ALONG ? tid / kDepth : tid % ROWS; }
+  __device__ __forceinline__ static int k(int tid) { return ALONG ? tid % kDepth : tid / ROWS; }
+  __device__ __forceinline__ void start(const FfnOperand& o, int64_t row0, int64_t k0, int tid) {
+    const int64_t ld = ALONG ? o.row_stride : o.k_stride, r = row0 + row(tid);
+    p = static_cast<const float*>(o.p) + (ALONG ? r * ld + k0 + k(tid) : r + (k0 + k(tid)) * ld);
+    step = (ALONG ? kRowStep : kStep) * ld;
+    advance = kGroups * kDepth * (ALONG ? 1 : ld);
     rows = 0;
 #pragma unroll
-    for (int i = 0; i < kLoads; ++i) rows |= (row0 + row + i * row_step < o.rows ? 1u : 0u) << i;
+    for (int i = 0; i < kLoads; ++i) rows |= (r + i * kRowStep < o.rows ? 1u : 0u) << i;
   }
-  __device__ __forceinline__ void load(int64_t left, float (&r)[kLoads]) {  // `left` steps of the sum from this stage on
+  __device__ __forceinline__ void fetch(uint32_t buffer, int64_t left, int tid) {  // `left` steps of the sum from this stage on
+    const float* q = p;
+    const uint32_t dst = buffer + 4 * (k(tid) * kPitch + row(tid));
+    constexpr int to = 4 * (kStep * kPitch + kRowStep);
+    if (left >= kDepth && rows == (1u << kLoads) - 1) {
 #pragma unroll
-    for (int i = 0; i < kLoads; ++i)
-      r[i] = (rows >> i & 1u) && k + i * k_step < left ? Elem<T>::to_f(__ldg(p + i * step)) : 0.f;
+      for (int i = 0; i < kLoads; ++i, q += step) copy4(dst + i * to, q);
+    } else {
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i, q += step) {
+        const bool there = (rows >> i & 1u) && k(tid) + i * kStep < left;
+        copy4_or_zero(dst + i * to, there ? q : p, there);
+      }
+    }
     p += advance;
-  }
-  __device__ __forceinline__ void put(const float (&r)[kLoads], float* buffer) const {
-#pragma unroll
-    for (int i = 0; i < kLoads; ++i) buffer[at + i * at_step] = r[i];
   }
 };
 
-template <typename T, int EPI>
-__global__ void __launch_bounds__(kThreads) ffn_simt_kernel(const __grid_constant__ FfnProduct p, float* parts, int splits) {
-  constexpr int NB = EPI == kGlu ? 2 : 1, V = kTile / 16;
-  __shared__ __align__(16) float sA[2][kDepth * kPitch], sB[2][NB][kDepth * kPitch];
-  const int tx = threadIdx.x % 16, ty = threadIdx.x / 16;
-  const int64_t m0 = static_cast<int64_t>(blockIdx.y) * kTile, n0 = static_cast<int64_t>(blockIdx.x) * kTile;
-  float acc[NB][V][V] = {};
-  // this CTA's stages of all terms' sums
-  const int64_t per_term = (p.K + kDepth - 1) / kDepth, stages = per_term * p.terms;
-  const int64_t s0 = stages * blockIdx.z / splits, s1 = stages * (blockIdx.z + 1) / splits;
-  for (int term = 0; term < p.terms; ++term) {
-    const int64_t first = s0 > term * per_term ? s0 - term * per_term : 0;
-    const int64_t last = s1 - term * per_term < per_term ? s1 - term * per_term : per_term;
-    if (first >= last) continue;
-    Loader<T> la(p.A[term], m0, first * kDepth);
-    Loader<T> lb(p.B[term], n0, first * kDepth), lb2(p.B[NB == 2 ? 1 : term], n0, first * kDepth);
-    float ra[Loader<T>::kLoads], rb[NB][Loader<T>::kLoads];
-    auto load = [&](int64_t st) {
-      la.load(p.K - st * kDepth, ra);
-      lb.load(p.K - st * kDepth, rb[0]);
-      if constexpr (NB == 2) lb2.load(p.K - st * kDepth, rb[NB - 1]);
-    };
-    auto put = [&](int buf) {
-      la.put(ra, sA[buf]);
-      lb.put(rb[0], sB[buf][0]);
-      if constexpr (NB == 2) lb2.put(rb[NB - 1], sB[buf][NB - 1]);
-    };
-    load(first);
-    put(0);
-    __syncthreads();
-    int buf = 0;
-    for (int64_t st = first; st < last; ++st, buf ^= 1) {
-      if (st + 1 < last) load(st + 1);  // the next stage travels while this one is used
+// Products of one launch, the jobs' tiles one after the other in blockIdx.x.
+struct Jobs {
+  FfnProduct p[kFfnMaxJobs];
+  float* parts[kFfnMaxJobs];
+  int tiles_n[kFfnMaxJobs], first[kFfnMaxJobs];  // tiles a row of tiles, and before the job
+  int count, splits;
+};
+
+__device__ __forceinline__ void read8(const float* p, float (&r)[8], int second) {
+  const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + second);
+  r[0] = a.x; r[1] = a.y; r[2] = a.z; r[3] = a.w;
+  r[4] = b.x; r[5] = b.y; r[6] = b.z; r[7] = b.w;
+}
+__device__ __forceinline__ bool on16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+// Four neighbouring values, of which the first `count` exist; `wide`: p is 16-byte aligned.
+__device__ __forceinline__ void write4(float* p, const float* v, int64_t count, bool wide) {
+  if (wide && count >= 4) {
+    *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
+  } else {
 #pragma unroll
-      for (int k = 0; k < kDepth; ++k) {
-        const float4 av = *reinterpret_cast<const float4*>(&sA[buf][k * kPitch + V * ty]);
-        const float a[V] = {av.x, av.y, av.z, av.w};
-#pragma unroll
-        for (int b = 0; b < NB; ++b) {
-          const float4 bv = *reinterpret_cast<const float4*>(&sB[buf][b][k * kPitch + V * tx]);
-          const float w[V] = {bv.x, bv.y, bv.z, bv.w};
-#pragma unroll
-          for (int i = 0; i < V; ++i)
-#pragma unroll
-            for (int j = 0; j < V; ++j) acc[b][i][j] = fmaf(a[i], w[j], acc[b][i][j]);
-        }
-      }
-      if (st + 1 < last) put(buf ^ 1);
-      __syncthreads();
-    }
+    for (int i = 0; i < 4; ++i)
+      if (i < count) p[i] = v[i];
   }
+}
+
+// AK, BK: whether A's and B's unit stride is the sum's.
+template <int EPI, bool AK, bool BK>
+__global__ void __launch_bounds__(kThreads, 2) ffn_simt_kernel(const __grid_constant__ Jobs jobs) {
+  extern __shared__ __align__(16) float smem[];
+  constexpr int kTileN = EPI == kGlu ? kTile / 2 : kTile;
+  int job = 0;
 #pragma unroll
-  for (int i = 0; i < V; ++i)
+  for (int j = 1; j < kFfnMaxJobs; ++j)
+    if (j < jobs.count && static_cast<int>(blockIdx.x) >= jobs.first[j]) job = j;
+  const FfnProduct& p = jobs.p[job];
+  const int tile = static_cast<int>(blockIdx.x) - jobs.first[job], tile_m = tile / jobs.tiles_n[job];
+  const int64_t m0 = static_cast<int64_t>(tile_m) * kTile;
+  const int64_t n0 = static_cast<int64_t>(tile - tile_m * jobs.tiles_n[job]) * kTileN;
+  const int group = threadIdx.x / kGroup, tid = threadIdx.x % kGroup, lane = threadIdx.x & 31;
+  const int ty = (tid >> 5) * 32 + 4 * (lane >> 3), tx = 4 * (lane & 7);
+  float* const mine = smem + group * kGroupFloats;  // the group's stages, [A, B][step][row] each
+  uint64_t acc[8][4] = {};  // pairs of columns
+
+  // the CTA's stages of each term's sum, dealt out to the groups
+  const int per_term = static_cast<int>((p.K + kDepth - 1) / kDepth), stages = per_term * p.terms;
+  const int s0 = static_cast<int>(static_cast<int64_t>(stages) * blockIdx.y / jobs.splits);
+  const int s1 = static_cast<int>(static_cast<int64_t>(stages) * (blockIdx.y + 1) / jobs.splits);
+  Loader<kTile, AK> la;
+  Loader<kTileN, BK> lb, lu;  // kGlu: rows of w_gate and of w_up
+  int term = -1, into = 0;
+  auto fetch = [&](int st) {
+    if (st < s1) {
+      const int t = st >= per_term ? 1 : 0, k0 = (st - t * per_term) * kDepth;
+      if (t != term) {
+        term = t;
+        la.start(p.A[t], m0, k0, tid);
+        lb.start(p.B[t], n0, k0, tid);
+        if constexpr (EPI == kGlu) lu.start(p.B[1], n0, k0, tid);
+      }
+      const int64_t left = p.K - k0;
+      const uint32_t a = smem_u32(mine + into * kStageFloats), b = a + 4 * kDepth * kPitch;
+      la.fetch(a, left, tid);
+      lb.fetch(b, left, tid);
+      if constexpr (EPI == kGlu) lu.fetch(b + 4 * kTileN, left, tid);
+      if (++into == kStages) into = 0;
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");  // one group of copies a stage, empty behind the last
+  };
 #pragma unroll
-    for (int j = 0; j < V; ++j) {
-      const int64_t m = m0 + V * ty + i, n = n0 + V * tx + j;
-      if (m >= p.M || n >= p.N) continue;
-      const int64_t at = m * p.ldo + n;
-      if constexpr (EPI == kStore) {
-        if (parts)
-          parts[(blockIdx.z * p.M + m) * p.N + n] = acc[0][i][j];
-        else
-          static_cast<T*>(p.out)[at] = Elem<T>::from_f(acc[0][i][j]);
-      } else if constexpr (EPI == kGlu) {
-        const float a = acc[0][i][j], b = acc[NB - 1][i][j];
-        float val, der;
-        ffn_act(p.act, a, val, der);
-        static_cast<T*>(p.out)[at] = Elem<T>::from_f(val * b);
+  for (int i = 0; i < kStages - 1; ++i) fetch(s0 + group + i * kGroups);
+  int slot = 0;
+  for (int st = s0 + group; st < s1; st += kGroups) {
+    asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2) : "memory");
+    asm volatile("bar.sync %0, %1;" ::"r"(1 + group), "n"(kGroup) : "memory");  // arrived, and the one before it has been read
+    fetch(st + (kStages - 1) * kGroups);
+    const float *sA = mine + slot * kStageFloats, *sB = sA + kDepth * kPitch;
+#pragma unroll
+    for (int k = 0; k < kDepth; ++k) {
+      float a[8];
+      read8(&sA[k * kPitch + ty], a, 16);
+      const ulonglong2 b0 = *reinterpret_cast<const ulonglong2*>(&sB[k * kPitch + tx]);
+      const ulonglong2 b1 = *reinterpret_cast<const ulonglong2*>(&sB[k * kPitch + tx + 32]);
+      const uint64_t b[4] = {b0.x, b0.y, b1.x, b1.y};
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        uint64_t aa;
+        asm("mov.b64 %0, {%1, %1};" : "=l"(aa) : "f"(a[i]));
+#pragma unroll
+        for (int j = 0; j < 4; ++j) asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(acc[i][j]) : "l"(aa), "l"(b[j]));
+      }
+    }
+    if (++slot == kStages) slot = 0;
+  }
+
+  // the groups' sums in their order, two rows of each thread's eight a group
+  asm volatile("cp.async.wait_group 0;" ::: "memory");
+  asm volatile("bar.sync %0, %1;" ::"r"(1 + group), "n"(kGroup) : "memory");
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      float lo, hi;
+      asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(acc[i][j]));
+      mine[(8 * i + 2 * j) * kGroup + tid] = lo;
+      mine[(8 * i + 2 * j + 1) * kGroup + tid] = hi;
+    }
+  __syncthreads();
+#pragma unroll
+  for (int r = 0; r < 8 / kGroups; ++r) {
+    const int i = 8 / kGroups * group + r;
+    float sum[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      sum[j] = smem[(8 * i + j) * kGroup + tid];
+#pragma unroll
+      for (int g = 1; g < kGroups; ++g) sum[j] += smem[g * kGroupFloats + (8 * i + j) * kGroup + tid];
+    }
+    const int64_t m = m0 + ty + (i & 3) + 16 * (i >> 2);
+    if (m >= p.M) continue;
+    if constexpr (EPI == kStore) {
+      float* parts = jobs.parts[job];
+      float* row = parts ? parts + (blockIdx.y * p.M + m) * p.N : static_cast<float*>(p.out) + m * p.ldo;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int64_t n = n0 + tx + 32 * h;
+        write4(row + n, sum + 4 * h, p.N - n, on16(row));
+      }
+    } else {
+      const bool wide = on16(p.out) && on16(p.out2) && on16(p.slope_gate) && on16(p.slope_up);  // rows are of whole 32 bytes
+      if constexpr (EPI == kGlu) {
+        const int64_t n = n0 + tx, at = m * p.ldo + n;
+        float h[4], sg[4], su[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          float der;
+          ffn_act(p.act, sum[j], su[j], der);
+          h[j] = su[j] * sum[4 + j];
+          sg[j] = der * sum[4 + j];
+        }
+        write4(static_cast<float*>(p.out) + at, h, p.N - n, wide);
         if (p.slope_gate) {
-          static_cast<T*>(p.slope_gate)[at] = Elem<T>::from_f(der * b);
-          static_cast<T*>(p.slope_up)[at] = Elem<T>::from_f(val);
+          write4(static_cast<float*>(p.slope_gate) + at, sg, p.N - n, wide);
+          write4(static_cast<float*>(p.slope_up) + at, su, p.N - n, wide);
         }
       } else {
-        const float dh = acc[0][i][j];
-        static_cast<T*>(p.out)[at] = Elem<T>::from_f(dh * Elem<T>::to_f(static_cast<const T*>(p.slope_gate)[at]));
-        static_cast<T*>(p.out2)[at] = Elem<T>::from_f(dh * Elem<T>::to_f(static_cast<const T*>(p.slope_up)[at]));
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int64_t n = n0 + tx + 32 * h, at = m * p.ldo + n;
+          float da[4], db[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const bool there = n + j < p.N;
+            da[j] = there ? sum[4 * h + j] * static_cast<const float*>(p.slope_gate)[at + j] : 0.f;
+            db[j] = there ? sum[4 * h + j] * static_cast<const float*>(p.slope_up)[at + j] : 0.f;
+          }
+          write4(static_cast<float*>(p.out) + at, da, p.N - n, wide);
+          write4(static_cast<float*>(p.out2) + at, db, p.N - n, wide);
+        }
       }
     }
+  }
 }
+
+int64_t tiles(int64_t M, int64_t N, int tile_n) { return ((M + kTile - 1) / kTile) * ((N + tile_n - 1) / tile_n); }
 
 }  // namespace
 
-namespace {
-template <int EPI> int launch(const FfnProduct& p, float* parts, int splits, cudaStream_t s) {
-  const dim3 grid(static_cast<unsigned>((p.N + kTile - 1) / kTile), static_cast<unsigned>((p.M + kTile - 1) / kTile), splits);
-  ffn_simt_kernel<float, EPI><<<grid, kThreads, 0, s>>>(p, parts, splits);
-  return launch_status();
-}
-}  // namespace
+int64_t ffn_simt_tiles(int64_t M, int64_t N) { return tiles(M, N, kTile); }
 
-// CTAs that share the sum of one tile: until there are four an SM, each with at
-// least 8 stages (128 steps) of its own. (517 x 333 x 887, forward and
-// backward: 210 us against 354 without.)
-int ffn_simt_splits(int64_t M, int64_t N, int64_t K, int terms) {
-  const int64_t tiles = ((M + kTile - 1) / kTile) * ((N + kTile - 1) / kTile);
-  const int64_t by_sms = 4 * sm_count() / tiles, by_depth = (K + kDepth - 1) / kDepth * terms / 8;
+// CTAs that share the sum of one tile: until there are two an SM, each with at
+// least 8 stages (128 steps), two a group.
+int ffn_simt_splits(int64_t tiles, int64_t K, int terms) {
+  const int64_t by_sms = 2 * sm_count() / tiles, by_depth = (K + kDepth - 1) / kDepth * terms / (2 * kGroups);
   const int64_t s = by_sms < by_depth ? by_sms : by_depth;
   return static_cast<int>(s < 1 ? 1 : s > 32 ? 32 : s);
 }
 
-int ffn_simt_launch(const FfnProduct& p, float* parts, cudaStream_t s) {
-  if (p.epilogue == kGlu) return launch<kGlu>(p, nullptr, 1, s);
-  if (p.epilogue == kGluBwd) return launch<kGluBwd>(p, nullptr, 1, s);
-  const int splits = ffn_simt_splits(p.M, p.N, p.K, p.terms);
-  if (splits > 1 && !parts) return HC_ERR_SCRATCH;
-  if (int rc = launch<kStore>(p, splits > 1 ? parts : nullptr, splits, s)) return rc;
-  return splits > 1 ? ffn_add_parts(parts, p.out, p.M * p.N, splits, HC_DTYPE_F32, s) : HC_OK;
+int ffn_simt_launch(const FfnProduct* ps, int count, float* parts, cudaStream_t s) {
+  const int epilogue = ps[0].epilogue, tile_n = epilogue == kGlu ? kTile / 2 : kTile;
+  Jobs jobs{};
+  jobs.count = count;
+  int64_t total = 0;
+  for (int j = 0; j < count; ++j) {
+    jobs.p[j] = ps[j];
+    jobs.tiles_n[j] = static_cast<int>((ps[j].N + tile_n - 1) / tile_n);
+    jobs.first[j] = static_cast<int>(total);
+    total += tiles(ps[j].M, ps[j].N, tile_n);
+    if (total > INT_MAX) return HC_ERR_BAD_SIZE;
+  }
+  jobs.splits = epilogue == kStore ? ffn_simt_splits(total, ps[0].K, ps[0].terms) : 1;
+  if (jobs.splits > 1) {
+    if (!parts) return HC_ERR_SCRATCH;
+    float* at = parts;
+    for (int j = 0; j < count; ++j) {
+      jobs.parts[j] = at;
+      at += jobs.splits * ps[j].M * ps[j].N;
+    }
+  }
+  const dim3 grid(static_cast<unsigned>(total), jobs.splits);
+  const bool ak = ps[0].A[0].k_stride == 1, bk = ps[0].B[0].k_stride == 1;
+  void (*kernel)(Jobs) = nullptr;  // the orders that occur: see ffn.cuh
+  if (epilogue == kGlu) kernel = ffn_simt_kernel<kGlu, true, true>;
+  else if (epilogue == kGluBwd) kernel = ffn_simt_kernel<kGluBwd, true, false>;
+  else if (ak) kernel = bk ? ffn_simt_kernel<kStore, true, true> : ffn_simt_kernel<kStore, true, false>;
+  else kernel = ffn_simt_kernel<kStore, false, false>;
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes) != cudaSuccess) {
+    cudaGetLastError();
+    return HC_ERR_LAUNCH;
+  }
+  kernel<<<grid, kThreads, kSmemBytes, s>>>(jobs);
+  if (int rc = launch_status()) return rc;
+  for (int j = 0; j < count && jobs.splits > 1; ++j)
+    if (int rc = ffn_add_parts(jobs.parts[j], ps[j].out, ps[j].M * ps[j].N, jobs.splits, HC_DTYPE_F32, s)) return rc;
+  return HC_OK;
 }
 
 }  // namespace hc
