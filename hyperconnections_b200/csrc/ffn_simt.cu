@@ -32,6 +32,11 @@ __device__ __forceinline__ void copy4_or_zero(uint32_t dst, const float* src, bo
   asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(there ? 4 : 0) : "memory");
 }
 
+// Where the lanes of a copy lie along the sum, two steps 8 apart would meet in
+// a bank (8 x kPitch is a multiple of 32): the pairs of four rows change places
+// in the later one.
+__device__ __forceinline__ constexpr int swap(bool along, int k) { return along && k >= 8 ? 2 : 0; }
+
 // ROWS rows of an operand, 16 steps at a time by the 64 threads of a group,
 // neighbouring threads along its unit stride (ALONG: the sum's), into a
 // [step][row] buffer. Rows and steps past the operand's end count as 0.
@@ -41,6 +46,7 @@ template <int ROWS, bool ALONG> struct Loader {
   const float* p;
   int64_t step, advance;  // from one of a thread's loads to the next; from the group's stage to its next
   uint32_t rows;          // bit i: the row of load i exists
+  static_assert(kRowStep % 4 == 0);  // swap() works within four rows
   __device__ __forceinline__ static int row(int tid) { return ALONG ? tid / kDepth : tid % ROWS; }
   __device__ __forceinline__ static int k(int tid) { return ALONG ? tid % kDepth : tid / ROWS; }
   __device__ __forceinline__ void start(const FfnOperand& o, int64_t row0, int64_t k0, int tid) {
@@ -54,7 +60,7 @@ template <int ROWS, bool ALONG> struct Loader {
   }
   __device__ __forceinline__ void fetch(uint32_t buffer, int64_t left, int tid) {  // `left` steps of the sum from this stage on
     const float* q = p;
-    const uint32_t dst = buffer + 4 * (k(tid) * kPitch + row(tid));
+    const uint32_t dst = buffer + 4 * (k(tid) * kPitch + (row(tid) ^ swap(ALONG, k(tid))));
     constexpr int to = 4 * (kStep * kPitch + kRowStep);
     if (left >= kDepth && rows == (1u << kLoads) - 1) {
 #pragma unroll
@@ -78,10 +84,15 @@ struct Jobs {
   int count, splits;
 };
 
-__device__ __forceinline__ void read8(const float* p, float (&r)[8], int second) {
-  const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + second);
-  r[0] = a.x; r[1] = a.y; r[2] = a.z; r[3] = a.w;
-  r[4] = b.x; r[5] = b.y; r[6] = b.z; r[7] = b.w;
+// Four neighbouring values, their pairs changed back.
+__device__ __forceinline__ void read4(const float* p, int swapped, float* r) {
+  const float4 v = *reinterpret_cast<const float4*>(p);
+  r[swapped] = v.x; r[swapped + 1] = v.y; r[2 - swapped] = v.z; r[3 - swapped] = v.w;
+}
+__device__ __forceinline__ void read_pairs(const float* p, int swapped, uint64_t* r) {
+  const ulonglong2 v = *reinterpret_cast<const ulonglong2*>(p);
+  r[swapped / 2] = v.x;
+  r[1 - swapped / 2] = v.y;
 }
 __device__ __forceinline__ bool on16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 // Four neighbouring values, of which the first `count` exist; `wide`: p is 16-byte aligned.
@@ -149,10 +160,11 @@ __global__ void __launch_bounds__(kThreads, 2) ffn_simt_kernel(const __grid_cons
 #pragma unroll
     for (int k = 0; k < kDepth; ++k) {
       float a[8];
-      read8(&sA[k * kPitch + ty], a, 16);
-      const ulonglong2 b0 = *reinterpret_cast<const ulonglong2*>(&sB[k * kPitch + tx]);
-      const ulonglong2 b1 = *reinterpret_cast<const ulonglong2*>(&sB[k * kPitch + tx + 32]);
-      const uint64_t b[4] = {b0.x, b0.y, b1.x, b1.y};
+      uint64_t b[4];
+      read4(&sA[k * kPitch + ty], swap(AK, k), a);
+      read4(&sA[k * kPitch + ty + 16], swap(AK, k), a + 4);
+      read_pairs(&sB[k * kPitch + tx], swap(BK, k), b);
+      read_pairs(&sB[k * kPitch + tx + 32], swap(BK, k), b + 2);
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         uint64_t aa;
