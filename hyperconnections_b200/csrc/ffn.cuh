@@ -58,9 +58,10 @@ int ffn_add_parts(const float* parts, void* out, int64_t count, int splits, int 
 // only), else nullptr.
 constexpr int kFfnMaxJobs = 3;
 
-// float32 (ffn_simt.cu).
-int64_t ffn_simt_tiles(int64_t M, int64_t N);
-int ffn_simt_splits(int64_t tiles, int64_t K, int terms);
+// float32 (ffn_simt.cu); few: every job has few rows.
+bool ffn_simt_few(int64_t M);
+int64_t ffn_simt_tiles(int64_t M, int64_t N, bool few);
+int ffn_simt_splits(int64_t tiles, int64_t K, int terms, bool few);
 int ffn_simt_launch(const FfnProduct* p, int jobs, float* parts, cudaStream_t s);
 
 // bf16 and fp16 (ffn_tc.cu): operands 16-byte aligned with strides of whole 16

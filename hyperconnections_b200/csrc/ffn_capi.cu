@@ -77,11 +77,13 @@ struct Size {
 };
 int64_t parts_bytes(std::initializer_list<Size> results, int64_t K, int terms, int dtype) {
   int64_t tiles = 0, count = 0;
+  bool rows_few = true;
+  for (const Size& r : results) rows_few = rows_few && ffn_simt_few(r.M);
   for (const Size& r : results) {
-    tiles += half(dtype) ? ffn_tc_tiles(r.M, r.N) : ffn_simt_tiles(r.M, r.N);
+    tiles += half(dtype) ? ffn_tc_tiles(r.M, r.N) : ffn_simt_tiles(r.M, r.N, rows_few);
     count += r.M * r.N;
   }
-  const int64_t splits = half(dtype) ? ffn_tc_splits(tiles, K, terms) : ffn_simt_splits(tiles, K, terms);
+  const int64_t splits = half(dtype) ? ffn_tc_splits(tiles, K, terms) : ffn_simt_splits(tiles, K, terms, rows_few);
   return splits > 1 ? splits * count * 4 : 0;
 }
 

@@ -8,10 +8,21 @@
 // x 8 values: four 16-byte reads of shared memory for 64 FMAs, where 4 x 4
 // values take two for 16 and the reads bound the kernel. A warp's lanes are 4
 // rows x 8 columns of such blocks, whose reads of a step are 64 and 128
-// consecutive bytes. Stages arrive by 4-byte asynchronous copies, which take any
+// consecutive bytes; columns go in pairs through fma.rn.f32x2, which halves the
+// instructions. Stages arrive by 4-byte asynchronous copies, which take any
 // alignment, stride and order, two of the group's stages ahead. Products with
 // few tiles also split their sum over CTAs, whose parts one more kernel adds in
 // order.
+//
+// Forward and backward of 4096 x 1024 x 2048: 48 TFLOP/s (3,217 us; 3,788 with
+// single FMAs), two thirds of the FMA units' peak: the reads of shared memory
+// return 128 bytes a cycle, as long as the FMAs they feed take. Of 517 x 333 x
+// 887: 136 us (204 with 4 x 4 values and no groups): five products of 20-39 us,
+// two thirds of them waits for the first stages and for each other's last ones.
+//
+// A few rows, at most 24, take tiles of 8 x 64, a thread all rows of four
+// columns for four of a stage's sixteen steps: the weights' way through shared
+// memory bounds it.
 #include "ffn.cuh"
 #include "mix_warp.cuh"  // smem_u32
 
@@ -20,9 +31,16 @@ namespace {
 
 constexpr int kTile = 64, kDepth = 16, kPitch = kTile + 4, kStages = 3;
 constexpr int kGroup = 64, kGroups = 4, kThreads = kGroup * kGroups;
-constexpr int kStageFloats = 2 * kDepth * kPitch, kGroupFloats = kStages * kStageFloats;
-constexpr int kSmemBytes = kGroups * kGroupFloats * 4;
-static_assert(kGroupFloats >= kTile * kTile);  // a group's sums take its stages' place
+constexpr int kFewRows = 8;  // of a tile for a few tokens
+
+// Shared memory by the tile's rows of A: a group's stages are A's [step][row] and B's.
+template <int TM> struct Layout {
+  static constexpr int kPitchA = TM + 4, kStageA = kDepth * kPitchA, kStage = kStageA + kDepth * kPitch;
+  static constexpr int kGroupFloats = kStages * kStage, kBytes = kGroups * kGroupFloats * 4;
+  static constexpr int kPerSm = TM == kTile ? 2 : 3;
+  static constexpr int kSums = TM == kTile ? kTile * kTile : 4 * TM * kTile;  // of a group, which take its stages' place
+  static_assert(kGroupFloats >= kSums);
+};
 
 __device__ __forceinline__ void copy4(uint32_t dst, const float* src) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
@@ -33,14 +51,14 @@ __device__ __forceinline__ void copy4_or_zero(uint32_t dst, const float* src, bo
 }
 
 // Where the lanes of a copy lie along the sum, two steps 8 apart would meet in
-// a bank (8 x kPitch is a multiple of 32): the pairs of four rows change places
+// a bank (8 x the pitch is a multiple of 32): the pairs of four rows change places
 // in the later one.
 __device__ __forceinline__ constexpr int swap(bool along, int k) { return along && k >= 8 ? 2 : 0; }
 
 // ROWS rows of an operand, 16 steps at a time by the 64 threads of a group,
 // neighbouring threads along its unit stride (ALONG: the sum's), into a
 // [step][row] buffer. Rows and steps past the operand's end count as 0.
-template <int ROWS, bool ALONG> struct Loader {
+template <int ROWS, bool ALONG, int PITCH> struct Loader {
   static constexpr int kLoads = ROWS * kDepth / kGroup;
   static constexpr int kRowStep = ALONG ? kGroup / kDepth : 0, kStep = ALONG ? 0 : kGroup / ROWS;  // from load to load
   const float* p;
@@ -60,8 +78,8 @@ template <int ROWS, bool ALONG> struct Loader {
   }
   __device__ __forceinline__ void fetch(uint32_t buffer, int64_t left, int tid) {  // `left` steps of the sum from this stage on
     const float* q = p;
-    const uint32_t dst = buffer + 4 * (k(tid) * kPitch + (row(tid) ^ swap(ALONG, k(tid))));
-    constexpr int to = 4 * (kStep * kPitch + kRowStep);
+    const uint32_t dst = buffer + 4 * (k(tid) * PITCH + (row(tid) ^ swap(ALONG, k(tid))));
+    constexpr int to = 4 * (kStep * PITCH + kRowStep);
     if (left >= kDepth && rows == (1u << kLoads) - 1) {
 #pragma unroll
       for (int i = 0; i < kLoads; ++i, q += step) copy4(dst + i * to, q);
@@ -80,7 +98,7 @@ template <int ROWS, bool ALONG> struct Loader {
 struct Jobs {
   FfnProduct p[kFfnMaxJobs];
   float* parts[kFfnMaxJobs];
-  int tiles_n[kFfnMaxJobs], first[kFfnMaxJobs];  // tiles a row of tiles, and before the job
+  int run[kFfnMaxJobs], first[kFfnMaxJobs];  // tiles a row (a few tokens: a column) of tiles, and before the job
   int count, splits;
 };
 
@@ -106,30 +124,36 @@ __device__ __forceinline__ void write4(float* p, const float* v, int64_t count, 
   }
 }
 
-// AK, BK: whether A's and B's unit stride is the sum's.
-template <int EPI, bool AK, bool BK>
-__global__ void __launch_bounds__(kThreads, 2) ffn_simt_kernel(const __grid_constant__ Jobs jobs) {
+// TM: the tile's rows. AK, BK: whether A's and B's unit stride is the sum's.
+template <int EPI, int TM, bool AK, bool BK>
+__global__ void __launch_bounds__(kThreads, Layout<TM>::kPerSm) ffn_simt_kernel(const __grid_constant__ Jobs jobs) {
+  using L = Layout<TM>;
   extern __shared__ __align__(16) float smem[];
   constexpr int kTileN = EPI == kGlu ? kTile / 2 : kTile;
+  constexpr bool few = TM == kFewRows;
   int job = 0;
 #pragma unroll
   for (int j = 1; j < kFfnMaxJobs; ++j)
     if (j < jobs.count && static_cast<int>(blockIdx.x) >= jobs.first[j]) job = j;
   const FfnProduct& p = jobs.p[job];
-  const int tile = static_cast<int>(blockIdx.x) - jobs.first[job], tile_m = tile / jobs.tiles_n[job];
-  const int64_t m0 = static_cast<int64_t>(tile_m) * kTile;
-  const int64_t n0 = static_cast<int64_t>(tile - tile_m * jobs.tiles_n[job]) * kTileN;
+  const int tile = static_cast<int>(blockIdx.x) - jobs.first[job], line = tile / jobs.run[job];
+  const int at = tile - line * jobs.run[job];
+  const int64_t m0 = static_cast<int64_t>(few ? at : line) * TM, n0 = static_cast<int64_t>(few ? line : at) * kTileN;
   const int group = threadIdx.x / kGroup, tid = threadIdx.x % kGroup, lane = threadIdx.x & 31;
-  const int ty = (tid >> 5) * 32 + 4 * (lane >> 3), tx = 4 * (lane & 7);
-  float* const mine = smem + group * kGroupFloats;  // the group's stages, [A, B][step][row] each
-  uint64_t acc[8][4] = {};  // pairs of columns
+  // 64 rows: a thread's 4 + 4 rows and columns begin at ty and tx. A few: all rows, four columns from tx, every fourth
+  // block of four steps.
+  const int ty = (tid >> 5) * 32 + 4 * (lane >> 3), tx = few ? 4 * (tid & 15) : 4 * (lane & 7);
+  const int quarter = tid >> 4;
+  float* const mine = smem + group * L::kGroupFloats;
+  constexpr int kPairs = few ? 2 : 4;
+  uint64_t acc[8][kPairs] = {};  // pairs of columns
 
   // the CTA's stages of each term's sum, dealt out to the groups
   const int per_term = static_cast<int>((p.K + kDepth - 1) / kDepth), stages = per_term * p.terms;
   const int s0 = static_cast<int>(static_cast<int64_t>(stages) * blockIdx.y / jobs.splits);
   const int s1 = static_cast<int>(static_cast<int64_t>(stages) * (blockIdx.y + 1) / jobs.splits);
-  Loader<kTile, AK> la;
-  Loader<kTileN, BK> lb, lu;  // kGlu: rows of w_gate and of w_up
+  Loader<TM, AK, L::kPitchA> la;
+  Loader<kTileN, BK, kPitch> lb, lu;  // kGlu: rows of w_gate and of w_up
   int term = -1, into = 0;
   auto fetch = [&](int st) {
     if (st < s1) {
@@ -141,7 +165,7 @@ __global__ void __launch_bounds__(kThreads, 2) ffn_simt_kernel(const __grid_cons
         if constexpr (EPI == kGlu) lu.start(p.B[1], n0, k0, tid);
       }
       const int64_t left = p.K - k0;
-      const uint32_t a = smem_u32(mine + into * kStageFloats), b = a + 4 * kDepth * kPitch;
+      const uint32_t a = smem_u32(mine + into * L::kStage), b = a + 4 * L::kStageA;
       la.fetch(a, left, tid);
       lb.fetch(b, left, tid);
       if constexpr (EPI == kGlu) lu.fetch(b + 4 * kTileN, left, tid);
@@ -156,122 +180,185 @@ __global__ void __launch_bounds__(kThreads, 2) ffn_simt_kernel(const __grid_cons
     asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2) : "memory");
     asm volatile("bar.sync %0, %1;" ::"r"(1 + group), "n"(kGroup) : "memory");  // arrived, and the one before it has been read
     fetch(st + (kStages - 1) * kGroups);
-    const float *sA = mine + slot * kStageFloats, *sB = sA + kDepth * kPitch;
+    const float *sA = mine + slot * L::kStage, *sB = sA + L::kStageA;
 #pragma unroll
-    for (int k = 0; k < kDepth; ++k) {
+    for (int step = 0; step < (few ? kDepth / 4 : kDepth); ++step) {
       float a[8];
-      uint64_t b[4];
-      read4(&sA[k * kPitch + ty], swap(AK, k), a);
-      read4(&sA[k * kPitch + ty + 16], swap(AK, k), a + 4);
-      read_pairs(&sB[k * kPitch + tx], swap(BK, k), b);
-      read_pairs(&sB[k * kPitch + tx + 32], swap(BK, k), b + 2);
+      uint64_t b[kPairs];
+      if constexpr (few) {
+        const int k = 4 * quarter + step;
+        read4(&sA[k * L::kPitchA], 0, a);
+        read4(&sA[k * L::kPitchA + 4], 0, a + 4);
+        read_pairs(&sB[k * kPitch + tx], 0, b);
+      } else {
+        const int k = step;
+        read4(&sA[k * L::kPitchA + ty], swap(AK, k), a);
+        read4(&sA[k * L::kPitchA + ty + 16], swap(AK, k), a + 4);
+        read_pairs(&sB[k * kPitch + tx], swap(BK, k), b);
+        read_pairs(&sB[k * kPitch + tx + 32], swap(BK, k), b + 2);
+      }
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         uint64_t aa;
         asm("mov.b64 %0, {%1, %1};" : "=l"(aa) : "f"(a[i]));
 #pragma unroll
-        for (int j = 0; j < 4; ++j) asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(acc[i][j]) : "l"(aa), "l"(b[j]));
+        for (int j = 0; j < kPairs; ++j) asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(acc[i][j]) : "l"(aa), "l"(b[j]));
       }
     }
     if (++slot == kStages) slot = 0;
   }
 
-  // the groups' sums in their order, two rows of each thread's eight a group
+  // the groups' sums in their order
   asm volatile("cp.async.wait_group 0;" ::: "memory");
   asm volatile("bar.sync %0, %1;" ::"r"(1 + group), "n"(kGroup) : "memory");
+  if constexpr (few) {  // [quarter][row][column]; a thread finishes one or two results
+    const bool back_a = AK && quarter >= 2, back_b = BK && quarter >= 2;  // swap() of steps 8 to 15
 #pragma unroll
-  for (int i = 0; i < 8; ++i)
+    for (int i = 0; i < 8; ++i)
+      *reinterpret_cast<ulonglong2*>(&mine[(quarter * 8 + (back_a ? i ^ 2 : i)) * kTile + tx]) =
+          make_ulonglong2(back_b ? acc[i][1] : acc[i][0], back_b ? acc[i][0] : acc[i][1]);
+    __syncthreads();
+    const auto sum = [&](int row, int col) {
+      float r = 0.f;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      float lo, hi;
-      asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(acc[i][j]));
-      mine[(8 * i + 2 * j) * kGroup + tid] = lo;
-      mine[(8 * i + 2 * j + 1) * kGroup + tid] = hi;
-    }
-  __syncthreads();
+      for (int g = 0; g < kGroups; ++g)
 #pragma unroll
-  for (int r = 0; r < 8 / kGroups; ++r) {
-    const int i = 8 / kGroups * group + r;
-    float sum[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      sum[j] = smem[(8 * i + j) * kGroup + tid];
-#pragma unroll
-      for (int g = 1; g < kGroups; ++g) sum[j] += smem[g * kGroupFloats + (8 * i + j) * kGroup + tid];
-    }
-    const int64_t m = m0 + ty + (i & 3) + 16 * (i >> 2);
-    if (m >= p.M) continue;
-    if constexpr (EPI == kStore) {
-      float* parts = jobs.parts[job];
-      float* row = parts ? parts + (blockIdx.y * p.M + m) * p.N : static_cast<float*>(p.out) + m * p.ldo;
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int64_t n = n0 + tx + 32 * h;
-        write4(row + n, sum + 4 * h, p.N - n, on16(row));
-      }
-    } else {
-      const bool wide = on16(p.out) && on16(p.out2) && on16(p.slope_gate) && on16(p.slope_up);  // rows are of whole 32 bytes
-      if constexpr (EPI == kGlu) {
-        const int64_t n = n0 + tx, at = m * p.ldo + n;
-        float h[4], sg[4], su[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          float der;
-          ffn_act(p.act, sum[j], su[j], der);
-          h[j] = su[j] * sum[4 + j];
-          sg[j] = der * sum[4 + j];
-        }
-        write4(static_cast<float*>(p.out) + at, h, p.N - n, wide);
+        for (int q = 0; q < 4; ++q) r += smem[g * L::kGroupFloats + (q * 8 + row) * kTile + col];
+      return r;
+    };
+    for (int o = threadIdx.x; o < 8 * kTileN; o += kThreads) {
+      const int row = o / kTileN, col = o % kTileN;
+      const int64_t m = m0 + row, n = n0 + col, to = m * p.ldo + n;
+      if (m >= p.M || n >= p.N) continue;
+      const float v = sum(row, col);
+      if constexpr (EPI == kStore) {
+        if (float* parts = jobs.parts[job]) parts[(blockIdx.y * p.M + m) * p.N + n] = v;
+        else static_cast<float*>(p.out)[to] = v;
+      } else if constexpr (EPI == kGlu) {
+        const float b = sum(row, col + kTileN);
+        float val, der;
+        ffn_act(p.act, v, val, der);
+        static_cast<float*>(p.out)[to] = val * b;
         if (p.slope_gate) {
-          write4(static_cast<float*>(p.slope_gate) + at, sg, p.N - n, wide);
-          write4(static_cast<float*>(p.slope_up) + at, su, p.N - n, wide);
+          static_cast<float*>(p.slope_gate)[to] = der * b;
+          static_cast<float*>(p.slope_up)[to] = val;
         }
       } else {
+        static_cast<float*>(p.out)[to] = v * static_cast<const float*>(p.slope_gate)[to];
+        static_cast<float*>(p.out2)[to] = v * static_cast<const float*>(p.slope_up)[to];
+      }
+    }
+  } else {  // two rows of each thread's eight a group
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        float lo, hi;
+        asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(acc[i][j]));
+        mine[(8 * i + 2 * j) * kGroup + tid] = lo;
+        mine[(8 * i + 2 * j + 1) * kGroup + tid] = hi;
+      }
+    __syncthreads();
+#pragma unroll
+    for (int r = 0; r < 8 / kGroups; ++r) {
+      const int i = 8 / kGroups * group + r;
+      float sum[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        sum[j] = smem[(8 * i + j) * kGroup + tid];
+#pragma unroll
+        for (int g = 1; g < kGroups; ++g) sum[j] += smem[g * L::kGroupFloats + (8 * i + j) * kGroup + tid];
+      }
+      const int64_t m = m0 + ty + (i & 3) + 16 * (i >> 2);
+      if (m >= p.M) continue;
+      if constexpr (EPI == kStore) {
+        float* parts = jobs.parts[job];
+        float* row = parts ? parts + (blockIdx.y * p.M + m) * p.N : static_cast<float*>(p.out) + m * p.ldo;
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          const int64_t n = n0 + tx + 32 * h, at = m * p.ldo + n;
-          float da[4], db[4];
+          const int64_t n = n0 + tx + 32 * h;
+          write4(row + n, sum + 4 * h, p.N - n, on16(row));
+        }
+      } else {
+        const bool wide = on16(p.out) && on16(p.out2) && on16(p.slope_gate) && on16(p.slope_up);  // rows are of whole 32 bytes
+        if constexpr (EPI == kGlu) {
+          const int64_t n = n0 + tx, to = m * p.ldo + n;
+          float h[4], sg[4], su[4];
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
-            const bool there = n + j < p.N;
-            da[j] = there ? sum[4 * h + j] * static_cast<const float*>(p.slope_gate)[at + j] : 0.f;
-            db[j] = there ? sum[4 * h + j] * static_cast<const float*>(p.slope_up)[at + j] : 0.f;
+            float der;
+            ffn_act(p.act, sum[j], su[j], der);
+            h[j] = su[j] * sum[4 + j];
+            sg[j] = der * sum[4 + j];
           }
-          write4(static_cast<float*>(p.out) + at, da, p.N - n, wide);
-          write4(static_cast<float*>(p.out2) + at, db, p.N - n, wide);
+          write4(static_cast<float*>(p.out) + to, h, p.N - n, wide);
+          if (p.slope_gate) {
+            write4(static_cast<float*>(p.slope_gate) + to, sg, p.N - n, wide);
+            write4(static_cast<float*>(p.slope_up) + to, su, p.N - n, wide);
+          }
+        } else {
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const int64_t n = n0 + tx + 32 * h, to = m * p.ldo + n;
+            float da[4], db[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const bool there = n + j < p.N;
+              da[j] = there ? sum[4 * h + j] * static_cast<const float*>(p.slope_gate)[to + j] : 0.f;
+              db[j] = there ? sum[4 * h + j] * static_cast<const float*>(p.slope_up)[to + j] : 0.f;
+            }
+            write4(static_cast<float*>(p.out) + to, da, p.N - n, wide);
+            write4(static_cast<float*>(p.out2) + to, db, p.N - n, wide);
+          }
         }
       }
     }
   }
 }
 
-int64_t tiles(int64_t M, int64_t N, int tile_n) { return ((M + kTile - 1) / kTile) * ((N + tile_n - 1) / tile_n); }
+int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+template <int TM> void (*kernel_of(int epilogue, bool ak, bool bk))(Jobs) {  // the orders that occur: see ffn.cuh
+  if (epilogue == kGlu) return ffn_simt_kernel<kGlu, TM, true, true>;
+  if (epilogue == kGluBwd) return ffn_simt_kernel<kGluBwd, TM, true, false>;
+  if (ak) return bk ? ffn_simt_kernel<kStore, TM, true, true> : ffn_simt_kernel<kStore, TM, true, false>;
+  return ffn_simt_kernel<kStore, TM, false, false>;
+}
 
 }  // namespace
 
-int64_t ffn_simt_tiles(int64_t M, int64_t N) { return tiles(M, N, kTile); }
+// Tiles of 8 rows rather than 64: the forward of 2048 x 8192 takes 78 us against
+// 182 at 8 rows, 128 against 183 at 16, 201 against 185 at 32; of 512 x 2048, 27
+// against 34 at 32.
+bool ffn_simt_few(int64_t M) { return M <= 24; }
 
-// CTAs that share the sum of one tile: until there are two an SM, each with at
-// least 8 stages (128 steps), two a group.
-int ffn_simt_splits(int64_t tiles, int64_t K, int terms) {
-  const int64_t by_sms = 2 * sm_count() / tiles, by_depth = (K + kDepth - 1) / kDepth * terms / (2 * kGroups);
+int64_t ffn_simt_tiles(int64_t M, int64_t N, bool few) { return ceil_div(M, few ? kFewRows : kTile) * ceil_div(N, kTile); }
+
+// CTAs that share the sum of one tile: until an SM has as many as it can hold,
+// each with at least 8 stages (128 steps), two a group.
+int ffn_simt_splits(int64_t tiles, int64_t K, int terms, bool few) {
+  const int per_sm = few ? Layout<kFewRows>::kPerSm : Layout<kTile>::kPerSm;
+  const int64_t by_sms = per_sm * sm_count() / tiles, by_depth = ceil_div(K, kDepth) * terms / (2 * kGroups);
   const int64_t s = by_sms < by_depth ? by_sms : by_depth;
   return static_cast<int>(s < 1 ? 1 : s > 32 ? 32 : s);
 }
 
 int ffn_simt_launch(const FfnProduct* ps, int count, float* parts, cudaStream_t s) {
   const int epilogue = ps[0].epilogue, tile_n = epilogue == kGlu ? kTile / 2 : kTile;
+  bool few = true;
+  for (int j = 0; j < count; ++j) few = few && ffn_simt_few(ps[j].M);
   Jobs jobs{};
   jobs.count = count;
   int64_t total = 0;
   for (int j = 0; j < count; ++j) {
+    const int64_t rows = ceil_div(ps[j].M, few ? kFewRows : kTile), cols = ceil_div(ps[j].N, tile_n);
     jobs.p[j] = ps[j];
-    jobs.tiles_n[j] = static_cast<int>((ps[j].N + tile_n - 1) / tile_n);
+    jobs.run[j] = static_cast<int>(few ? rows : cols);
     jobs.first[j] = static_cast<int>(total);
-    total += tiles(ps[j].M, ps[j].N, tile_n);
+    total += rows * cols;
     if (total > INT_MAX) return HC_ERR_BAD_SIZE;
   }
-  jobs.splits = epilogue == kStore ? ffn_simt_splits(total, ps[0].K, ps[0].terms) : 1;
+  jobs.splits = epilogue == kStore ? ffn_simt_splits(total, ps[0].K, ps[0].terms, few) : 1;
   if (jobs.splits > 1) {
     if (!parts) return HC_ERR_SCRATCH;
     float* at = parts;
@@ -280,18 +367,14 @@ int ffn_simt_launch(const FfnProduct* ps, int count, float* parts, cudaStream_t 
       at += jobs.splits * ps[j].M * ps[j].N;
     }
   }
-  const dim3 grid(static_cast<unsigned>(total), jobs.splits);
   const bool ak = ps[0].A[0].k_stride == 1, bk = ps[0].B[0].k_stride == 1;
-  void (*kernel)(Jobs) = nullptr;  // the orders that occur: see ffn.cuh
-  if (epilogue == kGlu) kernel = ffn_simt_kernel<kGlu, true, true>;
-  else if (epilogue == kGluBwd) kernel = ffn_simt_kernel<kGluBwd, true, false>;
-  else if (ak) kernel = bk ? ffn_simt_kernel<kStore, true, true> : ffn_simt_kernel<kStore, true, false>;
-  else kernel = ffn_simt_kernel<kStore, false, false>;
-  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes) != cudaSuccess) {
+  const auto kernel = few ? kernel_of<kFewRows>(epilogue, ak, bk) : kernel_of<kTile>(epilogue, ak, bk);
+  const int bytes = few ? Layout<kFewRows>::kBytes : Layout<kTile>::kBytes;
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) {
     cudaGetLastError();
     return HC_ERR_LAUNCH;
   }
-  kernel<<<grid, kThreads, kSmemBytes, s>>>(jobs);
+  kernel<<<dim3(static_cast<unsigned>(total), jobs.splits), kThreads, bytes, s>>>(jobs);
   if (int rc = launch_status()) return rc;
   for (int j = 0; j < count && jobs.splits > 1; ++j)
     if (int rc = ffn_add_parts(jobs.parts[j], ps[j].out, ps[j].M * ps[j].N, jobs.splits, HC_DTYPE_F32, s)) return rc;
