@@ -35,6 +35,7 @@
 #include <type_traits>
 
 #include "block_elem.cuh"
+#include "pairs.cuh"
 
 namespace hc {
 
@@ -47,38 +48,8 @@ constexpr int kNormSmemMax = 210 * 1024;  // of the 227 KB a CTA can have; up to
 constexpr int norm_bwd_threads(int N, int M, int esize) { return M >= 4 || (N == 8 && esize == 4) ? 256 : M == 2 || N == 8 ? 384 : 512; }
 // Chunks a thread may own in the forward (a token's rows then need fewer warps,
 // down to one without barriers): as many as keep a block's rows in registers.
-constexpr int norm_fwd_chunks(bool write, int N, int M, int esize) { return M == 1 && N <= 4 && esize == 2 ? 3 : 1; }
+constexpr int norm_fwd_chunks(int N, int M, int esize) { return M == 1 && N <= 4 && esize == 2 ? 3 : 1; }
 constexpr int norm_fwd_threads(int N, int M, int CH, int esize) { return M >= 4 ? 384 : CH > 1 ? 512 : 640; }
-
-// ------------------------------------------------------- pairs of float32
-using f2 = unsigned long long;
-__device__ __forceinline__ f2 pair(float a, float b) {
-  f2 r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
-  return r;
-}
-__device__ __forceinline__ f2 both(float a) { return pair(a, a); }
-__device__ __forceinline__ void split(f2 v, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
-__device__ __forceinline__ float fold2(f2 v) {
-  float a, b;
-  split(v, a, b);
-  return a + b;
-}
-__device__ __forceinline__ f2 fma2(f2 a, f2 b, f2 c) {
-  f2 r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-  return r;
-}
-__device__ __forceinline__ f2 mul2(f2 a, f2 b) {
-  f2 r;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
-__device__ __forceinline__ f2 add2(f2 a, f2 b) {
-  f2 r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
 
 // K pairs of a row of a small matrix, loaded where they are used: kept for both
 // halves of the columns, a mix of 8 streams alone would fill the registers.
@@ -1218,7 +1189,7 @@ template <typename T, bool WRITE, bool BWD, int N, int M, int CH> NormKernel nor
 }
 template <typename T, bool WRITE, int N, int M> NormKernel norm_kernel_for(bool bwd, int ch) {
   if (bwd) return norm_kernel_of<T, WRITE, true, N, M, 1>();
-  if constexpr (norm_fwd_chunks(WRITE, N, M, sizeof(T)) >= 3) {
+  if constexpr (norm_fwd_chunks(N, M, sizeof(T)) >= 3) {
     if (ch == 3) return norm_kernel_of<T, WRITE, false, N, M, 3>();
     if (ch == 2) return norm_kernel_of<T, WRITE, false, N, M, 2>();
   }
@@ -1241,7 +1212,7 @@ inline NormGeometry norm_geometry(bool write, bool bwd, int n, int m, int64_t D,
   const int N = padded_streams(n), M = padded_blocks(m);
   if (D % kColumns != 0 || M > N) return g;
   const int64_t lines = (D + 32 * kColumns - 1) / (32 * kColumns);  // warps with a chunk a thread
-  const int most = bwd ? 1 : norm_fwd_chunks(write, N, M, esize);
+  const int most = bwd ? 1 : norm_fwd_chunks(N, M, esize);
   g.chunks = static_cast<int>(lines < most ? lines : most);
   const int64_t warps = (lines + g.chunks - 1) / g.chunks;
   const int groups = warps == 1 ? kSmallGroups : 1;

@@ -54,8 +54,8 @@ int ffn_add_parts(const float* parts, void* out, int64_t count, int splits, int 
 
 // Up to kFfnMaxJobs products in one launch, which then share K, one term, the
 // order of their operands and the epilogue kStore. `parts`: the sum of splits *
-// M * N floats where *_splits of all their tiles says more than one (kStore
-// only), else nullptr.
+// M * N floats where the sum is split, more than one (kStore only), else
+// nullptr.
 constexpr int kFfnMaxJobs = 3;
 
 // float32 (ffn_simt.cu); few: every job has few rows.
@@ -66,8 +66,13 @@ int ffn_simt_launch(const FfnProduct* p, int jobs, float* parts, cudaStream_t s)
 
 // bf16 and fp16 (ffn_tc.cu): operands 16-byte aligned with strides of whole 16
 // bytes.
-int64_t ffn_tc_tiles(int64_t M, int64_t N);
-int ffn_tc_splits(int64_t tiles, int64_t K, int terms);
+struct FfnSize {
+  int64_t M, N;
+};
+struct FfnTcPlan {
+  int tile_n, splits;
+};
+FfnTcPlan ffn_tc_plan(const FfnSize* sizes, int jobs, int64_t K, int terms);
 int ffn_tc_launch(const FfnProduct* p, int jobs, int dtype, float* parts, cudaStream_t s);
 
 // bf16 and fp16, the forward's products for at most kFewTokens rows of A

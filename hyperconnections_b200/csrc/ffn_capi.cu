@@ -72,18 +72,16 @@ int fit(Matrix& out, Scratch& scratch, const void* p, int64_t rows, int64_t cols
 bool few(int64_t T, int dtype) { return half(dtype) && T <= kFewTokens; }
 
 // Float32 parts of products [M, N] summed over K in one launch.
-struct Size {
-  int64_t M, N;
-};
-int64_t parts_bytes(std::initializer_list<Size> results, int64_t K, int terms, int dtype) {
-  int64_t tiles = 0, count = 0;
+int64_t parts_bytes(std::initializer_list<FfnSize> results, int64_t K, int terms, int dtype) {
+  int64_t count = 0, tiles = 0;
   bool rows_few = true;
-  for (const Size& r : results) rows_few = rows_few && ffn_simt_few(r.M);
-  for (const Size& r : results) {
-    tiles += half(dtype) ? ffn_tc_tiles(r.M, r.N) : ffn_simt_tiles(r.M, r.N, rows_few);
+  for (const FfnSize& r : results) {
     count += r.M * r.N;
+    rows_few = rows_few && ffn_simt_few(r.M);
   }
-  const int64_t splits = half(dtype) ? ffn_tc_splits(tiles, K, terms) : ffn_simt_splits(tiles, K, terms, rows_few);
+  for (const FfnSize& r : results) tiles += ffn_simt_tiles(r.M, r.N, rows_few);
+  const int64_t splits = half(dtype) ? ffn_tc_plan(results.begin(), static_cast<int>(results.size()), K, terms).splits
+                                     : ffn_simt_splits(tiles, K, terms, rows_few);
   return splits > 1 ? splits * count * 4 : 0;
 }
 
@@ -91,7 +89,7 @@ int64_t parts_bytes(std::initializer_list<Size> results, int64_t K, int terms, i
 int64_t most_parts(int backward, int64_t T, int64_t D, int64_t F, int64_t O, int dtype) {
   if (!backward) return few(T, dtype) ? 0 : parts_bytes({{T, O}}, F, 1, dtype);
   int64_t most = parts_bytes({{T, D}}, F, 2, dtype);
-  const Size g{F, D}, d{O, F};  // w_gate's or w_up's, w_down's
+  const FfnSize g{F, D}, d{O, F};  // w_gate's or w_up's, w_down's
   for (const int64_t b : {parts_bytes({g}, T, 1, dtype), parts_bytes({g, g}, T, 1, dtype), parts_bytes({d}, T, 1, dtype),
                           parts_bytes({g, d}, T, 1, dtype), parts_bytes({g, g, d}, T, 1, dtype)})
     if (b > most) most = b;

@@ -25,6 +25,7 @@
 // memory bounds it.
 #include "ffn.cuh"
 #include "mix_warp.cuh"  // smem_u32
+#include "pairs.cuh"
 
 namespace hc {
 namespace {
@@ -107,7 +108,7 @@ __device__ __forceinline__ void read4(const float* p, int swapped, float* r) {
   const float4 v = *reinterpret_cast<const float4*>(p);
   r[swapped] = v.x; r[swapped + 1] = v.y; r[2 - swapped] = v.z; r[3 - swapped] = v.w;
 }
-__device__ __forceinline__ void read_pairs(const float* p, int swapped, uint64_t* r) {
+__device__ __forceinline__ void read_pairs(const float* p, int swapped, f2* r) {
   const ulonglong2 v = *reinterpret_cast<const ulonglong2*>(p);
   r[swapped / 2] = v.x;
   r[1 - swapped / 2] = v.y;
@@ -146,7 +147,7 @@ __global__ void __launch_bounds__(kThreads, Layout<TM>::kPerSm) ffn_simt_kernel(
   const int quarter = tid >> 4;
   float* const mine = smem + group * L::kGroupFloats;
   constexpr int kPairs = few ? 2 : 4;
-  uint64_t acc[8][kPairs] = {};  // pairs of columns
+  f2 acc[8][kPairs] = {};  // pairs of columns
 
   // the CTA's stages of each term's sum, dealt out to the groups
   const int per_term = static_cast<int>((p.K + kDepth - 1) / kDepth), stages = per_term * p.terms;
@@ -184,7 +185,7 @@ __global__ void __launch_bounds__(kThreads, Layout<TM>::kPerSm) ffn_simt_kernel(
 #pragma unroll
     for (int step = 0; step < (few ? kDepth / 4 : kDepth); ++step) {
       float a[8];
-      uint64_t b[kPairs];
+      f2 b[kPairs];
       if constexpr (few) {
         const int k = 4 * quarter + step;
         read4(&sA[k * L::kPitchA], 0, a);
@@ -199,10 +200,9 @@ __global__ void __launch_bounds__(kThreads, Layout<TM>::kPerSm) ffn_simt_kernel(
       }
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        uint64_t aa;
-        asm("mov.b64 %0, {%1, %1};" : "=l"(aa) : "f"(a[i]));
+        const f2 aa = both(a[i]);
 #pragma unroll
-        for (int j = 0; j < kPairs; ++j) asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(acc[i][j]) : "l"(aa), "l"(b[j]));
+        for (int j = 0; j < kPairs; ++j) acc[i][j] = fma2(aa, b[j], acc[i][j]);
       }
     }
     if (++slot == kStages) slot = 0;
@@ -254,7 +254,7 @@ __global__ void __launch_bounds__(kThreads, Layout<TM>::kPerSm) ffn_simt_kernel(
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         float lo, hi;
-        asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(acc[i][j]));
+        hc::split(acc[i][j], lo, hi);
         mine[(8 * i + 2 * j) * kGroup + tid] = lo;
         mine[(8 * i + 2 * j + 1) * kGroup + tid] = hi;
       }

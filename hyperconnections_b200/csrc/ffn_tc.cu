@@ -9,7 +9,7 @@
 // Clusters are persistent and walk the tiles; per CTA
 //
 //   warp 0      fetches: one lane issues the TMA copies of the CTA's halves of
-//               A and B into a ring of 5 stages of 32 KB (64 deep); both CTAs'
+//               A and B into a ring of 32 KB stages (64 deep); both CTAs'
 //               copies are counted on the leader's barrier
 //   warp 1      multiplies (in the leader CTA): one lane issues the four
 //               16-deep steps of a stage for both CTAs
@@ -45,6 +45,7 @@
 // copies in flight have landed.
 #include "ffn.cuh"
 #include "mix_warp.cuh"
+#include "pairs.cuh"
 
 namespace hc {
 namespace {
@@ -55,16 +56,20 @@ constexpr int kRows = 128;         // rows of A, and of B, that one CTA holds
 constexpr int kTileM = 2 * kRows;  // a pair's tile
 constexpr int kTileN = 2 * kRows;
 constexpr int kDepth = 64;         // elements of the sum in a stage: 128 bytes
-constexpr int kStages = 5;
 constexpr int kOperandBytes = kRows * kDepth * 2;
 constexpr int kStageBytes = 2 * kOperandBytes;
 constexpr int kFinishWarp = 4;    // the first of the finishing warps
 constexpr int kFinishWarps = 16;  // four a scheduler: with two, the activation's chains left it idle two cycles in three
 constexpr int kThreads = 32 * (kFinishWarp + kFinishWarps);
 constexpr int kSlotBytes = kOperandBytes;       // a quarter's: 32 columns of both slopes, and of da and db in their place
-constexpr int kWarpBytes = 4096;                // a finishing warp's results elsewhere: 32 rows of 128 bytes
-constexpr int kStagingBytes = 4 * kSlotBytes;   // the four slots, or the sixteen warps' results
-constexpr int kSmemBytes = kStages * kStageBytes + kStagingBytes + 1024;
+// The ring's stages and a finishing warp's results: 32 rows of 128 bytes, for
+// the three of h and the slopes 64 bytes each.
+constexpr int kMostStages = 5;
+constexpr int stages_of(int epi) { return epi == kGlu ? 4 : kMostStages; }
+constexpr int warp_bytes_of(int epi) { return epi == kGlu ? 3 * 2048 : 4096; }
+constexpr int kSmemBytes = kMostStages * kStageBytes + kFinishWarps * warp_bytes_of(kStore) + 1024;
+static_assert(kSmemBytes >= stages_of(kGlu) * kStageBytes + kFinishWarps * warp_bytes_of(kGlu) + 1024);
+static_assert(kFinishWarps * warp_bytes_of(kGluBwd) == 4 * kSlotBytes);  // or the quarters' slots
 constexpr int kGroupM = 8;  // tiles of A that neighbouring clusters share B with
 
 // Operands by term of a sum of two products, or by job of a launch of several.
@@ -73,7 +78,6 @@ struct alignas(64) TcMaps {
   CUtensorMap out[kFfnMaxJobs];  // kStore: by job; kGlu: h and the slopes; kGluBwd: da and db
   CUtensorMap in[2];             // kGluBwd: the slopes
 };
-static_assert(kStagingBytes == kFinishWarps * kWarpBytes);
 
 // One result. A launch of several shares the depth of the sum and the operands'
 // order.
@@ -91,13 +95,14 @@ struct TcArgs {
   int jobs, tiles, splits;  // tiles of all jobs
   int blocks_term, blocks;  // 64-deep blocks of one term, and of all
   int a_mn, b_mn;           // operands whose unit stride is their rows
+  int tile_n;               // columns of a tile's accumulator
   int act;
   uint32_t wait_limit;
   unsigned int* status;
 };
 
 struct Shared {
-  uint64_t full[kStages], empty[kStages];
+  uint64_t full[kMostStages], empty[kMostStages];
   uint64_t acc_full[2], acc_empty[2], drain;
   uint64_t part_full[4], part_done[4];  // a quarter's slopes have arrived, its results have left: twice a tile
   uint32_t tmem;
@@ -265,6 +270,11 @@ template <> __device__ __forceinline__ uint32_t pack2<__half>(float a, float b) 
   const __half2 h = __floats2half2_rn(a, b);
   return *reinterpret_cast<const uint32_t*>(&h);
 }
+template <typename T> __device__ __forceinline__ uint32_t pack2(f2 v) {
+  float a, b;
+  split(v, a, b);
+  return pack2<T>(a, b);
+}
 __device__ __forceinline__ void st_v8(void* p, const uint32_t* w) {
   asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]),
                "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
@@ -280,22 +290,30 @@ __device__ __forceinline__ float inverse_fast(float x) {
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
   return r;
 }
-// act(a) and act'(a) with the approximate exponential and inverse: their
-// errors, a few 2^-22 relative, are far below the half steps 2^-8 and 2^-11 of
-// the types they go to.
-__device__ __forceinline__ void fast_act(int act, float a, float& val, float& der) {
+// act(a) and act'(a) of two values with the approximate exponential and
+// inverse: their errors, a few 2^-22 relative, are far below the half steps 2^-8
+// and 2^-11 of the types they go to.
+__device__ __forceinline__ f2 sigmoid_of(f2 x) {  // 1 / (1 + 2^x)
+  float e0, e1;
+  split(x, e0, e1);
+  split(add2(pair(exp2_fast(e0), exp2_fast(e1)), both(1.f)), e0, e1);
+  return pair(inverse_fast(e0), inverse_fast(e1));
+}
+__device__ __forceinline__ void fast_act(int act, f2 a, f2& val, f2& der) {
   constexpr float kLog2e = 1.4426950408889634f;
   if (act == HC_ACT_SILU) {
-    const float s = inverse_fast(1.f + exp2_fast(-kLog2e * a));
-    val = a * s;
-    der = fmaf(val, 1.f - s, s);
-  } else {  // tanh(u) = 1 - 2 / (1 + e^2u); past |a| = 10 it is 1, and a^2 need not grow
+    const f2 s = sigmoid_of(mul2(a, both(-kLog2e)));
+    val = mul2(a, s);
+    der = fma2(val, fma2(s, both(-1.f), both(1.f)), s);
+  } else {  // tanh(u) = 1 - 2 i, i = 1 / (1 + e^2u); past |a| = 10 it is 1, and a^2 need not grow
     constexpr float c = 0.7978845608028654f;
-    const float a2 = fminf(a * a, 1e4f), half = 0.5f * a;
-    const float i = inverse_fast(1.f + exp2_fast((2.f * c * kLog2e) * a * fmaf(0.044715f, a2, 1.f)));
-    const float t = fmaf(-2.f, i, 1.f);
-    val = fmaf(half, t, half);
-    der = fmaf(half * fmaf(-t, t, 1.f), fmaf(3.f * 0.044715f * c, a2, c), fmaf(0.5f, t, 0.5f));
+    float q0, q1;
+    split(mul2(a, a), q0, q1);
+    const f2 a2 = pair(fminf(q0, 1e4f), fminf(q1, 1e4f)), half = mul2(a, both(0.5f));
+    const f2 i = sigmoid_of(mul2(mul2(a, both(2.f * c * kLog2e)), fma2(a2, both(0.044715f), both(1.f))));
+    const f2 t = fma2(i, both(-2.f), both(1.f)), less = fma2(i, both(2.f), both(-1.f));
+    val = fma2(half, t, half);
+    der = fma2(mul2(half, fma2(less, t, both(1.f))), fma2(a2, both(3.f * 0.044715f * c), both(c)), fma2(i, both(-1.f), both(1.f)));
   }
 }
 
@@ -309,10 +327,10 @@ template <typename T> struct Part {
   int lane, split, job_id;
   int64_t row0, n0;
   bool inside;  // any of it lies in the result
-  __device__ __forceinline__ Part(const TcArgs& args, const TcMaps& m, const Item& it, int rank, int quad, int part, int tile_n)
+  __device__ __forceinline__ Part(const TcArgs& args, const TcMaps& m, const Item& it, int rank, int quad, int tile_n, int col)
       : a(args), job(args.job[it.job]), maps(m), lane(threadIdx.x & 31), split(it.split), job_id(it.job) {
     row0 = static_cast<int64_t>(it.m) * kTileM + rank * kRows + 32 * quad;
-    n0 = static_cast<int64_t>(it.n) * tile_n + part * (tile_n / 4);
+    n0 = static_cast<int64_t>(it.n) * tile_n + col;
     inside = row0 < job.M && n0 < job.N;
   }
 
@@ -363,14 +381,12 @@ template <typename T> struct Part {
     }
   }
 
-  // 32 columns of h, act'(a) b and act(a); a at acc, b at acc + 128. Two of the
-  // three leave from the warp's two boxes, the third from the first's once it has.
+  // 32 columns of h, act'(a) b and act(a); a at acc, b at acc + 128.
   template <typename Release> __device__ __forceinline__ void glu(uint32_t acc, uint32_t mine, Release release) {
-    const uint32_t box0 = mine, box1 = mine + kWarpBytes / 2;
+    constexpr uint32_t kBox = 2048;
     const bool keep = a.slope_gate != nullptr;
-    if (lane == 0) store_wait_read<0>();
+    if (lane == 0) store_wait_read<0>();  // the last tile's results have left
     __syncwarp();
-    uint32_t su[16];
 #pragma unroll
     for (int st = 0; st < 2; ++st) {
       uint32_t r[16], q[16];
@@ -379,44 +395,37 @@ template <typename T> struct Part {
       acc_wait(r);
       acc_wait(q);
       if (st == 1) release();
-      uint32_t h[8], sg[8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        float v[2], d[2], b[2];
+      for (int c = 0; c < 2; ++c) {
+        uint32_t h[4], sg[4], su[4];
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          b[e] = __uint_as_float(q[2 * i + e]);
-          fast_act(a.act, __uint_as_float(r[2 * i + e]), v[e], d[e]);
+        for (int i = 0; i < 4; ++i) {
+          const int k = 8 * c + 2 * i;
+          const f2 b = pair(__uint_as_float(q[k]), __uint_as_float(q[k + 1]));
+          f2 v, d;
+          fast_act(a.act, pair(__uint_as_float(r[k]), __uint_as_float(r[k + 1])), v, d);
+          h[i] = pack2<T>(mul2(v, b));
+          sg[i] = pack2<T>(mul2(d, b));
+          su[i] = pack2<T>(v);
         }
-        h[i] = pack2<T>(v[0] * b[0], v[1] * b[1]);
-        sg[i] = pack2<T>(d[0] * b[0], d[1] * b[1]);
-        su[8 * st + i] = pack2<T>(v[0], v[1]);
-      }
-      put16(word64(box0, lane, 2 * st), h);
-      put16(word64(box0, lane, 2 * st + 1), h + 4);
-      if (keep) {
-        put16(word64(box1, lane, 2 * st), sg);
-        put16(word64(box1, lane, 2 * st + 1), sg + 4);
+        put16(word64(mine, lane, 2 * st + c), h);
+        if (keep) {
+          put16(word64(mine + kBox, lane, 2 * st + c), sg);
+          put16(word64(mine + 2 * kBox, lane, 2 * st + c), su);
+        }
       }
     }
-    const int x = static_cast<int>(n0), y = static_cast<int>(row0);
     fence_proxy_async_smem();
     __syncwarp();
     if (lane == 0) {
-      if (inside) store_box(&maps.out[0], x, y, box0);
-      store_commit();
-      if (inside && keep) store_box(&maps.out[1], x, y, box1);
-      store_commit();
-      if (keep) store_wait_read<1>();
-    }
-    if (!keep) return;
-    __syncwarp();
-#pragma unroll
-    for (int c = 0; c < 4; ++c) put16(word64(box0, lane, c), su + 4 * c);
-    fence_proxy_async_smem();
-    __syncwarp();
-    if (lane == 0) {
-      if (inside) store_box(&maps.out[2], x, y, box0);
+      if (inside) {
+        const int x = static_cast<int>(n0), y = static_cast<int>(row0);
+        store_box(&maps.out[0], x, y, mine);
+        if (keep) {
+          store_box(&maps.out[1], x, y, mine + kBox);
+          store_box(&maps.out[2], x, y, mine + 2 * kBox);
+        }
+      }
       store_commit();
     }
   }
@@ -466,6 +475,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     ffn_tc_kernel(const __grid_constant__ TcMaps maps, const __grid_constant__ TcArgs a) {
   extern __shared__ uint8_t raw[];
   __shared__ Shared sh;
+  constexpr int kStages = stages_of(EPI), kWarpBytes = warp_bytes_of(EPI);
   const uint32_t ring = (smem_u32(raw) + 1023) & ~1023u, staging = ring + kStages * kStageBytes;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = cluster_rank();
@@ -502,13 +512,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 
   if (warp == 0) {
     if (lane == 0) {
+      // both CTAs' boxes; B's across the sum are 64 columns wide, be there 96 or 128
+      const uint32_t stage_bytes =
+          2 * (kOperandBytes + (a.b_mn ? (a.tile_n > 128 ? 2 : 1) * (kOperandBytes / 2) : a.tile_n / 2 * kDepth * 2));
       int s = 0;
       uint32_t ph = 0;
       bool ok = true;
       for (int i = first; i < items && ok; i += step) {
         const Item it = item_at(a, i);
         const int row_a = it.m * kTileM + static_cast<int>(rank) * kRows;
-        const int row_b = EPI == kGlu ? it.n * kRows : it.n * kTileN + static_cast<int>(rank) * kRows;
+        const int row_b = EPI == kGlu ? it.n * kRows : it.n * a.tile_n + static_cast<int>(rank) * (a.tile_n / 2);
         for (int kb = it.k0; kb < it.k1; ++kb) {
           if (!pair_wait(sh, &sh.empty[s], ph ^ 1, a.wait_limit)) {
             ok = false;
@@ -520,7 +533,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           const CUtensorMap* mb = &maps.b[EPI == kGlu ? static_cast<int>(rank) : it.job + term];
           const uint32_t bar = cluster_addr(&sh.full[s], 0);
           const uint32_t da = ring + s * kStageBytes, db = da + kOperandBytes;
-          if (rank == 0) mbar_expect_tx(&sh.full[s], 2 * kStageBytes);
+          if (rank == 0) mbar_expect_tx(&sh.full[s], stage_bytes);
           if (a.a_mn) {
             fetch_box(da, ma, row_a, k, bar);
             fetch_box(da + kOperandBytes / 2, ma, row_a + 64, k, bar);
@@ -529,7 +542,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           }
           if (a.b_mn) {
             fetch_box(db, mb, row_b, k, bar);
-            fetch_box(db + kOperandBytes / 2, mb, row_b + 64, k, bar);
+            if (a.tile_n > 128) fetch_box(db + kOperandBytes / 2, mb, row_b + 64, k, bar);
           } else {
             fetch_box(db, mb, k, row_b, bar);
           }
@@ -551,10 +564,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     }
   } else if (warp == 1) {
     if (rank == 0 && lane == 0) {
-      // float32 sums of bf16 (format 1) or fp16 (0) operands, 256 x 256
+      // float32 sums of bf16 (format 1) or fp16 (0) operands, 256 x tile_n
       constexpr uint32_t fmt = sizeof(T) == 2 && std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
       const uint32_t idesc = (1u << 4) | (fmt << 7) | (fmt << 10) | (static_cast<uint32_t>(a.a_mn) << 15) |
-                             (static_cast<uint32_t>(a.b_mn) << 16) | ((kTileN >> 3) << 17) | ((kTileM >> 4) << 24);
+                             (static_cast<uint32_t>(a.b_mn) << 16) | (static_cast<uint32_t>(a.tile_n >> 3) << 17) |
+                             ((kTileM >> 4) << 24);
       const uint64_t step_a = (a.a_mn ? 16 * 128 : 32) >> 4, step_b = (a.b_mn ? 16 * 128 : 32) >> 4;
       int s = 0, buf = 0;
       uint32_t ph = 0, acc_ph = 0;
@@ -622,18 +636,19 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     }
   } else if (warp >= kFinishWarp) {
     const int quad = warp & 3, part = (warp - kFinishWarp) >> 2;
-    constexpr int tile_n = EPI == kGlu ? kRows : kTileN;
+    const int tile_n = EPI == kGlu ? kRows : a.tile_n;
+    constexpr int kPart = EPI == kGlu ? 32 : 64;  // columns of a quarter; a narrow tile has none for the last ones
     int buf = 0;
     uint32_t acc_ph = 0;
     for (int i = first; i < items; i += step) {
-      Part<T> tile(a, maps, item_at(a, i), static_cast<int>(rank), quad, part, tile_n);
+      Part<T> tile(a, maps, item_at(a, i), static_cast<int>(rank), quad, tile_n, part * kPart);
       bool ok = pair_wait(sh, &sh.acc_full[buf], acc_ph, a.wait_limit);
       if (!__all_sync(kFull, ok)) {
         if (lane == 0) tell_stop(sh, a);
         break;
       }
       tc_fence_after();
-      const uint32_t acc = tmem + buf * kTileN + (static_cast<uint32_t>(32 * quad) << 16) + part * (tile_n / 4);
+      const uint32_t acc = tmem + buf * kTileN + (static_cast<uint32_t>(32 * quad) << 16) + part * kPart;
       const auto release = [&] {
         tc_fence_before();
         __syncwarp();
@@ -656,6 +671,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           if (lane == 0) tell_stop(sh, a);
           break;
         }
+      } else if (part * kPart >= tile_n) {
+        release();
       } else {
         tile.store(acc, staging + (warp - kFinishWarp) * kWarpBytes, release);
       }
@@ -718,15 +735,16 @@ int pairs_resident() {
 
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
-// The matrix of an operand as a tensor map: 128-byte lines along its unit stride.
-bool encode_operand(CUtensorMap* map, const FfnOperand& o, int64_t K) {
+// The matrix of an operand as a tensor map: 128-byte lines along its unit
+// stride; `rows` of it in a box whose lines lie along the sum.
+bool encode_operand(CUtensorMap* map, const FfnOperand& o, int64_t K, int rows) {
   const auto encode = tensor_map_encoder();
   if (!encode) return false;
   const bool mn = o.k_stride != 1;
   const int64_t inner = mn ? o.rows : K, outer = mn ? K : o.rows, ld = mn ? o.k_stride : o.row_stride;
   const cuuint64_t dims[2] = {static_cast<cuuint64_t>(inner), static_cast<cuuint64_t>(outer)};
   const cuuint64_t strides[1] = {static_cast<cuuint64_t>(ld) * 2};
-  const cuuint32_t box[2] = {64, static_cast<cuuint32_t>(mn ? kDepth : kRows)};
+  const cuuint32_t box[2] = {64, static_cast<cuuint32_t>(mn ? kDepth : rows)};
   const cuuint32_t ones[2] = {1, 1};
   return encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT16, 2, const_cast<void*>(o.p), dims, strides, box, ones,
                 CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
@@ -754,15 +772,29 @@ template <typename T> Kernel kernel_of(int epi) {
 
 }  // namespace
 
-// Clusters that share the sum of one tile: as many as there are for every
-// tile, each with at least 4 blocks (256 deep) of its own.
-int ffn_tc_splits(int64_t tiles, int64_t K, int terms) {
-  const int64_t blocks = ceil_div(K, kDepth) * terms;
-  const int64_t by_pairs = pairs_resident() / tiles, by_depth = blocks / 4;
-  const int64_t s = by_pairs < by_depth ? by_pairs : by_depth;
-  return static_cast<int>(s < 1 ? 1 : s > 32 ? 32 : s);
+// The width of a launch's tiles and the clusters that share the sum of one: as
+// many as there are for every tile, each with at least 4 blocks (256 deep) of
+// its own. A narrower tile where it leaves the clusters less to do: a block
+// takes tile_n cycles twice over, and about 64 more for the rows of A that a
+// narrow tile reads as often. (32,768 tokens, 384 x 1536, fp16: y in NARROWY us with 192
+// columns, WIDEY with 256.)
+FfnTcPlan ffn_tc_plan(const FfnSize* sizes, int jobs, int64_t K, int terms) {
+  const int64_t pairs = pairs_resident(), blocks = ceil_div(K, kDepth) * terms;
+  FfnTcPlan best{};
+  int64_t least = 0;
+  for (int tile_n = kTileN; tile_n >= 128; tile_n -= 64) {
+    int64_t tiles = 0;
+    for (int j = 0; j < jobs; ++j) tiles += ceil_div(sizes[j].M, kTileM) * ceil_div(sizes[j].N, tile_n);
+    int64_t splits = pairs / tiles < blocks / 4 ? pairs / tiles : blocks / 4;
+    splits = splits < 1 ? 1 : splits > 32 ? 32 : splits;
+    const int64_t cost = ceil_div(tiles * splits, pairs) * ceil_div(blocks, splits) * (2 * tile_n + 64);
+    if (tile_n == kTileN || cost < least) {
+      least = cost;
+      best = {tile_n, static_cast<int>(splits)};
+    }
+  }
+  return best;
 }
-int64_t ffn_tc_tiles(int64_t M, int64_t N) { return ceil_div(M, kTileM) * ceil_div(N, kTileN); }
 
 int ffn_tc_launch(const FfnProduct* ps, int jobs, int dtype, float* parts, cudaStream_t s) {
   const FfnProduct& p = ps[0];
@@ -774,19 +806,25 @@ int ffn_tc_launch(const FfnProduct* ps, int jobs, int dtype, float* parts, cudaS
     cudaGetLastError();
     return HC_ERR_LAUNCH;
   }
+  FfnSize sizes[kFfnMaxJobs];
+  for (int j = 0; j < jobs; ++j) sizes[j] = {ps[j].M, ps[j].N};
+  const FfnTcPlan plan = p.epilogue == kStore ? ffn_tc_plan(sizes, jobs, p.K, p.terms) : FfnTcPlan{kTileN, 1};
+  const int rows_b = plan.tile_n / 2;
   TcMaps maps{};
   TcArgs a{};
   a.jobs = jobs;
+  a.tile_n = plan.tile_n;
+  a.splits = plan.splits;
   for (int j = 0; j < jobs; ++j) {
     const int nb = ps[j].epilogue == kGlu ? 2 : ps[j].terms;
     for (int t = 0; t < ps[j].terms; ++t)
-      if (!encode_operand(&maps.a[j + t], ps[j].A[t], p.K)) return HC_ERR_LAUNCH;
+      if (!encode_operand(&maps.a[j + t], ps[j].A[t], p.K, kRows)) return HC_ERR_LAUNCH;
     for (int t = 0; t < nb; ++t)
-      if (!encode_operand(&maps.b[j + t], ps[j].B[t], p.K)) return HC_ERR_LAUNCH;
+      if (!encode_operand(&maps.b[j + t], ps[j].B[t], p.K, rows_b)) return HC_ERR_LAUNCH;
     TcJob& job = a.job[j];
     job.M = ps[j].M; job.N = ps[j].N; job.ldo = ps[j].ldo; job.out = ps[j].out;
     job.tiles_m = static_cast<int>(ceil_div(job.M, kTileM));
-    job.tiles_n = static_cast<int>(ceil_div(job.N, p.epilogue == kGlu ? kRows : kTileN));
+    job.tiles_n = static_cast<int>(ceil_div(job.N, p.epilogue == kGlu ? kRows : plan.tile_n));
     // the hidden tensors' rows always start on 16-byte boundaries
     job.tma = job.ldo % 8 == 0;
     if (job.tma) {
@@ -803,7 +841,6 @@ int ffn_tc_launch(const FfnProduct* ps, int jobs, int dtype, float* parts, cudaS
                                 !encode_rows(&maps.in[1], p.slope_up, p.M, p.N, p.ldo, 32, kRows)))
     return HC_ERR_LAUNCH;
   a.slope_gate = p.slope_gate;
-  a.splits = p.epilogue == kStore ? ffn_tc_splits(a.tiles, p.K, p.terms) : 1;
   if (a.splits > 1) {
     if (!parts) return HC_ERR_SCRATCH;
     float* at = parts;
