@@ -61,15 +61,19 @@ constexpr int kStageBytes = 2 * kOperandBytes;
 constexpr int kFinishWarp = 4;    // the first of the finishing warps
 constexpr int kFinishWarps = 16;  // four a scheduler: with two, the activation's chains left it idle two cycles in three
 constexpr int kThreads = 32 * (kFinishWarp + kFinishWarps);
-constexpr int kSlotBytes = kOperandBytes;       // a quarter's: 32 columns of both slopes, and of da and db in their place
-// The ring's stages and a finishing warp's results: 32 rows of 128 bytes, for
-// the three of h and the slopes 64 bytes each.
-constexpr int kMostStages = 5;
-constexpr int stages_of(int epi) { return epi == kGlu ? 4 : kMostStages; }
-constexpr int warp_bytes_of(int epi) { return epi == kGlu ? 3 * 2048 : 4096; }
-constexpr int kSmemBytes = kMostStages * kStageBytes + kFinishWarps * warp_bytes_of(kStore) + 1024;
-static_assert(kSmemBytes >= stages_of(kGlu) * kStageBytes + kFinishWarps * warp_bytes_of(kGlu) + 1024);
-static_assert(kFinishWarps * warp_bytes_of(kGluBwd) == 4 * kSlotBytes);  // or the quarters' slots
+constexpr int kSlotBytes = kOperandBytes;  // kGluBwd: 32 columns of both slopes, and of da and db in their place
+constexpr int kSlots = 6;
+constexpr int kUses = 8;  // of slots by a tile: the quarters' first 32 columns, then their second ones
+// The ring's stages, and where results are put together: kStore's warps have 32
+// rows of 64 bytes each, kGlu's three of them (h and the slopes).
+constexpr int kMostStages = 6;
+constexpr int stages_of(int epi) { return epi == kStore ? kMostStages : 4; }
+constexpr int kBoxBytes = 32 * 64;
+constexpr int warp_bytes_of(int epi) { return epi == kGlu ? 3 * kBoxBytes : kBoxBytes; }
+constexpr int staging_of(int epi) { return epi == kGluBwd ? kSlots * kSlotBytes : kFinishWarps * warp_bytes_of(epi); }
+constexpr int kSmemBytes = kMostStages * kStageBytes + staging_of(kStore) + 1024;
+static_assert(kSmemBytes == stages_of(kGlu) * kStageBytes + staging_of(kGlu) + 1024);
+static_assert(kSmemBytes == stages_of(kGluBwd) * kStageBytes + staging_of(kGluBwd) + 1024);
 constexpr int kGroupM = 8;  // tiles of A that neighbouring clusters share B with
 
 // Operands by term of a sum of two products, or by job of a launch of several.
@@ -104,7 +108,10 @@ struct TcArgs {
 struct Shared {
   uint64_t full[kMostStages], empty[kMostStages];
   uint64_t acc_full[2], acc_empty[2], drain;
-  uint64_t part_full[4], part_done[4];  // a quarter's slopes have arrived, its results have left: twice a tile
+  // By a tile's use of a slot: its slopes have arrived, its da and db are in place. By use and not by slot, so that who
+  // waits for a phase has itself waited for the one before it; a slot passes from one quarter to another.
+  uint64_t use_full[kUses], use_ready[kUses];
+  uint64_t slot_done[kSlots];  // its results have left
   uint32_t tmem;
   volatile int stop;
 };
@@ -162,9 +169,8 @@ __device__ __forceinline__ uint4 get16(uint32_t at) {
   asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(q.x), "=r"(q.y), "=r"(q.z), "=r"(q.w) : "r"(at));
   return q;
 }
-// 16-byte word c of line r of a box as the TMA swizzles it: lines of 128 bytes
-// (8 words, the line's number modulo 8 mixed in) and of 64 bytes (4 words).
-__device__ __forceinline__ uint32_t word128(uint32_t base, int r, int c) { return base + r * 128 + ((c ^ (r & 7)) << 4); }
+// 16-byte word c of line r of a box of 64-byte lines as the TMA swizzles it: the
+// line's number over two modulo 4 mixed in.
 __device__ __forceinline__ uint32_t word64(uint32_t base, int r, int c) { return base + r * 64 + ((c ^ ((r >> 1) & 3)) << 4); }
 
 __device__ __forceinline__ void mma_pair(uint32_t acc, uint64_t a, uint64_t b, uint32_t idesc, uint32_t add) {
@@ -336,12 +342,13 @@ template <typename T> struct Part {
 
   // 64 columns of the result, or of a part of its sum.
   template <typename Release> __device__ __forceinline__ void store(uint32_t acc, uint32_t mine, Release release) {
-    if (job.tma && !job.parts) {
-      if (lane == 0) store_wait_read<0>();  // the last tile's results have left
-      __syncwarp();
-    }
+    const bool boxes = job.tma && !job.parts;
 #pragma unroll
     for (int st = 0; st < 4; ++st) {
+      if (boxes && (st & 1) == 0) {
+        if (lane == 0) store_wait_read<0>();  // the last 32 columns have left
+        __syncwarp();
+      }
       uint32_t r[16];
       acc_load16(acc + 16 * st, r);
       acc_wait(r);
@@ -363,8 +370,17 @@ template <typename T> struct Part {
         uint32_t w[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) w[i] = pack2<T>(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1]));
-        put16(word128(mine, lane, 2 * st), w);
-        put16(word128(mine, lane, 2 * st + 1), w + 4);
+        put16(word64(mine, lane, 2 * (st & 1)), w);
+        put16(word64(mine, lane, 2 * (st & 1) + 1), w + 4);
+        if (st & 1) {
+          fence_proxy_async_smem();
+          __syncwarp();
+          const int64_t x = n0 + 32 * (st >> 1);
+          if (lane == 0) {
+            if (row0 < job.M && x < job.N) store_box(&maps.out[job_id], static_cast<int>(x), static_cast<int>(row0), mine);
+            store_commit();
+          }
+        }
       } else if (row < job.M) {
         T* p = static_cast<T*>(job.out) + row * job.ldo + n;
 #pragma unroll
@@ -373,17 +389,10 @@ template <typename T> struct Part {
       }
       __syncwarp();  // the next load is the whole warp's
     }
-    if (job.tma && !job.parts) {
-      fence_proxy_async_smem();
-      __syncwarp();
-      if (lane == 0 && inside) store_box(&maps.out[job_id], static_cast<int>(n0), static_cast<int>(row0), mine);
-      if (lane == 0) store_commit();
-    }
   }
 
   // 32 columns of h, act'(a) b and act(a); a at acc, b at acc + 128.
   template <typename Release> __device__ __forceinline__ void glu(uint32_t acc, uint32_t mine, Release release) {
-    constexpr uint32_t kBox = 2048;
     const bool keep = a.slope_gate != nullptr;
     if (lane == 0) store_wait_read<0>();  // the last tile's results have left
     __syncwarp();
@@ -410,8 +419,8 @@ template <typename T> struct Part {
         }
         put16(word64(mine, lane, 2 * st + c), h);
         if (keep) {
-          put16(word64(mine + kBox, lane, 2 * st + c), sg);
-          put16(word64(mine + 2 * kBox, lane, 2 * st + c), su);
+          put16(word64(mine + kBoxBytes, lane, 2 * st + c), sg);
+          put16(word64(mine + 2 * kBoxBytes, lane, 2 * st + c), su);
         }
       }
     }
@@ -422,8 +431,8 @@ template <typename T> struct Part {
         const int x = static_cast<int>(n0), y = static_cast<int>(row0);
         store_box(&maps.out[0], x, y, mine);
         if (keep) {
-          store_box(&maps.out[1], x, y, mine + kBox);
-          store_box(&maps.out[2], x, y, mine + 2 * kBox);
+          store_box(&maps.out[1], x, y, mine + kBoxBytes);
+          store_box(&maps.out[2], x, y, mine + 2 * kBoxBytes);
         }
       }
       store_commit();
@@ -455,19 +464,6 @@ template <typename T> struct Part {
       __syncwarp();
     }
   }
-  __device__ __forceinline__ void glu_bwd_leave(int half, uint32_t gate, uint32_t up) {
-    fence_proxy_async_smem();
-    __syncwarp();
-    if (lane == 0) {
-      const int x = static_cast<int>(n0) + 32 * half, y = static_cast<int>(row0);
-      if (row0 < job.M && x < job.N) {
-        store_box(&maps.out[0], x, y, gate);
-        store_box(&maps.out[1], x, y, up);
-      }
-      store_commit();
-      store_wait_read<0>();  // before the slot is given back
-    }
-  }
 };
 
 template <typename T, int EPI>
@@ -491,10 +487,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       mbar_init(&sh.acc_full[b], 1);
       mbar_init(&sh.acc_empty[b], 2 * kFinishWarps);  // of both CTAs
     }
-    for (int q = 0; q < 4; ++q) {
-      mbar_init(&sh.part_full[q], 1);
-      mbar_init(&sh.part_done[q], 4);  // the quarter's warps
+    for (int u = 0; u < kUses; ++u) {
+      mbar_init(&sh.use_full[u], 1);
+      mbar_init(&sh.use_ready[u], 4);  // the quarter's warps
     }
+    for (int q = 0; q < kSlots; ++q) mbar_init(&sh.slot_done[q], 1);
     mbar_init(&sh.drain, 1);
     sh.stop = 0;
     fence_mbar_init();
@@ -613,25 +610,57 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       }
     }
   } else if (EPI == kGluBwd && warp == 3) {
-    if (lane == 0) {
+    if (lane == 0) {  // the tiles' uses, one after the other, go round the slots
       bool ok = true;
+      uint32_t slot = 0, ph = 0;
       for (int i = first; i < items && ok; i += step) {
         const Item it = item_at(a, i);
         const int row = it.m * kTileM + static_cast<int>(rank) * kRows;
-        for (int use = 0; use < 8; ++use) {  // the quarters' first halves, then their second ones
-          const int half = use >> 2, part = use & 3;
-          // the slot's use before this one has left: its parity is the other half's
-          if ((half || i != first) && !pair_wait(sh, &sh.part_done[part], half ^ 1, a.wait_limit)) {
+        for (int use = 0; use < kUses; ++use) {
+          if (!pair_wait(sh, &sh.slot_done[slot], ph ^ 1, a.wait_limit)) {
             ok = false;
             break;
           }
-          const uint32_t dst = staging + part * kSlotBytes;
-          const int n = it.n * kTileN + part * 64 + half * 32;
-          mbar_expect_tx(&sh.part_full[part], kSlotBytes);
-          fetch_own(dst, &maps.in[0], n, row, &sh.part_full[part]);
-          fetch_own(dst + kSlotBytes / 2, &maps.in[1], n, row, &sh.part_full[part]);
+          const uint32_t dst = staging + slot * kSlotBytes;
+          const int n = it.n * kTileN + (use & 3) * 64 + (use >> 2) * 32;
+          mbar_expect_tx(&sh.use_full[use], kSlotBytes);
+          fetch_own(dst, &maps.in[0], n, row, &sh.use_full[use]);
+          fetch_own(dst + kSlotBytes / 2, &maps.in[1], n, row, &sh.use_full[use]);
+          if (++slot == kSlots) {
+            slot = 0;
+            ph ^= 1;
+          }
         }
       }
+      if (!ok) tell_stop(sh, a);
+    }
+  } else if (EPI == kGluBwd && warp == 2) {
+    if (lane == 0) {  // da and db leave; a slot is given back when the one behind it is on its way
+      bool ok = true;
+      uint32_t slot = 0, ph = 0;
+      int last = -1;
+      for (int i = first; i < items && ok; i += step, ph ^= 1) {
+        const Item it = item_at(a, i);
+        const int row = it.m * kTileM + static_cast<int>(rank) * kRows;
+        for (int use = 0; use < kUses; ++use) {
+          if (!pair_wait(sh, &sh.use_ready[use], ph, a.wait_limit)) {
+            ok = false;
+            break;
+          }
+          const uint32_t src = staging + slot * kSlotBytes;
+          const int n = it.n * kTileN + (use & 3) * 64 + (use >> 2) * 32;
+          if (n < a.job[0].N && row < a.job[0].M) {
+            store_box(&maps.out[0], n, row, src);
+            store_box(&maps.out[1], n, row, src + kSlotBytes / 2);
+          }
+          store_commit();
+          store_wait_read<1>();
+          if (last >= 0) mbar_arrive(&sh.slot_done[last]);
+          last = static_cast<int>(slot);
+          if (++slot == kSlots) slot = 0;
+        }
+      }
+      store_wait_all();
       if (!ok) tell_stop(sh, a);
     }
   } else if (warp >= kFinishWarp) {
@@ -639,7 +668,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     const int tile_n = EPI == kGlu ? kRows : a.tile_n;
     constexpr int kPart = EPI == kGlu ? 32 : 64;  // columns of a quarter; a narrow tile has none for the last ones
     int buf = 0;
-    uint32_t acc_ph = 0;
+    uint32_t acc_ph = 0, uses = 0;  // of the slots, by the tiles before this one
     for (int i = first; i < items; i += step) {
       Part<T> tile(a, maps, item_at(a, i), static_cast<int>(rank), quad, tile_n, part * kPart);
       bool ok = pair_wait(sh, &sh.acc_full[buf], acc_ph, a.wait_limit);
@@ -657,20 +686,22 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       if constexpr (EPI == kGlu) {
         tile.glu(acc, staging + (warp - kFinishWarp) * kWarpBytes, release);
       } else if constexpr (EPI == kGluBwd) {
-        const uint32_t gate = staging + part * kSlotBytes + quad * 32 * 64, up = gate + kSlotBytes / 2;
         for (int half = 0; half < 2; ++half) {
-          ok = pair_wait(sh, &sh.part_full[part], half, a.wait_limit);
+          const int use = 4 * half + part;
+          ok = pair_wait(sh, &sh.use_full[use], uses / kUses & 1, a.wait_limit);
           if (!__all_sync(kFull, ok)) break;
-          tile.glu_bwd(acc, half, gate, up);
+          const uint32_t gate = staging + (uses + use) % kSlots * kSlotBytes + quad * 32 * 64;
+          tile.glu_bwd(acc, half, gate, gate + kSlotBytes / 2);
           if (half) release();
-          tile.glu_bwd_leave(half, gate, up);
+          fence_proxy_async_smem();
           __syncwarp();
-          if (lane == 0) mbar_arrive(&sh.part_done[part]);
+          if (lane == 0) mbar_arrive(&sh.use_ready[use]);
         }
         if (!__all_sync(kFull, ok)) {
           if (lane == 0) tell_stop(sh, a);
           break;
         }
+        uses += kUses;
       } else if (part * kPart >= tile_n) {
         release();
       } else {
@@ -751,17 +782,16 @@ bool encode_operand(CUtensorMap* map, const FfnOperand& o, int64_t K, int rows) 
                 CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-// Rows of a result or of the slopes in boxes of `cols` x `rows`, a box's line of
-// 64 or 128 bytes swizzled.
-bool encode_rows(CUtensorMap* map, void* p, int64_t M, int64_t N, int64_t ld, int cols, int rows) {
+// A result or slopes in boxes of `rows` x 32, the lines of 64 bytes swizzled.
+bool encode_rows(CUtensorMap* map, void* p, int64_t M, int64_t N, int64_t ld, int rows) {
   const auto encode = tensor_map_encoder();
   if (!encode) return false;
   const cuuint64_t dims[2] = {static_cast<cuuint64_t>(N), static_cast<cuuint64_t>(M)};
   const cuuint64_t strides[1] = {static_cast<cuuint64_t>(ld) * 2};
-  const cuuint32_t box[2] = {static_cast<cuuint32_t>(cols), static_cast<cuuint32_t>(rows)};
+  const cuuint32_t box[2] = {32, static_cast<cuuint32_t>(rows)};
   const cuuint32_t ones[2] = {1, 1};
   return encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT16, 2, p, dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                cols == 32 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                 CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
@@ -831,14 +861,14 @@ int ffn_tc_launch(const FfnProduct* ps, int jobs, int dtype, float* parts, cudaS
       const FfnProduct& q = ps[j];
       void* const outs[3] = {q.out, q.epilogue == kGlu ? q.slope_gate : q.out2, q.epilogue == kGlu ? q.slope_up : nullptr};
       for (int k = 0; k < (q.epilogue == kStore ? 1 : 3); ++k)
-        if (outs[k] && !encode_rows(&maps.out[j + k], outs[k], job.M, job.N, job.ldo, q.epilogue == kStore ? 64 : 32, 32))
+        if (outs[k] && !encode_rows(&maps.out[j + k], outs[k], job.M, job.N, job.ldo, q.epilogue == kGluBwd ? kRows : 32))
           return HC_ERR_LAUNCH;
     }
     if (static_cast<int64_t>(job.tiles_m) * job.tiles_n > (int64_t(1) << 24)) return HC_ERR_BAD_SIZE;
     a.tiles += job.tiles_m * job.tiles_n;
   }
-  if (p.epilogue == kGluBwd && (!encode_rows(&maps.in[0], p.slope_gate, p.M, p.N, p.ldo, 32, kRows) ||
-                                !encode_rows(&maps.in[1], p.slope_up, p.M, p.N, p.ldo, 32, kRows)))
+  if (p.epilogue == kGluBwd && (!encode_rows(&maps.in[0], p.slope_gate, p.M, p.N, p.ldo, kRows) ||
+                                !encode_rows(&maps.in[1], p.slope_up, p.M, p.N, p.ldo, kRows)))
     return HC_ERR_LAUNCH;
   a.slope_gate = p.slope_gate;
   if (a.splits > 1) {
