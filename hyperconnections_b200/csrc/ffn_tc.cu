@@ -43,6 +43,8 @@
 // Every wait is bounded (poll limit of status.cu): a warp that gives up
 // reports it, tells both CTAs to stop, and the pair leaves together after its
 // copies in flight have landed.
+#include <cstring>
+
 #include "ffn.cuh"
 #include "mix_warp.cuh"
 #include "pairs.cuh"
@@ -100,6 +102,7 @@ struct TcArgs {
   int blocks_term, blocks;  // 64-deep blocks of one term, and of all
   int a_mn, b_mn;           // operands whose unit stride is their rows
   int tile_n;               // columns of a tile's accumulator
+  uint32_t maps;            // bit i: the i-th of TcMaps is in use
   int act;
   uint32_t wait_limit;
   unsigned int* status;
@@ -148,6 +151,9 @@ __device__ __forceinline__ void fetch_own(uint32_t dst, const CUtensorMap* map, 
       "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
       "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(smem_u32(bar))
       : "memory");
+}
+__device__ __forceinline__ void prefetch_map(const CUtensorMap* map) {
+  asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(map)) : "memory");
 }
 __device__ __forceinline__ void store_box(const CUtensorMap* map, int x, int y, uint32_t src) {
   asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%1, %2}], [%3];" ::"l"(
@@ -478,6 +484,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   const int items = a.tiles * a.splits;
   const int first = blockIdx.x >> 1, step = gridDim.x >> 1;
 
+  pdl_launch_dependents();
+  if (warp == 3 && lane < static_cast<int>(sizeof(TcMaps) / sizeof(CUtensorMap)) && (a.maps >> lane & 1u))
+    prefetch_map(reinterpret_cast<const CUtensorMap*>(&maps) + lane);
   if (threadIdx.x == 0) {
     for (int s = 0; s < kStages; ++s) {
       mbar_init(&sh.full[s], 1);
@@ -506,6 +515,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   cluster_sync();
   tc_fence_after();
   const uint32_t tmem = sh.tmem;
+  pdl_wait_prior_grid();  // no memory is touched before the launches before this one are done
 
   if (warp == 0) {
     if (lane == 0) {
@@ -870,6 +880,11 @@ int ffn_tc_launch(const FfnProduct* ps, int jobs, int dtype, float* parts, cudaS
   if (p.epilogue == kGluBwd && (!encode_rows(&maps.in[0], p.slope_gate, p.M, p.N, p.ldo, kRows) ||
                                 !encode_rows(&maps.in[1], p.slope_up, p.M, p.N, p.ldo, kRows)))
     return HC_ERR_LAUNCH;
+  const CUtensorMap* all = reinterpret_cast<const CUtensorMap*>(&maps);
+  for (size_t i = 0; i < sizeof(TcMaps) / sizeof(CUtensorMap); ++i) {
+    const CUtensorMap none{};
+    if (memcmp(all + i, &none, sizeof(none)) != 0) a.maps |= 1u << i;
+  }
   a.slope_gate = p.slope_gate;
   if (a.splits > 1) {
     if (!parts) return HC_ERR_SCRATCH;
@@ -887,8 +902,20 @@ int ffn_tc_launch(const FfnProduct* ps, int jobs, int dtype, float* parts, cudaS
   a.wait_limit = wait_poll_limit();
   a.status = timeout_word(s);
   const int items = a.tiles * a.splits, pairs = items < pairs_resident() ? items : pairs_resident();
-  kernel<<<2 * pairs, kThreads, kSmemBytes, s>>>(maps, a);
-  if (int rc = launch_status()) return rc;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(2 * pairs);
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = kSmemBytes;
+  cfg.stream = s;
+  cudaLaunchAttribute at[1];  // a product's CTAs come up while the last ones of the product before it leave
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  if (cudaLaunchKernelEx(&cfg, kernel, maps, a) != cudaSuccess) {
+    cudaGetLastError();
+    return HC_ERR_LAUNCH;
+  }
   if (a.splits > 1)
     for (int j = 0; j < jobs; ++j)
       if (int rc = ffn_add_parts(a.job[j].parts, ps[j].out, ps[j].M * ps[j].N, a.splits, dtype, s)) return rc;
