@@ -106,6 +106,7 @@ struct NormArgs {
 struct NormGeometry {
   int warps;   // warps of one token's group (the 8-column kernels); 0 = element by element
   int chunks;  // 8-column chunks a thread owns (forward)
+  bool ragged; // rows that are not whole chunks on 16-byte boundaries
   int grid;    // CTAs
   int rows;    // rows of `partial` that are written
 };

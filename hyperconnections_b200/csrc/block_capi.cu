@@ -38,15 +38,16 @@ bool drop_args(DropArgs& d, double p, const int64_t* state, int64_t seed, int64_
   return true;
 }
 
-// The 8-column kernels take rows of whole 8-column chunks whose group fits a
-// CTA, with every stream and parameter on a 16-byte boundary; the others go
-// element by element. (16,384 tokens of n = 4, D = 768, bf16, forward and
-// backward: 180 us against 3,222 for the mix-write, 90 against 668 for the read.)
+// The 8-column kernels take rows whose group fits a CTA, those of whole chunks
+// on 16-byte boundaries by 16 bytes; the others go element by element. (16,384
+// tokens of n = 4, D = 768, bf16, forward and backward: 180 us against 3,222 for
+// the mix-write, 90 against 668 for the read.)
 NormGeometry geometry(bool write, bool bwd, int n, int m, int64_t D, int esize,
-                      std::initializer_list<const void*> ps) {
-  for (const void* p : ps)
-    if (!aligned16(p)) return NormGeometry{};
-  return norm_geometry(write, bwd, n, m, D, esize);
+                      std::initializer_list<const void*> ps, const float* stats) {
+  if ((reinterpret_cast<uintptr_t>(stats) & 7u) != 0) return NormGeometry{};
+  bool aligned = true;
+  for (const void* p : ps) aligned = aligned && aligned16(p);
+  return norm_geometry(write, bwd, n, m, D, esize, aligned);
 }
 
 int launch(int sdt, bool write, bool bwd, NormGeometry& g, const NormArgs& a, cudaStream_t s) {
@@ -146,7 +147,7 @@ extern "C" int hc_read_norm_fwd(const float* R, const void* x, const float* weig
   a.R = R; a.x = x; a.weight = weight; a.bias = bias; a.out = y; a.stats = stats;
   a.T = T; a.D = D; a.n = n; a.m = m; a.norm = norm; a.eps = eps;
   NormGeometry geo = geometry(false, false, n, m, D, dtype_size(stream_dtype),
-                              {x, y, weight, bias, stats});
+                              {x, y, weight, bias}, stats);
   return launch(stream_dtype, false, false, geo, a, static_cast<cudaStream_t>(stream));
 }
 
@@ -175,7 +176,7 @@ extern "C" int hc_read_norm_bwd(const void* g, const float* R, const void* x, co
   a.grad_x = grad_x; a.grad_R = grad_R; a.partial = params ? scratch : nullptr;
   a.T = T; a.D = D; a.n = n; a.m = m; a.norm = norm;
   NormGeometry geo = geometry(false, true, n, m, D, dtype_size(stream_dtype),
-                              {g, x, grad_x, weight, scratch});
+                              {g, x, grad_x, weight, scratch}, nullptr);
   if (int rc = launch(stream_dtype, false, true, geo, a, s)) return rc;
   return params ? norm_param_grads(scratch, geo.rows, E, weight, nullptr, nullptr, grad_weight, grad_bias, nullptr, s)
                 : HC_OK;
@@ -206,7 +207,7 @@ extern "C" int hc_mix_write_norm_fwd(const float* H, const void* x, const float*
   a.out = out; a.stats = stats; a.T = T; a.D = D; a.n = n; a.m = m; a.norm = norm; a.gate_act = gate_act; a.eps = eps;
   drop_args(a.drop, p, state, seed, offset);
   NormGeometry geo = geometry(true, false, n, m, D, dtype_size(stream_dtype),
-                              {x, f, gate, out, weight, bias, scale, stats});
+                              {x, f, gate, out, weight, bias, scale}, stats);
   return launch(stream_dtype, true, false, geo, a, static_cast<cudaStream_t>(stream));
 }
 
@@ -243,7 +244,7 @@ extern "C" int hc_mix_write_norm_bwd(const void* g, const float* H, const void* 
   a.T = T; a.D = D; a.n = n; a.m = m; a.norm = norm; a.gate_act = gate_act;
   drop_args(a.drop, p, state, seed, offset);
   NormGeometry geo = geometry(true, true, n, m, D, dtype_size(stream_dtype),
-                              {g, x, f, gate, grad_x, grad_f, grad_gate, weight, bias, scale, scratch});
+                              {g, x, f, gate, grad_x, grad_f, grad_gate, weight, bias, scale, scratch}, nullptr);
   if (int rc = launch(stream_dtype, true, true, geo, a, s)) return rc;
   return params ? norm_param_grads(scratch, geo.rows, E, weight, bias, scale, grad_weight, grad_bias, grad_scale, s)
                 : HC_OK;

@@ -1,5 +1,5 @@
-// block_norm.cuh — the norm kernels for rows of whole 8-column chunks (D a
-// multiple of 8, streams and parameters on 16-byte boundaries).
+// block_norm.cuh — the norm kernels by eight columns a thread: for rows of whole
+// chunks on 16-byte boundaries (D a multiple of 8), and, ragged, for any others.
 //
 // A token belongs to a group of W = ceil(D / 256) warps: a CTA for W > 1, one
 // of a CTA's four warps for W = 1. A thread owns eight columns of every row,
@@ -27,6 +27,12 @@
 //     gradients wait for, and the token's small matrices', which nothing waits
 //     for: those are added behind the next token's barrier. A token costs one
 //     barrier.
+// Ragged rows cost more instructions, not more bytes: they travel in 4-byte
+// copies and are shifted when they are read, g x^T is summed on the FMA units,
+// and outputs are put together in shared memory. (16,384 tokens, n = 4, bf16,
+// forward and backward: 165 us at D = 769 against 122 at 768 for the read, 440
+// against 182 for the mix-write.)
+//
 // The [m D] parameters' gradients are sums over tokens: a thread keeps its
 // columns' sums in registers over all of its group's tokens and writes them
 // once; block_capi.cu adds the groups' sums in order.
@@ -62,6 +68,8 @@ template <int K> __device__ __forceinline__ void pairs(const f2* p, f2 (&v)[K]) 
     for (int i = 0; i < K; i += 2) asm volatile("ld.shared.v2.b64 {%0, %1}, [%2];" : "=l"(v[i]), "=l"(v[i + 1]) : "r"(at + 8 * i));
   }
 }
+
+__device__ __forceinline__ bool on16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
 struct V8 {  // eight columns
   f2 v[4];
@@ -121,11 +129,18 @@ template <typename T> __device__ __forceinline__ void put8(T* p, const V8& r) {
 #pragma unroll
   for (int i = 0; i < kWords<T>; ++i) st_v4(p + i * (16 / sizeof(T)), pack<T>(f + i * (16 / sizeof(T))));
 }
-// Eight values of a float32 parameter, or `none`.
-__device__ __forceinline__ V8 param8(const float* p, int64_t c, bool ok, float none) {
+// Eight values of a float32 parameter, or `none`; of the first `cols` columns where rows are ragged.
+template <bool RAGGED> __device__ __forceinline__ V8 param8(const float* p, int64_t c, int cols, float none) {
   V8 r;
   r.fill(none);
-  if (p && ok) {
+  if (!p || cols == 0) return r;
+  if (RAGGED && (cols < kColumns || !on16(p + c))) {
+    float f[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) f[i] = i < cols ? __ldg(p + c + i) : none;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) r.v[i] = pair(f[2 * i], f[2 * i + 1]);
+  } else {
     const float4 a = __ldg(reinterpret_cast<const float4*>(p + c)), b = __ldg(reinterpret_cast<const float4*>(p + c) + 1);
     r.v[0] = pair(a.x, a.y);
     r.v[1] = pair(a.z, a.w);
@@ -175,6 +190,7 @@ struct Place {
   int W, group, warp, lane, tid;
   int64_t d0;
   bool live;  // owns columns of the row
+  int cols, warp_cols;  // how many: of the thread's first chunk, and of its warp's
   __device__ __forceinline__ Place(int warps, int64_t D) {
     W = warps;
     lane = threadIdx.x & 31;
@@ -184,6 +200,9 @@ struct Place {
     tid = warp * 32 + lane;
     d0 = static_cast<int64_t>(tid) * kColumns;
     live = d0 < D;
+    const int64_t w0 = static_cast<int64_t>(warp) * 256;
+    cols = !live ? 0 : D - d0 < kColumns ? static_cast<int>(D - d0) : kColumns;
+    warp_cols = D <= w0 ? 0 : D - w0 < 256 ? static_cast<int>(D - w0) : 256;
   }
   __device__ __forceinline__ void sync() const {
     if (W == 1)
@@ -203,7 +222,7 @@ struct Place {
 
 // Chunks of eight columns that a thread owns, 32 W apart.
 __device__ __forceinline__ int owned_chunks(const Place& p, int64_t D) {
-  const int total = static_cast<int>(D / kColumns), per = 32 * p.W;
+  const int total = static_cast<int>((D + kColumns - 1) / kColumns), per = 32 * p.W;
   return p.tid < total ? (total - p.tid + per - 1) / per : 0;
 }
 
@@ -213,7 +232,7 @@ __device__ __forceinline__ int owned_chunks(const Place& p, int64_t D) {
 // variance of a LayerNorm is merged from (count, mean, sum of squared
 // deviations) triples pair by pair, which loses nothing where the mean is large
 // against the deviations.
-template <int CH, int M, int MAXW>
+template <bool RAGGED, int CH, int M, int MAXW>
 __device__ __forceinline__ void group_stats(const Place& p, const V8 (&u)[CH][M], int chunks, int m, int norm, float eps,
                                             float inv, float4 (&red)[MAXW], float& mean, float& rstd) {
   mean = 0.f;
@@ -237,7 +256,7 @@ __device__ __forceinline__ void group_stats(const Place& p, const V8 (&u)[CH][M]
     rstd = rsqrtf(fmaf(s, inv, eps));
     return;
   }
-  float c = static_cast<float>(8 * m * chunks), mu = 0.f, m2 = 0.f;
+  float c = static_cast<float>((RAGGED ? p.cols : 8 * chunks) * m), mu = 0.f, m2 = 0.f;
   if (chunks > 0) {
     f2 s2 = both(0.f);
 #pragma unroll
@@ -257,7 +276,12 @@ __device__ __forceinline__ void group_stats(const Place& p, const V8 (&u)[CH][M]
         if (k >= m) break;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const f2 d = add2(u[j][k].v[i], less);
+          f2 d = add2(u[j][k].v[i], less);
+          if (RAGGED && 2 * i + 2 > p.cols) {
+            float lo, hi;
+            split(d, lo, hi);
+            d = pair(2 * i < p.cols ? lo : 0.f, 0.f);
+          }
           q2 = fma2(d, d, q2);
         }
       }
@@ -306,21 +330,50 @@ __device__ __forceinline__ void group_stats(const Place& p, const V8 (&u)[CH][M]
 // bytes of padding, so that the same lane's words of eight rows lie in
 // different banks (warp_gram). All of a thread's addresses are one register and
 // a constant.
+//
+// RAGGED: rows begin where they like and end inside a chunk (one chunk a
+// thread). They travel in 4-byte copies; of 16-bit values the words that hold
+// them, four or, where the first begins inside one, five, the fifth behind the
+// lanes' others, and are shifted when they are read. Outputs are put together
+// in STAGE rows a warp, which it then stores side by side.
 constexpr int kRowPitch = 32 * 16 + 16;
-template <typename T, int ROWS, int CH> struct Rows {
+template <typename T, bool RAGGED> constexpr int kPitchOf = kRowPitch + (RAGGED && sizeof(T) == 2 ? 128 : 0);
+template <typename T, int ROWS, int CH, bool RAGGED = false, int STAGE = 0> struct Rows {
+  static constexpr int kPitch = kPitchOf<T, RAGGED>, kStageRow = 256 * sizeof(T);
+  static_assert(!RAGGED || (CH == 1 && ROWS <= 32));
   uint8_t* mem;
-  int base;
-  __device__ __forceinline__ Rows(uint8_t* smem)
-      : mem(smem), base((threadIdx.x >> 5) * (CH * ROWS * kWords<T> * kRowPitch) + (threadIdx.x & 31) * 16) {
+  int base, cols;
+  mutable uint32_t inside;  // bit i: row i's first value is the second of its word
+  __device__ __forceinline__ Rows(uint8_t* smem, const Place& p)
+      : mem(smem), base((threadIdx.x >> 5) * (CH * ROWS * kWords<T> * kPitch) + (threadIdx.x & 31) * 16), cols(p.cols), inside(0) {
     for (int i = 0; i < CH * ROWS * kWords<T>; ++i)
-      *reinterpret_cast<uint4*>(mem + base + i * kRowPitch) = make_uint4(0u, 0u, 0u, 0u);
+      *reinterpret_cast<uint4*>(mem + base + i * kPitch) = make_uint4(0u, 0u, 0u, 0u);
   }
-  __device__ __forceinline__ int at(int c, int row) const { return base + (c * ROWS + row) * kWords<T> * kRowPitch; }
-  __device__ __forceinline__ int bytes() const { return (blockDim.x >> 5) * (CH * ROWS * kWords<T> * kRowPitch); }
+  __device__ __forceinline__ int at(int c, int row) const { return base + (c * ROWS + row) * kWords<T> * kPitch; }
+  __device__ __forceinline__ int fifth(int row) const { return at(0, row) + kRowPitch - static_cast<int>(threadIdx.x & 31) * 12; }
+  __device__ __forceinline__ int stage_base() const { return static_cast<int>(blockDim.x >> 5) * (CH * ROWS * kWords<T> * kPitch); }
+  __device__ __forceinline__ int bytes() const {
+    return stage_base() + (RAGGED ? static_cast<int>(blockDim.x >> 5) * STAGE * kStageRow : 0);
+  }
   __device__ __forceinline__ void fetch(int c, int row, const T* src) const {
     const uint32_t dst = shared_addr(mem) + at(c, row);
+    if constexpr (!RAGGED) {
 #pragma unroll
-    for (int i = 0; i < kWords<T>; ++i) copy16(dst + i * kRowPitch, src + i * (16 / sizeof(T)));
+      for (int i = 0; i < kWords<T>; ++i) copy16(dst + i * kPitch, src + i * (16 / sizeof(T)));
+    } else if constexpr (sizeof(T) == 4) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (i < cols) copy4(dst + (i >> 2) * kPitch + (i & 3) * 4, src + i);
+    } else {
+      const uint32_t in = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(src) >> 1) & 1u;
+      inside = (inside & ~(1u << row)) | in << row;
+      const T* word = src - in;
+      const int count = cols + static_cast<int>(in);  // values from the first word's beginning on
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (2 * i < count) copy4(dst + 4 * i, word + 2 * i);
+      if (8 < count) copy4(shared_addr(mem) + fifth(row), word + 8);
+    }
   }
   // Rows row .. row + K - 1 of a chunk, of which the first `count` exist, D elements apart.
   template <int K> __device__ __forceinline__ void fetch_rows(int c, int row, const T* src, int count, int64_t D) const {
@@ -330,12 +383,24 @@ template <typename T, int ROWS, int CH> struct Rows {
       src += D;
     }
   }
+  // Two words of 16-bit values of which the first is value `first` of the row; `next` is the word behind them.
+  __device__ __forceinline__ uint2 settle(uint2 q, uint32_t next, int row, int first) const {
+    if (inside >> row & 1u) q = make_uint2(__funnelshift_r(q.x, q.y, 16), __funnelshift_r(q.y, next, 16));
+    const int left = cols - first;
+    if (left < 4) {
+      q.x = left >= 2 ? q.x : left == 1 ? q.x & 0xffffu : 0u;
+      q.y = left == 3 ? q.y & 0xffffu : 0u;
+    }
+    return q;
+  }
   __device__ __forceinline__ V4 half(int c, int row, int h) const {  // columns 4 h .. 4 h + 3
     float f[8];
     if constexpr (kWords<T> == 2) {
-      unpack<T>(*reinterpret_cast<const uint4*>(mem + at(c, row) + h * kRowPitch), f);
+      unpack<T>(*reinterpret_cast<const uint4*>(mem + at(c, row) + h * kPitch), f);
     } else {
-      const uint2 q = *reinterpret_cast<const uint2*>(mem + at(c, row) + h * 8);
+      uint2 q = *reinterpret_cast<const uint2*>(mem + at(c, row) + h * 8);
+      if constexpr (RAGGED)
+        q = settle(q, *reinterpret_cast<const uint32_t*>(mem + (h ? fifth(row) : at(c, row) + 8)), row, 4 * h);
       unpack<T>(make_uint4(q.x, q.y, 0u, 0u), f);
     }
     return V4{{pair(f[0], f[1]), pair(f[2], f[3])}};
@@ -343,8 +408,53 @@ template <typename T, int ROWS, int CH> struct Rows {
   __device__ __forceinline__ V8 get(int c, int row) const {
     uint4 q[kWords<T>];
 #pragma unroll
-    for (int i = 0; i < kWords<T>; ++i) q[i] = *reinterpret_cast<const uint4*>(mem + at(c, row) + i * kRowPitch);
+    for (int i = 0; i < kWords<T>; ++i) q[i] = *reinterpret_cast<const uint4*>(mem + at(c, row) + i * kPitch);
+    if constexpr (RAGGED && kWords<T> == 1) {
+      const uint2 a = settle(make_uint2(q[0].x, q[0].y), q[0].z, row, 0);
+      const uint2 b = settle(make_uint2(q[0].z, q[0].w), *reinterpret_cast<const uint32_t*>(mem + fifth(row)), row, 4);
+      q[0] = make_uint4(a.x, a.y, b.x, b.y);
+    }
     return expand<T>(q);
+  }
+  // Ragged outputs: columns into a staged row, then `count` of the staged rows, D elements apart in memory, from the
+  // thread's column of the first on.
+  __device__ __forceinline__ T* staged(int row) const {
+    return reinterpret_cast<T*>(mem + stage_base() + ((threadIdx.x >> 5) * STAGE + row) * kStageRow);
+  }
+  __device__ __forceinline__ void stage8(int row, const V8& v) const {
+    float f[8];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) split(v.v[i], f[2 * i], f[2 * i + 1]);
+#pragma unroll
+    for (int i = 0; i < kWords<T>; ++i)
+      *reinterpret_cast<uint4*>(staged(row) + (threadIdx.x & 31) * 8 + i * (16 / sizeof(T))) = pack<T>(f + i * (16 / sizeof(T)));
+  }
+  __device__ __forceinline__ void stage4(int row, int h, const V4& v) const {
+    float f[8] = {};
+    split(v.v[0], f[0], f[1]);
+    split(v.v[1], f[2], f[3]);
+    const uint4 q = pack<T>(f);
+    T* to = staged(row) + (threadIdx.x & 31) * 8 + 4 * h;
+    if constexpr (sizeof(T) == 4)
+      *reinterpret_cast<uint4*>(to) = q;
+    else
+      *reinterpret_cast<uint2*>(to) = make_uint2(q.x, q.y);
+  }
+  template <int K> __device__ __forceinline__ void unstage(T* dst, int count, int64_t D, int warp_cols) const {
+    const int lane = threadIdx.x & 31;
+    dst -= 8 * lane;
+    __syncwarp();
+#pragma unroll
+    for (int r = 0; r < K; ++r) {
+      if (r < count) {
+        const T* from = staged(r);
+#pragma unroll
+        for (int e = 0; e < 256; e += 32)
+          if (e + lane < warp_cols) dst[e + lane] = from[e + lane];
+      }
+      dst += D;
+    }
+    __syncwarp();
   }
 };
 __device__ __forceinline__ float one(f2 v) {
@@ -438,7 +548,7 @@ template <int R> struct SmallGrads {
 
 // The groups' sums of the [m D] parameters' gradients; with several groups a
 // CTA each adds its own row.
-template <int CH, int M>
+template <bool RAGGED, int CH, int M>
 __device__ __forceinline__ void store_param_sums(const NormArgs& a, const Place& p, int chunks, const V8 (&A)[CH][M],
                                                  const V8 (&B)[CH][M]) {
   if (!a.partial) return;
@@ -451,6 +561,19 @@ __device__ __forceinline__ void store_param_sums(const NormArgs& a, const Place&
 #pragma unroll
     for (int k = 0; k < M; ++k) {
       if (k >= a.m) break;
+      if constexpr (RAGGED) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          float s[2][2];
+          split(A[c][k].v[i >> 1], s[0][0], s[0][1]);
+          split(B[c][k].v[i >> 1], s[1][0], s[1][1]);
+          if (i < p.cols) {
+            dst[k * a.D + i] = s[0][i & 1];
+            dst[E + k * a.D + i] = s[1][i & 1];
+          }
+        }
+        continue;
+      }
       put8<float>(dst + k * a.D + c * 256 * p.W, A[c][k]);
       put8<float>(dst + E + k * a.D + c * 256 * p.W, B[c][k]);
     }
@@ -473,7 +596,7 @@ __device__ __forceinline__ Memory& group_memory(uint8_t* dyn, const Place& p, in
 }
 
 // ------------------------------------------------------------------- read
-template <typename T, int N, int M, int CH>
+template <typename T, int N, int M, int CH, bool RAGGED>
 __global__ void __launch_bounds__(norm_fwd_threads(N, M, CH, sizeof(T)))
     read_norm_fwd_kernel(const __grid_constant__ NormArgs a, int warps) {
   constexpr int MAXW = norm_fwd_threads(N, M, CH, sizeof(T)) / 32;
@@ -483,7 +606,7 @@ __global__ void __launch_bounds__(norm_fwd_threads(N, M, CH, sizeof(T)))
   const int n = a.n, m = a.m, chunks = owned_chunks(p, a.D), step = 256 * p.W;
   const int64_t D = a.D, E = D * m;
   const float inv = 1.f / static_cast<float>(E);
-  const Rows<T, N, CH> rows(dyn);
+  const Rows<T, N, CH, RAGGED, M> rows(dyn, p);
   auto& sR = group_memory<ReadMemory<N, M>>(dyn, p, rows.bytes()).R;
   clear_small(p, sR);
   const SmallCopies<(N * M + 31) / 32> copies(p, n * m, [&](int id, const float*& src, int& stride, int& dst) {
@@ -519,28 +642,33 @@ __global__ void __launch_bounds__(norm_fwd_threads(N, M, CH, sizeof(T)))
           if (next < a.T) fetch(next, c);
         }
         float mean, rstd;
-        group_stats<CH, M, MAXW>(p, u, chunks, m, a.norm, a.eps, inv, red[parity], mean, rstd);
+        group_stats<RAGGED, CH, M, MAXW>(p, u, chunks, m, a.norm, a.eps, inv, red[parity], mean, rstd);
         if (a.stats && p.tid == 0) *reinterpret_cast<float2*>(a.stats + 2 * t) = make_float2(mean, rstd);
         T* y = static_cast<T*>(a.out) + t * E + p.d0;
         const f2 less = both(-mean), r2 = both(rstd);
 #pragma unroll
         for (int c = 0; c < CH; ++c) {
-          if (c >= chunks) break;
+          if (!RAGGED && c >= chunks) break;
+          const int cols = RAGGED ? p.cols : kColumns;
 #pragma unroll
           for (int k = 0; k < M; ++k) {
             if (k >= m) break;
             const int64_t col = k * D + c * step;
-            const V8 w = param8(a.weight, col + p.d0, true, 1.f), b = param8(a.bias, col + p.d0, true, 0.f);
+            const V8 w = param8<RAGGED>(a.weight, col + p.d0, cols, 1.f), b = param8<RAGGED>(a.bias, col + p.d0, cols, 0.f);
 #pragma unroll
             for (int i = 0; i < 4; ++i) u[c][k].v[i] = fma2(mul2(add2(u[c][k].v[i], less), r2), w.v[i], b.v[i]);
-            put8<T>(y + col, u[c][k]);
+            if constexpr (RAGGED)
+              rows.stage8(k, u[c][k]);
+            else
+              put8<T>(y + col, u[c][k]);
           }
         }
+        if constexpr (RAGGED) rows.template unstage<M>(y, m, D, p.warp_cols);
         __syncwarp();
       });
 }
 
-template <typename T, int N, int M, int CH>
+template <typename T, int N, int M, int CH, bool RAGGED>
 __global__ void __launch_bounds__(norm_bwd_threads(N, M, sizeof(T)))
     read_norm_bwd_kernel(const __grid_constant__ NormArgs a, int warps) {
   static_assert(CH == 1, "the backward's threads own one chunk");
@@ -551,7 +679,7 @@ __global__ void __launch_bounds__(norm_bwd_threads(N, M, sizeof(T)))
   const int n = a.n, m = a.m;
   const int64_t D = a.D, E = D * m;
   const float inv = 1.f / static_cast<float>(E);
-  const Rows<T, N + M, 1> rows(dyn);
+  const Rows<T, N + M, 1, RAGGED, N> rows(dyn, p);
   auto& sR = group_memory<ReadMemory<N, M>>(dyn, p, rows.bytes()).R;
   clear_small(p, sR);
   const SmallCopies<(G + 33) / 32> copies(p, n * m + 2, [&](int id, const float*& src, int& stride, int& dst) {
@@ -610,7 +738,7 @@ __global__ void __launch_bounds__(norm_bwd_threads(N, M, sizeof(T)))
 #pragma unroll
         for (int k = 0; k < M; ++k) {
           const V8 g = rows.get(0, N + k);
-          const V8 w = param8(a.weight, k * D + p.d0, p.live && k < m, 1.f);
+          const V8 w = param8<RAGGED>(a.weight, k * D + p.d0, k < m ? p.cols : 0, 1.f);
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             u[k].v[i] = mul2(add2(u[k].v[i], less), r2);  // xhat
@@ -645,11 +773,18 @@ __global__ void __launch_bounds__(norm_bwd_threads(N, M, sizeof(T)))
           r.fill(0.f);
 #pragma unroll
           for (int k = 0; k < M; ++k) axpy(R[j * M + k], u[k], r);
-          if (store && j < n) put8<T>(gx, r);
-          gx += D;
+          if constexpr (RAGGED) {
+            rows.stage8(j, r);
+          } else {
+            if (store && j < n) put8<T>(gx, r);
+            gx += D;
+          }
           const V8 x = rows.get(0, j);  // 0 where there are no columns
 #pragma unroll
           for (int k = 0; k < M; ++k) acc[j * M + k] = dot(u[k], x);
+        }
+        if constexpr (RAGGED) {
+          if (a.grad_x) rows.template unstage<N>(gx, n, D, p.warp_cols);
         }
         if (next < a.T) fetch_x(next);
         fold_to<G>(acc, p.lane, gram[parity][p.slot()]);
@@ -658,7 +793,7 @@ __global__ void __launch_bounds__(norm_bwd_threads(N, M, sizeof(T)))
       });
   p.sync();
   flush();
-  store_param_sums<1, M>(a, p, p.live ? 1 : 0, A, B);
+  store_param_sums<RAGGED, 1, M>(a, p, p.live ? 1 : 0, A, B);
 }
 
 // -------------------------------------------------------------- mix-write
@@ -681,6 +816,18 @@ __device__ __forceinline__ void keep_mul(V8& v, float scale, const uint32_t (&ma
     split(mul2(v.v[i], both(scale)), x, y);
     v.v[i] = pair(__uint_as_float(__float_as_uint(x) & mask[2 * i]), __uint_as_float(__float_as_uint(y) & mask[2 * i + 1]));
   }
+}
+// The same of eight columns that begin inside a block of four.
+__device__ __forceinline__ void keep_ragged(const DropArgs& d, const DropKey& key, uint64_t element, uint32_t (&mask)[8]) {
+  uint32_t bits = 0;
+#pragma unroll
+  for (int h = 0; h < 3; ++h) {
+    const uint4 w = philox4(key, (element >> 2) + h);
+    bits |= ((w.x > d.below ? 1u : 0u) | (w.y > d.below ? 2u : 0u) | (w.z > d.below ? 4u : 0u) | (w.w > d.below ? 8u : 0u)) << (4 * h);
+  }
+  bits >>= static_cast<uint32_t>(element) & 3u;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) mask[i] = bits >> i & 1u ? 0xffffffffu : 0u;
 }
 // act(a) of a gate, and act'(a).
 __device__ __forceinline__ void gate8(int act, const V8& a, V8& val, V8& der) {
@@ -808,10 +955,11 @@ template <int N> __device__ __forceinline__ void store_gram(const float (&c)[4],
 }
 
 // scale * weight and scale * bias of eight columns from c on.
-__device__ __forceinline__ void scaled_params(const NormArgs& a, int64_t c, bool ok, V8& ws, V8& bs) {
-  const V8 sc = param8(a.scale, c, ok, 1.f);
-  ws = param8(a.weight, c, ok, 1.f);
-  bs = param8(a.bias, c, ok, 0.f);
+template <bool RAGGED>
+__device__ __forceinline__ void scaled_params(const NormArgs& a, int64_t c, int cols, V8& ws, V8& bs) {
+  const V8 sc = param8<RAGGED>(a.scale, c, cols, 1.f);
+  ws = param8<RAGGED>(a.weight, c, cols, 1.f);
+  bs = param8<RAGGED>(a.bias, c, cols, 0.f);
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     ws.v[i] = mul2(ws.v[i], sc.v[i]);
@@ -819,7 +967,7 @@ __device__ __forceinline__ void scaled_params(const NormArgs& a, int64_t c, bool
   }
 }
 
-template <typename T, int N, int M, int CH>
+template <typename T, int N, int M, int CH, bool RAGGED>
 __global__ void __launch_bounds__(norm_fwd_threads(N, M, CH, sizeof(T)))
     write_norm_fwd_kernel(const __grid_constant__ NormArgs a, int warps) {
   constexpr int MAXW = norm_fwd_threads(N, M, CH, sizeof(T)) / 32;
@@ -831,7 +979,7 @@ __global__ void __launch_bounds__(norm_fwd_threads(N, M, CH, sizeof(T)))
   const int64_t D = a.D, E = D * m;
   const float inv = 1.f / static_cast<float>(E);
   const DropKey key = a.drop.on ? drop_key(a.drop) : DropKey{};
-  const Rows<T, N + 2 * M, CH> rows(dyn);  // x, f, gate
+  const Rows<T, N + 2 * M, CH, RAGGED, N> rows(dyn, p);  // x, f, gate
   auto& memory = group_memory<WriteMemory<N, M>>(dyn, p, rows.bytes());
   auto& small = memory.small;
   auto& mixed = memory.mixed;
@@ -871,7 +1019,7 @@ __global__ void __launch_bounds__(norm_fwd_threads(N, M, CH, sizeof(T)))
         }
         float mean = 0.f, rstd = 1.f;
         if (a.norm != HC_NORM_NONE) {
-          group_stats<CH, M, MAXW>(p, z, chunks, m, a.norm, a.eps, inv, red[parity], mean, rstd);
+          group_stats<RAGGED, CH, M, MAXW>(p, z, chunks, m, a.norm, a.eps, inv, red[parity], mean, rstd);
           if (a.stats && p.tid == 0) *reinterpret_cast<float2*>(a.stats + 2 * t) = make_float2(mean, rstd);
         } else {
           p.sync();
@@ -890,7 +1038,7 @@ __global__ void __launch_bounds__(norm_fwd_threads(N, M, CH, sizeof(T)))
             }
             const int64_t col = k * D + p.d0 + c * step;
             V8 ws, bs;
-            scaled_params(a, col, c < chunks, ws, bs);
+            scaled_params<RAGGED>(a, col, RAGGED ? p.cols : c < chunks ? kColumns : 0, ws, bs);
 #pragma unroll
             for (int i = 0; i < 4; ++i) z[c][k].v[i] = fma2(mul2(add2(z[c][k].v[i], less), r2), ws.v[i], bs.v[i]);
             if (a.gate) {
@@ -901,7 +1049,10 @@ __global__ void __launch_bounds__(norm_fwd_threads(N, M, CH, sizeof(T)))
             }
             if (a.drop.on) {
               uint32_t keep[8];
-              keep8(a.drop, key, static_cast<uint64_t>(t * E + col), keep);
+              if constexpr (RAGGED)
+                keep_ragged(a.drop, key, static_cast<uint64_t>(t * E + col), keep);
+              else
+                keep8(a.drop, key, static_cast<uint64_t>(t * E + col), keep);
               keep_mul(z[c][k], a.drop.scale, keep);
             }
           }
@@ -927,17 +1078,22 @@ __global__ void __launch_bounds__(norm_fwd_threads(N, M, CH, sizeof(T)))
               for (int j = 0; j < N; ++j) axpy(hi[j], x[j], r);
 #pragma unroll
               for (int k = 0; k < M; ++k) axpy(wi[k], zh[k], r);
-              if (c < chunks && i < n) put4<T>(dst, r);
-              dst += D;
+              if constexpr (RAGGED) {
+                rows.stage4(i, h, r);
+              } else {
+                if (c < chunks && i < n) put4<T>(dst, r);
+                dst += D;
+              }
             }
           }
+          if constexpr (RAGGED) rows.template unstage<N>(out, n, D, p.warp_cols);
           if (next < a.T) fetch_rest(next, c);
         }
         __syncwarp();
       });
 }
 
-template <typename T, int N, int M, int CH>
+template <typename T, int N, int M, int CH, bool RAGGED>
 __global__ void __launch_bounds__(norm_bwd_threads(N, M, sizeof(T)))
     write_norm_bwd_kernel(const __grid_constant__ NormArgs a, int warps) {
   static_assert(CH == 1, "the backward's threads own one chunk");
@@ -951,7 +1107,7 @@ __global__ void __launch_bounds__(norm_bwd_threads(N, M, sizeof(T)))
   const int64_t D = a.D, E = D * m;
   const float inv = 1.f / static_cast<float>(E);
   const DropKey key = a.drop.on ? drop_key(a.drop) : DropKey{};
-  const Rows<T, 2 * N + 2 * M, 1> rows(dyn);  // g, x, f, gate
+  const Rows<T, 2 * N + 2 * M, 1, RAGGED, N> rows(dyn, p);  // g, x, f, gate
   auto& memory = group_memory<WriteMemory<N, M>>(dyn, p, rows.bytes());
   auto& small = memory.small;
   auto& mixed = memory.mixed;
@@ -1053,11 +1209,18 @@ __global__ void __launch_bounds__(norm_bwd_threads(N, M, sizeof(T)))
             pairs<N>(H + j * N, hj);
 #pragma unroll
             for (int i = 0; i < N; ++i) axpy(hj[i], g[i], r);
-            if (store && j < n) put4<T>(dst, r);
-            dst += D;
+            if constexpr (RAGGED) {
+              rows.stage4(j, h, r);
+            } else {
+              if (store && j < n) put4<T>(dst, r);
+              dst += D;
+            }
           }
         }
-        if constexpr (sizeof(T) == 4) {  // g x^T of float32 streams
+        if constexpr (RAGGED) {
+          if (a.grad_x) rows.template unstage<N>(gx, n, D, p.warp_cols);
+        }
+        if constexpr (sizeof(T) == 4 || RAGGED) {  // g x^T of float32 streams, and of rows that are shifted when they are read
           float acc[GB];
 #pragma unroll
           for (int j = 0; j < N; ++j) {
@@ -1067,7 +1230,7 @@ __global__ void __launch_bounds__(norm_bwd_threads(N, M, sizeof(T)))
             if ((j + 1) * N % GB == 0) fold_to<GB>(acc, p.lane, &gram[parity][p.slot()][(j + 1) * N - GB]);
           }
         }
-        if constexpr (sizeof(T) == 2) {
+        if constexpr (sizeof(T) == 2 && !RAGGED) {
           float gsum[4] = {0.f, 0.f, 0.f, 0.f};
           warp_gram<T, N>(rows, gsum);
           store_gram<N>(gsum, p.lane, gram[parity][p.slot()]);
@@ -1084,11 +1247,14 @@ __global__ void __launch_bounds__(norm_bwd_threads(N, M, sizeof(T)))
           const int64_t col = k * D + p.d0;
           uint32_t keep[8];
           if (a.drop.on) {
-            keep8(a.drop, key, static_cast<uint64_t>(t * E + col), keep);
+            if constexpr (RAGGED)
+                keep_ragged(a.drop, key, static_cast<uint64_t>(t * E + col), keep);
+              else
+                keep8(a.drop, key, static_cast<uint64_t>(t * E + col), keep);
             keep_mul(q[k], a.drop.scale, keep);
           }
           V8 ws, bs, xh = rows.get(0, 2 * N + k);
-          scaled_params(a, col, p.live, ws, bs);
+          scaled_params<RAGGED>(a, col, p.cols, ws, bs);
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             xh.v[i] = mul2(add2(xh.v[i], less), r2);
@@ -1103,7 +1269,10 @@ __global__ void __launch_bounds__(norm_bwd_threads(N, M, sizeof(T)))
               q[k].v[i] = mul2(q[k].v[i], val.v[i]);
               z[k].v[i] = mul2(z[k].v[i], val.v[i]);
             }
-            if (a.grad_gate && p.live) put8<T>(static_cast<T*>(a.grad_gate) + t * E + col, der);
+            if constexpr (RAGGED)
+              rows.stage8(k, der);
+            else if (a.grad_gate && p.live)
+              put8<T>(static_cast<T*>(a.grad_gate) + t * E + col, der);
           }
           if (a.drop.on) keep_mul(z[k], a.drop.scale, keep);
 #pragma unroll
@@ -1114,6 +1283,10 @@ __global__ void __launch_bounds__(norm_bwd_threads(N, M, sizeof(T)))
             s1 = fma2(q[k].v[i], xh.v[i], s1);
             s2 = add2(q[k].v[i], s2);
           }
+        }
+        if constexpr (RAGGED) {
+          if (a.gate && a.grad_gate)
+            rows.template unstage<M>(static_cast<T*>(a.grad_gate) + t * E + p.d0, m, D, p.warp_cols);
         }
         float sums[2] = {fold2(s1), fold2(s2)};  // g is 0 where there are no columns
         fold_to<2>(sums, p.lane, red[parity][p.slot()]);
@@ -1139,7 +1312,7 @@ __global__ void __launch_bounds__(norm_bwd_threads(N, M, sizeof(T)))
           c2 += red[parity][p.slot0() + i][1];
         }
         const f2 k1 = both(-c1 * inv), k2 = both(a.norm == HC_NORM_LAYER ? -c2 * inv : 0.f);
-        if (a.grad_f && p.live) {
+        if (a.grad_f && (RAGGED || p.live)) {
 #pragma unroll
           for (int k = 0; k < M; ++k) {
             if (k >= m) break;
@@ -1149,8 +1322,12 @@ __global__ void __launch_bounds__(norm_bwd_threads(N, M, sizeof(T)))
               for (int i = 0; i < 4; ++i)
                 q[k].v[i] = mul2(r2, fma2(mul2(add2(f.v[i], less), r2), k1, add2(q[k].v[i], k2)));
             }
-            put8<T>(static_cast<T*>(a.grad_f) + t * E + k * D + p.d0, q[k]);
+            if constexpr (RAGGED)
+              rows.stage8(k, q[k]);
+            else
+              put8<T>(static_cast<T*>(a.grad_f) + t * E + k * D + p.d0, q[k]);
           }
+          if constexpr (RAGGED) rows.template unstage<M>(static_cast<T*>(a.grad_f) + t * E + p.d0, m, D, p.warp_cols);
         }
         if (next < a.T) fetch_f(next);
         last = t;
@@ -1159,21 +1336,24 @@ __global__ void __launch_bounds__(norm_bwd_threads(N, M, sizeof(T)))
       });
   p.sync();
   flush();
-  store_param_sums<1, M>(a, p, p.live ? 1 : 0, A, B);
+  store_param_sums<RAGGED, 1, M>(a, p, p.live ? 1 : 0, A, B);
 }
 
 // ------------------------------------------------------------------- host
 using NormKernel = void (*)(NormArgs, int);
 
-inline int padded_streams(int n) { return n <= 1 ? 1 : n <= 2 ? 2 : n <= 4 ? 4 : 8; }
+// Rows of whole chunks have kernels for 1, 2, 4 and 8 streams, ragged ones for 4 and 8.
+inline int padded_streams(int n, bool ragged) { return ragged ? (n <= 4 ? 4 : 8) : n <= 1 ? 1 : n <= 2 ? 2 : n <= 4 ? 4 : 8; }
 inline int padded_blocks(int m) { return m <= 1 ? 1 : m <= 2 ? 2 : 4; }
 
 // Shared memory of a CTA: its threads' rows and its groups' small matrices.
-inline int64_t norm_smem_bytes(bool write, bool bwd, int N, int M, int chunks, int threads, int groups, int esize) {
+inline int64_t norm_smem_bytes(bool write, bool bwd, bool ragged, int N, int M, int chunks, int threads, int groups, int esize) {
   const int rows = write ? (bwd ? 2 * N : N) + 2 * M : N + (bwd ? M : 0);
+  const int pitch = ragged && esize == 2 ? kPitchOf<__half, true> : kRowPitch, stage = !ragged ? 0 : write || bwd ? N : M;
   const int64_t entries = write ? (N * N + N * M + N + 3) / 2 * 2 : N * M + 2;
   const int64_t group = (entries * 8 * kSmallSlots + (write ? N * N * 20 : 0) + 15) / 16 * 16;
-  return static_cast<int64_t>(rows * esize / 2) * chunks * kRowPitch * (threads / 32) + groups * group;
+  const int64_t warp = static_cast<int64_t>(rows * esize / 2) * chunks * pitch + stage * 256 * esize;
+  return warp * (threads / 32) + groups * group;
 }
 static_assert(sizeof(ReadMemory<8, 4>) == (34 * 8 * kSmallSlots + 15) / 16 * 16);
 static_assert(sizeof(WriteMemory<8, 4>) == (106 * 8 * kSmallSlots + 64 * 20 + 15) / 16 * 16);
@@ -1181,61 +1361,89 @@ static_assert(sizeof(WriteMemory<1, 1>) == (6 * 8 * kSmallSlots + 20 + 15) / 16 
 
 // The kernel for n streams, m blocks and ch chunks a thread: the next larger of
 // 1, 2, 4, 8 and of 1, 2, 4 (rows past n and m are neither read nor written).
-template <typename T, bool WRITE, bool BWD, int N, int M, int CH> NormKernel norm_kernel_of() {
-  if constexpr (WRITE && BWD) return write_norm_bwd_kernel<T, N, M, CH>;
-  if constexpr (WRITE && !BWD) return write_norm_fwd_kernel<T, N, M, CH>;
-  if constexpr (!WRITE && BWD) return read_norm_bwd_kernel<T, N, M, CH>;
-  if constexpr (!WRITE && !BWD) return read_norm_fwd_kernel<T, N, M, CH>;
+template <typename T, bool WRITE, bool BWD, int N, int M, int CH, bool RAGGED> NormKernel norm_kernel_of() {
+  if constexpr (WRITE && BWD) return write_norm_bwd_kernel<T, N, M, CH, RAGGED>;
+  if constexpr (WRITE && !BWD) return write_norm_fwd_kernel<T, N, M, CH, RAGGED>;
+  if constexpr (!WRITE && BWD) return read_norm_bwd_kernel<T, N, M, CH, RAGGED>;
+  if constexpr (!WRITE && !BWD) return read_norm_fwd_kernel<T, N, M, CH, RAGGED>;
 }
-template <typename T, bool WRITE, int N, int M> NormKernel norm_kernel_for(bool bwd, int ch) {
-  if (bwd) return norm_kernel_of<T, WRITE, true, N, M, 1>();
-  if constexpr (norm_fwd_chunks(N, M, sizeof(T)) >= 3) {
-    if (ch == 3) return norm_kernel_of<T, WRITE, false, N, M, 3>();
-    if (ch == 2) return norm_kernel_of<T, WRITE, false, N, M, 2>();
+template <typename T, bool WRITE, int N, int M> NormKernel norm_kernel_for(bool bwd, bool ragged, int ch) {
+  if constexpr (N >= 4) {
+    if (ragged)
+      return bwd ? norm_kernel_of<T, WRITE, true, N, M, 1, true>() : norm_kernel_of<T, WRITE, false, N, M, 1, true>();
   }
-  return norm_kernel_of<T, WRITE, false, N, M, 1>();
+  if (bwd) return norm_kernel_of<T, WRITE, true, N, M, 1, false>();
+  if constexpr (norm_fwd_chunks(N, M, sizeof(T)) >= 3) {
+    if (ch == 3) return norm_kernel_of<T, WRITE, false, N, M, 3, false>();
+    if (ch == 2) return norm_kernel_of<T, WRITE, false, N, M, 2, false>();
+  }
+  return norm_kernel_of<T, WRITE, false, N, M, 1, false>();
 }
-template <typename T, bool WRITE> NormKernel norm_kernel(bool bwd, int n, int m, int ch) {
-#define HC_NM(N, M) norm_kernel_for<T, WRITE, N, M>(bwd, ch)
-  if (n == 1) return HC_NM(1, 1);
-  if (n == 2) return m == 1 ? HC_NM(2, 1) : HC_NM(2, 2);
-  if (n <= 4) return m == 1 ? HC_NM(4, 1) : m == 2 ? HC_NM(4, 2) : HC_NM(4, 4);
-  return m == 1 ? HC_NM(8, 1) : m == 2 ? HC_NM(8, 2) : HC_NM(8, 4);
+template <typename T, bool WRITE> NormKernel norm_kernel(bool bwd, bool ragged, int N, int M, int ch) {
+#define HC_NM(N, M) norm_kernel_for<T, WRITE, N, M>(bwd, ragged, ch)
+  if (N == 1) return HC_NM(1, 1);
+  if (N == 2) return M == 1 ? HC_NM(2, 1) : HC_NM(2, 2);
+  if (N == 4) return M == 1 ? HC_NM(4, 1) : M == 2 ? HC_NM(4, 2) : HC_NM(4, 4);
+  return M == 1 ? HC_NM(8, 1) : M == 2 ? HC_NM(8, 2) : HC_NM(8, 4);
 #undef HC_NM
 }
 
 // Warps of a token's group, and for the forward the chunks a thread owns; 0
-// warps where the 8-column kernels do not take the shape (rows that are not
-// whole chunks or do not fit a CTA, more blocks than streams).
-inline NormGeometry norm_geometry(bool write, bool bwd, int n, int m, int64_t D, int esize) {
+// warps where the 8-column kernels do not take the shape (rows that do not fit a
+// CTA, more blocks than streams). `aligned`: streams and parameters on 16-byte
+// boundaries.
+inline NormGeometry norm_geometry(bool write, bool bwd, int n, int m, int64_t D, int esize, bool aligned) {
   NormGeometry g{};
-  const int N = padded_streams(n), M = padded_blocks(m);
-  if (D % kColumns != 0 || M > N) return g;
+  g.ragged = !aligned || D % kColumns != 0;
+  const int N = padded_streams(n, g.ragged), M = padded_blocks(m);
+  if (M > N) return g;
   const int64_t lines = (D + 32 * kColumns - 1) / (32 * kColumns);  // warps with a chunk a thread
-  const int most = bwd ? 1 : norm_fwd_chunks(N, M, esize);
+  const int most = bwd || g.ragged ? 1 : norm_fwd_chunks(N, M, esize);
   g.chunks = static_cast<int>(lines < most ? lines : most);
   const int64_t warps = (lines + g.chunks - 1) / g.chunks;
   const int groups = warps == 1 ? kSmallGroups : 1;
   if (32 * warps * groups > (bwd ? norm_bwd_threads(N, M, esize) : norm_fwd_threads(N, M, g.chunks, esize)) ||
-      norm_smem_bytes(write, bwd, N, M, g.chunks, static_cast<int>(32 * warps * groups), groups, esize) > kNormSmemMax)
+      norm_smem_bytes(write, bwd, g.ragged, N, M, g.chunks, static_cast<int>(32 * warps * groups), groups, esize) > kNormSmemMax)
     return g;
   g.warps = static_cast<int>(warps);
   return g;
+}
+
+// CTAs of a kernel that an SM holds, 0 on an error; the kernel is made ready for
+// that much shared memory. The driver is asked once a kernel, size and device on
+// each thread (a decoding step's read + pre-norm 10.8 -> 10.5 us a call).
+inline int ctas_per_sm(const void* kernel, int threads, int smem) {
+  struct Known {
+    const void* kernel;
+    int threads, smem, device, ctas;
+  };
+  thread_local Known known[64] = {};
+  int device = 0;
+  if (cudaGetDevice(&device) != cudaSuccess) {
+    cudaGetLastError();
+    return 0;
+  }
+  Known& at = known[(reinterpret_cast<uintptr_t>(kernel) / 16 + threads / 32) % 64];
+  if (at.kernel == kernel && at.threads == threads && at.smem == smem && at.device == device) return at.ctas;
+  int ctas = 0;
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kNormSmemMax) != cudaSuccess ||
+      cudaOccupancyMaxActiveBlocksPerMultiprocessor(&ctas, kernel, threads, smem) != cudaSuccess || ctas < 1) {
+    cudaGetLastError();
+    return 0;
+  }
+  at = Known{kernel, threads, smem, device, ctas};
+  return ctas;
 }
 
 template <typename T, bool WRITE>
 int norm_launch(bool bwd, NormGeometry& geo, const NormArgs& a, cudaStream_t s) {
   if (geo.warps == 0) return norm_launch_elem<T>(WRITE, bwd, geo, a, s);
   const int groups = geo.warps == 1 ? kSmallGroups : 1, threads = 32 * geo.warps * groups;
-  const NormKernel k = norm_kernel<T, WRITE>(bwd, a.n, a.m, geo.chunks);
-  const int smem = static_cast<int>(norm_smem_bytes(WRITE, bwd, padded_streams(a.n), padded_blocks(a.m), geo.chunks,
-                                                    threads, groups, sizeof(T)));
-  int per_sm = 0;
-  if (cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, kNormSmemMax) != cudaSuccess ||
-      cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, k, threads, smem) != cudaSuccess || per_sm < 1) {
-    cudaGetLastError();
-    return HC_ERR_LAUNCH;
-  }
+  const int N = padded_streams(a.n, geo.ragged), M = padded_blocks(a.m);
+  const NormKernel k = norm_kernel<T, WRITE>(bwd, geo.ragged, N, M, geo.chunks);
+  const int smem = static_cast<int>(norm_smem_bytes(WRITE, bwd, geo.ragged, N, M, geo.chunks, threads, groups, sizeof(T)));
+  const int per_sm = ctas_per_sm(reinterpret_cast<const void*>(k), threads, smem);
+  if (per_sm < 1) return HC_ERR_LAUNCH;
   const int64_t want = (a.T + groups - 1) / groups, most = static_cast<int64_t>(per_sm) * sm_count();
   geo.grid = static_cast<int>(want < most ? want : most);
   geo.rows = geo.grid * groups;
