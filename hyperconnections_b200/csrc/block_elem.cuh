@@ -1,8 +1,7 @@
 // block_elem.cuh — the norm kernels element by element: any n <= 8, m <= 4, D
 // and alignment, one CTA a token (grid-strided). Every pass reads the token
 // again (from L2 after the first), so these are for the shapes that the
-// 8-column kernels (block_norm.cuh) do not take: tokens too wide for a CTA and
-// more blocks than streams.
+// 8-column kernels (block_norm.cuh) do not take: tokens too wide for a CTA.
 #pragma once
 
 #include "block.cuh"

@@ -1342,9 +1342,13 @@ __global__ void __launch_bounds__(norm_bwd_threads(N, M, sizeof(T)))
 // ------------------------------------------------------------------- host
 using NormKernel = void (*)(NormArgs, int);
 
-// Rows of whole chunks have kernels for 1, 2, 4 and 8 streams, ragged ones for 4 and 8.
-inline int padded_streams(int n, bool ragged) { return ragged ? (n <= 4 ? 4 : 8) : n <= 1 ? 1 : n <= 2 ? 2 : n <= 4 ? 4 : 8; }
+// Rows of whole chunks have kernels for 1, 2, 4 and 8 streams, ragged ones for 4
+// and 8; none for fewer streams than blocks.
 inline int padded_blocks(int m) { return m <= 1 ? 1 : m <= 2 ? 2 : 4; }
+inline int padded_streams(int n, int M, bool ragged) {
+  const int least = ragged ? 4 : M > n ? M : n;
+  return least <= 1 && n <= 1 ? 1 : least <= 2 && n <= 2 ? 2 : n <= 4 ? 4 : 8;
+}
 
 // Shared memory of a CTA: its threads' rows and its groups' small matrices.
 inline int64_t norm_smem_bytes(bool write, bool bwd, bool ragged, int N, int M, int chunks, int threads, int groups, int esize) {
@@ -1390,13 +1394,12 @@ template <typename T, bool WRITE> NormKernel norm_kernel(bool bwd, bool ragged, 
 
 // Warps of a token's group, and for the forward the chunks a thread owns; 0
 // warps where the 8-column kernels do not take the shape (rows that do not fit a
-// CTA, more blocks than streams). `aligned`: streams and parameters on 16-byte
+// CTA). `aligned`: streams and parameters on 16-byte
 // boundaries.
 inline NormGeometry norm_geometry(bool write, bool bwd, int n, int m, int64_t D, int esize, bool aligned) {
   NormGeometry g{};
   g.ragged = !aligned || D % kColumns != 0;
-  const int N = padded_streams(n, g.ragged), M = padded_blocks(m);
-  if (M > N) return g;
+  const int M = padded_blocks(m), N = padded_streams(n, M, g.ragged);
   const int64_t lines = (D + 32 * kColumns - 1) / (32 * kColumns);  // warps with a chunk a thread
   const int most = bwd || g.ragged ? 1 : norm_fwd_chunks(N, M, esize);
   g.chunks = static_cast<int>(lines < most ? lines : most);
@@ -1439,7 +1442,7 @@ template <typename T, bool WRITE>
 int norm_launch(bool bwd, NormGeometry& geo, const NormArgs& a, cudaStream_t s) {
   if (geo.warps == 0) return norm_launch_elem<T>(WRITE, bwd, geo, a, s);
   const int groups = geo.warps == 1 ? kSmallGroups : 1, threads = 32 * geo.warps * groups;
-  const int N = padded_streams(a.n, geo.ragged), M = padded_blocks(a.m);
+  const int M = padded_blocks(a.m), N = padded_streams(a.n, M, geo.ragged);
   const NormKernel k = norm_kernel<T, WRITE>(bwd, geo.ragged, N, M, geo.chunks);
   const int smem = static_cast<int>(norm_smem_bytes(WRITE, bwd, geo.ragged, N, M, geo.chunks, threads, groups, sizeof(T)));
   const int per_sm = ctas_per_sm(reinterpret_cast<const void*>(k), threads, smem);
