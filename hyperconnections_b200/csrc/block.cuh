@@ -107,6 +107,7 @@ struct NormGeometry {
   int warps;   // warps of one token's group (the 8-column kernels); 0 = element by element
   int chunks;  // 8-column chunks a thread owns (forward)
   bool ragged; // rows that are not whole chunks on 16-byte boundaries
+  bool wide;   // kernels for more threads
   int grid;    // CTAs
   int rows;    // rows of `partial` that are written
 };

@@ -50,12 +50,19 @@ constexpr int kSmallGroups = 4;  // groups of a CTA when a group is one warp
 constexpr int kSmallSlots = 8;   // tokens whose small matrices are held (5 are live; a power of two)
 constexpr int kNormSmemMax = 210 * 1024;  // of the 227 KB a CTA can have; up to 10 KB are static
 
-// Threads of a CTA at most, which bounds the registers of one.
-constexpr int norm_bwd_threads(int N, int M, int esize) { return M >= 4 || (N == 8 && esize == 4) ? 256 : M == 2 || N == 8 ? 384 : 512; }
+// Threads of a CTA at most, which bounds the registers of one. WIDE: kernels
+// with room for 4096 columns, whose registers spill, for tokens that the others
+// have too few threads for.
+constexpr int kWideThreads = 512;
+constexpr int norm_bwd_threads(int N, int M, int esize, bool wide) {
+  return wide ? kWideThreads : M >= 4 || (N == 8 && esize == 4) ? 256 : M == 2 || N == 8 ? 384 : 512;
+}
 // Chunks a thread may own in the forward (a token's rows then need fewer warps,
 // down to one without barriers): as many as keep a block's rows in registers.
 constexpr int norm_fwd_chunks(int N, int M, int esize) { return M == 1 && N <= 4 && esize == 2 ? 3 : 1; }
-constexpr int norm_fwd_threads(int N, int M, int CH, int esize) { return M >= 4 ? 384 : CH > 1 ? 512 : 640; }
+constexpr int norm_fwd_threads(int N, int M, int CH, int esize, bool wide) {
+  return wide ? kWideThreads : M >= 4 ? 384 : CH > 1 ? 512 : 640;
+}
 
 // K pairs of a row of a small matrix, loaded where they are used: kept for both
 // halves of the columns, a mix of 8 streams alone would fill the registers.
@@ -596,10 +603,10 @@ __device__ __forceinline__ Memory& group_memory(uint8_t* dyn, const Place& p, in
 }
 
 // ------------------------------------------------------------------- read
-template <typename T, int N, int M, int CH, bool RAGGED>
-__global__ void __launch_bounds__(norm_fwd_threads(N, M, CH, sizeof(T)))
+template <typename T, int N, int M, int CH, bool RAGGED, bool WIDE>
+__global__ void __launch_bounds__(norm_fwd_threads(N, M, CH, sizeof(T), WIDE))
     read_norm_fwd_kernel(const __grid_constant__ NormArgs a, int warps) {
-  constexpr int MAXW = norm_fwd_threads(N, M, CH, sizeof(T)) / 32;
+  constexpr int MAXW = norm_fwd_threads(N, M, CH, sizeof(T), WIDE) / 32;
   extern __shared__ __align__(16) uint8_t dyn[];
   __shared__ float4 red[2][MAXW];
   const Place p(warps, a.D);
@@ -668,11 +675,11 @@ __global__ void __launch_bounds__(norm_fwd_threads(N, M, CH, sizeof(T)))
       });
 }
 
-template <typename T, int N, int M, int CH, bool RAGGED>
-__global__ void __launch_bounds__(norm_bwd_threads(N, M, sizeof(T)))
+template <typename T, int N, int M, int CH, bool RAGGED, bool WIDE>
+__global__ void __launch_bounds__(norm_bwd_threads(N, M, sizeof(T), WIDE))
     read_norm_bwd_kernel(const __grid_constant__ NormArgs a, int warps) {
   static_assert(CH == 1, "the backward's threads own one chunk");
-  constexpr int MAXW = norm_bwd_threads(N, M, sizeof(T)) / 32, G = N * M;
+  constexpr int MAXW = norm_bwd_threads(N, M, sizeof(T), WIDE) / 32, G = N * M;
   extern __shared__ __align__(16) uint8_t dyn[];
   __shared__ float red[2][MAXW][2], gram[2][MAXW][G];
   const Place p(warps, a.D);
@@ -967,10 +974,10 @@ __device__ __forceinline__ void scaled_params(const NormArgs& a, int64_t c, int 
   }
 }
 
-template <typename T, int N, int M, int CH, bool RAGGED>
-__global__ void __launch_bounds__(norm_fwd_threads(N, M, CH, sizeof(T)))
+template <typename T, int N, int M, int CH, bool RAGGED, bool WIDE>
+__global__ void __launch_bounds__(norm_fwd_threads(N, M, CH, sizeof(T), WIDE))
     write_norm_fwd_kernel(const __grid_constant__ NormArgs a, int warps) {
-  constexpr int MAXW = norm_fwd_threads(N, M, CH, sizeof(T)) / 32;
+  constexpr int MAXW = norm_fwd_threads(N, M, CH, sizeof(T), WIDE) / 32;
   using S = Small<N, M, false>;
   extern __shared__ __align__(16) uint8_t dyn[];
   __shared__ float4 red[2][MAXW];
@@ -1093,11 +1100,11 @@ __global__ void __launch_bounds__(norm_fwd_threads(N, M, CH, sizeof(T)))
       });
 }
 
-template <typename T, int N, int M, int CH, bool RAGGED>
-__global__ void __launch_bounds__(norm_bwd_threads(N, M, sizeof(T)))
+template <typename T, int N, int M, int CH, bool RAGGED, bool WIDE>
+__global__ void __launch_bounds__(norm_bwd_threads(N, M, sizeof(T), WIDE))
     write_norm_bwd_kernel(const __grid_constant__ NormArgs a, int warps) {
   static_assert(CH == 1, "the backward's threads own one chunk");
-  constexpr int MAXW = norm_bwd_threads(N, M, sizeof(T)) / 32;
+  constexpr int MAXW = norm_bwd_threads(N, M, sizeof(T), WIDE) / 32;
   constexpr int GB = N * N < 32 ? N * N : 32, G = N * N + N * M;  // H's sums [column][row] by batches of GB, then W's
   using S = Small<N, M, true>;
   extern __shared__ __align__(16) uint8_t dyn[];
@@ -1365,30 +1372,36 @@ static_assert(sizeof(WriteMemory<1, 1>) == (6 * 8 * kSmallSlots + 20 + 15) / 16 
 
 // The kernel for n streams, m blocks and ch chunks a thread: the next larger of
 // 1, 2, 4, 8 and of 1, 2, 4 (rows past n and m are neither read nor written).
-template <typename T, bool WRITE, bool BWD, int N, int M, int CH, bool RAGGED> NormKernel norm_kernel_of() {
-  if constexpr (WRITE && BWD) return write_norm_bwd_kernel<T, N, M, CH, RAGGED>;
-  if constexpr (WRITE && !BWD) return write_norm_fwd_kernel<T, N, M, CH, RAGGED>;
-  if constexpr (!WRITE && BWD) return read_norm_bwd_kernel<T, N, M, CH, RAGGED>;
-  if constexpr (!WRITE && !BWD) return read_norm_fwd_kernel<T, N, M, CH, RAGGED>;
+template <typename T, bool WRITE, bool BWD, int N, int M, int CH, bool RAGGED, bool WIDE> NormKernel norm_kernel_of() {
+  if constexpr (WRITE && BWD) return write_norm_bwd_kernel<T, N, M, CH, RAGGED, WIDE>;
+  if constexpr (WRITE && !BWD) return write_norm_fwd_kernel<T, N, M, CH, RAGGED, WIDE>;
+  if constexpr (!WRITE && BWD) return read_norm_bwd_kernel<T, N, M, CH, RAGGED, WIDE>;
+  if constexpr (!WRITE && !BWD) return read_norm_fwd_kernel<T, N, M, CH, RAGGED, WIDE>;
 }
-template <typename T, bool WRITE, int N, int M> NormKernel norm_kernel_for(bool bwd, bool ragged, int ch) {
-  if constexpr (N >= 4) {
-    if (ragged)
-      return bwd ? norm_kernel_of<T, WRITE, true, N, M, 1, true>() : norm_kernel_of<T, WRITE, false, N, M, 1, true>();
+template <typename T, bool WRITE, int N, int M, bool RAGGED> NormKernel norm_kernel_for(bool bwd, bool wide, int ch) {
+  if (bwd) {
+    if constexpr (norm_bwd_threads(N, M, sizeof(T), false) < kWideThreads)
+      if (wide) return norm_kernel_of<T, WRITE, true, N, M, 1, RAGGED, true>();
+    return norm_kernel_of<T, WRITE, true, N, M, 1, RAGGED, false>();
   }
-  if (bwd) return norm_kernel_of<T, WRITE, true, N, M, 1, false>();
-  if constexpr (norm_fwd_chunks(N, M, sizeof(T)) >= 3) {
-    if (ch == 3) return norm_kernel_of<T, WRITE, false, N, M, 3, false>();
-    if (ch == 2) return norm_kernel_of<T, WRITE, false, N, M, 2, false>();
+  if constexpr (norm_fwd_threads(N, M, 1, sizeof(T), false) < kWideThreads)
+    if (wide) return norm_kernel_of<T, WRITE, false, N, M, 1, RAGGED, true>();
+  if constexpr (!RAGGED && norm_fwd_chunks(N, M, sizeof(T)) >= 3) {
+    if (ch == 3) return norm_kernel_of<T, WRITE, false, N, M, 3, false, false>();
+    if (ch == 2) return norm_kernel_of<T, WRITE, false, N, M, 2, false, false>();
   }
-  return norm_kernel_of<T, WRITE, false, N, M, 1, false>();
+  return norm_kernel_of<T, WRITE, false, N, M, 1, RAGGED, false>();
 }
-template <typename T, bool WRITE> NormKernel norm_kernel(bool bwd, bool ragged, int N, int M, int ch) {
-#define HC_NM(N, M) norm_kernel_for<T, WRITE, N, M>(bwd, ragged, ch)
-  if (N == 1) return HC_NM(1, 1);
-  if (N == 2) return M == 1 ? HC_NM(2, 1) : HC_NM(2, 2);
-  if (N == 4) return M == 1 ? HC_NM(4, 1) : M == 2 ? HC_NM(4, 2) : HC_NM(4, 4);
-  return M == 1 ? HC_NM(8, 1) : M == 2 ? HC_NM(8, 2) : HC_NM(8, 4);
+template <typename T, bool WRITE> NormKernel norm_kernel(const NormGeometry& geo, bool bwd, int N, int M) {
+#define HC_NM(N, M, RAGGED) norm_kernel_for<T, WRITE, N, M, RAGGED>(bwd, geo.wide, geo.chunks)
+  if (geo.ragged) {
+    if (N == 4) return M == 1 ? HC_NM(4, 1, true) : M == 2 ? HC_NM(4, 2, true) : HC_NM(4, 4, true);
+    return M == 1 ? HC_NM(8, 1, true) : M == 2 ? HC_NM(8, 2, true) : HC_NM(8, 4, true);
+  }
+  if (N == 1) return HC_NM(1, 1, false);
+  if (N == 2) return M == 1 ? HC_NM(2, 1, false) : HC_NM(2, 2, false);
+  if (N == 4) return M == 1 ? HC_NM(4, 1, false) : M == 2 ? HC_NM(4, 2, false) : HC_NM(4, 4, false);
+  return M == 1 ? HC_NM(8, 1, false) : M == 2 ? HC_NM(8, 2, false) : HC_NM(8, 4, false);
 #undef HC_NM
 }
 
@@ -1405,8 +1418,11 @@ inline NormGeometry norm_geometry(bool write, bool bwd, int n, int m, int64_t D,
   g.chunks = static_cast<int>(lines < most ? lines : most);
   const int64_t warps = (lines + g.chunks - 1) / g.chunks;
   const int groups = warps == 1 ? kSmallGroups : 1;
-  if (32 * warps * groups > (bwd ? norm_bwd_threads(N, M, esize) : norm_fwd_threads(N, M, g.chunks, esize)) ||
-      norm_smem_bytes(write, bwd, g.ragged, N, M, g.chunks, static_cast<int>(32 * warps * groups), groups, esize) > kNormSmemMax)
+  const int64_t threads = 32 * warps * groups;
+  const int most_threads = bwd ? norm_bwd_threads(N, M, esize, false) : norm_fwd_threads(N, M, g.chunks, esize, false);
+  g.wide = threads > most_threads && most_threads < kWideThreads;
+  if (threads > (g.wide ? kWideThreads : most_threads) ||
+      norm_smem_bytes(write, bwd, g.ragged, N, M, g.chunks, static_cast<int>(threads), groups, esize) > kNormSmemMax)
     return g;
   g.warps = static_cast<int>(warps);
   return g;
@@ -1443,7 +1459,7 @@ int norm_launch(bool bwd, NormGeometry& geo, const NormArgs& a, cudaStream_t s) 
   if (geo.warps == 0) return norm_launch_elem<T>(WRITE, bwd, geo, a, s);
   const int groups = geo.warps == 1 ? kSmallGroups : 1, threads = 32 * geo.warps * groups;
   const int M = padded_blocks(a.m), N = padded_streams(a.n, M, geo.ragged);
-  const NormKernel k = norm_kernel<T, WRITE>(bwd, geo.ragged, N, M, geo.chunks);
+  const NormKernel k = norm_kernel<T, WRITE>(geo, bwd, N, M);
   const int smem = static_cast<int>(norm_smem_bytes(WRITE, bwd, geo.ragged, N, M, geo.chunks, threads, groups, sizeof(T)));
   const int per_sm = ctas_per_sm(reinterpret_cast<const void*>(k), threads, smem);
   if (per_sm < 1) return HC_ERR_LAUNCH;

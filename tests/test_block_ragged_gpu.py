@@ -35,6 +35,16 @@ READ = [
     (11, 6, 2, 1, "fp16", "rms", "wb"),
     (6, 4, 1, 257, "bf16", "layer", "w"),
     (6, 4, 1, 255, "fp32", "layer", "w"),
+    # tokens that take more threads, and tokens too wide for a CTA
+    (300, 8, 4, 4096, "bf16", "layer", "wb"),
+    (5, 8, 1, 4095, "fp16", "rms", "w"),
+    (5, 4, 4, 4096, "fp16", "layer", "wb"),
+    (5, 8, 2, 2600, "fp32", "rms", "w"),
+    (3, 8, 4, 6000, "fp32", "layer", "wb"),
+    (3, 4, 4, 5001, "bf16", "rms", "w"),
+    (600, 8, 1, 4100, "fp32", "layer", "wb"),
+    (3, 1, 4, 100, "fp32", "layer", "wb"),
+    (3, 2, 3, 77, "bf16", "rms", "wb"),
 ]
 
 
@@ -67,6 +77,15 @@ WRITE = [
     (11, 6, 2, 1, "fp16", "rms", "wb", "", True, 0.0),
     (6, 4, 1, 257, "bf16", "layer", "w", "sigmoid", False, 0.1),
     (6, 4, 1, 255, "fp32", "layer", "w", "sigmoid", False, 0.1),
+    (200, 8, 4, 4096, "bf16", "layer", "wbs", "sigmoid", True, 0.1),
+    (5, 8, 1, 4095, "fp16", "rms", "ws", "linear", False, 0.3),
+    (5, 4, 4, 4096, "fp16", "layer", "wb", "", True, 0.1),
+    (5, 8, 2, 2056, "fp32", "rms", "ws", "sigmoid", True, 0.0),
+    (3, 8, 4, 6000, "fp32", "layer", "wbs", "sigmoid", True, 0.2),
+    (3, 4, 4, 5001, "bf16", "rms", "w", "linear", False, 0.1),
+    (600, 8, 1, 4100, "fp32", "layer", "wb", "sigmoid", True, 0.1),
+    (3, 1, 4, 100, "fp32", "layer", "wbs", "linear", True, 0.1),
+    (3, 2, 3, 77, "bf16", "none", "s", "sigmoid", False, 0.1),
 ]
 
 
