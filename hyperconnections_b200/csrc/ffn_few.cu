@@ -22,6 +22,10 @@ constexpr int kThreads = 256, kWarps = kThreads / 32;
 constexpr int kRows = 16;   // rows of the weights of a CTA
 constexpr int kChunk = 32;  // elements of the sum that a warp's 16-byte loads cover
 constexpr int kUnroll = 4;  // chunks in flight
+// CTAs of an SM. (8 tokens, 2048 x 8192: 22.6 us with four of the down product's,
+// 24.7 with its 80 registers and three; two chunks in flight and four CTAs for h
+// were slower.)
+constexpr int per_sm_of(int mats, int tiles) { return mats == 1 && tiles == 1 ? 4 : 2; }
 // CTAs of a cluster at most: 8, or as many as shared memory holds the sums of.
 constexpr int most_slices(int mats, int tiles) { return mats * tiles >= 8 ? 4 : 8; }
 
@@ -56,7 +60,7 @@ __device__ __forceinline__ uint4 weight16(const void* p, bool ok) {
 
 // MATS weights (2: w_gate and w_up of the same rows), TILES eights of tokens.
 template <typename T, int MATS, int TILES>
-__global__ void __launch_bounds__(kThreads, 2) ffn_few_kernel(const __grid_constant__ FewArgs a) {
+__global__ void __launch_bounds__(kThreads, per_sm_of(MATS, TILES)) ffn_few_kernel(const __grid_constant__ FewArgs a) {
   constexpr int kSums = MATS * TILES * 4;  // accumulators of a lane
   __shared__ float sums[kWarps][kSums][32];
   __shared__ float total[most_slices(MATS, TILES)][kSums][32];  // the leader's: every slice's sums
@@ -64,6 +68,8 @@ __global__ void __launch_bounds__(kThreads, 2) ffn_few_kernel(const __grid_const
   const int slice = blockIdx.x % a.slices;
   const int64_t row0 = static_cast<int64_t>(blockIdx.x / a.slices) * kRows;
   float acc[MATS][TILES][4] = {};
+  const bool cluster = a.slices > 1;  // whose first CTA has to run before the others write to it
+  if (cluster) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
 
   // this warp's chunks of the sum: every (slices * 8)th run of kUnroll chunks
   const int64_t chunks = (a.K + kChunk - 1) / kChunk, runs = (chunks + kUnroll - 1) / kUnroll;
@@ -119,18 +125,19 @@ __global__ void __launch_bounds__(kThreads, 2) ffn_few_kernel(const __grid_const
 #pragma unroll
   for (int i = 0; i < kSums; ++i) sums[warp][i][lane] = acc[i / (TILES * 4)][i / 4 % TILES][i % 4];
   __syncthreads();
+  if (cluster) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
   for (int i = threadIdx.x; i < kSums * 32; i += kThreads) {
     float s = 0.f;
 #pragma unroll
     for (int k = 0; k < kWarps; ++k) s += (&sums[k][0][0])[i];
-    if (a.slices == 1) {
+    if (!cluster) {
       (&total[0][0][0])[i] = s;
     } else {  // to the cluster's first CTA
       uint32_t dst = static_cast<uint32_t>(__cvta_generic_to_shared(&total[slice][0][0] + i));
       asm volatile("mapa.shared::cluster.u32 %0, %0, 0;\n\tst.shared::cluster.f32 [%0], %1;" : "+r"(dst) : "f"(s) : "memory");
     }
   }
-  if (a.slices == 1) {
+  if (!cluster) {
     __syncthreads();
   } else {
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
