@@ -134,8 +134,10 @@ __device__ __forceinline__ uint32_t cluster_addr(const void* p, uint32_t rank) {
   asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(smem_u32(p)), "r"(rank));
   return r;
 }
+// Relaxed: what it gives back has been read (tcgen05.wait::ld), and a release
+// would wait for the warp's stores to shared memory as well.
 __device__ __forceinline__ void arrive_cluster(uint32_t addr) {
-  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(addr) : "memory");
+  asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(addr) : "memory");
 }
 // A box of a matrix into this CTA, counted on a barrier of the pair.
 __device__ __forceinline__ void fetch_box(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
