@@ -49,6 +49,26 @@ __device__ __forceinline__ void ffn_act(int act, float a, float& val, float& der
   }
 }
 
+// A launch whose CTAs come up while the last ones of the launch before it leave:
+// the kernel touches no memory before pdl_wait_prior_grid(), and lets the next
+// launch in with pdl_launch_dependents().
+template <typename... Args>
+int ffn_launch(void (*kernel)(Args...), dim3 grid, int threads, int smem, cudaStream_t s, const Args&... args) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  if (cudaLaunchKernelEx(&cfg, kernel, args...) == cudaSuccess) return HC_OK;
+  cudaGetLastError();
+  return HC_ERR_LAUNCH;
+}
+
 // Up to kFfnMaxJobs products in one launch, which then share K, one term, the
 // order of their operands and the epilogue kStore. `parts`: the sum of splits *
 // M * N floats where the sum is split, more than one (kStore only), else
@@ -61,6 +81,7 @@ struct FfnParts {
   const float* parts;
   void* out;
   int64_t count;
+  bool fours;  // (set by ffn_add_parts) four at a time
 };
 int ffn_add_parts(const FfnParts* jobs, int count, int splits, int dtype, cudaStream_t s);
 

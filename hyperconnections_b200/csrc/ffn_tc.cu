@@ -743,18 +743,37 @@ struct AddJobs {
   FfnParts job[kFfnMaxJobs];
   int jobs, splits;
 };
+template <typename T> __device__ __forceinline__ void put_sum(T* p, float4 s) {
+  if constexpr (sizeof(T) == 4)
+    *reinterpret_cast<float4*>(p) = s;
+  else
+    *reinterpret_cast<uint2*>(p) = make_uint2(pack2<T>(s.x, s.y), pack2<T>(s.z, s.w));
+}
 template <typename T> __global__ void __launch_bounds__(256) add_parts_kernel(const __grid_constant__ AddJobs a) {
   const int64_t stride = static_cast<int64_t>(gridDim.x) * 256, first = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  pdl_launch_dependents();
+  pdl_wait_prior_grid();
 #pragma unroll
   for (int j = 0; j < kFfnMaxJobs; ++j) {
     if (j >= a.jobs) break;
     const float* parts = a.job[j].parts;
     T* out = static_cast<T*>(a.job[j].out);
     const int64_t count = a.job[j].count;
-    for (int64_t i = first; i < count; i += stride) {
-      float s = 0.f;
-      for (int p = 0; p < a.splits; ++p) s += parts[p * count + i];
-      out[i] = Elem<T>::from_f(s);
+    if (a.job[j].fours) {
+      for (int64_t i = 4 * first; i < count; i += 4 * stride) {
+        float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int p = 0; p < a.splits; ++p) {
+          const float4 v = *reinterpret_cast<const float4*>(parts + p * count + i);
+          s = make_float4(s.x + v.x, s.y + v.y, s.z + v.z, s.w + v.w);
+        }
+        put_sum<T>(out + i, s);
+      }
+    } else {
+      for (int64_t i = first; i < count; i += stride) {
+        float s = 0.f;
+        for (int p = 0; p < a.splits; ++p) s += parts[p * count + i];
+        out[i] = Elem<T>::from_f(s);
+      }
     }
   }
 }
@@ -914,23 +933,10 @@ int ffn_tc_launch(const FfnProduct* ps, int jobs, int dtype, float* parts, cudaS
   a.wait_limit = wait_poll_limit();
   a.status = timeout_word(s);
   const int items = a.tiles * a.splits, pairs = items < pairs_resident() ? items : pairs_resident();
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(2 * pairs);
-  cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = kSmemBytes;
-  cfg.stream = s;
-  cudaLaunchAttribute at[1];  // a product's CTAs come up while the last ones of the product before it leave
-  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  at[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = at;
-  cfg.numAttrs = 1;
-  if (cudaLaunchKernelEx(&cfg, kernel, maps, a) != cudaSuccess) {
-    cudaGetLastError();
-    return HC_ERR_LAUNCH;
-  }
+  if (int rc = ffn_launch(kernel, dim3(2 * pairs), kThreads, kSmemBytes, s, maps, a)) return rc;
   if (a.splits == 1) return HC_OK;
   FfnParts sums[kFfnMaxJobs];
-  for (int j = 0; j < jobs; ++j) sums[j] = {a.job[j].parts, ps[j].out, ps[j].M * ps[j].N};
+  for (int j = 0; j < jobs; ++j) sums[j] = {a.job[j].parts, ps[j].out, ps[j].M * ps[j].N, false};
   return ffn_add_parts(sums, jobs, a.splits, dtype, s);
 }
 
@@ -941,16 +947,15 @@ int ffn_add_parts(const FfnParts* jobs, int count, int splits, int dtype, cudaSt
   int64_t most = 0;
   for (int j = 0; j < count; ++j) {
     a.job[j] = jobs[j];
-    if (jobs[j].count > most) most = jobs[j].count;
+    a.job[j].fours = jobs[j].count % 4 == 0 && aligned16(jobs[j].parts) && aligned16(jobs[j].out);
+    const int64_t items = a.job[j].fours ? jobs[j].count / 4 : jobs[j].count;
+    if (items > most) most = items;
   }
   const int64_t want = ceil_div(most, 256), cap = 8 * static_cast<int64_t>(sm_count());
   const int grid = static_cast<int>(want < cap ? want : cap);
-  switch (dtype) {
-    case HC_DTYPE_F32: add_parts_kernel<float><<<grid, 256, 0, s>>>(a); break;
-    case HC_DTYPE_F16: add_parts_kernel<__half><<<grid, 256, 0, s>>>(a); break;
-    default: add_parts_kernel<__nv_bfloat16><<<grid, 256, 0, s>>>(a); break;
-  }
-  return launch_status();
+  const auto kernel = dtype == HC_DTYPE_F32 ? add_parts_kernel<float> : dtype == HC_DTYPE_F16 ? add_parts_kernel<__half>
+                                                                                              : add_parts_kernel<__nv_bfloat16>;
+  return ffn_launch(kernel, dim3(grid), 256, 0, s, a);
 }
 
 unsigned int ffn_take_timeouts(bool reset) {
