@@ -17,12 +17,12 @@
 // Forward and backward of 4096 x 1024 x 2048: 48 TFLOP/s (3,217 us; 3,788 with
 // single FMAs), two thirds of the FMA units' peak: the reads of shared memory
 // return 128 bytes a cycle, as long as the FMAs they feed take. Of 517 x 333 x
-// 887: 136 us (204 with 4 x 4 values and no groups): five products of 20-39 us,
+// 887: 133 us (204 with 4 x 4 values and no groups): five products of 20-39 us,
 // two thirds of them waits for the first stages and for each other's last ones.
 //
 // A few rows, at most 24, take tiles of 8 x 64, a thread all rows of four
 // columns for four of a stage's sixteen steps: the weights' way through shared
-// memory bounds it.
+// memory bounds it. The forward of at most 4 rows streams the weights.
 #include "ffn.cuh"
 #include "mix_warp.cuh"  // smem_u32
 #include "pairs.cuh"
@@ -316,7 +316,116 @@ __global__ void __launch_bounds__(kThreads, Layout<TM>::kPerSm) ffn_simt_kernel(
   }
 }
 
+// The forward's products for at most 4 rows of A, bound by the weights: a CTA
+// takes four rows of them (two of w_gate and the same two of w_up), its lanes 16
+// bytes of each at a time and its warps every eighth 512 bytes, straight into
+// registers; x comes from L1. No stage, no barrier until the sums meet. (Forward
+// of 2048 x 8192: 46 us, 4.3 TB/s of weights, for one token and 57 for four, against
+// 75 and 77 with tiles; for eight, whose x costs more loads than the weights, 81
+// against 78.)
+constexpr int kStreamThreads = 256, kStreamWarps = kStreamThreads / 32, kStreamTokens = 4;
+
+__device__ __forceinline__ float4 weight4(const float* p) {
+  float4 v;
+  asm volatile("ld.global.nc.L1::no_allocate.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "l"(p));
+  return v;
+}
+
+template <int MATS> __global__ void __launch_bounds__(kStreamThreads, 3) ffn_stream_kernel(const __grid_constant__ FfnProduct p) {
+  constexpr int kRows = 4 / MATS;
+  __shared__ float sums[kStreamWarps][4 * kStreamTokens];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t row0 = static_cast<int64_t>(blockIdx.x) * kRows;
+  const int tokens = static_cast<int>(p.M);
+  const float* w[4];
+  bool there[4];
+#pragma unroll
+  for (int v = 0; v < 4; ++v) {
+    const FfnOperand& b = p.B[v / kRows];
+    const int64_t row = row0 + v % kRows;
+    there[v] = row < b.rows;
+    w[v] = static_cast<const float*>(b.p) + (there[v] ? row : 0) * b.row_stride;
+  }
+  const float* x = static_cast<const float*>(p.A[0].p);
+  const int64_t ldx = p.A[0].row_stride;
+  f2 acc[4][kStreamTokens] = {};  // of even and odd steps
+  constexpr int64_t kStep = 4 * kStreamThreads;
+  const int64_t first = 4 * threadIdx.x;
+  float4 next[4];
+  const auto load = [&](int64_t k) {
+#pragma unroll
+    for (int v = 0; v < 4; ++v) next[v] = k < p.K && there[v] ? weight4(w[v] + k) : make_float4(0.f, 0.f, 0.f, 0.f);
+  };
+  load(first);
+  for (int64_t k = first; k < p.K; k += kStep) {  // K is a multiple of 4
+    f2 lo[4], hi[4];
+#pragma unroll
+    for (int v = 0; v < 4; ++v) {
+      lo[v] = pair(next[v].x, next[v].y);
+      hi[v] = pair(next[v].z, next[v].w);
+    }
+    load(k + kStep);
+#pragma unroll
+    for (int t = 0; t < kStreamTokens; ++t) {
+      if (t >= tokens) break;
+      const float4 xv = __ldg(reinterpret_cast<const float4*>(x + t * ldx + k));
+      const f2 x0 = pair(xv.x, xv.y), x1 = pair(xv.z, xv.w);
+#pragma unroll
+      for (int v = 0; v < 4; ++v) acc[v][t] = fma2(hi[v], x1, fma2(lo[v], x0, acc[v][t]));
+    }
+  }
+  // the lanes' sums: every exchange sends half of the live values, lanes l and l + 16 end with value l (row l / 4, token
+  // l % 4)
+  constexpr int kValues = 4 * kStreamTokens;
+  float s[kValues];
+#pragma unroll
+  for (int i = 0; i < kValues; ++i) s[i] = fold2(acc[i / kStreamTokens][i % kStreamTokens]);
+#pragma unroll
+  for (int o = kValues / 2; o > 0; o >>= 1)
+#pragma unroll
+    for (int i = 0; i < o; ++i) {
+      const float keep = lane & o ? s[i + o] : s[i], give = lane & o ? s[i] : s[i + o];
+      s[i] = keep + __shfl_xor_sync(kFull, give, o);
+    }
+  s[0] += __shfl_xor_sync(kFull, s[0], kValues);
+  if (lane < kValues) sums[warp][lane] = s[0];
+  __syncthreads();
+  if (warp != 0) return;
+  float r = 0.f;
+#pragma unroll
+  for (int i = 0; i < kStreamWarps; ++i) r += sums[i][lane % kValues];
+  const float b = __shfl_down_sync(kFull, r, kValues / 2);  // MATS 2: of w_up
+  const int64_t t = lane % kStreamTokens, n = row0 + lane / kStreamTokens, to = t * p.ldo + n;
+  if (lane >= kValues / MATS || t >= tokens || n >= p.N) return;
+  if constexpr (MATS == 2) {
+    float val, der;
+    ffn_act(p.act, r, val, der);
+    static_cast<float*>(p.out)[to] = val * b;
+    if (p.slope_gate) {
+      static_cast<float*>(p.slope_gate)[to] = der * b;
+      static_cast<float*>(p.slope_up)[to] = val;
+    }
+  } else {
+    static_cast<float*>(p.out)[to] = r;
+  }
+}
+
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+// Whether the streaming kernel takes a product: rows of whole 16 bytes, summed along them.
+bool streams(const FfnProduct& p) {
+  if (p.M > kStreamTokens || p.terms != 1 || p.epilogue == kGluBwd || p.K % 4 != 0) return false;
+  for (const FfnOperand* o : {&p.A[0], &p.B[0], &p.B[p.epilogue == kGlu ? 1 : 0]})
+    if (o->k_stride != 1 || o->row_stride % 4 != 0 || !aligned16(o->p)) return false;
+  return true;
+}
+int stream_launch(const FfnProduct& p, cudaStream_t s) {
+  if (p.epilogue == kGlu)
+    ffn_stream_kernel<2><<<static_cast<unsigned>(ceil_div(p.N, 2)), kStreamThreads, 0, s>>>(p);
+  else
+    ffn_stream_kernel<1><<<static_cast<unsigned>(ceil_div(p.N, 4)), kStreamThreads, 0, s>>>(p);
+  return launch_status();
+}
 
 template <int TM> void (*kernel_of(int epilogue, bool ak, bool bk))(Jobs) {  // the orders that occur: see ffn.cuh
   if (epilogue == kGlu) return ffn_simt_kernel<kGlu, TM, true, true>;
@@ -345,6 +454,7 @@ int ffn_simt_splits(int64_t tiles, int64_t K, int terms, bool few) {
 
 int ffn_simt_launch(const FfnProduct* ps, int count, float* parts, cudaStream_t s) {
   const int epilogue = ps[0].epilogue, tile_n = epilogue == kGlu ? kTile / 2 : kTile;
+  if (count == 1 && streams(ps[0])) return stream_launch(ps[0], s);
   bool few = true;
   for (int j = 0; j < count; ++j) few = few && ffn_simt_few(ps[j].M);
   Jobs jobs{};

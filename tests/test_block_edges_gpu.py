@@ -30,7 +30,7 @@ def ops():
 
 
 # ------------------------------------------------------------ a few tokens
-@pytest.mark.parametrize("T", [1, 2, 7, 8, 9, 16, 24, 31, 32, 33, 64, 65])
+@pytest.mark.parametrize("T", [1, 2, 3, 4, 5, 7, 8, 9, 16, 24, 25, 31, 32, 33, 64, 65])
 @pytest.mark.parametrize("dt,act", [("bf16", "silu"), ("fp16", "gelu_tanh"), ("fp32", "silu")])
 def test_ffn_around_the_few_token_limit(T, dt, act):
     t, g = inputs(T, 264, 520, 136, dt, seed=T)

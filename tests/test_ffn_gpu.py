@@ -112,6 +112,10 @@ SHAPES = [
     (65, 333, 200, 77, "fp32", "silu"),
     (130, 128, 192, 64, "fp32", "gelu_tanh"),
     (700, 40, 24, 56, "fp32", "silu"),
+    (3, 64, 100, 37, "fp32", "gelu_tanh"),
+    (4, 1028, 2052, 1030, "fp32", "silu"),
+    (24, 72, 136, 260, "fp32", "silu"),
+    (25, 72, 136, 260, "fp32", "silu"),
 ]
 
 
