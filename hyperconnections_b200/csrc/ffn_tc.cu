@@ -13,9 +13,9 @@
 //               copies are counted on the leader's barrier
 //   warp 1      multiplies (in the leader CTA): one lane issues the four
 //               16-deep steps of a stage for both CTAs
-//   warp 2      owns the tensor memory
-//   warp 3      (for da, db) fetches the tile's slopes, 32 columns at a time for
-//               each quarter, into the quarters' 16 KB slots
+//   warp 2      owns the tensor memory, and (for da, db) stores what is finished
+//   warp 3      (for da, db) fetches the tile's slopes, 32 columns of a quarter
+//               at a time, into six slots of 16 KB that go round
 //   warps 4-19  finish: four groups of four warps read the accumulator out of
 //               tensor memory, a quarter of the columns each, and write the
 //               result while the next tile is multiplied into the other half of
@@ -23,9 +23,17 @@
 //
 // Results leave through shared memory and TMA stores, and slopes come by TMA
 // loads: a warp holds a row a lane, so its own loads and stores would touch 32
-// lines each (da and db of 32,768 tokens, 384 x 1536, fp16: 134 us that way, 99
-// with the copies). A quarter's slopes come in two halves of 32 columns, so that
-// all four quarters fetch and finish at once.
+// lines each (da and db of 32,768 tokens, 384 x 1536, fp16: 134 us that way, 84
+// with the copies). da and db take their slopes' places; a warp of its own stores
+// them, so that the finishing warps need not wait for their slots to empty.
+//
+// What bounds the products is L2: at 10-13.6 TB/s in each of the five of that
+// shape (100, 47, 84, 89 and 128 us for h and the slopes, y, da and db, dx, the
+// weights' gradients); those of 16,384 tokens, 2048 x 8192, bf16 keep the tensor
+// pipe 58-91% active. Fetching the next blocks into L2 ahead of their copies made
+// every product 20-30% slower; a sixth stage and a release fence less changed
+// nothing, and 128-byte lines for slopes and results cost the first shape what
+// they gave the other.
 //
 // An operand is read as it lies: summed along its unit stride ("K-major", x
 // and the weights of the forward) or across it ("MN-major", the weights of dx

@@ -24,6 +24,9 @@ or bfloat16); the rest in float32, and every gradient comes back in its
 tensor's own dtype. norm is "rms" (x / sqrt(mean x^2 + eps)) or "layer"
 ((x - mean) / sqrt(var + eps)), and for ``hc_mix_write_norm`` also "none".
 Dropout's bits are those of ``hc_dropout`` on z as a tensor [*, m, D].
+
+With one stream and one block the norm takes R's size out of y: R's gradient is
+then 0 but for eps, and what comes out is mostly rounding.
 """
 
 from __future__ import annotations
