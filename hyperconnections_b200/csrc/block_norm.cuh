@@ -23,10 +23,12 @@
 //   * a warp folds k sums by halving exchanges (every exchange sends half of
 //     the live values: about k + 5 - log k shuffles), writes them to shared
 //     memory, and behind the group's barrier every thread adds the W warps' in
-//     order. The backward's sums come in two rounds, the norm's two, which the
-//     gradients wait for, and the token's small matrices', which nothing waits
-//     for: those are added behind the next token's barrier. A token costs one
-//     barrier.
+//     order. The backward's sums are the norm's two and the token's small
+//     matrices'. The mix-write has all of them before its barrier and adds them
+//     behind it; the read's second ones come out of the gradients, behind the
+//     barrier, and are added behind the next token's. A token costs one barrier
+//     (the mix-write's backward with a projection, whose matrices pass from
+//     thread to thread, three).
 // Ragged rows cost more instructions, not more bytes: they travel in 4-byte
 // copies and are shifted when they are read, g x^T is summed on the FMA units,
 // and outputs are put together in shared memory. (16,384 tokens, n = 4, bf16,
@@ -1143,15 +1145,13 @@ __global__ void __launch_bounds__(norm_bwd_threads(N, M, sizeof(T), WIDE))
     A[0][k].fill(0.f);
     B[0][k].fill(0.f);
   }
-  int64_t last = -1;
-  int last_parity = 0, last_slot = 0;
-  // grad_H, grad_v and grad_W of the last token, whose warps' sums lie in the other buffer
-  auto flush = [&] {
-    if (last < 0) return;
-    grads.store(p, last, [&](int q, int id) { return gram[last_parity][p.slot0() + q][id]; });
+  // grad_H, grad_v and grad_W of the token whose warps' sums lie in gram[parity], behind the barrier that completes
+  // them: the next sums to go there are those of the token after next, behind one more barrier
+  auto add_sums = [&](int64_t t, int slot, int parity) {
+    grads.store(p, t, [&](int q, int id) { return gram[parity][p.slot0() + q][id]; });
     if (a.v) {
       p.sync();
-      S::grads(a, p, small[last_slot], memory.G, last);
+      S::grads(a, p, small[slot], memory.G, t);
     }
   };
   auto fetch_outer = [&](int64_t t) {  // g, x and gate
@@ -1310,7 +1310,7 @@ __global__ void __launch_bounds__(norm_bwd_threads(N, M, sizeof(T), WIDE))
         __syncwarp();  // warp_gram's reads are done before the next token's copies overwrite the rows
         if (next < a.T) fetch_outer(next);
         p.sync();
-        flush();
+        add_sums(t, slot, parity);
         if (a.v) {  // the next token's mix, which its work begins with
           S::project(p, small[(slot + 1) & (kSmallSlots - 1)], mixed[parity ^ 1]);
           p.sync();
@@ -1339,12 +1339,7 @@ __global__ void __launch_bounds__(norm_bwd_threads(N, M, sizeof(T), WIDE))
           if constexpr (RAGGED) rows.template unstage<M>(static_cast<T*>(a.grad_f) + t * E + p.d0, m, D, p.warp_cols);
         }
         if (next < a.T) fetch_f(next);
-        last = t;
-        last_parity = parity;
-        last_slot = slot;
       });
-  p.sync();
-  flush();
   store_param_sums<RAGGED, 1, M>(a, p, p.live ? 1 : 0, A, B);
 }
 
