@@ -239,10 +239,10 @@ __device__ __forceinline__ int owned_chunks(const Place& p, int64_t D) {
 
 // Mean and 1 / root of the group's values: u[c][k] of each chunk c that the
 // thread owns (`chunks` of them) and each block k < m; what does not exist
-// holds 0. `red` is one buffer, a float4 a warp; one barrier where W > 1. The
-// variance of a LayerNorm is merged from (count, mean, sum of squared
-// deviations) triples pair by pair, which loses nothing where the mean is large
-// against the deviations.
+// holds 0. `red` is one buffer, a float4 a warp; one barrier where W > 1, none
+// where W = 1. The variance of a LayerNorm is merged from (count, mean, sum of
+// squared deviations) triples pair by pair, which loses nothing where the mean
+// is large against the deviations.
 template <bool RAGGED, int CH, int M, int MAXW>
 __device__ __forceinline__ void group_stats(const Place& p, const V8 (&u)[CH][M], int chunks, int m, int norm, float eps,
                                             float inv, float4 (&red)[MAXW], float& mean, float& rstd) {
@@ -477,9 +477,10 @@ __device__ __forceinline__ float one(f2 v) {
 // The loop over a group's tokens. all(t) issues the copies of a token's rows,
 // small(t, slot) those of its small matrices. work(t, next, slot, parity) does
 // token t, whose rows have arrived and whose small matrices have since the
-// barrier before; it passes the group's barrier exactly once, and where
-// next < T asks for that token's rows, each as soon as it has read this
-// token's.
+// barrier before; between two tokens' uses of a buffer, and between a token's
+// wait for copies and another thread's use of them, it passes a barrier of the
+// group (of a warp for W = 1, where a shuffle is none). Where next < T it asks
+// for that token's rows, each as soon as it has read this token's.
 template <typename All, typename Small, typename Start, typename Work>
 __device__ __forceinline__ void walk_tokens(const Place& p, int64_t T, All all, Small small, Start start, Work work) {
   const int64_t t0 = p.first(), step = p.stride();
@@ -1035,6 +1036,9 @@ __global__ void __launch_bounds__(norm_fwd_threads(N, M, CH, sizeof(T), WIDE))
         } else {
           p.sync();
         }
+        // a group of one warp has passed no barrier in group_stats: what its lanes copied (the next token's matrices) and
+        // wrote (this token's mix) is read by one another below
+        if (p.W == 1) __syncwarp();
         const f2* s = small[slot];
         if (a.v) S::project(p, small[(slot + 1) & (kSmallSlots - 1)], mixed[parity ^ 1]);
         const f2* H = a.v ? mixed[parity] : s;

@@ -53,3 +53,18 @@ def test_mix_write_gradients_of_a_token(T, n, m, D, dt, norm, proj):
     for _ in range(3):
         for a, b in zip(write_step(t, g, **kw), alone):
             assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("T,n,m,D,dt,norm", [
+    (FEW * 120, 4, 1, 256, "bf16", "rms"),
+    (FEW * 120, 4, 1, 768, "bf16", "layer"),  # one warp, three chunks a thread
+    (FEW * 60, 8, 2, 200, "fp16", "layer"),
+    (FEW * 60, 3, 1, 77, "fp32", "rms"),
+])
+def test_projected_mix_of_one_warp(T, n, m, D, dt, norm):
+    """The projected mix of a token is made by its warp's lanes for one another."""
+    t, _ = write_inputs(T, n, m, D, dt, "wbs", "sigmoid", True)
+    kw = dict(norm=norm, gate_activation="sigmoid")
+    alone = torch.cat([ops().hc_mix_write_norm(**part(t, i), **kw) for i in range(0, T, FEW)])
+    for _ in range(3):
+        assert torch.equal(ops().hc_mix_write_norm(**t, **kw), alone)
