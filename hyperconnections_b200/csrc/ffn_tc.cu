@@ -32,8 +32,8 @@
 // weights' gradients); those of 16,384 tokens, 2048 x 8192, bf16 keep the tensor
 // pipe 58-91% active. Fetching the next blocks into L2 ahead of their copies made
 // every product 20-30% slower; a sixth stage and a release fence less changed
-// nothing, and 128-byte lines for slopes and results cost the first shape what
-// they gave the other.
+// nothing (the fence is there), and 128-byte lines for slopes and results cost
+// the first shape what they gave the other.
 //
 // An operand is read as it lies: summed along its unit stride ("K-major", x
 // and the weights of the forward) or across it ("MN-major", the weights of dx
@@ -142,10 +142,23 @@ __device__ __forceinline__ uint32_t cluster_addr(const void* p, uint32_t rank) {
   asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(smem_u32(p)), "r"(rank));
   return r;
 }
-// Relaxed: what it gives back has been read (tcgen05.wait::ld), and a release
-// would wait for the warp's stores to shared memory as well.
+// An arrival on a barrier of either CTA of the pair. Release: it gives back tensor memory whose reads (tcgen05.ld,
+// waited for and fenced) have to come before the other side's next products. A relaxed one, which no rule of the memory
+// model orders so, was no faster in any product.
 __device__ __forceinline__ void arrive_cluster(uint32_t addr) {
-  asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(addr) : "memory");
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(addr) : "memory");
+}
+// The wait that goes with it.
+__device__ __forceinline__ bool try_wait_cluster(uint64_t* bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(smem_u32(bar)), "r"(parity)
+      : "memory");
+  return ok;
 }
 // A box of a matrix into this CTA, counted on a barrier of the pair.
 __device__ __forceinline__ void fetch_box(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
@@ -233,10 +246,11 @@ __device__ __forceinline__ uint64_t matrix_desc(uint32_t addr, bool mn) {
   return static_cast<uint64_t>((addr & 0x3ffff) >> 4) | (lead << 16) | (step << 32) | (1ull << 46) | (2ull << 61);
 }
 
-// Bounded wait that also ends when the pair has been told to stop.
+// Bounded wait that also ends when the pair has been told to stop. CLUSTER: for threads of both CTAs.
+template <bool CLUSTER = false>
 __device__ __forceinline__ bool pair_wait(Shared& sh, uint64_t* bar, uint32_t parity, uint32_t limit) {
   for (uint32_t i = 0; i < limit; ++i) {
-    if (mbar_try_wait(bar, parity)) return true;
+    if (CLUSTER ? try_wait_cluster(bar, parity) : mbar_try_wait(bar, parity)) return true;
     if (sh.stop) return false;
   }
   return false;
@@ -592,7 +606,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       bool ok = true;
       for (int i = first; i < items && ok; i += step) {
         const Item it = item_at(a, i);
-        if (!pair_wait(sh, &sh.acc_empty[buf], acc_ph ^ 1, a.wait_limit)) {
+        if (!pair_wait<true>(sh, &sh.acc_empty[buf], acc_ph ^ 1, a.wait_limit)) {
           ok = false;
           break;
         }
