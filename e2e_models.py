@@ -41,6 +41,7 @@ import torch.nn.functional as F
 
 from hyperconnections_b200.block import BlockOptions
 from hyperconnections_b200.cghc import ContinuousGenHyperConnections
+from hyperconnections_b200.drop_state import DropState
 from hyperconnections_b200.ops import gated_ffn, hc_dropout
 
 N_STREAMS = 4
@@ -122,15 +123,13 @@ class EmbeddingDropout(nn.Module):
     def __init__(self, p: float):
         super().__init__()
         self.p = p
-        self.register_buffer("state", torch.stack([torch.randint(1 << 62, ()), torch.zeros((), dtype=torch.int64)]),
-                             persistent=False)
+        self.bits = DropState()
 
     def forward(self, h):
         if not self.training:
             return h
-        out = hc_dropout(h, self.p, self.state)
-        self.state[1].add_(1)
-        return out
+        with self.bits.drawn(h.device) as seed:
+            return hc_dropout(h, self.p, seed)
 
 
 def hc(dim: int, module: nn.Module, block: BlockOptions | None = None) -> ContinuousGenHyperConnections:

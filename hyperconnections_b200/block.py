@@ -18,12 +18,14 @@ its parameters, ``state_dict`` keys and results.
 
 from __future__ import annotations
 
+from contextlib import nullcontext
 from dataclasses import dataclass
 from typing import Literal, Optional
 
 import torch
 import torch.nn as nn
 
+from .drop_state import DropState
 from .ops import hc_mix_write, hc_mix_write_norm, hc_read, hc_read_norm
 
 NormKind = Literal["rms", "layer"]
@@ -63,10 +65,11 @@ class _Norm(nn.Module):
 class BlockParts(nn.Module):
     """The parameters of a layer's ``BlockOptions`` and its read and write.
 
-    Dropout's bits come from ``drop_state``, an int64 buffer (seed, offset) on
+    Dropout's bits come from ``drop_state``, an int64 tensor (seed, offset) on
     the layer's device (seeded from torch's generator, not part of the
     ``state_dict``): every training step's write draws with the next offset, also
-    when a graph that holds it is replayed."""
+    when a graph that holds it is replayed, and a write that a checkpoint runs
+    again with the offset of its first run (``drop_state.py``)."""
 
     def __init__(self, options: BlockOptions, embed_dim: int):
         super().__init__()
@@ -76,8 +79,11 @@ class BlockParts(nn.Module):
         self.gate = nn.Linear(embed_dim, embed_dim) if options.gate else None
         self.scale = None if options.residual_scale is None else nn.Parameter(
             torch.full((embed_dim,), float(options.residual_scale)))
-        seed = torch.randint(1 << 62, (1,)) if options.dropout else torch.zeros(1, dtype=torch.int64)
-        self.register_buffer("drop_state", torch.cat([seed, torch.zeros(1, dtype=torch.int64)]), persistent=False)
+        self.bits = DropState(seeded=options.dropout > 0)
+
+    @property
+    def drop_state(self) -> torch.Tensor:
+        return self.bits.state
 
     def read(self, R: torch.Tensor, x: torch.Tensor) -> torch.Tensor:
         """The block's input [T, m, D] from the streams x [T, n, D]."""
@@ -93,13 +99,10 @@ class BlockParts(nn.Module):
         if p is None and self.gate is None and self.scale is None and drop == 0.0:
             return hc_mix_write(H, x, W, f, v)
         gate = None if self.gate is None else self.gate(u.reshape(-1, self.embed_dim)).view(f.shape)
-        out = hc_mix_write_norm(H, x, W, f, v, norm="none" if p is None else p.kind,
-                                weight=None if p is None else p.weight, bias=None if p is None else p.bias, eps=o.eps,
-                                gate=gate, gate_activation="sigmoid", scale=self.scale, dropout_p=drop,
-                                seed=self.drop_state if drop else None)
-        if drop:
-            self.drop_state[1].add_(1)
-        return out
+        with self.bits.drawn(x.device) if drop else nullcontext() as seed:
+            return hc_mix_write_norm(H, x, W, f, v, norm="none" if p is None else p.kind,
+                                     weight=None if p is None else p.weight, bias=None if p is None else p.bias, eps=o.eps,
+                                     gate=gate, gate_activation="sigmoid", scale=self.scale, dropout_p=drop, seed=seed)
 
 
 def read_block(parts: Optional[BlockParts], R, x):
