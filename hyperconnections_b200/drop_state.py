@@ -17,6 +17,7 @@ from collections import OrderedDict
 from contextlib import contextmanager
 
 import torch
+import torch.distributed as dist
 import torch.nn as nn
 
 
@@ -27,10 +28,28 @@ def _may_run_again() -> bool:
     return not torch.is_grad_enabled() or torch._C._autograd._top_saved_tensors_default_hooks(True) is not None
 
 
+def _number() -> int:
+    return int(torch.randint(1 << 62, (), device="cpu"))
+
+
+_RANK_STEP = 0x1E3779B97F4A7C15  # odd: no two ranks below 2^62 meet
+
+
+def _rank() -> int:
+    return dist.get_rank() if dist.is_available() and dist.is_initialized() else 0
+
+
 class DropState(nn.Module):
     """``state``: int64 (seed, offset), seeded from torch's generator and not
     part of the ``state_dict``. Each draw has the state as it is and adds 1 to
     the offset.
+
+    The ranks of a job seed torch alike and drop out different tokens, so with
+    ``torch.distributed`` set up before the module is made, each rank's seed is
+    its own (rank 0's is the generator's). The state is no buffer:
+    DistributedDataParallel would put rank 0's on every rank before each forward.
+    It moves with the module, or to where it is first drawn. Ranks that hold the
+    same tokens want the same state: set it.
 
     A checkpoint's second forward runs inside the backward pass, from the same
     state of torch's CPU generator as the first (``preserve_rng_state``, its
@@ -50,8 +69,21 @@ class DropState(nn.Module):
     def __init__(self, seeded: bool = True):
         super().__init__()
         seed = torch.randint(1 << 62, (1,)) if seeded else torch.zeros(1, dtype=torch.int64)
-        self.register_buffer("state", torch.cat([seed, torch.zeros(1, dtype=torch.int64)]), persistent=False)
+        if seed.is_meta:  # a module without memory yet
+            seed = torch.randint(1 << 62, (1,), device="cpu")
+        if seeded and _rank() > 0:
+            seed = (seed + _rank() * _RANK_STEP) % (1 << 62)
+        self.state = torch.cat([seed, torch.zeros_like(seed)])
         self._filed = OrderedDict()  # number -> [(seed, offset), drawn again, two of them]
+
+    def _apply(self, fn, recurse=True):
+        super()._apply(fn, recurse)
+        self._move(fn(self.state).device)
+        return self
+
+    def _move(self, device: torch.device) -> None:
+        if device.type != "meta":
+            self.state = self.state.to(device)
 
     def __getstate__(self):  # of a copy: its own draws
         return {**self.__dict__, "_filed": OrderedDict()}
@@ -79,6 +111,7 @@ class DropState(nn.Module):
     @contextmanager
     def drawn(self, device: torch.device):
         """The (seed, offset) of one forward, on `device`."""
+        self._move(device)
         if torch._C._current_graph_task_id() != -1:  # a backward pass is running on this thread
             yield self._find()
         elif _may_run_again():
@@ -89,7 +122,3 @@ class DropState(nn.Module):
         else:
             yield self.state
             self.state[1].add_(1)
-
-
-def _number() -> int:
-    return int(torch.randint(1 << 62, (), device="cpu"))

@@ -4,9 +4,14 @@ the (seed, offset) it is given; on the GPU the layers and the embedding's
 dropout, whose gradients under a checkpoint are those of the plain step."""
 
 import copy
+import os
+import socket
+from datetime import timedelta
 
 import pytest
 import torch
+import torch.distributed as dist
+import torch.multiprocessing as mp
 import torch.nn as nn
 from torch.utils.checkpoint import checkpoint
 
@@ -107,6 +112,70 @@ def test_copies_have_their_own_draws():
     assert len(a.bits._filed) == 1 and not b.bits._filed and b.bits.state.tolist() == [3, 101]
     assert not b.state_dict()
     assert grad_of(out, x) == 100
+
+
+def test_the_state_goes_with_its_module():
+    a = Stand()
+    a.bits.state.copy_(torch.tensor([1 << 61, 1 << 60]))
+    for moved in (a.double(), a.half(), a.to("cpu", torch.bfloat16), a.to_empty(device="cpu"), a.to("meta"), a.cpu()):
+        assert moved.bits.state.dtype == torch.int64 and moved.bits.state.tolist() == [1 << 61, 1 << 60]
+    with torch.device("meta"):
+        made = DropState()
+    assert made.state.device.type == "cpu" and made.state[0] != 0
+    assert not dict(a.named_buffers()) and not dict(a.named_parameters())
+    assert DropState(seeded=False).state.tolist() == [0, 0]
+
+
+def _worker(rank, world, port, q):
+    os.environ.update(MASTER_ADDR="127.0.0.1", MASTER_PORT=str(port))
+    dist.init_process_group("gloo", rank=rank, world_size=world, timeout=timedelta(seconds=60))
+    try:
+        torch.manual_seed(0)
+
+        class Net(nn.Module):
+            def __init__(self):
+                super().__init__()
+                self.drop, self.fc = Stand(), nn.Linear(4, 4)
+                self.drop.bits = DropState()
+
+            def forward(self, x):
+                return self.fc(self.drop(x))
+
+        net = nn.parallel.DistributedDataParallel(Net())
+        states = [net.module.drop.bits.state.tolist()]
+        for _ in range(2):
+            net(torch.ones(2, 4)).sum().backward()
+            states.append(net.module.drop.bits.state.tolist())
+        q.put((rank, states, net.module.drop.seen, net.module.fc.weight.detach().sum().item()))
+    finally:
+        dist.destroy_process_group()
+
+
+def test_ranks_that_seed_alike_draw_other_bits():
+    """Two ranks build the same model from the same seed: their states differ from the beginning and after forwards of
+    DistributedDataParallel; rank 0 has what one process alone has."""
+    world = 2
+    ctx = mp.get_context("spawn")
+    q = ctx.Queue()
+    with socket.socket() as s:
+        s.bind(("127.0.0.1", 0))
+        port = s.getsockname()[1]
+    procs = [ctx.Process(target=_worker, args=(r, world, port, q)) for r in range(world)]
+    for p in procs:
+        p.start()
+    res = sorted(q.get(timeout=120) for _ in range(world))
+    for p in procs:
+        p.join(timeout=60)
+        assert p.exitcode == 0
+    torch.manual_seed(0)
+    Stand(), nn.Linear(4, 4)
+    alone = DropState().state[0].item()
+    (_, first, seen0, w0), (_, second, seen1, w1) = res
+    assert w0 == w1
+    assert first == [[alone, k] for k in range(3)] and seen0 == [[alone, 0], [alone, 1]]
+    other = second[0][0]
+    assert other != alone and 0 <= other < 1 << 62
+    assert second == [[other, k] for k in range(3)] and seen1 == [[other, 0], [other, 1]]
 
 
 # --------------------------------------------------------------------- GPU
