@@ -66,10 +66,14 @@ template <typename Saved> tensor_list wanted(AutogradContext* ctx, const Saved& 
   return d;
 }
 
+// Whether a call goes through its autograd Function: a gradient may be asked of
+// it, or an input carries a tangent of forward-mode differentiation (with or
+// without gradients enabled), which the Function refuses; without it the tangent
+// would be lost.
 bool wants_grad(std::initializer_list<const Tensor*> ts) {
-  if (!at::GradMode::is_enabled()) return false;
+  const bool grads = at::GradMode::is_enabled();
   for (const Tensor* t : ts)
-    if (t->defined() && t->requires_grad()) return true;
+    if (t->defined() && ((grads && t->requires_grad()) || t->_fw_grad(/*level=*/0).defined())) return true;
   return false;
 }
 
