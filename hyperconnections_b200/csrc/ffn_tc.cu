@@ -327,8 +327,9 @@ __device__ __forceinline__ float inverse_fast(float x) {
   return r;
 }
 // act(a) and act'(a) of two values with the approximate exponential and
-// inverse: their errors, a few 2^-22 relative, are far below the half steps 2^-8
-// and 2^-11 of the types they go to.
+// inverse: their errors, a few 2^-22 relative, and that of the exponent's
+// argument (at most 36 for |a| <= 6: some 125 2^-24 of the result) are far below
+// the half steps 2^-8 and 2^-11 of the types they go to.
 __device__ __forceinline__ f2 sigmoid_of(f2 x) {  // 1 / (1 + 2^x)
   float e0, e1;
   split(x, e0, e1);
@@ -341,15 +342,14 @@ __device__ __forceinline__ void fast_act(int act, f2 a, f2& val, f2& der) {
     const f2 s = sigmoid_of(mul2(a, both(-kLog2e)));
     val = mul2(a, s);
     der = fma2(val, fma2(s, both(-1.f), both(1.f)), s);
-  } else {  // tanh(u) = 1 - 2 i, i = 1 / (1 + e^2u); past |a| = 10 it is 1, and a^2 need not grow
-    constexpr float c = 0.7978845608028654f;
+  } else {  // a / (1 + e^-2u), see ffn_act
+    constexpr float c2 = 2.f * 0.7978845608028654f;
     float q0, q1;
     split(mul2(a, a), q0, q1);
-    const f2 a2 = pair(fminf(q0, 1e4f), fminf(q1, 1e4f)), half = mul2(a, both(0.5f));
-    const f2 i = sigmoid_of(mul2(mul2(a, both(2.f * c * kLog2e)), fma2(a2, both(0.044715f), both(1.f))));
-    const f2 t = fma2(i, both(-2.f), both(1.f)), less = fma2(i, both(2.f), both(-1.f));
-    val = fma2(half, t, half);
-    der = fma2(mul2(half, fma2(less, t, both(1.f))), fma2(a2, both(3.f * 0.044715f * c), both(c)), fma2(i, both(-1.f), both(1.f)));
+    const f2 a2 = pair(fminf(q0, 1e4f), fminf(q1, 1e4f));
+    const f2 s = sigmoid_of(mul2(mul2(a, both(-c2 * kLog2e)), fma2(a2, both(0.044715f), both(1.f))));
+    val = mul2(a, s);
+    der = fma2(mul2(val, fma2(s, both(-1.f), both(1.f))), fma2(a2, both(3.f * 0.044715f * c2), both(c2)), s);
   }
 }
 
