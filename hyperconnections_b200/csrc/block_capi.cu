@@ -25,6 +25,15 @@ bool f32_ok(std::initializer_list<const float*> ps) {
   return true;
 }
 
+// Streams are read by their elements where they are not on wider boundaries.
+bool streams_ok(int sdt, std::initializer_list<const void*> ps) {
+  for (const void* p : ps)
+    if (reinterpret_cast<uintptr_t>(p) % dtype_size(sdt) != 0) return false;
+  return true;
+}
+
+bool state_ok(const int64_t* state) { return reinterpret_cast<uintptr_t>(state) % sizeof(int64_t) == 0; }
+
 // Dropout's arguments; false when p is not in [0, 1].
 bool drop_args(DropArgs& d, double p, const int64_t* state, int64_t seed, int64_t offset) {
   if (!(p >= 0.0 && p <= 1.0)) return false;
@@ -142,7 +151,7 @@ extern "C" int hc_read_norm_fwd(const float* R, const void* x, const float* weig
   if (!(eps >= 0.f)) return HC_ERR_BAD_SIZE;
   if (T == 0 || D == 0) return HC_OK;
   if (!R || !x || !y) return HC_ERR_NULL_POINTER;
-  if (!f32_ok({R, weight, bias, stats})) return HC_ERR_ALIGNMENT;
+  if (!f32_ok({R, weight, bias, stats}) || !streams_ok(stream_dtype, {x, y})) return HC_ERR_ALIGNMENT;
   NormArgs a{};
   a.R = R; a.x = x; a.weight = weight; a.bias = bias; a.out = y; a.stats = stats;
   a.T = T; a.D = D; a.n = n; a.m = m; a.norm = norm; a.eps = eps;
@@ -168,7 +177,8 @@ extern "C" int hc_read_norm_bwd(const void* g, const float* R, const void* x, co
     return HC_OK;
   }
   if (!g || !R || !x || !stats) return HC_ERR_NULL_POINTER;
-  if (!f32_ok({R, weight, stats, grad_R, grad_weight, grad_bias, scratch})) return HC_ERR_ALIGNMENT;
+  if (!f32_ok({R, weight, stats, grad_R, grad_weight, grad_bias, scratch}) || !streams_ok(stream_dtype, {g, x, grad_x}))
+    return HC_ERR_ALIGNMENT;
   const bool params = grad_weight || grad_bias;
   if (params && (!scratch || scratch_words < hc_norm_scratch_words(T, n, m, D, stream_dtype))) return HC_ERR_SCRATCH;
   NormArgs a{};
@@ -201,7 +211,8 @@ extern "C" int hc_mix_write_norm_fwd(const float* H, const void* x, const float*
   if (!(eps >= 0.f)) return HC_ERR_BAD_SIZE;
   if (T == 0 || D == 0) return HC_OK;
   if (!H || !x || !W || !f || !out) return HC_ERR_NULL_POINTER;
-  if (!f32_ok({H, W, v, weight, bias, scale, stats})) return HC_ERR_ALIGNMENT;
+  if (!f32_ok({H, W, v, weight, bias, scale, stats}) || !streams_ok(stream_dtype, {x, f, gate, out}) || !state_ok(state))
+    return HC_ERR_ALIGNMENT;
   NormArgs a{};
   a.H = H; a.x = x; a.W = W; a.f = f; a.v = v; a.weight = weight; a.bias = bias; a.gate = gate; a.scale = scale;
   a.out = out; a.stats = stats; a.T = T; a.D = D; a.n = n; a.m = m; a.norm = norm; a.gate_act = gate_act; a.eps = eps;
@@ -224,7 +235,8 @@ extern "C" int hc_mix_write_norm_bwd(const void* g, const float* H, const void* 
   if (int rc = check_write(norm, gate_act, p)) return rc;
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
   const int64_t E = m * D;
-  if (!f32_ok({H, W, v, weight, bias, scale, stats, grad_H, grad_W, grad_v, grad_weight, grad_bias, grad_scale, scratch}))
+  if (!f32_ok({H, W, v, weight, bias, scale, stats, grad_H, grad_W, grad_v, grad_weight, grad_bias, grad_scale, scratch}) ||
+      !streams_ok(stream_dtype, {g, x, f, gate, grad_x, grad_f, grad_gate}) || !state_ok(state))
     return HC_ERR_ALIGNMENT;
   if (T == 0 || D == 0) {  // sums over nothing
     const struct { float* p; int64_t words; } zero[] = {{grad_H, T * n * n}, {grad_W, T * n * m}, {grad_v, T * n},
@@ -258,6 +270,7 @@ extern "C" int hc_dropout(const void* x, void* y, int64_t N, double p, const int
   if (!drop_args(d, p, state, seed, offset)) return HC_ERR_BAD_SIZE;
   if (N == 0) return HC_OK;
   if (!x || !y) return HC_ERR_NULL_POINTER;
+  if (!streams_ok(stream_dtype, {x, y}) || !state_ok(state)) return HC_ERR_ALIGNMENT;
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (!d.on) {  // every element is kept, times 1
     if (x == y) return HC_OK;

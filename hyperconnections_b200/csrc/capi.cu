@@ -8,7 +8,7 @@ extern "C" const char* hc_error_string(int code) {
     case HC_ERR_BAD_SIZE: return "negative or out-of-range size";
     case HC_ERR_UNSUPPORTED_N: return "number of streams / matrix order n must be in 1..8";
     case HC_ERR_DTYPE: return "unsupported dtype or dtype combination";
-    case HC_ERR_ALIGNMENT: return "a float32 pointer is not 4-byte aligned";
+    case HC_ERR_ALIGNMENT: return "a pointer is not aligned (float32 to 4 bytes)";
     case HC_ERR_SCRATCH: return "scratch buffer missing or too small";
     case HC_ERR_LAUNCH: return "CUDA kernel launch failed";
     case HC_ERR_TIMEOUT:

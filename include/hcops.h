@@ -53,7 +53,8 @@ extern "C" {
 #define HC_ERR_BAD_SIZE       2  /* negative size, or n / D out of range           */
 #define HC_ERR_UNSUPPORTED_N  3  /* n (or m) outside the entry point's range      */
 #define HC_ERR_DTYPE          4  /* unknown dtype code or unsupported combination  */
-#define HC_ERR_ALIGNMENT      5  /* a float32 pointer is not 4-byte aligned        */
+#define HC_ERR_ALIGNMENT      5  /* a pointer is not aligned: float32 to 4 bytes;  */
+                                 /* the block's operators: as each says            */
 #define HC_ERR_SCRATCH        6  /* scratch buffer missing or too small            */
 #define HC_ERR_LAUNCH         7  /* the CUDA launch itself failed                  */
 #define HC_ERR_TIMEOUT        8  /* a bounded wait in an earlier launch gave up    */
@@ -378,6 +379,12 @@ int hc_mix_write_bwd(const void* g, const float* H, const void* x,
  * hc_mix_write_norm needs for the gradients of its [E] parameters. Returns 0
  * in error cases. Depends on the current device's SM count. */
 int64_t hc_norm_scratch_words(int64_t T, int n, int m, int64_t D, int stream_dtype);
+
+/* Tensors of the norm operators and of hc_dropout are aligned to their own
+ * type, `state` to 8 bytes; 16-byte boundaries are faster. Rows of 16-bit
+ * streams that are not on 4-byte boundaries are read by the aligned words that
+ * hold them: up to one element before and behind a tensor is read with them
+ * and not used. */
 
 /* u[t,k,:] = sum_j R[t,k,j] x[t,j,:];  y[t] = weight * norm(u[t]) + bias over
  * the E values of a token. R [T,m,n], x [T,n,D] -> y [T,m,D]; weight, bias
