@@ -83,7 +83,7 @@ __global__ void __launch_bounds__(kThreads, per_sm_of(MATS, TILES)) ffn_few_kern
     uint4 wa[kUnroll][MATS][2], xb[kUnroll][TILES];
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u) {
-      const int64_t k = (run * kUnroll + u) * kChunk + q * 8;  // K is a multiple of 8
+      const int64_t k = (run * kUnroll + u) * kChunk + q * 8;  // rows hold whole eights, zeros behind K
 #pragma unroll
       for (int m = 0; m < MATS; ++m) {
         const T* p = w[m] + (row0 + r) * a.ldw + k;
@@ -157,6 +157,7 @@ __global__ void __launch_bounds__(kThreads, per_sm_of(MATS, TILES)) ffn_few_kern
     if constexpr (MATS == 2) {
       float val, der;
       ffn_act(a.act, s[0], val, der);
+      if (row >= a.rows) val = der = s[MATS - 1] = 0.f;  // read by the down product: 0 also where an infinite x made 0 x inf
       static_cast<T*>(a.out)[at] = Elem<T>::from_f(val * s[MATS - 1]);
       if (a.slope_gate) {
         static_cast<T*>(a.slope_gate)[at] = Elem<T>::from_f(der * s[MATS - 1]);

@@ -451,7 +451,7 @@ int hc_dropout(const void* x, void* y, int64_t N, double p,
  * and b but what dh is multiplied with: slope_gate = act'(a) b, slope_up =
  * act(a), computed in float32 and rounded once, like h. These three are
  * [T,Fp] with Fp = F rounded up to a multiple of 8 (their last columns are
- * written 0); the slopes are NULL when no backward follows. Half-precision
+ * written too: 0 for a finite row of x, and unused); the slopes are NULL when no backward follows. Half-precision
  * tensors start on 16-byte boundaries. scratch:
  * hc_gated_ffn_scratch_bytes(0, ...) bytes, 256-byte aligned. */
 int hc_gated_ffn_fwd(const void* x, const void* w_gate, const void* w_up,
