@@ -238,8 +238,8 @@ __device__ __forceinline__ int owned_chunks(const Place& p, int64_t D) {
 }
 
 // Mean and 1 / root of the group's values: u[c][k] of each chunk c that the
-// thread owns (`chunks` of them) and each block k < m; what does not exist
-// holds 0. `red` is one buffer, a float4 a warp; one barrier where W > 1, none
+// thread owns (`chunks` of them) and each block k < m; columns that do not exist
+// hold 0. `red` is one buffer, a float4 a warp; one barrier where W > 1, none
 // where W = 1. The variance of a LayerNorm is merged from (count, mean, sum of
 // squared deviations) triples pair by pair, which loses nothing where the mean
 // is large against the deviations.
@@ -252,9 +252,11 @@ __device__ __forceinline__ void group_stats(const Place& p, const V8 (&u)[CH][M]
 #pragma unroll
     for (int c = 0; c < CH; ++c)
 #pragma unroll
-      for (int k = 0; k < M; ++k)
+      for (int k = 0; k < M; ++k) {
+        if (M > 2 && k >= m) break;  // three blocks of four: 0 x inf in the last one is not theirs
 #pragma unroll
         for (int i = 0; i < 4; ++i) s2 = fma2(u[c][k].v[i], u[c][k].v[i], s2);
+      }
     float s = fold2(s2);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(kFull, s, o);
