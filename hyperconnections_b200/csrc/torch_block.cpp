@@ -317,6 +317,8 @@ MaybeTensor dropout(const Tensor& x, const MaybeTensor& state_, double p, int64_
 
 // ----------------------------------------------------------------- gated_ffn
 struct GatedFfn : public torch::autograd::Function<GatedFfn> {
+  // A width of 0: every sum is empty, and y and all gradients are 0.
+  static bool nothing(const tensor_list& t) { return t[0].size(-1) == 0 || t[3].numel() == 0; }
   static Tensor scratch_bytes(int backward, int64_t T, int64_t D, int64_t F, int64_t O, const Tensor& x,
                               int64_t* size) {
     *size = hc_gated_ffn_scratch_bytes(backward, T, D, F, O, code_of(x.scalar_type()));
@@ -330,6 +332,7 @@ struct GatedFfn : public torch::autograd::Function<GatedFfn> {
     int64_t T = 1;
     for (size_t i = 0; i + 1 < sizes.size(); ++i) T *= sizes[i];
     sizes.back() = O;
+    if (nothing(t)) return torch::zeros(sizes, x.options());
     Tensor y = torch::empty(sizes, x.options()), h = torch::empty({T, Fp}, x.options()), sg, su;
     if (keep) {
       sg = torch::empty_like(h);
@@ -345,7 +348,7 @@ struct GatedFfn : public torch::autograd::Function<GatedFfn> {
   }
   static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& w_gate, const Tensor& w_up,
                         const Tensor& w_down, int64_t act) {
-    tensor_list t = {dense16(x), dense16(w_gate), dense16(w_up), dense16(w_down)}, inner;
+    tensor_list t = {dense16(x), dense16(w_gate), dense16(w_up), dense16(w_down)}, inner(3);
     Tensor y = run(t, act, true, &inner);
     t.insert(t.end(), inner.begin(), inner.end());
     ctx->save_for_backward(t);
@@ -356,9 +359,15 @@ struct GatedFfn : public torch::autograd::Function<GatedFfn> {
     const auto t = ctx->get_saved_variables();
     const Tensor &x = t[0], &h = t[4];
     const c10::cuda::CUDAGuard guard(x.device());
+    tensor_list d = wanted(ctx, t, 4);
+    if (nothing(t)) {
+      for (Tensor& a : d)
+        if (a.defined()) a.zero_();
+      d.emplace_back();
+      return once(std::move(d));
+    }
     const int64_t D = x.size(-1), F = t[1].size(0), O = t[3].size(0), T = h.size(0);
     const Tensor g = dense16(grads[0].to(x.scalar_type()));
-    tensor_list d = wanted(ctx, t, 4);
     const bool inner = d[0].defined() || d[1].defined() || d[2].defined();
     const Tensor da = like(inner, h), db = like(inner, h);
     int64_t size = 0;
