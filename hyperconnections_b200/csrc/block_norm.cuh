@@ -32,8 +32,8 @@
 // Ragged rows cost more instructions, not more bytes: they travel in 4-byte
 // copies and are shifted when they are read, g x^T is summed on the FMA units,
 // and outputs are put together in shared memory. (16,384 tokens, n = 4, bf16,
-// forward and backward: 165 us at D = 769 against 122 at 768 for the read, 440
-// against 182 for the mix-write.)
+// forward and backward: 168 us at D = 769 against 95 at 768 for the read, 444
+// against 180 for the mix-write.)
 //
 // The [m D] parameters' gradients are sums over tokens: a thread keeps its
 // columns' sums in registers over all of its group's tokens and writes them
@@ -50,7 +50,8 @@ namespace hc {
 constexpr int kColumns = 8;      // a thread's columns
 constexpr int kSmallGroups = 4;  // groups of a CTA when a group is one warp
 constexpr int kSmallSlots = 8;   // tokens whose small matrices are held (5 are live; a power of two)
-constexpr int kNormSmemMax = 210 * 1024;  // of the 227 KB a CTA can have; up to 10 KB are static
+constexpr int kCtaSmemMax = 227 * 1024;
+constexpr int kNormSmemMax = 210 * 1024;  // dynamic; the sums of a token are static, up to 12.3 KB (n = 8, m = 4, 512 threads)
 
 // Threads of a CTA at most, which bounds the registers of one. WIDE: kernels
 // with room for 4096 columns, whose registers spill, for tokens that the others
@@ -689,6 +690,7 @@ __global__ void __launch_bounds__(norm_bwd_threads(N, M, sizeof(T), WIDE))
   constexpr int MAXW = norm_bwd_threads(N, M, sizeof(T), WIDE) / 32, G = N * M;
   extern __shared__ __align__(16) uint8_t dyn[];
   __shared__ float red[2][MAXW][2], gram[2][MAXW][G];
+  static_assert(kNormSmemMax + sizeof(red) + sizeof(gram) <= kCtaSmemMax);
   const Place p(warps, a.D);
   const int n = a.n, m = a.m;
   const int64_t D = a.D, E = D * m;
@@ -1119,6 +1121,7 @@ __global__ void __launch_bounds__(norm_bwd_threads(N, M, sizeof(T), WIDE))
   using S = Small<N, M, true>;
   extern __shared__ __align__(16) uint8_t dyn[];
   __shared__ float red[2][MAXW][2], gram[2][MAXW][G];
+  static_assert(kNormSmemMax + sizeof(red) + sizeof(gram) <= kCtaSmemMax);
   const Place p(warps, a.D);
   const int n = a.n, m = a.m;
   const int64_t D = a.D, E = D * m;
@@ -1353,7 +1356,11 @@ __global__ void __launch_bounds__(norm_bwd_threads(N, M, sizeof(T), WIDE))
 using NormKernel = void (*)(NormArgs, int);
 
 // Rows of whole chunks have kernels for 1, 2, 4 and 8 streams, ragged ones for 4
-// and 8; none for fewer streams than blocks.
+// and 8; none for fewer streams than blocks. Numbers between are cheap to read
+// and dear to mix (16,384 x n x 768 bf16, forward and backward, n = 3, 4, 5, 6, 7,
+// 8: read 86, 95, 110, 120, 128, 136 us, mix-write 173, 180, 283, 291, 297, 303;
+// m = 3 and 4 at n = 4: read 187, 199, mix-write 449, 525): the work of the mix
+// is the larger kernel's.
 inline int padded_blocks(int m) { return m <= 1 ? 1 : m <= 2 ? 2 : 4; }
 inline int padded_streams(int n, int M, bool ragged) {
   const int least = ragged ? 4 : M > n ? M : n;
@@ -1410,8 +1417,10 @@ template <typename T, bool WRITE> NormKernel norm_kernel(const NormGeometry& geo
 
 // Warps of a token's group, and for the forward the chunks a thread owns; 0
 // warps where the 8-column kernels do not take the shape (rows that do not fit a
-// CTA). `aligned`: streams and parameters on 16-byte
-// boundaries.
+// CTA: a backward's threads own one chunk, so from 4104 columns on; 4,096 tokens,
+// n = 4, bf16: backward of 4096, 5120 and 8192 columns in 81, 706 and 1,183 us for
+// the read, 151, 3,062 and 5,052 for the mix-write). `aligned`: streams and
+// parameters on 16-byte boundaries.
 inline NormGeometry norm_geometry(bool write, bool bwd, int n, int m, int64_t D, int esize, bool aligned) {
   NormGeometry g{};
   g.ragged = !aligned || D % kColumns != 0;

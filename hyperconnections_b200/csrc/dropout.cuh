@@ -1,9 +1,12 @@
 // dropout.cuh — y = x / (1 - p) where the element's Philox word says so, else 0.
 //
-// Bound by HBM as long as the generator keeps up: a block of four words is ten
-// rounds of two 32 x 32 -> 64 bit products and two three-input xors (the round
-// keys, the same for all, stay in registers), about 80 instructions for the
-// eight elements that a thread moves at a time.
+// A block of four words is ten rounds of two 32 x 32 -> 64 bit products and two
+// three-input xors (the round keys, the same for all, stay in registers), about
+// 80 instructions for the eight elements that a thread moves at a time. 33.5M
+// elements in one direction: bf16 36 us (floor 20.5), float32 47 (41). In bf16
+// no pipe is full (ALU 56%, the multipliers 37%, issue 59 of 100 cycles at 86% of
+// the warps): a warp waits 28% of its time for its 16 bytes, half of it for a pipe
+// or its turn.
 #pragma once
 
 #include "block.cuh"

@@ -23,17 +23,20 @@
 //
 // Results leave through shared memory and TMA stores, and slopes come by TMA
 // loads: a warp holds a row a lane, so its own loads and stores would touch 32
-// lines each (da and db of 32,768 tokens, 384 x 1536, fp16: 134 us that way, 84
+// lines each (da and db of 32,768 tokens, 384 x 1536, fp16: 134 us that way, 88
 // with the copies). da and db take their slopes' places; a warp of its own stores
 // them, so that the finishing warps need not wait for their slots to empty.
 //
-// What bounds the products is L2: at 10-13.6 TB/s in each of the five of that
-// shape (100, 47, 84, 89 and 128 us for h and the slopes, y, da and db, dx, the
-// weights' gradients); those of 16,384 tokens, 2048 x 8192, bf16 keep the tensor
-// pipe 58-91% active. Fetching the next blocks into L2 ahead of their copies made
-// every product 20-30% slower; a sixth stage and a release fence less changed
-// nothing (the fence is there), and 128-byte lines for slopes and results cost
-// the first shape what they gave the other.
+// What bounds the products: the wide ones (16,384 tokens, 2048 x 8192, bf16) keep
+// the tensor pipe 58-91% active, under the power limit. In the narrow ones of the
+// shape above (101, 48, 88, 91 and 131 us under the profiler for h and the slopes,
+// y, da and db, dx, the weights' gradients) no unit is full: tensor pipe 42, 45,
+// 23, 49 and 66%, L2 44, 28, 49, 33 and 37%, what the SMs read from it 17-30%. Of
+// each some 13 us are its start and end, and y and dx have tiles for 3.5 rounds of
+// the clusters, which take four. Fetching the next blocks into L2 ahead of their
+// copies made every product 20-30% slower; a sixth stage and a release fence less
+// changed nothing (the fence is there), and 128-byte lines for slopes and results
+// cost the first shape what they gave the other.
 //
 // An operand is read as it lies: summed along its unit stride ("K-major", x
 // and the weights of the forward) or across it ("MN-major", the weights of dx
