@@ -125,6 +125,10 @@ class EmbeddingDropout(nn.Module):
         self.p = p
         self.bits = DropState()
 
+    @property
+    def state(self) -> torch.Tensor:
+        return self.bits.state
+
     def forward(self, h):
         if not self.training:
             return h

@@ -85,6 +85,10 @@ class BlockParts(nn.Module):
     def drop_state(self) -> torch.Tensor:
         return self.bits.state
 
+    @drop_state.setter
+    def drop_state(self, state: torch.Tensor) -> None:
+        self.bits.state = state
+
     def read(self, R: torch.Tensor, x: torch.Tensor) -> torch.Tensor:
         """The block's input [T, m, D] from the streams x [T, n, D]."""
         if self.pre_norm is None:

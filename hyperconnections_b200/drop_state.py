@@ -83,7 +83,8 @@ class DropState(nn.Module):
 
     def _move(self, device: torch.device) -> None:
         if device.type != "meta":
-            self.state = self.state.to(device)
+            with torch.inference_mode(False):  # which makes tensors that no later step could move on
+                self.state = self.state.to(device)
 
     def __getstate__(self):  # of a copy: its own draws
         return {**self.__dict__, "_filed": OrderedDict()}

@@ -12,7 +12,8 @@ same places. Give every call of a step its own offset (or seed).
 seed and offset are whole numbers (taken modulo 2^64), or seed is an int64
 CUDA tensor of two elements (seed, offset), which the kernel reads when it
 runs: a step captured into a CUDA graph draws new bits at each replay when the
-step also moves that tensor on.
+step also moves that tensor on. ``drop_state.DropState`` does that for a module,
+with checkpoints and several ranks in mind.
 """
 
 from __future__ import annotations

@@ -126,6 +126,26 @@ def test_the_state_goes_with_its_module():
     assert DropState(seeded=False).state.tolist() == [0, 0]
 
 
+def test_the_state_of_a_layer_can_be_set():
+    from tests.test_block_layers import CGHC, FULL, layer
+
+    lay = layer(CGHC, 4, 2, 16, FULL)
+    lay.block.drop_state = torch.tensor([5, 6])
+    assert lay.block.bits.state.tolist() == [5, 6]
+    lay.block.drop_state.copy_(torch.tensor([7, 8]))
+    assert lay.block.drop_state.tolist() == [7, 8] and not any("state" in k for k in lay.state_dict())
+
+
+def test_a_draw_without_autograd_leaves_a_state_that_moves_on():
+    m, x = Stand(), torch.ones(1, requires_grad=True)
+    with torch.inference_mode():
+        m.float()
+        m(torch.ones(1))
+    with torch.no_grad():
+        m(x)
+    assert grad_of(m(x), x) == 102
+
+
 def _worker(rank, world, port, q):
     os.environ.update(MASTER_ADDR="127.0.0.1", MASTER_PORT=str(port))
     dist.init_process_group("gloo", rank=rank, world_size=world, timeout=timedelta(seconds=60))
