@@ -55,9 +55,9 @@ constexpr int kNormSmemMax = 210 * 1024;  // dynamic; the sums of a token are st
 
 // Threads of a CTA at most, which bounds the registers of one. WIDE: kernels
 // with room for 4096 columns, whose registers spill, for tokens that the others
-// have too few threads for. (Forward and backward of the mix-write, n = 8, m = 2:
-// 4,096 x 1024 fp16 in 192 us against 152 with fewer threads, 3,072 x 4096 bf16 in
-// 510 against 3,815 element by element.)
+// have too few threads for. (The mix-write's backward, n = 8, m = 2: 2,048 x 4096
+// bf16 in 203 us, at 4104 columns element by element 2,302; 4,096 x 1024 fp16,
+// which needs no such room, forward and backward in 192 against 152.)
 constexpr int kWideThreads = 512;
 constexpr int norm_bwd_threads(int N, int M, int esize, bool wide) {
   return wide ? kWideThreads : M >= 4 || (N == 8 && esize == 4) ? 256 : M == 2 || N == 8 ? 384 : 512;
