@@ -72,7 +72,7 @@ class DropState(nn.Module):
         if seed.is_meta:  # a module without memory yet
             seed = torch.randint(1 << 62, (1,), device="cpu")
         if seeded and _rank() > 0:
-            seed = (seed + _rank() * _RANK_STEP) % (1 << 62)
+            seed = (seed + _rank() * _RANK_STEP % (1 << 62)) % (1 << 62)  # the sum stays below 2^63
         self.state = torch.cat([seed, torch.zeros_like(seed)])
         self._filed = OrderedDict()  # number -> [(seed, offset), drawn again, two of them]
 

@@ -4,7 +4,7 @@
     y = (act(x w_gate^T) * (x w_up^T)) w_down^T
 
 x [*, D], w_gate and w_up [F, D], w_down [O, F] (the layouts of
-``nn.Linear.weight``) -> y [*, O]; activation "silu" or "gelu_tanh" (the
+``nn.Linear.weight``) -> y [*, O], at most 2^22 rows of x and widths of 2^20; activation "silu" or "gelu_tanh" (the
 tanh form of GELU). Both projections, the activation and the product are one
 kernel, which writes h = act(a) * b and, when a backward follows, what dh is
 multiplied with there: act'(a) b and act(a). The backward does that where it

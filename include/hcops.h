@@ -451,9 +451,10 @@ int hc_dropout(const void* x, void* y, int64_t N, double p,
  * and b but what dh is multiplied with: slope_gate = act'(a) b, slope_up =
  * act(a), computed in float32 and rounded once, like h. These three are
  * [T,Fp] with Fp = F rounded up to a multiple of 8 (their last columns are
- * written too: 0 for a finite row of x, and unused); the slopes are NULL when no backward follows. Half-precision
- * tensors start on 16-byte boundaries. scratch:
- * hc_gated_ffn_scratch_bytes(0, ...) bytes, 256-byte aligned. */
+ * written too: 0 for a finite row of x, and unused); the slopes are NULL when
+ * no backward follows. Half-precision tensors start on 16-byte boundaries.
+ * T <= 2^22; 1 <= D, F, O <= 2^20. scratch: hc_gated_ffn_scratch_bytes(0, ...)
+ * bytes, 256-byte aligned. */
 int hc_gated_ffn_fwd(const void* x, const void* w_gate, const void* w_up,
                      const void* w_down, void* y, void* h, void* slope_gate,
                      void* slope_up, void* scratch, int64_t scratch_bytes,

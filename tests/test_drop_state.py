@@ -126,6 +126,19 @@ def test_the_state_goes_with_its_module():
     assert DropState(seeded=False).state.tolist() == [0, 0]
 
 
+def test_every_rank_has_a_seed_of_its_own(monkeypatch):
+    import hyperconnections_b200.drop_state as ds
+
+    for first in (0, 1, 2):  # seeds of the generator
+        seeds = []
+        for rank in [*range(64), 1000, 4095, 1 << 20]:
+            monkeypatch.setattr(ds, "_rank", lambda: rank)
+            torch.manual_seed(first)
+            seeds.append(DropState().state.tolist())
+        assert len({s for s, _ in seeds}) == len(seeds)
+        assert all(0 <= s < 1 << 62 and o == 0 for s, o in seeds)
+
+
 def test_the_state_of_a_layer_can_be_set():
     from tests.test_block_layers import CGHC, FULL, layer
 
